@@ -39,29 +39,29 @@ def listed():
 
     return [
         # one decode step of one sequence that reports the sampled token and 20 alternatives
-        logprobs("decode 1 row, top 20", 1, 50304, "bf16", top_k=20, temperature=0.8),
+        logprobs("decode 1 row top 20", 1, 50304, "bf16", top_k=20, temperature=0.8),
         # one decode step of a batch with capped fp32 logits of a large vocabulary
-        logprobs("decode 64 rows, fp32, top 5", 64, 131072, "fp32", top_k=5, softcap=30.0),
+        logprobs("decode 64 rows fp32 top 5", 64, 131072, "fp32", top_k=5, softcap=30.0),
         # scoring given text: no alternatives
-        logprobs("score 4096 rows, fp16", 4096, 32768, "fp16"),
+        logprobs("score 4096 rows fp16", 4096, 32768, "fp16"),
         # a teacher's pass over a training batch: its 64 most likely tokens per position
-        logprobs("teacher 8192 rows, top 64", 8192, 50304, "bf16", top_k=64, entropy=False, temperature=2.0),
+        logprobs("teacher 8192 rows top 64", 8192, 50304, "bf16", top_k=64, entropy=False, temperature=2.0),
         # a short policy-gradient batch with an odd vocabulary
-        logprobs("policy 37 rows, fp32, odd", 37, 50257, "fp32", train=True),
+        logprobs("policy 37 rows fp32 odd", 37, 50257, "fp32", train=True),
         # a policy-gradient step with an entropy bonus
         logprobs("policy 8192 rows", 8192, 50304, "bf16", train=True),
         # a small batch distilled with the rest of the vocabulary as one bucket
-        distill("distill 24 rows, fp32", 24, 32000, "fp32", 8, tail=True),
+        distill("distill 24 rows fp32", 24, 32000, "fp32", 8, tail=True),
         # fp16 with a loss scale, odd sizes, renormalised teacher
-        distill("distill 1023 rows, fp16, odd", 1023, 50257, "fp16", 33, tail=False, temperature=2.0),
+        distill("distill 1023 rows fp16 odd", 1023, 50257, "fp16", 33, tail=False, temperature=2.0),
         # a full distillation step
         distill("distill 8192 rows", 8192, 50304, "bf16", 64, tail=True, temperature=2.0),
         # the last positions of a few sequences scored from their hidden states
         head("head 8 rows", 8, 768, 50304, "bf16"),
         # scoring under a wider model, rows that fill no tile
-        head("head 2001 rows, fp16", 2001, 1536, 32000, "fp16"),
+        head("head 2001 rows fp16", 2001, 1536, 32000, "fp16"),
         # a policy-gradient step from the hidden states
-        head("head 4096 rows, train", 4096, 768, 50304, "bf16", train=True),
+        head("head 4096 rows train", 4096, 768, 50304, "bf16", train=True),
     ]
 
 
