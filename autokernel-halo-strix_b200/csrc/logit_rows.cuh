@@ -1,0 +1,280 @@
+// Device helpers shared by the operators over rows of logits (token log-probabilities,
+// distillation): addressing of strided rows, 32-byte groups, running softmax statistics.
+#pragma once
+
+#include "ak_common.cuh"
+
+namespace ak {
+
+// Rows of logits: row r is (outer, inner) = (r / inner, r % inner) and starts at
+// base + outer * s_outer + inner * s_inner elements, so a (B, T, V) view such as
+// logits[:, :-1] needs no copy.  Elements of a row are adjacent.
+struct RowAddr {
+  int64_t inner, s_outer, s_inner;
+  __host__ __device__ __forceinline__ int64_t off(int64_t r) const {
+    const int64_t o = r / inner;
+    return o * s_outer + (r - o * inner) * s_inner;
+  }
+};
+
+// What a logit x means: y = softcap(x), log-probabilities of y / temperature.
+// kl = log2(e) / temperature turns a difference of y into an exponent of 2.
+struct Squash {
+  float cap, inv_cap, inv_t, kl;
+};
+
+inline Squash make_squash(float temperature, float softcap) {
+  Squash q;
+  q.cap = softcap > 0.f ? softcap : 0.f;
+  q.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
+  q.inv_t = 1.f / temperature;
+  q.kl = (float)(1.4426950408889634 / (double)temperature);
+  return q;
+}
+
+template <bool CAP>
+__device__ __forceinline__ float squash(float x, const Squash& q) {
+  return CAP ? q.cap * tanhf(x * q.inv_cap) : x;
+}
+
+// Derivative of squash at its output y.
+template <bool CAP>
+__device__ __forceinline__ float squash_slope(float y, const Squash& q) {
+  if constexpr (!CAP) return 1.f;
+  const float t = y * q.inv_cap;
+  return 1.f - t * t;
+}
+
+// A row is cut into a head (elements before the first 32-byte boundary), groups of 16
+// elements (32 bytes of a 16-bit type, 64 bytes of fp32) and a tail of fewer than 16.
+constexpr int kGroup = 16;
+
+struct RowCut {
+  int head, groups, tail;
+};
+
+template <typename T>
+__device__ __forceinline__ RowCut cut_row(const T* row, int V) {
+  RowCut c;
+  const int mis = (int)(reinterpret_cast<uintptr_t>(row) & 31u);
+  c.head = min(V, mis ? (32 - mis) / (int)sizeof(T) : 0);
+  c.groups = (V - c.head) / kGroup;
+  c.tail = V - c.head - c.groups * kGroup;
+  return c;
+}
+
+// 32 bytes with one load or store (addresses 32-byte aligned).
+struct Words8 {
+  uint32_t w[8];
+};
+__device__ __forceinline__ Words8 load32(const void* p) {
+  Words8 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                 "=r"(r.w[7])
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ void store32(void* p, const Words8& r) {
+  asm volatile("st.global.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]),
+               "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7]), "l"(p)
+               : "memory");
+}
+
+// One group as it lies in memory, and as fp32 values.
+template <typename T>
+struct RawGroup {
+  Words8 r[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ RawGroup<T> load_group(const T* p) {
+  RawGroup<T> g;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) g.r[i] = load32(reinterpret_cast<const char*>(p) + 32 * i);
+  return g;
+}
+
+__device__ __forceinline__ float2 unpack2(uint32_t w, const __nv_bfloat16*) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, const __half*) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_group(float (&x)[kGroup], const RawGroup<T>& g) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(g.r[i / 8].w[i % 8]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = unpack2(g.r[0].w[i], (const T*)nullptr);
+      x[2 * i] = v.x;
+      x[2 * i + 1] = v.y;
+    }
+  }
+}
+
+// Stores 16 values rounded to T: one or two 32-byte stores where the address allows, else
+// element by element (the output's rows start at another phase than the input's).
+template <typename T>
+__device__ __forceinline__ void store_group(T* p, const float (&x)[kGroup], bool vec) {
+  if (vec) {
+    RawGroup<T> g;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) g.r[i / 8].w[i % 8] = __float_as_uint(x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g.r[0].w[i] = pack2(x[2 * i], x[2 * i + 1], (const T*)nullptr);
+    }
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) store32(reinterpret_cast<char*>(p) + 32 * i, g.r[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = from_f<T>(x[i]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Running softmax statistics of a set of logits
+// ---------------------------------------------------------------------------
+//   m   largest x (before squash; -inf for an empty set, NaN is passed over)
+//   mu  what exponents are taken against: squash(m), or 0 where m is -inf and uncapped
+//   s   sum of e = 2^(kl (y - mu))
+//   w   sum of e * kl (y - mu)    (entropy only)
+// y - mu is formed before the scaling: the product with kl of a number near the type's lowest
+// value would overflow, and a fused x * kl - mu * kl would turn that into NaN.  A -inf logit
+// adds nothing (its term of w is cut off at a finite exponent); a NaN reaches s.
+template <bool CAP, bool ENT>
+struct RowStats {
+  float m, mu, s, w;
+
+  __device__ __forceinline__ void init(const Squash& q) {
+    m = -INFINITY;
+    mu = CAP ? -q.cap : 0.f;
+    s = 0.f;
+    w = 0.f;
+  }
+
+  // Moves the statistics to the larger maximum mn.
+  __device__ __forceinline__ void rebase(float mn, const Squash& q) {
+    const float nu = CAP ? squash<CAP>(mn, q) : mn;
+    if (CAP || m != -INFINITY) {  // s is 0 or NaN for an uncapped m = -inf
+      const float d = fmaxf((mu - nu) * q.kl, -1e30f);
+      const float f = ex2(d);
+      if constexpr (ENT) w = f * fmaf(d, s, w);
+      s *= f;
+    }
+    m = mn;
+    mu = nu;
+  }
+
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], const Squash& q) {
+    float lm = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) lm = fmaxf(lm, x[i]);
+    add(x, lm, q);
+  }
+
+  // lm: the largest of x
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float lm, const Squash& q) {
+    static_assert(N % 2 == 0 || N == 1, "pairs");
+    if (lm > m) rebase(lm, q);
+    if constexpr (N == 1) {
+      const float d = (squash<CAP>(x[0], q) - mu) * q.kl;
+      const float e = ex2(d);
+      s += e;
+      if constexpr (ENT) w = fmaf(e, fmaxf(d, -1e4f), w);
+    } else {
+      const float2 nmu = make_float2(-mu, -mu), kl = make_float2(q.kl, q.kl);
+      float2 s2 = make_float2(s, 0.f), w2 = make_float2(w, 0.f);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 y = make_float2(squash<CAP>(x[i], q), squash<CAP>(x[i + 1], q));
+        const float2 d = __fmul2_rn(__fadd2_rn(y, nmu), kl);
+        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+        s2 = __fadd2_rn(s2, e);
+        if constexpr (ENT) w2 = __ffma2_rn(e, make_float2(fmaxf(d.x, -1e4f), fmaxf(d.y, -1e4f)), w2);
+      }
+      s = s2.x + s2.y;
+      if constexpr (ENT) w = w2.x + w2.y;
+    }
+  }
+
+  // Adds the statistics of another set.
+  __device__ __forceinline__ void merge(RowStats o, const Squash& q) {
+    if (o.m > m) rebase(o.m, q);
+    else if (m > o.m) o.rebase(m, q);
+    s += o.s;
+    if constexpr (ENT) w += o.w;
+  }
+
+  // Sums over the warp, the same on every lane.
+  __device__ __forceinline__ void warp_merge(const Squash& q) {
+    const float M = warp_max(m);
+    if (M > m) rebase(M, q);
+    s = warp_sum(s);
+    if constexpr (ENT) w = warp_sum(w);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Thread-block clusters: CTAs of one row
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t row_cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void row_cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// A word at the same shared-memory offset in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t ld_cluster_u32(const void* p, uint32_t rank) {
+  uint32_t a, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint64_t ld_cluster_u64(const void* p, uint32_t rank) {
+  uint32_t a;
+  uint64_t v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// Launches `kern` with clusters of `cs` CTAs (none for 1).
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_rows(void (*kern)(KArgs...), int64_t grid, int threads, int cs, size_t smem,
+                               cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cs;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cs > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+}  // namespace ak

@@ -1,0 +1,561 @@
+// Log-probabilities of given tokens from logit rows, with each row's entropy and its most
+// likely alternatives; sm_100a.
+//
+//   y = softcap(x) / T,  lse = log sum exp y,  logprob = y_t - lse
+//   H = lse - sum p y,   p = exp(y - lse)
+//   dx_i = [ g_lp (1[i = t] - p_i) - g_H p_i (log p_i + H) ] dy_i/dx_i
+//
+// Forward: one pass over the row with the running maximum and the two sums of RowStats, by one
+// CTA per row, or by a cluster of CTAs whose shares are joined through distributed shared memory
+// where there are few rows.
+//
+// Alternatives, without a second pass over the row: a thread writes the maximum of each group of
+// 16 adjacent elements it reads to shared memory.  Order groups by (maximum, lowest position) and
+// elements by (value, lowest position): an element outside the first k groups is preceded by the k
+// largest elements of those groups, so the k groups hold the k best elements, ties included.  Only
+// they are read again, from L2.
+#include "logit_rows.cuh"
+
+#include <algorithm>
+
+namespace ak {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTop = 128;         // alternatives
+constexpr int kMaxCluster = 8;       // the portable cluster size
+constexpr int kMaxGroupKeys = 8194;  // group maxima of one CTA's share (32 KB), head and tail included
+constexpr int kCandGroups = 512;     // candidates of the short way through the selection
+constexpr int kCandElems = 768;
+
+// Unsigned keys in the order of the values: -0 and +0 are equal, NaN is below every number, 0 is
+// no value at all.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 1u;
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return (b >> 31) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k <= 1u) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
+}
+
+// One CTA's share of a row as the selection sees it: local group 0 is the row's head (first CTA
+// only), 1 .. n are whole groups, n + 1 is the tail (last CTA only).
+template <typename T>
+struct Share {
+  const T* row;
+  int head, tail, g0, n, body_end;  // body_end: first element of the tail
+  int head_here, tail_here;
+  __device__ __forceinline__ int start(int j) const {
+    return j == 0 ? 0 : (j <= n ? head + (g0 + j - 1) * kGroup : body_end);
+  }
+  __device__ __forceinline__ int size(int j) const { return j == 0 ? head_here : (j <= n ? kGroup : tail_here); }
+  __device__ __forceinline__ int elems() const { return head_here + n * kGroup + tail_here; }
+};
+
+struct SelectScratch {
+  union {
+    struct {
+      uint32_t groups[kCandGroups];
+      uint64_t elems[kCandElems];
+    } cand;
+    uint32_t keys[kMaxTop * kGroup];  // the exact way: elements of the chosen groups
+  };
+  uint32_t chosen[kMaxTop];  // groups, then elements, in order of position
+  uint32_t warp_n[2][kWarps];
+  uint32_t ngroups, nelems;
+};
+
+// The first k of n keys in the order (key descending, position ascending): their positions,
+// ascending, in out.  Needs n >= k.  A binary search over the key's bits for the k-th largest,
+// then everything above it and the first of those equal to it.
+__device__ void select_exact(const uint32_t* keys, int n, int k, uint32_t* out, SelectScratch& sc) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t t = 0;
+  int above = 0;  // number of keys > t, known at the end
+  for (int bit = 31; bit >= -1; --bit) {
+    const uint32_t probe = bit >= 0 ? (t | (1u << bit)) : t;
+    int c = 0;
+    for (int i = tid; i < n; i += kThreads) c += bit >= 0 ? (keys[i] >= probe) : (keys[i] > probe);
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) sc.warp_n[0][warp] = (uint32_t)c;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) total += (int)sc.warp_n[0][i];
+    __syncthreads();
+    if (bit < 0) above = total;
+    else if (total >= k) t = probe;
+  }
+  const int equal_wanted = k - above;
+  int taken = 0, equal_seen = 0;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + tid;
+    const uint32_t key = i < n ? keys[i] : 0u;
+    const bool eq = i < n && key == t;
+    const uint32_t eq_ballot = __ballot_sync(0xffffffffu, eq);
+    if (lane == 0) sc.warp_n[0][warp] = __popc(eq_ballot);
+    __syncthreads();
+    int eq_before = equal_seen, eq_total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) eq_before += (int)sc.warp_n[0][w];
+      eq_total += (int)sc.warp_n[0][w];
+    }
+    eq_before += __popc(eq_ballot & ((1u << lane) - 1u));
+    const bool take = i < n && (key > t || (eq && eq_before < equal_wanted));
+    const uint32_t ballot = __ballot_sync(0xffffffffu, take);
+    if (lane == 0) sc.warp_n[1][warp] = __popc(ballot);
+    __syncthreads();
+    int before = taken, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += (int)sc.warp_n[1][w];
+      total += (int)sc.warp_n[1][w];
+    }
+    if (take) out[before + __popc(ballot & ((1u << lane) - 1u))] = (uint32_t)i;
+    taken += total;
+    equal_seen += eq_total;
+    __syncthreads();
+  }
+}
+
+// Entry of the sorted list: larger is better.
+__device__ __forceinline__ uint64_t entry(uint32_t key, int index) {
+  return ((uint64_t)key << 32) | (uint32_t)(~(uint32_t)index);
+}
+
+// The k best elements of the share, best first, in top[0 .. k).  gkeys holds the n + 2 group
+// maxima (a barrier has passed since they were written), mine the largest key this thread wrote.
+template <typename T>
+__device__ void select_top(uint64_t* top, const Share<T>& sh, const uint32_t* gkeys, uint32_t mine, int k,
+                           SelectScratch& sc) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // A lower bound of the k-th best group: each warp's j-th largest thread maximum, j = ceil(k /
+  // warps), and the smallest of these; at least warps * j >= k groups reach it.
+  const int j = (k + kWarps - 1) / kWarps;
+  uint32_t v = mine, bound = 0;
+  for (int i = 0; i < j; ++i) {
+    bound = __reduce_max_sync(0xffffffffu, v);
+    const uint32_t at = __ballot_sync(0xffffffffu, v == bound);
+    if (lane == __ffs(at) - 1) v = 0;
+  }
+  if (lane == 0) sc.warp_n[0][warp] = bound;
+  if (tid == 0) { sc.ngroups = 0; sc.nelems = 0; }
+  __syncthreads();
+  bound = sc.warp_n[0][0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) bound = min(bound, sc.warp_n[0][w]);
+  bound = max(bound, 1u);  // key 0 is no value
+  const int ng = sh.n + 2;
+  for (int i = tid; i < ng; i += kThreads) {
+    if (gkeys[i] >= bound) {
+      const uint32_t at = atomicAdd(&sc.ngroups, 1u);
+      if (at < kCandGroups) sc.cand.groups[at] = (uint32_t)i;
+    }
+  }
+  __syncthreads();
+  const uint32_t ncg = sc.ngroups;
+  bool exact = ncg > kCandGroups;
+  if (!exact) {
+    for (int i = tid; i < (int)ncg * kGroup; i += kThreads) {
+      const int g = (int)sc.cand.groups[i / kGroup], e = i % kGroup;
+      if (e < sh.size(g)) {
+        const int idx = sh.start(g) + e;
+        const uint32_t key = order_key(to_f<T>(sh.row[idx]));
+        if (key >= bound) {
+          const uint32_t at = atomicAdd(&sc.nelems, 1u);
+          if (at < kCandElems) sc.cand.elems[at] = entry(key, idx);
+        }
+      }
+    }
+    __syncthreads();
+    exact = sc.nelems > kCandElems;
+  }
+  if (!exact) {
+    const int ne = (int)sc.nelems;
+    for (int i = tid; i < ne; i += kThreads) {
+      const uint64_t e = sc.cand.elems[i];
+      int rank = 0;
+      for (int o = 0; o < ne; ++o) rank += sc.cand.elems[o] > e;
+      if (rank < k) top[rank] = e;
+    }
+    __syncthreads();
+    return;
+  }
+  // Many equal values (masked or constant rows): choose the k groups, then the k elements, exactly.
+  __syncthreads();
+  const int kg = min(k, ng);
+  select_exact(gkeys, ng, kg, sc.chosen, sc);
+  for (int i = tid; i < kg * kGroup; i += kThreads) {
+    const int g = (int)sc.chosen[i / kGroup], e = i % kGroup;
+    sc.keys[i] = e < sh.size(g) ? order_key(to_f<T>(sh.row[sh.start(g) + e])) : 0u;
+  }
+  __syncthreads();
+  // positions in the list of chosen groups ascend with the position in the row
+  __shared__ uint32_t groups[kMaxTop];
+  for (int i = tid; i < kg; i += kThreads) groups[i] = sc.chosen[i];
+  __syncthreads();
+  select_exact(sc.keys, kg * kGroup, k, sc.chosen, sc);
+  uint64_t e = 0;
+  if (tid < k) {
+    const int at = (int)sc.chosen[tid], g = (int)groups[at / kGroup];
+    e = entry(sc.keys[at], sh.start(g) + at % kGroup);
+  }
+  __syncthreads();
+  uint64_t* all = sc.cand.elems;  // the keys have been read
+  if (tid < k) all[tid] = e;
+  __syncthreads();
+  if (tid < k) {
+    int rank = 0;
+    for (int o = 0; o < k; ++o) rank += all[o] > e;
+    top[rank] = e;
+  }
+  __syncthreads();
+}
+
+struct FwdArgs {
+  float* logprobs;      // nullable
+  float* entropy;       // nullable
+  float* lse;           // nullable
+  float2* stats;        // nullable: (mu, log S) for the backward
+  float* top_lp;        // nullable with top_idx
+  int64_t* top_idx;
+  const int64_t* targets;  // nullable
+  RowAddr addr;
+  int64_t ignore_index;
+  int V, k, cs;
+  Squash q;
+};
+
+constexpr int kBatch = 2;  // groups of a thread in flight
+
+template <typename T, bool CAP, bool ENT, bool TOP>
+__global__ void __launch_bounds__(kThreads)
+token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
+  using Stats = RowStats<CAP, ENT>;
+  extern __shared__ uint32_t gkeys[];  // TOP: group maxima
+  __shared__ Stats s_warp[kWarps];
+  __shared__ float s_share[4];         // this CTA's statistics, read by the others of the cluster
+  __shared__ uint64_t s_top[TOP ? kMaxTop : 1];
+  __shared__ __align__(8) unsigned char s_scratch[TOP ? sizeof(SelectScratch) : 8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cs = a.cs;
+  const int64_t r = cs > 1 ? blockIdx.x / cs : blockIdx.x;
+  const int rank = cs > 1 ? (int)row_cluster_rank() : 0;
+  const Squash q = a.q;
+  const T* row = logits + a.addr.off(r);
+  const RowCut cut = cut_row(row, a.V);
+  Share<T> sh;
+  sh.row = row;
+  sh.head = cut.head;
+  sh.tail = cut.tail;
+  sh.g0 = (int)((int64_t)cut.groups * rank / cs);
+  sh.n = (int)((int64_t)cut.groups * (rank + 1) / cs) - sh.g0;
+  sh.body_end = cut.head + cut.groups * kGroup;
+  sh.head_here = rank == 0 ? cut.head : 0;
+  sh.tail_here = rank == cs - 1 ? cut.tail : 0;
+
+  Stats st;
+  st.init(q);
+  uint32_t mine = 0;
+  const T* body = row + cut.head + (int64_t)sh.g0 * kGroup;
+  int g = tid;
+  for (; g + (kBatch - 1) * kThreads < sh.n; g += kBatch * kThreads) {
+    RawGroup<T> raw[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) raw[u] = load_group<T>(body + (int64_t)(g + u * kThreads) * kGroup);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      float x[kGroup];
+      unpack_group<T>(x, raw[u]);
+      float lm = x[0];
+#pragma unroll
+      for (int i = 1; i < kGroup; ++i) lm = fmaxf(lm, x[i]);
+      if constexpr (TOP) {
+        const uint32_t key = order_key(lm);
+        gkeys[1 + g + u * kThreads] = key;
+        mine = max(mine, key);
+      }
+      st.add(x, lm, q);
+    }
+  }
+  for (; g < sh.n; g += kThreads) {
+    float x[kGroup];
+    unpack_group<T>(x, load_group<T>(body + (int64_t)g * kGroup));
+    float lm = x[0];
+#pragma unroll
+    for (int i = 1; i < kGroup; ++i) lm = fmaxf(lm, x[i]);
+    if constexpr (TOP) {
+      const uint32_t key = order_key(lm);
+      gkeys[1 + g] = key;
+      mine = max(mine, key);
+    }
+    st.add(x, lm, q);
+  }
+  // head and tail: one element a lane of the first and the last warp
+  if (warp == 0 || warp == kWarps - 1) {
+    const bool first = warp == 0;
+    const int n = first ? sh.head_here : sh.tail_here;
+    uint32_t key = 0;
+    if (lane < n) {
+      const float x[1] = {to_f<T>(row[(first ? 0 : sh.body_end) + lane])};
+      st.add(x, q);
+      key = order_key(x[0]);
+    }
+    if constexpr (TOP) {
+      const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+      if (lane == 0) {
+        gkeys[first ? 0 : sh.n + 1] = best;
+        mine = max(mine, best);
+      }
+    }
+  }
+  st.warp_merge(q);
+  if (lane == 0) s_warp[warp] = st;
+  __syncthreads();
+  st = s_warp[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) st.merge(s_warp[w], q);
+  const int kl = TOP ? min(a.k, sh.elems()) : 0;
+  if constexpr (TOP)
+    if (kl > 0) select_top<T>(s_top, sh, gkeys, mine, kl, *reinterpret_cast<SelectScratch*>(s_scratch));
+  if (cs > 1) {
+    if (tid == 0) {
+      s_share[0] = st.m;
+      s_share[1] = st.s;
+      s_share[2] = ENT ? st.w : 0.f;
+      s_share[3] = __int_as_float(kl);
+    }
+    row_cluster_sync();
+    st.init(q);
+    for (int c = 0; c < cs; ++c) {  // the same order in every CTA
+      Stats o;
+      o.init(q);
+      const float m = __uint_as_float(ld_cluster_u32(&s_share[0], c));
+      if (m != -INFINITY) { o.m = m; o.mu = squash<CAP>(m, q); }
+      o.s = __uint_as_float(ld_cluster_u32(&s_share[1], c));
+      o.w = __uint_as_float(ld_cluster_u32(&s_share[2], c));
+      st.merge(o, q);
+    }
+  }
+  // S = 0: every logit is -inf and the row has no distribution: log-probabilities -inf, entropy 0
+  const float logs = logf(st.s);
+  if constexpr (TOP) {
+    for (int i = tid; i < kl; i += kThreads) {
+      const uint64_t e = s_top[i];
+      int pos = i;
+      for (int c = 0; c < cs; ++c) {
+        if (c == rank) continue;
+        // entries of the other list that are better: it is sorted
+        int lo = 0, hi = __float_as_int(__uint_as_float(ld_cluster_u32(&s_share[3], c)));
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (ld_cluster_u64(&s_top[mid], c) > e) lo = mid + 1;
+          else hi = mid;
+        }
+        pos += lo;
+      }
+      if (pos < a.k) {
+        const float x = key_value((uint32_t)(e >> 32));
+        a.top_idx[r * a.k + pos] = (int64_t)(uint32_t)~(uint32_t)e;
+        a.top_lp[r * a.k + pos] = st.s == 0.f ? -INFINITY : (squash<CAP>(x, q) - st.mu) * q.inv_t - logs;
+      }
+    }
+  }
+  if (rank == 0 && tid == 0) {
+    const int64_t t = a.targets ? a.targets[r] : 0;
+    const bool ignored = a.targets && t == a.ignore_index;
+    if (a.logprobs) {
+      float lp = 0.f;
+      if (!ignored) {
+        if (t < 0 || t >= a.V) lp = NAN;  // not a token
+        else if (st.s == 0.f) lp = -INFINITY;
+        else lp = (squash<CAP>(to_f<T>(row[t]), q) - st.mu) * q.inv_t - logs;
+      }
+      a.logprobs[r] = lp;
+    }
+    if constexpr (ENT)
+      a.entropy[r] = (ignored || st.s == 0.f) ? 0.f : logs - kLn2 * (st.w / st.s);
+    if (a.lse) a.lse[r] = st.mu * q.inv_t + logs;
+    if (a.stats) a.stats[r] = make_float2(st.mu, logs);
+  }
+  if (cs > 1) row_cluster_sync();  // the other CTAs have read this one's shared memory
+}
+
+struct BwdArgs {
+  const float2* stats;
+  const float* entropy;    // nullable with g_ent
+  const float* g_lp;       // nullable
+  const float* g_ent;      // nullable
+  const int64_t* targets;  // nullable
+  RowAddr addr;
+  int64_t ignore_index;
+  int V, segs;
+  Squash q;
+};
+
+constexpr int kBwdBatch = 2;
+constexpr int kBwdGroups = kThreads * kBwdBatch;  // groups of one CTA
+
+// Elementwise from the saved (mu, log S, H): each CTA takes one segment of a row.
+template <typename T, bool CAP, bool ENT>
+__global__ void __launch_bounds__(kThreads)
+token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const BwdArgs a) {
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x / a.segs;
+  const int seg = (int)(blockIdx.x - r * a.segs);
+  const Squash q = a.q;
+  const T* row = logits + a.addr.off(r);
+  T* grow = grad + r * a.V;
+  const RowCut cut = cut_row(row, a.V);
+  const bool vec = (reinterpret_cast<uintptr_t>(grow + cut.head) & 31u) == 0;
+  const int64_t t = a.targets ? a.targets[r] : -1;
+  const float2 ml = a.stats[r];
+  // rows without a gradient: ignored ones, and those whose every logit is -inf (S = 0)
+  const bool none = (a.targets && t == a.ignore_index) || ml.y == -INFINITY;
+  float gl = (a.targets && a.g_lp) ? a.g_lp[r] : 0.f;
+  if (a.targets && !none && (t < 0 || t >= a.V)) gl = NAN;
+  const float ge = ENT ? a.g_ent[r] : 0.f, H = ENT ? a.entropy[r] : 0.f;
+  // d = (y - mu) kl - log2 S; p = 2^d; dx = p (c0 + c1 d) (+ gl at the target), all times 1 / T
+  const float l2s = ml.y * kLog2e;
+  const float c0 = -(gl + ge * H) * q.inv_t, c1 = -ge * kLn2 * q.inv_t, ct = gl * q.inv_t;
+
+  auto one = [&](float x, int i) {
+    const float y = squash<CAP>(x, q);
+    const float d = (y - ml.x) * q.kl - l2s;
+    float o = ex2(d);
+    o *= ENT ? fmaf(c1, fmaxf(d, -1e4f), c0) : c0;
+    if (i == (int)t) o += ct;
+    return o * squash_slope<CAP>(y, q);
+  };
+
+  const int gbeg = seg * kBwdGroups;
+  const T* body = row + cut.head;
+  T* gbody = grow + cut.head;
+  RawGroup<T> raw[kBwdBatch];
+#pragma unroll
+  for (int u = 0; u < kBwdBatch; ++u) {
+    const int g = gbeg + u * kThreads + tid;
+    if (g < cut.groups) raw[u] = load_group<T>(body + (int64_t)g * kGroup);
+  }
+#pragma unroll
+  for (int u = 0; u < kBwdBatch; ++u) {
+    const int g = gbeg + u * kThreads + tid;
+    if (g < cut.groups) {
+      float x[kGroup];
+      unpack_group<T>(x, raw[u]);
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) x[i] = none ? 0.f : one(x[i], cut.head + g * kGroup + i);
+      store_group<T>(gbody + (int64_t)g * kGroup, x, vec);
+    }
+  }
+  if (seg == 0 && tid < cut.head) grow[tid] = from_f<T>(none ? 0.f : one(to_f<T>(row[tid]), tid));
+  const int tail0 = cut.head + cut.groups * kGroup;
+  if (seg == a.segs - 1 && tid < cut.tail)
+    grow[tail0 + tid] = from_f<T>(none ? 0.f : one(to_f<T>(row[tail0 + tid]), tail0 + tid));
+}
+
+// CTAs per row: one where the rows fill the GPU, else as many (2, 4, 8) as give every SM a CTA and
+// each CTA at least half a group per thread; more where one CTA's group maxima would not fit.
+int cluster_for(int64_t rows, int64_t V, bool top) {
+  int cs = 1;
+  while (cs < kMaxCluster && rows * cs * 2 <= sm_count() * 2 && V / (2 * cs) >= kThreads * kGroup / 2) cs *= 2;
+  if (top)
+    while (cs < kMaxCluster && (V / kGroup) / cs + 2 > kMaxGroupKeys - 2) cs *= 2;
+  return cs;
+}
+
+int check_rows(const char* what, const void* logits, int64_t rows, int64_t inner, int64_t V, float temperature,
+               float softcap, int dt) {
+  AK_REQUIRE(valid_dtype(dt), AK_ERR_DTYPE, "%s: unsupported dtype %d", what, dt);
+  AK_REQUIRE(rows >= 0 && inner > 0 && V > 0 && V < (1LL << 30) && rows < (1LL << 27), AK_ERR_SHAPE,
+             "%s: bad shape: %lld rows of %lld", what, (long long)rows, (long long)V);
+  AK_REQUIRE(temperature > 0.f && temperature < INFINITY, AK_ERR_ARG, "%s: temperature must be positive and finite",
+             what);
+  AK_REQUIRE(softcap >= 0.f && softcap < INFINITY, AK_ERR_ARG, "%s: softcap must be >= 0 and finite", what);
+  AK_REQUIRE(rows == 0 || logits, AK_ERR_ARG, "%s: null pointer", what);
+  AK_REQUIRE((reinterpret_cast<uintptr_t>(logits) % elem_size(dt)) == 0, AK_ERR_ARG,
+             "%s: logits not aligned to their type", what);
+  return AK_OK;
+}
+
+template <typename T>
+int launch_fwd(const T* logits, const FwdArgs& a, int64_t rows, cudaStream_t st) {
+  const bool cap = a.q.cap > 0.f, ent = a.entropy != nullptr, top = a.k > 0;
+  void (*kern)(const T*, FwdArgs) = nullptr;
+#define AK_PICK(C, E, P) \
+  if (cap == C && ent == E && top == P) kern = token_logprobs_fwd_kernel<T, C, E, P>;
+  AK_PICK(false, false, false) AK_PICK(false, false, true) AK_PICK(false, true, false) AK_PICK(false, true, true)
+  AK_PICK(true, false, false) AK_PICK(true, false, true) AK_PICK(true, true, false) AK_PICK(true, true, true)
+#undef AK_PICK
+  const size_t smem = top ? ((size_t)(a.V / kGroup) / a.cs + 4) * 4 : 0;
+  AK_CUDA_TRY(launch_rows(kern, rows * a.cs, kThreads, a.cs, smem, st, logits, a), "ak_token_logprobs_fwd");
+  return AK_OK;
+}
+
+}  // namespace
+}  // namespace ak
+
+using namespace ak;
+
+extern "C" int ak_token_logprobs_fwd(float* logprobs, float* entropy, float* lse, float* row_stats, float* top_lp,
+                                     int64_t* top_idx, const void* logits, const int64_t* targets, int64_t rows,
+                                     int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t V, int64_t k,
+                                     float temperature, float softcap, int64_t ignore_index, int dt, void* stream) {
+  clear_error();
+  int rc = check_rows("ak_token_logprobs_fwd", logits, rows, inner, V, temperature, softcap, dt);
+  if (rc) return rc;
+  AK_REQUIRE(k >= 0 && k <= kMaxTop && k <= V, AK_ERR_SHAPE,
+             "ak_token_logprobs_fwd: top_k %lld must be at most %d and at most the vocabulary", (long long)k, kMaxTop);
+  AK_REQUIRE(k == 0 || V <= (int64_t)kMaxCluster * kGroup * (kMaxGroupKeys - 4), AK_ERR_SHAPE,
+             "ak_token_logprobs_fwd: vocabulary of %lld too large for top_k", (long long)V);
+  if (rows == 0) return AK_OK;
+  AK_REQUIRE((k == 0) || (top_lp && top_idx), AK_ERR_ARG, "ak_token_logprobs_fwd: null top_lp or top_idx");
+  AK_REQUIRE(!logprobs || targets, AK_ERR_ARG, "ak_token_logprobs_fwd: logprobs need targets");
+  FwdArgs a{};
+  a.logprobs = logprobs; a.entropy = entropy; a.lse = lse;
+  a.stats = reinterpret_cast<float2*>(row_stats);
+  a.top_lp = top_lp; a.top_idx = top_idx; a.targets = targets;
+  a.addr = RowAddr{inner, stride_outer, stride_inner};
+  a.ignore_index = ignore_index;
+  a.V = (int)V; a.k = (int)k; a.cs = cluster_for(rows, V, k > 0);
+  a.q = make_squash(temperature, softcap);
+  AK_DISPATCH_DTYPE(dt, T, return launch_fwd<T>((const T*)logits, a, rows, (cudaStream_t)stream));
+  return AK_OK;
+}
+
+extern "C" int ak_token_logprobs_bwd(void* grad, const void* logits, const int64_t* targets, const float* row_stats,
+                                     const float* entropy, const float* g_logprobs, const float* g_entropy,
+                                     int64_t rows, int64_t inner, int64_t stride_outer, int64_t stride_inner,
+                                     int64_t V, float temperature, float softcap, int64_t ignore_index, int dt,
+                                     void* stream) {
+  clear_error();
+  int rc = check_rows("ak_token_logprobs_bwd", logits, rows, inner, V, temperature, softcap, dt);
+  if (rc) return rc;
+  if (rows == 0) return AK_OK;
+  AK_REQUIRE(grad && row_stats, AK_ERR_ARG, "ak_token_logprobs_bwd: null pointer");
+  AK_REQUIRE(!g_logprobs || targets, AK_ERR_ARG, "ak_token_logprobs_bwd: a gradient of logprobs needs targets");
+  AK_REQUIRE(!g_entropy || entropy, AK_ERR_ARG, "ak_token_logprobs_bwd: a gradient of the entropy needs the entropy");
+  AK_REQUIRE((reinterpret_cast<uintptr_t>(grad) % elem_size(dt)) == 0, AK_ERR_ARG,
+             "ak_token_logprobs_bwd: grad not aligned to its type");
+  BwdArgs a{};
+  a.stats = reinterpret_cast<const float2*>(row_stats);
+  a.entropy = entropy; a.g_lp = g_logprobs; a.g_ent = g_entropy; a.targets = targets;
+  a.addr = RowAddr{inner, stride_outer, stride_inner};
+  a.ignore_index = ignore_index;
+  a.V = (int)V;
+  a.segs = (int)std::max<int64_t>(1, (V / kGroup + kBwdGroups - 1) / kBwdGroups);
+  a.q = make_squash(temperature, softcap);
+  AK_REQUIRE(rows * a.segs < (1LL << 31), AK_ERR_SHAPE, "ak_token_logprobs_bwd: too many rows");
+  const bool cap = a.q.cap > 0.f, ent = g_entropy != nullptr;
+  AK_DISPATCH_DTYPE(dt, T, {
+    auto kern = cap ? (ent ? token_logprobs_bwd_kernel<T, true, true> : token_logprobs_bwd_kernel<T, true, false>)
+                    : (ent ? token_logprobs_bwd_kernel<T, false, true> : token_logprobs_bwd_kernel<T, false, false>);
+    kern<<<(unsigned)(rows * a.segs), kThreads, 0, (cudaStream_t)stream>>>((T*)grad, (const T*)logits, a);
+  });
+  AK_CHECK_LAUNCH("ak_token_logprobs_bwd");
+  return AK_OK;
+}

@@ -47,6 +47,8 @@ SIGNATURES = {
     "ak_ce_rows_bwd": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _i64, _f, _f, _vp, _f, _i, _vp],
     "ak_ce_rows_reduce": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _vp],
     "ak_ce_inv_valid": [_vp, _vp, _i64, _i64, _vp],
+    "ak_token_logprobs_fwd": [_vp] * 8 + [_i64] * 6 + [_f, _f, _i64, _i, _vp],
+    "ak_token_logprobs_bwd": [_vp] * 7 + [_i64] * 5 + [_f, _f, _i64, _i, _vp],
     "ak_linear_ce_logits_grad_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
     "ak_linear_ce_logits_grad": [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp],
     "ak_linear_ce_workspace_size": [_i64, _i64, _i64, ctypes.POINTER(_sz)],
@@ -577,6 +579,80 @@ def ce_inv_valid(targets: torch.Tensor, ignore_index: int = -100) -> torch.Tenso
     inv = torch.empty((), dtype=torch.float32, device=dev)
     call("ak_ce_inv_valid", ptr(inv), ptr(targets), targets.numel(), int(ignore_index), stream(dev))
     return inv
+
+
+# ---------------------------------------------------------------------------
+# Token log-probabilities over logit rows
+# ---------------------------------------------------------------------------
+def call_on(device: torch.device, name: str, *args) -> None:
+    """`call` with `device` current, which a launch on one of its streams needs."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
+def logit_rows(logits: torch.Tensor):
+    """(tensor, rows, inner, stride_outer, stride_inner): the rows of logits (..., V) as the library
+    addresses them.  A view whose leading dimensions are at most two runs of evenly spaced rows
+    (logits[:, :-1], a slice of a padded vocabulary) is taken as it lies, others are copied."""
+    V = logits.shape[-1]
+    if logits.is_contiguous():
+        rows = logits.numel() // V
+        return logits, rows, max(rows, 1), 0, V
+    if V > 1 and logits.stride(-1) != 1:
+        return logit_rows(logits.contiguous())
+    runs = []  # [size, stride], outermost first, merged where evenly spaced
+    for size, stride in zip(logits.shape[:-1], logits.stride()[:-1]):
+        if size == 1:
+            continue
+        if runs and runs[-1][1] == stride * size:
+            runs[-1] = [runs[-1][0] * size, stride]
+        else:
+            runs.append([size, stride])
+    if len(runs) > 2:
+        return logit_rows(logits.contiguous())
+    runs = [[1, 0]] * (2 - len(runs)) + runs
+    (n0, s0), (n1, s1) = runs
+    return logits, n0 * n1, max(n1, 1), s0, s1
+
+
+def token_logprobs_fwd(logits: torch.Tensor, targets: Optional[torch.Tensor], top_k: int = 0,
+                       temperature: float = 1.0, softcap: float = 0.0, ignore_index: int = -100,
+                       want_entropy: bool = False, want_stats: bool = False):
+    """Returns [logprobs, entropy, lse, top_logprobs, top_indices, row_stats], shaped like the leading
+    dimensions of logits (absent ones are None); targets int64, contiguous or None."""
+    dev = require_cuda(logits, targets)
+    x, rows, inner, so, si = logit_rows(logits)
+    lead = logits.shape[:-1]
+    f32 = dict(dtype=torch.float32, device=dev)
+    lp = torch.empty(lead, **f32) if targets is not None else None
+    ent = torch.empty(lead, **f32) if want_entropy else None
+    lse = torch.empty(lead, **f32)
+    stats = torch.empty(rows, 2, **f32) if want_stats else None
+    top_lp = torch.empty(*lead, top_k, **f32) if top_k else None
+    top_idx = torch.empty(*lead, top_k, dtype=torch.int64, device=dev) if top_k else None
+    call_on(dev, "ak_token_logprobs_fwd", ptr(lp), ptr(ent), ptr(lse), ptr(stats), ptr(top_lp), ptr(top_idx), ptr(x),
+            ptr(targets), rows, inner, so, si, logits.shape[-1], top_k, temperature, softcap, ignore_index,
+            dtype_code(logits), stream(dev))
+    return [lp, ent, lse, top_lp, top_idx, stats]
+
+
+def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], row_stats: torch.Tensor,
+                       entropy: Optional[torch.Tensor], g_logprobs: Optional[torch.Tensor],
+                       g_entropy: Optional[torch.Tensor], temperature: float = 1.0, softcap: float = 0.0,
+                       ignore_index: int = -100) -> torch.Tensor:
+    """Gradient of the logits (dense, their dtype) from those of logprobs and entropy (either may be None)."""
+    dev = require_cuda(logits, targets, row_stats, entropy, g_logprobs, g_entropy)
+    x, rows, inner, so, si = logit_rows(logits)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    glp = g_logprobs.to(torch.float32).contiguous() if g_logprobs is not None else None
+    gent = g_entropy.to(torch.float32).contiguous() if g_entropy is not None else None
+    call_on(dev, "ak_token_logprobs_bwd", ptr(grad), ptr(x), ptr(targets), ptr(row_stats), ptr(entropy), ptr(glp),
+            ptr(gent), rows, inner, so, si, logits.shape[-1], temperature, softcap, ignore_index,
+            dtype_code(logits), stream(dev))
+    return grad
 
 
 def linear_ce_supported(hidden: torch.Tensor, weight: torch.Tensor) -> bool:

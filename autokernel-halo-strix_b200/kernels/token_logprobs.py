@@ -1,0 +1,113 @@
+"""Log-probabilities of given tokens on B200, with entropies and top alternatives.
+
+`token_logprobs` reads logit rows once and answers, per row: how likely the target token was,
+how uncertain the distribution is, and which tokens were most likely.  It serves scoring and
+decoding (no gradient is kept then), a teacher's pass over a batch for `kernels.distill`, and
+policy-gradient losses: `logprobs` and `entropy` are differentiable.  The cross-entropy in
+`kernels.ce_fused` is the loss over the same rows.
+
+The reference has only the loss (kernels/ce_fused.py:557-785).
+"""
+import math
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from kernels import _ak
+
+KERNEL_TYPE = "token_logprobs"
+BACKEND = "cuda_sm100a"
+
+MAX_TOP_K = 128
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row of the input; fp32, indices int64.  Fields that were not asked for are None."""
+    logprobs: Optional[torch.Tensor]
+    entropy: Optional[torch.Tensor]
+    lse: torch.Tensor
+    top_logprobs: Optional[torch.Tensor] = None
+    top_indices: Optional[torch.Tensor] = None
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    """Saves the logits and two numbers a row; the backward recomputes the softmax from them."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, top_k, temperature, softcap, ignore_index, entropy):
+        lp, ent, lse, top_lp, top_idx, stats = _ak.token_logprobs_fwd(
+            logits, targets, top_k, temperature, softcap, ignore_index, want_entropy=entropy, want_stats=True)
+        ctx.save_for_backward(logits, targets, stats, ent)
+        ctx.args = (temperature, softcap, ignore_index)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (lse, top_lp, top_idx) if t is not None))
+        return lp, ent, lse, top_lp, top_idx
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, *rest):
+        if g_lp is None and g_ent is None:
+            return (None,) * 7
+        logits, targets, stats, ent = ctx.saved_tensors
+        grad = _ak.token_logprobs_bwd(logits, targets, stats, ent, g_lp, g_ent, *ctx.args)
+        return (grad,) + (None,) * 6
+
+
+def check_scales(what: str, temperature: float, softcap: float):
+    temperature, softcap = float(temperature), float(softcap)
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
+    if not (softcap >= 0.0 and math.isfinite(softcap)):
+        raise ValueError(f"{what}: softcap must be >= 0 (0: none) and finite, got {softcap}")
+    return temperature, softcap
+
+
+def check_targets(what: str, targets: torch.Tensor, lead) -> torch.Tensor:
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: targets must be int64 or int32, got {targets.dtype}")
+    if targets.shape != lead:
+        raise ValueError(f"{what}: targets {tuple(targets.shape)} do not match the rows {tuple(lead)}")
+    return targets.to(torch.int64).contiguous()
+
+
+def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, *, top_k: int = 0,
+                   temperature: float = 1.0, softcap: float = 0.0, ignore_index: int = -100,
+                   entropy: bool = False) -> TokenLogprobs:
+    """Log-probabilities under softmax(softcap(logits) / temperature) over the last dimension.
+
+    logits (..., V): fp32, bf16 or fp16 on the GPU.  Row views (logits[:, :-1], logits[..., :V]) are
+    read in place; an input whose last dimension is strided, or with more than two uneven leading
+    dimensions, is copied.
+    targets (...): the tokens whose `logprobs` are wanted, or None.  Where a target is `ignore_index`
+    its log-probability and entropy are 0 and its row gets no gradient, whatever the row holds; a
+    target outside the vocabulary gives NaN.
+    top_k: alternatives per row, at most 128: `top_logprobs` and `top_indices` (..., top_k), most
+    likely first, equal logits by lowest index.  They and `lse` carry no gradient.
+    entropy: whether to compute the entropy (nats).
+
+    -inf logits are tokens without probability.  A row of nothing else has log-probabilities -inf,
+    entropy 0 and no gradient; a row with NaN is NaN.
+    """
+    what = "token_logprobs"
+    _ak.require_cuda(logits, targets)
+    _ak.dtype_code(logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits must be (..., V) with V >= 1, got {tuple(logits.shape)}")
+    if targets is not None:
+        targets = check_targets(what, targets, logits.shape[:-1])
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
+        raise ValueError(f"{what}: top_k must be in 0..{min(MAX_TOP_K, logits.shape[-1])}, got {top_k}")
+    temperature, softcap = check_scales(what, temperature, softcap)
+    ignore_index = int(ignore_index)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k, temperature, softcap, ignore_index,
+                                                   bool(entropy)))
+    return TokenLogprobs(*_ak.token_logprobs_fwd(logits, targets, top_k, temperature, softcap, ignore_index,
+                                                 want_entropy=bool(entropy))[:5])
+
+
+def kernel_fn(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    """Log-probability of each row's target (0 where it is -100)."""
+    return token_logprobs(logits, targets).logprobs

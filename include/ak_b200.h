@@ -176,6 +176,44 @@ AK_API int ak_scale_by_device_scalar(void* x, int64_t n, const float* scale, int
                                      void* stream);
 
 /* ------------------------------------------------------------------------ *
+ * Token log-probabilities from logit rows
+ * ------------------------------------------------------------------------ */
+
+/* For each row x of logits: y = softcap(x) / temperature (softcap(x) = c tanh(x / c),
+ * c = softcap; 0 leaves x), lse = log sum exp y, p = exp(y - lse):
+ *   logprobs[rows]  y_target - lse; 0 where target == ignore_index, NaN where it is no token
+ *   entropy[rows]   -sum p log p; 0 where target == ignore_index
+ *   lse[rows]
+ *   row_stats[rows][2]  what ak_token_logprobs_bwd needs
+ *   top_lp / top_idx[rows][k]  log-probability and index of the k largest logits, largest first,
+ *                   equal ones by lowest index; 0 <= k <= min(128, V), V <= 1048320 for k > 0
+ * Each output is fp32 (top_idx int64) and nullable; logprobs needs targets (int64, nullable).
+ * Row r of logits (dt) starts at logits + (r / inner) * stride_outer + (r % inner) * stride_inner
+ * elements, aligned to the element only; a row's V elements are adjacent.
+ * -inf logits have no probability; a row of nothing else has lse and log-probabilities -inf and
+ * entropy 0.  A row with NaN (or +inf, without softcap) has NaN results; among its alternatives'
+ * indices NaN ranks below every number.  Reads the logits once.
+ * No counterpart in the reference, which has the loss only (kernels/ce_fused.py:122-382). */
+AK_API int ak_token_logprobs_fwd(float* logprobs, float* entropy, float* lse, float* row_stats,
+                                 float* top_lp, int64_t* top_idx, const void* logits,
+                                 const int64_t* targets, int64_t rows, int64_t inner,
+                                 int64_t stride_outer, int64_t stride_inner, int64_t V,
+                                 int64_t k, float temperature, float softcap,
+                                 int64_t ignore_index, int dt, void* stream);
+
+/* Gradient of the logits, grad[rows][V] (dt, dense), given those of logprobs (g_logprobs) and
+ * entropy (g_entropy), fp32 [rows], each nullable:
+ *   dx_i = [ g_lp (1[i = t] - p_i) - g_H p_i (log p_i + H) ] dy_i/dx_i.
+ * row_stats and entropy are the forward's, with the same arguments.  Ignored rows and rows of
+ * -inf get zeros.  Reads the logits once and writes the gradient once. */
+AK_API int ak_token_logprobs_bwd(void* grad, const void* logits, const int64_t* targets,
+                                 const float* row_stats, const float* entropy,
+                                 const float* g_logprobs, const float* g_entropy, int64_t rows,
+                                 int64_t inner, int64_t stride_outer, int64_t stride_inner,
+                                 int64_t V, float temperature, float softcap,
+                                 int64_t ignore_index, int dt, void* stream);
+
+/* ------------------------------------------------------------------------ *
  * Fused linear + cross-entropy on the tensor cores (tcgen05 / TMEM / TMA)
  * ------------------------------------------------------------------------ */
 
