@@ -19,6 +19,7 @@ struct RowAddr {
 
 // What a logit x means: y = softcap(x), log-probabilities of y / temperature.
 // kl = log2(e) / temperature turns a difference of y into an exponent of 2.
+// -inf stays -inf under softcap: a masked token has no probability there either.
 struct Squash {
   float cap, inv_cap, inv_t, kl;
 };
@@ -34,7 +35,9 @@ inline Squash make_squash(float temperature, float softcap) {
 
 template <bool CAP>
 __device__ __forceinline__ float squash(float x, const Squash& q) {
-  return CAP ? q.cap * tanhf(x * q.inv_cap) : x;
+  if constexpr (!CAP) return x;
+  const float y = q.cap * tanhf(x * q.inv_cap);
+  return x == -INFINITY ? x : y;
 }
 
 // Derivative of squash at its output y.
@@ -42,7 +45,7 @@ template <bool CAP>
 __device__ __forceinline__ float squash_slope(float y, const Squash& q) {
   if constexpr (!CAP) return 1.f;
   const float t = y * q.inv_cap;
-  return 1.f - t * t;
+  return y == -INFINITY ? 0.f : 1.f - t * t;
 }
 
 // A row is cut into a head (elements before the first 32-byte boundary), groups of 16
@@ -150,7 +153,7 @@ __device__ __forceinline__ void store_group(T* p, const float (&x)[kGroup], bool
 // Running softmax statistics of a set of logits
 // ---------------------------------------------------------------------------
 //   m   largest x (before squash; -inf for an empty set, NaN is passed over)
-//   mu  what exponents are taken against: squash(m), or 0 where m is -inf and uncapped
+//   mu  what exponents are taken against: squash(m), or 0 where m is -inf
 //   s   sum of e = 2^(kl (y - mu))
 //   w   sum of e * kl (y - mu)    (entropy only)
 // y - mu is formed before the scaling: the product with kl of a number near the type's lowest
@@ -160,9 +163,9 @@ template <bool CAP, bool ENT>
 struct RowStats {
   float m, mu, s, w;
 
-  __device__ __forceinline__ void init(const Squash& q) {
+  __device__ __forceinline__ void init() {
     m = -INFINITY;
-    mu = CAP ? -q.cap : 0.f;
+    mu = 0.f;
     s = 0.f;
     w = 0.f;
   }
@@ -170,7 +173,7 @@ struct RowStats {
   // Moves the statistics to the larger maximum mn.
   __device__ __forceinline__ void rebase(float mn, const Squash& q) {
     const float nu = CAP ? squash<CAP>(mn, q) : mn;
-    if (CAP || m != -INFINITY) {  // s is 0 or NaN for an uncapped m = -inf
+    if (m != -INFINITY) {  // there s is 0 or NaN
       const float d = fmaxf((mu - nu) * q.kl, -1e30f);
       const float f = ex2(d);
       if constexpr (ENT) w = f * fmaf(d, s, w);

@@ -259,7 +259,7 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
   sh.tail_here = rank == cs - 1 ? cut.tail : 0;
 
   Stats st;
-  st.init(q);
+  st.init();
   uint32_t mine = 0;
   const T* body = row + cut.head + (int64_t)sh.g0 * kGroup;
   int g = tid;
@@ -330,10 +330,10 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
       s_share[3] = __int_as_float(kl);
     }
     row_cluster_sync();
-    st.init(q);
+    st.init();
     for (int c = 0; c < cs; ++c) {  // the same order in every CTA
       Stats o;
-      o.init(q);
+      o.init();
       const float m = __uint_as_float(ld_cluster_u32(&s_share[0], c));
       if (m != -INFINITY) { o.m = m; o.mu = squash<CAP>(m, q); }
       o.s = __uint_as_float(ld_cluster_u32(&s_share[1], c));

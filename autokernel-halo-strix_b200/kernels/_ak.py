@@ -49,6 +49,8 @@ SIGNATURES = {
     "ak_ce_inv_valid": [_vp, _vp, _i64, _i64, _vp],
     "ak_token_logprobs_fwd": [_vp] * 8 + [_i64] * 6 + [_f, _f, _i64, _i, _vp],
     "ak_token_logprobs_bwd": [_vp] * 7 + [_i64] * 5 + [_f, _f, _i64, _i, _vp],
+    "ak_distill_topk_fwd": [_vp] * 10 + [_i64] * 6 + [_f, _f, _i, _i, _vp, _vp],
+    "ak_distill_topk_bwd": [_vp] * 8 + [_i64] * 6 + [_f, _f, _i, _vp],
     "ak_linear_ce_logits_grad_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
     "ak_linear_ce_logits_grad": [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp],
     "ak_linear_ce_workspace_size": [_i64, _i64, _i64, ctypes.POINTER(_sz)],
@@ -156,7 +158,7 @@ def _size_query(name: str, *dims: int) -> int:
 # Device status words (bounded-wait timeouts)
 # ---------------------------------------------------------------------------
 AK_ERR_TIMEOUT = 5
-STATUS_SLOTS = ("selective_scan_fwd", "selective_scan_bwd", "linear_ce", "bounded_wait_test")
+STATUS_SLOTS = ("selective_scan_fwd", "selective_scan_bwd", "linear_ce", "bounded_wait_test", "distill_topk")
 
 
 class _StatusWords:
@@ -651,6 +653,43 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], ro
     gent = g_entropy.to(torch.float32).contiguous() if g_entropy is not None else None
     call_on(dev, "ak_token_logprobs_bwd", ptr(grad), ptr(x), ptr(targets), ptr(row_stats), ptr(entropy), ptr(glp),
             ptr(gent), rows, inner, so, si, logits.shape[-1], temperature, softcap, ignore_index,
+            dtype_code(logits), stream(dev))
+    return grad
+
+
+# ---------------------------------------------------------------------------
+# Distillation from a teacher's top-K log-probabilities
+# ---------------------------------------------------------------------------
+def distill_topk_fwd(logits: torch.Tensor, teacher_idx: torch.Tensor, teacher_lp: torch.Tensor,
+                     mask: Optional[torch.Tensor] = None, temperature: float = 1.0, softcap: float = 0.0,
+                     tail: bool = False, want_grad: bool = False, want_stats: bool = False):
+    """Returns [loss, losses, inv_n, grad, rest_stats, gk] (absent ones are None); teacher_idx int64 and
+    teacher_lp fp32 (..., K), mask bool, all contiguous."""
+    dev = require_cuda(logits, teacher_idx, teacher_lp, mask)
+    x, rows, inner, so, si = logit_rows(logits)
+    K = teacher_idx.shape[-1]
+    f32 = dict(dtype=torch.float32, device=dev)
+    loss = torch.empty((), **f32)
+    losses = torch.empty(logits.shape[:-1], **f32)
+    inv_n = torch.empty((), **f32) if mask is not None else None
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
+    rest = torch.empty(rows, 2, **f32) if want_stats else None
+    gk = torch.empty(rows, K, **f32) if want_stats else None
+    call_on(dev, "ak_distill_topk_fwd", ptr(loss), ptr(losses), ptr(inv_n), ptr(grad), ptr(rest), ptr(gk), ptr(x),
+            ptr(teacher_idx), ptr(teacher_lp), ptr(mask), rows, inner, so, si, logits.shape[-1], K, temperature,
+            softcap, int(tail), dtype_code(logits), status_ptr(dev, "distill_topk"), stream(dev))
+    return [loss, losses, inv_n, grad, rest, gk]
+
+
+def distill_topk_bwd(logits: torch.Tensor, teacher_idx: torch.Tensor, rest_stats: torch.Tensor, gk: torch.Tensor,
+                     mask: Optional[torch.Tensor], inv_n: Optional[torch.Tensor], g_loss: torch.Tensor,
+                     temperature: float = 1.0, softcap: float = 0.0) -> torch.Tensor:
+    dev = require_cuda(logits, teacher_idx, rest_stats, gk, mask, inv_n, g_loss)
+    x, rows, inner, so, si = logit_rows(logits)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    g = g_loss.reshape(1).to(torch.float32)
+    call_on(dev, "ak_distill_topk_bwd", ptr(grad), ptr(x), ptr(teacher_idx), ptr(rest_stats), ptr(gk), ptr(mask),
+            ptr(inv_n), ptr(g), rows, inner, so, si, logits.shape[-1], teacher_idx.shape[-1], temperature, softcap,
             dtype_code(logits), stream(dev))
     return grad
 

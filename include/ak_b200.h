@@ -15,7 +15,7 @@
  *   - Functions keep no mutable global state beyond a per-device attribute
  *     cache, so they are reentrant and thread-safe.
  *   - Kernels that wait on asynchronous copies or on each other (the mamba
- *     scan and the tensor-core linear + CE) bound every wait.  When a wait runs
+ *     scan, the distillation and the tensor-core linear + CE) bound every wait.  When a wait runs
  *     out they write AK_ERR_TIMEOUT to the caller's `status` word (nullable; a
  *     device int, or a pinned host int whose device address comes from
  *     ak_status_device_pointer), stop issuing work, wait (again bounded) for
@@ -180,7 +180,7 @@ AK_API int ak_scale_by_device_scalar(void* x, int64_t n, const float* scale, int
  * ------------------------------------------------------------------------ */
 
 /* For each row x of logits: y = softcap(x) / temperature (softcap(x) = c tanh(x / c),
- * c = softcap; 0 leaves x), lse = log sum exp y, p = exp(y - lse):
+ * c = softcap; 0 leaves x; -inf stays -inf), lse = log sum exp y, p = exp(y - lse):
  *   logprobs[rows]  y_target - lse; 0 where target == ignore_index, NaN where it is no token
  *   entropy[rows]   -sum p log p; 0 where target == ignore_index
  *   lse[rows]
@@ -212,6 +212,44 @@ AK_API int ak_token_logprobs_bwd(void* grad, const void* logits, const int64_t* 
                                  int64_t inner, int64_t stride_outer, int64_t stride_inner,
                                  int64_t V, float temperature, float softcap,
                                  int64_t ignore_index, int dt, void* stream);
+
+/* ------------------------------------------------------------------------ *
+ * Distillation from a teacher's top-K log-probabilities
+ * ------------------------------------------------------------------------ */
+
+/* loss[0] = temperature^2 * mean over the rows with mask (uint8, nullable: all) of the divergence of
+ * the student p = softmax(softcap(x) / temperature) from the teacher's K entries (teacher_idx int64,
+ * teacher_lp fp32, both [rows][K], 1 <= K <= 128; log-probabilities at that temperature):
+ *   tail = 0: q = softmax of the entries;   sum_k q_k (log q_k - log p_{i_k})
+ *   tail = 1: q_k = exp(lp_k), r = max(0, 1 - sum q);  the same sum + r (log r - log p_r), p_r the
+ *             student's probability outside the K tokens (left out where it has no logit there
+ *             within 30000 of its largest: -inf or lowest-value masks)
+ * A negative index is padding; a row of nothing else has loss 0 and no gradient (it counts in the
+ * mean).  An index >= V makes its row's loss and gradient NaN.  Entries of one token add up.
+ * losses[rows] fp32: the rows' divergences (0 without mask).  inv_n (needed with a mask): receives
+ * 1 / max(1, rows with mask).
+ * grad (nullable): d loss / d logits, dense [rows][V] dt.  Without it, rest_stats [rows][2] and
+ * gk [rows][K] (both nullable, fp32) receive what ak_distill_topk_bwd needs.
+ * Rows of logits as in ak_token_logprobs_fwd; a row has to fit the shared memory of 8 CTAs
+ * (about 880,000 16-bit or 440,000 fp32 elements).  Reads the logits once.
+ * No counterpart in the reference, which trains on hard labels only (kernels/ce_fused.py:122-382). */
+AK_API int ak_distill_topk_fwd(float* loss, float* losses, float* inv_n, void* grad,
+                               float* rest_stats, float* gk, const void* logits,
+                               const int64_t* teacher_idx, const float* teacher_lp,
+                               const uint8_t* mask, int64_t rows, int64_t inner,
+                               int64_t stride_outer, int64_t stride_inner, int64_t V, int64_t K,
+                               float temperature, float softcap, int tail, int dt, int* status,
+                               void* stream);
+
+/* grad[rows][V] (dt, dense) = *g_loss (device fp32) * d loss / d logits from the forward's
+ * rest_stats, gk and inv_n, with the same arguments: one rounding, whatever g_loss is (an fp16
+ * gradient of a scaled loss does not underflow on the way). */
+AK_API int ak_distill_topk_bwd(void* grad, const void* logits, const int64_t* teacher_idx,
+                               const float* rest_stats, const float* gk, const uint8_t* mask,
+                               const float* inv_n, const float* g_loss, int64_t rows,
+                               int64_t inner, int64_t stride_outer, int64_t stride_inner,
+                               int64_t V, int64_t K, float temperature, float softcap, int dt,
+                               void* stream);
 
 /* ------------------------------------------------------------------------ *
  * Fused linear + cross-entropy on the tensor cores (tcgen05 / TMEM / TMA)

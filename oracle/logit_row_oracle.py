@@ -17,11 +17,11 @@ LN2 = 0.6931471805599453
 
 
 def squash(x, temperature=1.0, softcap=0.0):
-    """(softcap(x) / temperature, its derivative)."""
+    """(softcap(x) / temperature, its derivative); -inf stays -inf."""
     d = torch.ones_like(x)
     if softcap > 0:
-        t = torch.tanh(x / softcap)
-        x, d = softcap * t, 1 - t * t
+        t, gone = torch.tanh(x / softcap), torch.isneginf(x)
+        x, d = torch.where(gone, x, softcap * t), torch.where(gone, torch.zeros_like(t), 1 - t * t)
     return x / temperature, d / temperature
 
 
@@ -123,3 +123,80 @@ def assert_within(actual, expected, tol, what=""):
         i = tuple(bad.nonzero()[0].tolist())
         raise AssertionError(f"{what}: {int(bad.sum())} values out of tolerance, first at {i}: {a[i].item():.9g} vs "
                              f"{b[i].item():.9g}, tolerance {(tol + half)[i].item():.3g}")
+
+
+def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=False, g_loss=1.0):
+    """dict of loss, losses, grad of double rows (N, V) and the fp32 bounds tol_loss, tol_losses, tol_grad.
+
+    Student log-probabilities are off as in token_logprobs.  q: an exponential off by 4 u, its
+    argument t - max by u each, K additions and a division; 1 - sum q by (K + 6) u; losses are sums of
+    K terms, and the mean one of N / 1024 + 64."""
+    n, v = x.shape
+    k = idx.shape[1]
+    live = torch.ones(n, dtype=torch.bool, device=x.device) if mask is None else mask
+    r = token_logprobs(x, None, temperature=temperature, softcap=softcap)
+    p, logp, empty = r["p"], r["logp"], r["empty"]
+    used = idx >= 0
+    bad = (idx >= v).any(1)
+    at = idx.clamp(0, v - 1)
+    t = torch.where(used, tlp.double(), torch.full_like(tlp, -torch.inf, dtype=torch.float64))
+    if tail:
+        none = ~used.any(1)
+        q, logq = torch.where(used, t.exp(), 0.0), t
+        rel_q = torch.full_like(q, 4 * U)
+        rest = (1 - q.sum(1)).clamp(min=0)
+    else:
+        tm = t.amax(1, keepdim=True)
+        none = torch.isneginf(tm[:, 0])
+        d = torch.where(none[:, None], torch.full_like(t, -torch.inf), t - torch.where(none[:, None], 0.0, tm))
+        z = d.exp().sum(1, keepdim=True)
+        q = torch.where(none[:, None], torch.zeros_like(t), d.exp() / z)
+        logq = d - torch.log(z)
+        rel_q = (torch.where(q > 0, d.abs(), 0.0) + 10 + k) * U
+        rest = torch.zeros(n, dtype=torch.float64, device=x.device)
+    lpk = logp.gather(1, at)
+    diff = torch.where(q > 0, logq - lpk, torch.zeros_like(q))
+    terms = q * diff
+    inside = torch.zeros(n, v + 1, dtype=torch.bool, device=x.device)
+    inside.scatter_(1, torch.where(used, at, v), True)
+    inside = inside[:, :v]
+    outside = ~inside & ~torch.isneginf(x)
+    logpr = torch.logsumexp(torch.where(outside, logp, torch.full_like(logp, -torch.inf)), 1)
+    # a rest that lies 30000 below the largest logit is masked
+    y = squash(x, 1.0, softcap)[0]
+    low = torch.where(outside, y, torch.full_like(y, -torch.inf)).amax(1) - y.amax(1)
+    has_rest = outside.any(1) & ~none & (torch.tensor(tail, device=x.device)) & (low >= -3e4)
+    dr = (k + 6) * U
+    tail_term = torch.where(has_rest & (rest > 0), rest * (torch.log(rest) - logpr), torch.zeros_like(rest))
+    losses = terms.sum(1) + tail_term
+    tol_lp = r["tol_logs"][:, None] + 8 * U * (lpk.abs().nan_to_num(0, 0, 0) + torch.log(torch.tensor(v + 1.0)).item()) + 8 * U * softcap / temperature
+    absl = torch.where(q > 0, logq.abs(), 0.0)
+    tol = (q * (rel_q * diff.abs().nan_to_num(0, 0, 0) + tol_lp + (4 + k) * U * (absl + 1))).sum(1)
+    tol = tol + torch.where(has_rest, dr * (3 + torch.log(rest + dr).abs() + logpr.abs().nan_to_num(0, 0, 0))
+                            + rest * (2 * r["tol_logs"] + 12 * U * (1 + logpr.abs().nan_to_num(0, 0, 0)) + 16 * U * softcap / temperature),
+                            torch.zeros_like(rest))
+    tol = tol + 24 * U * (terms.abs().nan_to_num(0, 0, 0).sum(1) + tail_term.abs())
+    losses = torch.where(none, torch.zeros_like(losses), losses)
+    losses = torch.where(bad, torch.full_like(losses, torch.nan), losses)
+    losses, tol = torch.where(live, losses, 0.0), torch.where(live, tol, 0.0)
+    cnt = max(1, int(live.sum()))
+    mult = temperature ** 2 / cnt
+    # gradient
+    mass = torch.zeros_like(p).scatter_add_(1, at, torch.where(used, q, 0.0))
+    cond = torch.where(has_rest[:, None] & outside, (logp - logpr[:, None]).exp(), torch.zeros_like(p))  # p_i / p_r
+    g = torch.where(inside, p - mass, p - rest[:, None] * cond)
+    _, dy = squash(x, temperature, softcap)
+    logv = torch.log(torch.tensor(v + 1.0)).item()
+    lgp = torch.where(p > 0, logp, torch.zeros_like(p))
+    lpr = torch.where(has_rest, logpr, torch.zeros_like(rest)).abs()[:, None]
+    rel = 10 * U + (4 * lgp.abs() + 6 * logv + 6 * lpr) * U + 2 * r["tol_logs"][:, None] + 16 * U * softcap / temperature
+    relm = torch.zeros_like(p).scatter_add_(1, at, torch.where(used, q * (rel_q + k * U), torch.zeros_like(q)))
+    tg = torch.where(inside, p * rel + relm, p * rel + cond * (rest[:, None] * rel + dr)) + 6 * U * g.abs()
+    tg = tg * dy.abs() + (g.abs() * 16 * U / temperature if softcap > 0 else 0.0)
+    off = (none | empty | ~live)[:, None]
+    g, tg = torch.where(off, torch.zeros_like(g), g * dy), torch.where(off, torch.zeros_like(tg), tg)
+    g = torch.where((bad & live)[:, None], torch.full_like(g, torch.nan), g)
+    f = mult * g_loss
+    return {"losses": losses, "tol_losses": tol, "loss": losses.sum() * mult,
+            "tol_loss": (tol.sum() + (n / 1024 + 64) * U * losses.abs().nan_to_num(0, 0, 0).sum()) * mult,
+            "grad": g * f, "tol_grad": tg * abs(f)}

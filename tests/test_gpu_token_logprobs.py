@@ -94,6 +94,7 @@ def test_masks_and_ties(v, dtype):
     t = torch.full((x.shape[0],), v // 2, device=DEV)
     for k in sorted({1, min(20, v), min(128, v)}):
         check(x, t, token_logprobs(x, t, top_k=k, entropy=True), top_k=k)
+    check(x, t, token_logprobs(x, t, top_k=min(20, v), entropy=True, softcap=9.0), top_k=min(20, v), softcap=9.0)
     big = x.repeat(60, 1)  # a CTA per row
     check(big, t.repeat(60), token_logprobs(big, t.repeat(60), top_k=min(9, v), entropy=True), top_k=min(9, v))
 
@@ -204,6 +205,10 @@ def test_backward_masked_rows(dtype):
     ref, tol = O.token_logprobs_grad(x.double().cpu(), t.cpu(), gl, ge)
     O.assert_within(got, ref, tol, "grad")
     assert (got[0] == 0).all() and (got[2] == 0).all()
+    r = token_logprobs(xg, t, entropy=True, softcap=9.0)
+    got, = torch.autograd.grad([r.logprobs, r.entropy], xg, [gl.to(DEV), ge.to(DEV)])
+    ref, tol = O.token_logprobs_grad(x.double().cpu(), t.cpu(), gl, ge, softcap=9.0)
+    O.assert_within(got, ref, tol, "softcap grad")
     # a row of NaN that is ignored gets zeros
     xn = torch.full((2, 77), torch.nan, dtype=dtype, device=DEV, requires_grad=True)
     r = token_logprobs(xn, torch.tensor([-100, 5], device=DEV))
