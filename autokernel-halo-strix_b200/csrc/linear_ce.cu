@@ -36,7 +36,12 @@
 // list-scheduled, see sched_tile).  Every mbarrier wait is bounded: on a
 // timeout AK_ERR_TIMEOUT goes to the caller's status word, the CTA stops
 // issuing loads and MMAs, drains what it issued, frees TMEM and finishes.
-#include "ak_common.cuh"
+//
+// The same GEMM also answers token log-probabilities from hidden states (EPI_LOGP: each tile is
+// reduced to per-row softmax statistics with the sums the entropy needs, nothing is stored) and
+// their gradients (EPI_LOGP_GRAD: the logits are formed again and leave the accumulators as
+// dL/dlogits in 16 bits, from the forward's statistics; then the grouped dW / dH launch).
+#include "logit_rows.cuh"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -62,7 +67,8 @@ constexpr int TMEM_COLS = 2 * BN;  // two accumulators
 constexpr int64_t kChunkRows = 16384;
 constexpr int kTileOverheadK = 4;  // per-tile cost beyond its K blocks, in K blocks (list schedule)
 
-enum Epi : int { EPI_STATS = 0, EPI_STORE = 1, EPI_NONE = 2 };  // EPI_NONE: accumulate only (timing)
+// EPI_NONE: accumulate only (timing)
+enum Epi : int { EPI_STATS = 0, EPI_STORE = 1, EPI_NONE = 2, EPI_LOGP = 3, EPI_LOGP_GRAD = 4 };
 
 struct Prob {
   int M, N, K;
@@ -81,6 +87,14 @@ struct Prob {
   const float* add_f32;     // nullable, same layout as C
   const float* scale;       // nullable device scalar multiplying acc (before add_f32 / accumulate)
   int c_f32, accumulate;
+  // EPI_LOGP: part (largest logit, S), partw (sum of e * argument; nullable) and tlogit.
+  // EPI_LOGP_GRAD: C (ldc) = gradient of the logits / *scale, from the rows' statistics
+  float* partw;             // [M][kEpiGroups * ntiles]
+  const float2* stats;      // [M] (mu, log S)
+  const float* entropy;     // [M], with g_ent
+  const float* g_lp;        // nullable [M]
+  const float* g_ent;       // nullable [M]
+  Squash q;
 };
 
 // Two problems whose tiles differ in K (dW's short-K tiles and dH's long-K ones)
@@ -544,10 +558,157 @@ __device__ __forceinline__ void epi_store(const Prob& P, uint32_t tbase, int row
   }
 }
 
+// One 32-column chunk into a row's statistics; columns from P.N on hold nothing.
+template <bool CAP, bool ENT>
+__device__ __forceinline__ void logp_chunk(const float (&v)[32], RowStats<true, true>& st, const Squash& q) {
+  RowStats<CAP, ENT> a;
+  a.m = st.m; a.mu = st.mu; a.s = st.s;
+  if constexpr (ENT) a.w = st.w;
+  a.add(v, q);
+  st.m = a.m; st.mu = a.mu; st.s = a.s;
+  if constexpr (ENT) st.w = a.w;
+}
+
+// Per-row softmax statistics of this warpgroup's 128 columns, with the entropy's sum if P.partw,
+// and the target logit.  Nothing else is stored.
+template <typename T>
+__device__ __forceinline__ void epi_logp(const Prob& P, uint32_t tbase, int row0, int lane, int64_t lab, int col0,
+                                         int eg) {
+  const int row = row0 + lane;
+  const int c0 = eg * kGroupCols;
+  const Squash q = P.q;
+  const bool cap = q.cap > 0.f, ent = P.partw != nullptr;
+  RowStats<true, true> st;
+  st.init();
+  Tm32 buf[2];
+  __syncwarp();
+  tmem_ld_issue(tbase + (uint32_t)c0, buf[0]);
+  tmem_ld_wait(buf[0]);
+#pragma unroll
+  for (int k = 0; k < kGroupCols / 32; ++k) {
+    if (k + 1 < kGroupCols / 32) tmem_ld_issue(tbase + (uint32_t)(c0 + 32 * (k + 1)), buf[(k + 1) & 1]);
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[k & 1].r[j]);
+    const int cbase = col0 + c0 + 32 * k;
+    const int rel = (int)(lab - cbase);  // lab is -1 where the row has no target (or is no row)
+    if ((unsigned)rel < 32u) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j == rel) P.tlogit[row] = v[j];
+    }
+    if (cbase + 32 > P.N) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (cbase + j >= P.N) v[j] = -INFINITY;
+    }
+    if (!cap && ent) logp_chunk<false, true>(v, st, q);
+    else if (!cap) logp_chunk<false, false>(v, st, q);
+    else if (ent) logp_chunk<true, true>(v, st, q);
+    else logp_chunk<true, false>(v, st, q);
+    if (k + 1 < kGroupCols / 32) tmem_ld_wait(buf[(k + 1) & 1]);
+  }
+  if (row < P.M) {
+    const int64_t at = (int64_t)row * (kEpiGroups * P.ntiles) + kEpiGroups * (col0 / BN) + eg;
+    P.part[at] = make_float2(st.m, st.s);
+    if (ent) P.partw[at] = st.w;
+  }
+}
+
+// What a lane needs to turn its row's logits into their gradient: with d = (y - mu) kl - log2 S and
+// p = 2^d, dx = (p (c0 + c1 d) [+ ct at the target]) * slope of the softcap.
+struct LogpRow {
+  float mu, l2s, c0, c1, ct;
+  int t;      // target column, or -1
+  bool none;  // no gradient: ignored, no distribution, or no such row
+};
+
+__device__ __forceinline__ LogpRow load_logp_row(const Prob& P, int row) {
+  LogpRow r{};
+  r.t = -1;
+  r.none = true;
+  if (row >= P.M) return r;
+  const int64_t lab = P.labels ? P.labels[row] : -1;
+  const float2 ml = P.stats[row];
+  r.none = (P.labels && lab == P.ignore_index) || ml.y == -INFINITY;
+  float gl = (P.labels && P.g_lp) ? P.g_lp[row] : 0.f;
+  if (P.labels && !r.none && (lab < 0 || lab >= P.N)) gl = NAN;
+  else r.t = (int)lab;
+  const float ge = P.g_ent ? P.g_ent[row] : 0.f, H = P.g_ent ? P.entropy[row] : 0.f;
+  const float f = P.q.inv_t / (P.scale ? *P.scale : 1.f);
+  r.mu = ml.x;
+  r.l2s = ml.y * kLog2e;
+  r.c0 = -(gl + ge * H) * f;
+  r.c1 = -ge * kLn2 * f;
+  r.ct = gl * f;
+  return r;
+}
+
+// The logits' gradient, rounded to T once: the operand type of the dW / dH products.
+template <typename T>
+__device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int row0, int lane, const LogpRow& lr,
+                                              int col0, int eg, uint32_t stg) {
+  const int row = row0 + lane;
+  const int nrows = min(32, P.M - row0);
+  const int c0 = eg * kGroupCols;
+  const Squash q = P.q;
+  const bool cap = q.cap > 0.f;
+  T* C = reinterpret_cast<T*>(P.C);
+  Tm32 buf[2];
+  __syncwarp();
+  tmem_ld_issue(tbase + (uint32_t)c0, buf[0]);
+  tmem_ld_wait(buf[0]);
+#pragma unroll
+  for (int k = 0; k < kGroupCols / 32; ++k) {
+    if (k + 1 < kGroupCols / 32) tmem_ld_issue(tbase + (uint32_t)(c0 + 32 * (k + 1)), buf[(k + 1) & 1]);
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[k & 1].r[j]);
+    const int cbase = col0 + c0 + 32 * k;
+    const int rel = lr.t - cbase;
+    if (lr.none) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = 0.f;
+    } else if (!cap) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float d = (v[j] - lr.mu) * q.kl - lr.l2s;
+        float o = ex2(d) * fmaf(lr.c1, fmaxf(d, -1e4f), lr.c0);
+        if (j == rel) o += lr.ct;
+        v[j] = o;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float y = squash<true>(v[j], q);
+        const float d = (y - lr.mu) * q.kl - lr.l2s;
+        float o = ex2(d) * fmaf(lr.c1, fmaxf(d, -1e4f), lr.c0);
+        if (j == rel) o += lr.ct;
+        v[j] = o * squash_slope<true>(y, q);
+      }
+    }
+    if (col0 + c0 + 32 * (k | 1) + 32 <= P.N) {
+      stage_put<T>(stg, lane, k & 1, v);
+      if (k & 1) {
+        __syncwarp();
+        stage_flush<T>(stg, lane, C, P.ldc, row0, nrows, cbase - 32);
+        __syncwarp();
+      }
+    } else if (row < P.M) {
+      T* crow = C + (int64_t)row * P.ldc + cbase;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (cbase + j < P.N) crow[j] = from_f<T>(v[j]);
+    }
+    if (k + 1 < kGroupCols / 32) tmem_ld_wait(buf[(k + 1) & 1]);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // The GEMM kernel (clusters of 2 CTAs)
 // ---------------------------------------------------------------------------
-template <typename T, bool kList>
+// kLogp: the log-probability epilogues, kept out of the instances that the other launches use.
+template <typename T, bool kList, bool kLogp>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 tc_gemm2_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tB0,
                 const __grid_constant__ CUtensorMap tA1, const __grid_constant__ CUtensorMap tB1,
@@ -682,13 +843,30 @@ tc_gemm2_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__
       const Prob& P = pi ? g.p[1] : g.p[0];
       const int acc = local & 1;
       const int row0 = mt * (2 * BM) + (int)rank * BM + quad * 32;  // this warp's 32 rows
-      // the row's label is loaded before the wait, so its latency hides behind the MMAs
-      const int64_t lab = (P.epi == EPI_STATS && row0 + lane < P.M) ? P.labels[row0 + lane] : -1;
+      // the row's label (and coefficients) are loaded before the wait, so their latency hides
+      // behind the MMAs
+      int64_t lab = -1;
+      [[maybe_unused]] LogpRow lr;
+      if constexpr (kLogp) {
+        if (P.epi == EPI_LOGP) {
+          if (P.labels && row0 + lane < P.M) lab = P.labels[row0 + lane];
+          if (lab < 0 || lab >= P.N) lab = -1;
+        } else {
+          lr = load_logp_row(P, row0 + lane);
+        }
+      } else {
+        lab = (P.epi == EPI_STATS && row0 + lane < P.M) ? P.labels[row0 + lane] : -1;
+      }
       if (!wait_bar<false>(&tfull[acc], (uint32_t)(local >> 1) & 1u, wt)) break;  // no accumulator to read
       tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
-      if (P.epi == EPI_STATS) epi_stats<T>(P, tbase, row0, lane, lab, nt * BN, eg, stg);
-      else if (P.epi == EPI_STORE) epi_store<T>(P, tbase, row0, lane, nt * BN, eg, stg);
+      if constexpr (kLogp) {
+        if (P.epi == EPI_LOGP) epi_logp<T>(P, tbase, row0, lane, lab, nt * BN, eg);
+        else epi_logp_grad<T>(P, tbase, row0, lane, lr, nt * BN, eg, stg);
+      } else {
+        if (P.epi == EPI_STATS) epi_stats<T>(P, tbase, row0, lane, lab, nt * BN, eg, stg);
+        else if (P.epi == EPI_STORE) epi_store<T>(P, tbase, row0, lane, nt * BN, eg, stg);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty0 + (uint32_t)(acc * 8));
@@ -804,15 +982,71 @@ lce_grad_inplace(T* __restrict__ L, const float* __restrict__ lse, const int64_t
   }
 }
 
+// Merge the per-tile partials of a row (one warp each) into its log-probability, entropy and lse.
+template <bool CAP>
+__global__ void __launch_bounds__(256)
+logp_rows_reduce(float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ lse,
+                 float2* __restrict__ stats, const float2* __restrict__ part, const float* __restrict__ partw,
+                 const float* __restrict__ tlogit, const int64_t* __restrict__ labels, int M, int V, int nparts,
+                 int64_t ignore_index, const Squash q) {
+  const int row = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+  if (row >= M) return;
+  RowStats<CAP, true> st;
+  st.init();
+  for (int t = lane; t < nparts; t += 32) {
+    const float2 p = part[(int64_t)row * nparts + t];
+    RowStats<CAP, true> o;
+    o.init();
+    if (p.x != -INFINITY) { o.m = p.x; o.mu = squash<CAP>(p.x, q); }
+    o.s = p.y;
+    o.w = partw ? partw[(int64_t)row * nparts + t] : 0.f;
+    st.merge(o, q);
+  }
+  st.warp_merge(q);
+  if (lane != 0) return;
+  const float logs = logf(st.s);
+  const int64_t t = labels ? labels[row] : -1;
+  const bool ignored = labels && t == ignore_index;
+  if (logprobs) {
+    float lp = 0.f;
+    if (!ignored) {
+      if (t < 0 || t >= V) lp = NAN;  // not a token
+      else if (st.s == 0.f) lp = -INFINITY;
+      else lp = (squash<CAP>(tlogit[row], q) - st.mu) * q.inv_t - logs;
+    }
+    logprobs[row] = lp;
+  }
+  if (entropy) entropy[row] = (ignored || st.s == 0.f) ? 0.f : logs - kLn2 * (st.w / st.s);
+  lse[row] = st.mu * q.inv_t + logs;
+  if (stats) stats[row] = make_float2(st.mu, logs);
+}
+
+// scale[0] = largest |g_lp| + |g_ent| over the rows (1 where that is 0 or not finite): divides the
+// 16-bit gradient of the logits, so that small upstream gradients do not underflow in fp16.
+__global__ void __launch_bounds__(1024)
+logp_grad_scale(float* __restrict__ scale, const float* __restrict__ g_lp, const float* __restrict__ g_ent, int64_t M) {
+  __shared__ float s[32];
+  float m = 0.f;
+  for (int64_t i = threadIdx.x; i < M; i += blockDim.x)
+    m = fmaxf(m, (g_lp ? fabsf(g_lp[i]) : 0.f) + (g_ent ? fabsf(g_ent[i]) : 0.f));
+  m = warp_max(m);
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 32; ++i) m = fmaxf(m, s[i]);
+    scale[0] = (m > 0.f && m < INFINITY) ? m : 1.f;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-// Tensor map over a row-major [rows][cols] 16-bit matrix.  K-major operands
+// Tensor map over a row-major [rows][cols] 16-bit matrix with rows ld elements apart.  K-major operands
 // (cols = K) load 64 x 128 boxes; MN-major operands (cols = M or N) load 64 x 64
 // boxes, two per operand and stage.
-int make_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, bool mn, bool bf16) {
+int make_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, bool mn, bool bf16) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
   const cuuint32_t box[2] = {64u, mn ? 64u : 128u};
   const cuuint32_t estr[2] = {1, 1};
   // Resolved through the runtime so the library does not link libcuda directly.
@@ -837,11 +1071,12 @@ int make_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, bo
 constexpr size_t kSmem = (size_t)STAGES * STAGE_BYTES + 256 + (size_t)kEpiWarps * kStageWarpBytes + 1024;
 
 // One GEMM operand: a row-major [rows][cols] matrix read K-major (cols = K) or
-// MN-major (cols = M or N).
+// MN-major (cols = M or N).  ld: elements between rows, 0 for cols.
 struct Operand {
   const void* base;
   int64_t rows, cols;
   int mn;
+  int64_t ld = 0;
 };
 
 void finish_prob(Prob& P) {
@@ -865,7 +1100,7 @@ int resident_pairs() {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmem;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, tc_gemm2_kernel<T, false>, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, tc_gemm2_kernel<T, false, false>, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
       n = sm_count() / 2;
     }
@@ -877,11 +1112,22 @@ int resident_pairs() {
 template <typename T>
 int launch_group(const Operand* A, const Operand* B, Group& g, cudaStream_t st) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  // before the tensor maps: the runtime call binds the device's context to this thread, which the
+  // driver's encoder needs (an autograd worker may come here with none bound yet)
+  auto prepare = [](auto kern) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+  };
+  const bool logp = g.p[0].epi == EPI_LOGP || g.p[0].epi == EPI_LOGP_GRAD;
+  AK_CUDA_TRY(logp ? prepare(tc_gemm2_kernel<T, false, true>) : prepare(tc_gemm2_kernel<T, false, false>),
+              "linear_ce: smem attribute");
   CUtensorMap maps[4];
   int rc;
   for (int i = 0; i < g.nprob; ++i) {
-    if ((rc = make_tmap(&maps[2 * i], A[i].base, A[i].rows, A[i].cols, A[i].mn, bf16))) return rc;
-    if ((rc = make_tmap(&maps[2 * i + 1], B[i].base, B[i].rows, B[i].cols, B[i].mn, bf16))) return rc;
+    if ((rc = make_tmap(&maps[2 * i], A[i].base, A[i].rows, A[i].cols, A[i].ld ? A[i].ld : A[i].cols, A[i].mn, bf16)))
+      return rc;
+    if ((rc = make_tmap(&maps[2 * i + 1], B[i].base, B[i].rows, B[i].cols, B[i].ld ? B[i].ld : B[i].cols, B[i].mn,
+                        bf16)))
+      return rc;
     g.p[i].a_mn = A[i].mn;
     g.p[i].b_mn = B[i].mn;
     finish_prob(g.p[i]);
@@ -900,9 +1146,11 @@ int launch_group(const Operand* A, const Operand* B, Group& g, cudaStream_t st) 
     }
   }
   if (g.total == 0) return AK_OK;
-  auto kern = g.lp >= 0 ? tc_gemm2_kernel<T, true> : tc_gemm2_kernel<T, false>;
-  AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem),
-              "linear_ce: smem attribute");
+  auto kern = logp ? tc_gemm2_kernel<T, false, true> : tc_gemm2_kernel<T, false, false>;
+  if (g.lp >= 0) {
+    kern = tc_gemm2_kernel<T, true, false>;
+    AK_CUDA_TRY(prepare(kern), "linear_ce: smem attribute");
+  }
   const int pairs = std::max(1, std::min(g.total, resident_pairs<T>()));
   kern<<<2 * pairs, kThreads, kSmem, st>>>(maps[0], maps[1], maps[2], maps[3], g);
   AK_CHECK_LAUNCH("linear_ce: tcgen05 gemm");
@@ -1039,6 +1287,151 @@ int run(float* loss, float* lse, void* dH, void* dW, const Ws& w, const void* H,
   return AK_OK;
 }
 
+// Token log-probabilities.  Workspace: the tiles' statistics of one chunk (forward), or the chunk's
+// 16-bit gradient of the logits, rows padded to 8 elements, and the fp32 dW accumulator (backward).
+struct LogpWs {
+  float2* part;
+  float* partw;
+  float* tlogit;
+  void* G;
+  float* scale;
+  float* dWacc;
+  size_t bytes;
+};
+
+LogpWs carve_logp(void* base, int64_t N, int64_t D, int64_t V, bool backward) {
+  LogpWs w{};
+  const int64_t nparts = kEpiGroups * ((V + BN - 1) / BN), Nc = chunk_rows(N);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    off = (off + 255) & ~size_t(255);
+    char* p = base ? static_cast<char*>(base) + off : nullptr;
+    off += bytes;
+    return p;
+  };
+  if (backward) {
+    w.G = take((size_t)Nc * ((V + 7) / 8 * 8) * 2);
+    w.scale = reinterpret_cast<float*>(take(4));
+    w.dWacc = N > Nc ? reinterpret_cast<float*>(take((size_t)V * D * 4)) : nullptr;
+  } else {
+    w.part = reinterpret_cast<float2*>(take((size_t)Nc * nparts * sizeof(float2)));
+    w.partw = reinterpret_cast<float*>(take((size_t)Nc * nparts * 4));
+    w.tlogit = reinterpret_cast<float*>(take((size_t)Nc * 4));
+  }
+  w.bytes = off + 256;
+  return w;
+}
+
+template <typename T>
+int logp_fwd(float* logprobs, float* entropy, float* lse, float2* stats, const LogpWs& w, const void* H,
+             const void* W, const int64_t* labels, int64_t N, int64_t D, int64_t V, const Squash& q,
+             int64_t ignore_index, int* status, cudaStream_t st) {
+  const int64_t Nc = chunk_rows(N);
+  const int nparts = kEpiGroups * (int)((V + BN - 1) / BN);
+  for (int64_t r0 = 0; r0 < N; r0 += Nc) {
+    const int64_t nr = std::min(Nc, N - r0);
+    Operand A[1] = {{static_cast<const T*>(H) + r0 * D, nr, D, 0}};
+    Operand B[1] = {{W, V, D, 0}};
+    Group g{};
+    g.nprob = 1;
+    g.status = status;
+    Prob& P = g.p[0];
+    P.M = (int)nr; P.N = (int)V; P.K = (int)D;
+    P.epi = EPI_LOGP;
+    P.part = w.part; P.partw = entropy ? w.partw : nullptr; P.tlogit = w.tlogit;
+    P.labels = labels ? labels + r0 : nullptr; P.ignore_index = ignore_index;
+    P.q = q;
+    const int rc = launch_group<T>(A, B, g, st);
+    if (rc) return rc;
+    auto kern = q.cap > 0.f ? logp_rows_reduce<true> : logp_rows_reduce<false>;
+    kern<<<(unsigned)((nr * 32 + 255) / 256), 256, 0, st>>>(
+        logprobs ? logprobs + r0 : nullptr, entropy ? entropy + r0 : nullptr, lse + r0, stats ? stats + r0 : nullptr,
+        w.part, P.partw, w.tlogit, P.labels, (int)nr, (int)V, nparts, ignore_index, q);
+    AK_CHECK_LAUNCH("ak_linear_logprobs_fwd: rows");
+  }
+  return AK_OK;
+}
+
+template <typename T>
+int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, const int64_t* labels,
+             const float2* stats, const float* entropy, const float* g_lp, const float* g_ent, int64_t N, int64_t D,
+             int64_t V, const Squash& q, int64_t ignore_index, int* status, cudaStream_t st) {
+  const int64_t Nc = chunk_rows(N), ldg = (V + 7) / 8 * 8;
+  // bf16 has fp32's range; only fp16 is scaled
+  const float* scale = nullptr;
+  if (std::is_same<T, __half>::value) {
+    logp_grad_scale<<<1, 1024, 0, st>>>(w.scale, g_lp, g_ent, N);
+    AK_CHECK_LAUNCH("ak_linear_logprobs_bwd: scale");
+    scale = w.scale;
+  }
+  int rc;
+  for (int64_t r0 = 0; r0 < N; r0 += Nc) {
+    const int64_t nr = std::min(Nc, N - r0);
+    const bool first = r0 == 0, last = r0 + nr >= N;
+    Operand A[2], B[2];
+    Group g{};
+    g.status = status;
+    g.nprob = 1;
+    A[0] = {static_cast<const T*>(H) + r0 * D, nr, D, 0};
+    B[0] = {W, V, D, 0};
+    Prob& L = g.p[0];
+    L.M = (int)nr; L.N = (int)V; L.K = (int)D;
+    L.epi = EPI_LOGP_GRAD;
+    L.C = w.G; L.ldc = ldg;
+    L.labels = labels ? labels + r0 : nullptr; L.ignore_index = ignore_index;
+    L.stats = stats + r0; L.entropy = entropy ? entropy + r0 : nullptr;
+    L.g_lp = g_lp ? g_lp + r0 : nullptr; L.g_ent = g_ent ? g_ent + r0 : nullptr;
+    L.scale = scale; L.q = q;
+    if ((rc = launch_group<T>(A, B, g, st))) return rc;
+    // dW (+)= G^T H_c and dH_c = G W in one launch, as in the linear + CE
+    g = Group{};
+    g.status = status;
+    int np = 0;
+    if (dW) {
+      A[np] = {w.G, nr, V, 1, ldg};
+      B[np] = {static_cast<const T*>(H) + r0 * D, nr, D, 1};
+      Prob& P = g.p[np++];
+      P.M = (int)V; P.N = (int)D; P.K = (int)nr;
+      P.epi = EPI_STORE;
+      P.ldc = D;
+      P.scale = scale;
+      if (first && last) {
+        P.C = dW;
+      } else if (!last) {
+        P.C = w.dWacc; P.c_f32 = 1; P.accumulate = first ? 0 : 1;
+      } else {
+        P.C = dW; P.add_f32 = w.dWacc;
+      }
+    }
+    if (dH) {
+      A[np] = {w.G, nr, V, 0, ldg};
+      B[np] = {W, V, D, 1};
+      Prob& P = g.p[np++];
+      P.M = (int)nr; P.N = (int)D; P.K = (int)V;
+      P.epi = EPI_STORE;
+      P.C = static_cast<T*>(dH) + r0 * D; P.ldc = D;
+      P.scale = scale;
+    }
+    g.nprob = np;
+    if ((rc = launch_group<T>(A, B, g, st))) return rc;
+  }
+  return AK_OK;
+}
+
+int check_logp(const char* what, const void* H, const void* W, int64_t N, int64_t D, int64_t V, float temperature,
+               float softcap, int dt) {
+  AK_REQUIRE(dt == AK_BF16 || dt == AK_F16, AK_ERR_DTYPE, "%s: hidden states and weight must be bf16 or fp16", what);
+  AK_REQUIRE(N >= 0 && D > 0 && V > 0 && D % 8 == 0 && D <= (1 << 20) && N < (1LL << 31) && V < (1LL << 30),
+             AK_ERR_SHAPE, "%s: bad shape: %lld x %lld, vocabulary %lld (the hidden size must be a multiple of 8)", what,
+             (long long)N, (long long)D, (long long)V);
+  AK_REQUIRE(temperature > 0.f && temperature < INFINITY, AK_ERR_ARG, "%s: temperature must be positive and finite",
+             what);
+  AK_REQUIRE(softcap >= 0.f && softcap < INFINITY, AK_ERR_ARG, "%s: softcap must be >= 0 and finite", what);
+  AK_REQUIRE(N == 0 || (H && W && aligned16(H) && aligned16(W)), AK_ERR_ARG,
+             "%s: hidden states and weight must be 16-byte aligned", what);
+  return AK_OK;
+}
+
 int check_shape(int64_t N, int64_t D, int64_t V, int dt) {
   AK_REQUIRE(dt == AK_BF16 || dt == AK_F16, AK_ERR_DTYPE, "linear_ce: tensor-core path takes bf16 or fp16");
   AK_REQUIRE(N > 0 && D > 0 && V > 0, AK_ERR_SHAPE, "linear_ce: empty problem");
@@ -1149,4 +1542,55 @@ extern "C" int ak_linear_ce_logits_grad(float* loss, float* lse, void* G, void* 
   lce_loss<<<1, 1024, 0, st>>>(loss, w.losses, w.inv_valid, N);
   AK_CHECK_LAUNCH("ak_linear_ce_logits_grad");
   return AK_OK;
+}
+
+extern "C" int ak_linear_logprobs_workspace_size(int64_t N, int64_t D, int64_t V, int backward, size_t* bytes) {
+  clear_error();
+  AK_REQUIRE(bytes != nullptr, AK_ERR_ARG, "ak_linear_logprobs_workspace_size: null bytes");
+  AK_REQUIRE(N >= 0 && D > 0 && V > 0, AK_ERR_SHAPE, "ak_linear_logprobs_workspace_size: bad shape");
+  *bytes = carve_logp(nullptr, N, D, V, backward != 0).bytes;
+  return AK_OK;
+}
+
+extern "C" int ak_linear_logprobs_fwd(float* logprobs, float* entropy, float* lse, float* row_stats, void* workspace,
+                                      size_t ws_bytes, const void* H, const void* W, const int64_t* targets, int64_t N,
+                                      int64_t D, int64_t V, float temperature, float softcap, int64_t ignore_index,
+                                      int dt, int* status, void* stream) {
+  clear_error();
+  const int rc = check_logp("ak_linear_logprobs_fwd", H, W, N, D, V, temperature, softcap, dt);
+  if (rc) return rc;
+  if (N == 0) return AK_OK;
+  AK_REQUIRE(lse && (!logprobs || targets), AK_ERR_ARG, "ak_linear_logprobs_fwd: null pointer");
+  AK_REQUIRE(workspace && ws_bytes >= carve_logp(nullptr, N, D, V, false).bytes, AK_ERR_WORKSPACE,
+             "ak_linear_logprobs_fwd: workspace too small");
+  void* base = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  const LogpWs w = carve_logp(base, N, D, V, false);
+  const Squash q = make_squash(temperature, softcap);
+  auto fn = dt == AK_BF16 ? logp_fwd<__nv_bfloat16> : logp_fwd<__half>;
+  return fn(logprobs, entropy, lse, reinterpret_cast<float2*>(row_stats), w, H, W, targets, N, D, V, q, ignore_index,
+            status, (cudaStream_t)stream);
+}
+
+extern "C" int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_t ws_bytes, const void* H,
+                                      const void* W, const int64_t* targets, const float* row_stats,
+                                      const float* entropy, const float* g_logprobs, const float* g_entropy, int64_t N,
+                                      int64_t D, int64_t V, float temperature, float softcap, int64_t ignore_index,
+                                      int dt, int* status, void* stream) {
+  clear_error();
+  const int rc = check_logp("ak_linear_logprobs_bwd", H, W, N, D, V, temperature, softcap, dt);
+  if (rc) return rc;
+  if (N == 0 || (!dH && !dW)) return AK_OK;
+  AK_REQUIRE(row_stats, AK_ERR_ARG, "ak_linear_logprobs_bwd: null pointer");
+  AK_REQUIRE(!g_logprobs || targets, AK_ERR_ARG, "ak_linear_logprobs_bwd: a gradient of logprobs needs targets");
+  AK_REQUIRE(!g_entropy || entropy, AK_ERR_ARG, "ak_linear_logprobs_bwd: a gradient of the entropy needs the entropy");
+  AK_REQUIRE((!dH || aligned16(dH)) && (!dW || aligned16(dW)), AK_ERR_ARG,
+             "ak_linear_logprobs_bwd: dH and dW must be 16-byte aligned");
+  AK_REQUIRE(workspace && ws_bytes >= carve_logp(nullptr, N, D, V, true).bytes, AK_ERR_WORKSPACE,
+             "ak_linear_logprobs_bwd: workspace too small");
+  void* base = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  const LogpWs w = carve_logp(base, N, D, V, true);
+  const Squash q = make_squash(temperature, softcap);
+  auto fn = dt == AK_BF16 ? logp_bwd<__nv_bfloat16> : logp_bwd<__half>;
+  return fn(dH, dW, w, H, W, targets, reinterpret_cast<const float2*>(row_stats), entropy, g_logprobs, g_entropy, N, D,
+            V, q, ignore_index, status, (cudaStream_t)stream);
 }

@@ -51,6 +51,9 @@ SIGNATURES = {
     "ak_token_logprobs_bwd": [_vp] * 7 + [_i64] * 5 + [_f, _f, _i64, _i, _vp],
     "ak_distill_topk_fwd": [_vp] * 10 + [_i64] * 6 + [_f, _f, _i, _i, _vp, _vp],
     "ak_distill_topk_bwd": [_vp] * 8 + [_i64] * 6 + [_f, _f, _i, _vp],
+    "ak_linear_logprobs_workspace_size": [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)],
+    "ak_linear_logprobs_fwd": [_vp] * 5 + [_sz] + [_vp] * 3 + [_i64] * 3 + [_f, _f, _i64, _i, _vp, _vp],
+    "ak_linear_logprobs_bwd": [_vp] * 3 + [_sz] + [_vp] * 7 + [_i64] * 3 + [_f, _f, _i64, _i, _vp, _vp],
     "ak_linear_ce_logits_grad_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
     "ak_linear_ce_logits_grad": [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp],
     "ak_linear_ce_workspace_size": [_i64, _i64, _i64, ctypes.POINTER(_sz)],
@@ -158,7 +161,8 @@ def _size_query(name: str, *dims: int) -> int:
 # Device status words (bounded-wait timeouts)
 # ---------------------------------------------------------------------------
 AK_ERR_TIMEOUT = 5
-STATUS_SLOTS = ("selective_scan_fwd", "selective_scan_bwd", "linear_ce", "bounded_wait_test", "distill_topk")
+STATUS_SLOTS = ("selective_scan_fwd", "selective_scan_bwd", "linear_ce", "bounded_wait_test", "distill_topk",
+                "linear_logprobs")
 
 
 class _StatusWords:
@@ -743,6 +747,44 @@ def linear_ce_fwdbwd(hidden, weight, labels, ignore_index=-100, need_dh=True, ne
     call("ak_linear_ce_fwdbwd", ptr(loss), ptr(lse), ptr(dH), ptr(dW), ptr(ws), ws_bytes, ptr(h), ptr(w), ptr(lab),
          ptr(inv_valid), N, D, V, int(ignore_index), dtype_code(h), status_ptr(dev, "linear_ce"), stream(dev))
     return loss, lse, dH, dW
+
+
+def linear_logprobs_fwd(hidden, weight, targets, temperature=1.0, softcap=0.0, ignore_index=-100,
+                        want_entropy=False, want_stats=False):
+    """Returns [logprobs, entropy, lse, row_stats] of the logits hidden @ weight.T (absent ones are None);
+    hidden (N, D) and weight (V, D) dense, 16-byte aligned, of one 16-bit type."""
+    dev = require_cuda(hidden, weight, targets)
+    N, D = hidden.shape
+    V = weight.shape[0]
+    f32 = dict(dtype=torch.float32, device=dev)
+    lp = torch.empty(N, **f32) if targets is not None else None
+    ent = torch.empty(N, **f32) if want_entropy else None
+    lse = torch.empty(N, **f32)
+    stats = torch.empty(N, 2, **f32) if want_stats else None
+    ws_bytes = _size_query("ak_linear_logprobs_workspace_size", N, D, V, 0)
+    ws = workspace(ws_bytes, dev)
+    call_on(dev, "ak_linear_logprobs_fwd", ptr(lp), ptr(ent), ptr(lse), ptr(stats), ptr(ws), ws_bytes, ptr(hidden),
+            ptr(weight), ptr(targets), N, D, V, temperature, softcap, ignore_index, dtype_code(hidden),
+            status_ptr(dev, "linear_logprobs"), stream(dev))
+    return [lp, ent, lse, stats]
+
+
+def linear_logprobs_bwd(hidden, weight, targets, row_stats, entropy, g_logprobs, g_entropy, temperature=1.0,
+                        softcap=0.0, ignore_index=-100, need_dh=True, need_dw=True):
+    """Returns (dH or None, dW or None) from the gradients of logprobs and entropy (either may be None)."""
+    dev = require_cuda(hidden, weight, targets, row_stats, entropy, g_logprobs, g_entropy)
+    N, D = hidden.shape
+    V = weight.shape[0]
+    dH = torch.empty_like(hidden) if need_dh else None
+    dW = (torch.empty_like(weight) if N else torch.zeros_like(weight)) if need_dw else None
+    glp = g_logprobs.to(torch.float32).contiguous() if g_logprobs is not None else None
+    gent = g_entropy.to(torch.float32).contiguous() if g_entropy is not None else None
+    ws_bytes = _size_query("ak_linear_logprobs_workspace_size", N, D, V, 1)
+    ws = workspace(ws_bytes, dev)
+    call_on(dev, "ak_linear_logprobs_bwd", ptr(dH), ptr(dW), ptr(ws), ws_bytes, ptr(hidden), ptr(weight),
+            ptr(targets), ptr(row_stats), ptr(entropy), ptr(glp), ptr(gent), N, D, V, temperature, softcap,
+            ignore_index, dtype_code(hidden), status_ptr(dev, "linear_logprobs"), stream(dev))
+    return dH, dW
 
 
 def tc_gemm(a: torch.Tensor, b: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:

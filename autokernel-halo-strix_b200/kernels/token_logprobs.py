@@ -6,7 +6,11 @@ decoding (no gradient is kept then), a teacher's pass over a batch for `kernels.
 policy-gradient losses: `logprobs` and `entropy` are differentiable.  The cross-entropy in
 `kernels.ce_fused` is the loss over the same rows.
 
-The reference has only the loss (kernels/ce_fused.py:557-785).
+`linear_token_logprobs` answers the same (without alternatives) from hidden states and the output
+projection on the tensor cores; logits are never stored, as in `ChunkedLinearCrossEntropyLoss`.
+
+The reference has only the losses (kernels/ce_fused.py:557-785,
+kernels/hip/chunked_linear_cross_entropy.py:50-229).
 """
 import math
 from typing import NamedTuple, Optional
@@ -106,6 +110,76 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
                                                    bool(entropy)))
     return TokenLogprobs(*_ak.token_logprobs_fwd(logits, targets, top_k, temperature, softcap, ignore_index,
                                                  want_entropy=bool(entropy))[:5])
+
+
+class _LinearTokenLogprobs(torch.autograd.Function):
+    """Saves its operands and two numbers a row; the backward forms the logits again, chunk by chunk."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, temperature, softcap, ignore_index, entropy):
+        w = weight.to(hidden.dtype)
+        lp, ent, lse, stats = _ak.linear_logprobs_fwd(hidden, w, targets, temperature, softcap, ignore_index,
+                                                      want_entropy=entropy, want_stats=True)
+        ctx.save_for_backward(hidden, w, targets, stats, ent)
+        ctx.args, ctx.weight_dtype = (temperature, softcap, ignore_index), weight.dtype
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(lse)
+        return lp, ent, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, *rest):
+        if g_lp is None and g_ent is None:
+            return (None,) * 7
+        hidden, w, targets, stats, ent = ctx.saved_tensors
+        dh, dw = _ak.linear_logprobs_bwd(hidden, w, targets, stats, ent, g_lp, g_ent, *ctx.args,
+                                         need_dh=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
+        return (dh, dw.to(ctx.weight_dtype) if dw is not None else None) + (None,) * 5
+
+
+def _dense16(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and on a 16-byte boundary (a TMA operand)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: Optional[torch.Tensor] = None, *,
+                          temperature: float = 1.0, softcap: float = 0.0, ignore_index: int = -100,
+                          entropy: bool = False) -> TokenLogprobs:
+    """`token_logprobs(hidden @ weight.T, targets, ...)` without the logits and without alternatives.
+
+    hidden (..., D): bf16 or fp16 on the GPU, D a multiple of 8; weight (V, D): cast to hidden's type
+    if it has another.  The log-probabilities are of the fp32 accumulators: nothing between the
+    products and the result is rounded to 16 bits.  In the backward the gradient of the logits is, as
+    the operand of the two products that follow.  The hidden states of ignored rows have to be
+    finite where a gradient of weight is wanted (they enter it times 0).
+    """
+    what = "linear_token_logprobs"
+    _ak.require_cuda(hidden, weight, targets)
+    if hidden.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: hidden must be bfloat16 or float16, got {hidden.dtype}")
+    _ak.dtype_code(weight)
+    if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[0] < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: hidden (..., D) and weight (V, D), got {tuple(hidden.shape)} and "
+                         f"{tuple(weight.shape)}")
+    D = hidden.shape[-1]
+    if D < 8 or D % 8:
+        raise ValueError(f"{what}: the hidden size must be a multiple of 8, got {D}")
+    lead = hidden.shape[:-1]
+    if targets is not None:
+        targets = check_targets(what, targets, lead).view(-1)
+    temperature, softcap = check_scales(what, temperature, softcap)
+    ignore_index = int(ignore_index)
+    h = _dense16(hidden.reshape(-1, D))
+    w = _dense16(weight)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        lp, ent, lse = _LinearTokenLogprobs.apply(h, w, targets, temperature, softcap, ignore_index, bool(entropy))
+    else:
+        lp, ent, lse, _ = _ak.linear_logprobs_fwd(h, w.to(h.dtype), targets, temperature, softcap, ignore_index,
+                                                  want_entropy=bool(entropy))
+    if len(lead) != 1:
+        lp, ent, lse = (t.view(lead) if t is not None else None for t in (lp, ent, lse))
+    return TokenLogprobs(lp, ent, lse)
 
 
 def kernel_fn(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:

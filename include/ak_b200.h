@@ -308,6 +308,33 @@ AK_API int ak_linear_ce_logits_grad(float* loss, float* lse, void* G, void* work
                    int64_t N, int64_t D, int64_t V, int64_t ignore_index, int dt,
                    int* status, void* stream);
 
+/* Workspace bytes for ak_linear_logprobs_fwd (backward = 0) / _bwd (1). */
+AK_API int ak_linear_logprobs_workspace_size(int64_t N, int64_t D, int64_t V, int backward,
+                                             size_t* bytes);
+
+/* ak_token_logprobs_fwd's logprobs, entropy, lse and row_stats for the logits H W^T of hidden
+ * states H[N, D] and an output projection W[V, D] (bf16 or fp16, dense, 16-byte aligned), without
+ * the logits: the tcgen05 GEMM reduces its fp32 accumulators to each row's statistics.  N and V
+ * are any, D is a multiple of 8.  entropy, row_stats and logprobs / targets are nullable. */
+AK_API int ak_linear_logprobs_fwd(float* logprobs, float* entropy, float* lse, float* row_stats,
+                                  void* workspace, size_t ws_bytes, const void* H, const void* W,
+                                  const int64_t* targets, int64_t N, int64_t D, int64_t V,
+                                  float temperature, float softcap, int64_t ignore_index, int dt,
+                                  int* status, void* stream);
+
+/* dH[N, D] and dW[V, D] (dt, each nullable) from the gradients of logprobs and entropy (fp32 [N],
+ * each nullable) and the forward's row_stats and entropy.  Per chunk of at most 16384 rows the
+ * logits are formed again and leave the accumulators as their gradient, rounded to dt once (in
+ * fp16 divided by the largest upstream gradient, which the next products' fp32 accumulators
+ * restore); then dW += G^T H and dH = G W in one launch.  Ignored rows have G = 0: their hidden
+ * states enter dW as 0 * h. */
+AK_API int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_t ws_bytes,
+                                  const void* H, const void* W, const int64_t* targets,
+                                  const float* row_stats, const float* entropy,
+                                  const float* g_logprobs, const float* g_entropy, int64_t N,
+                                  int64_t D, int64_t V, float temperature, float softcap,
+                                  int64_t ignore_index, int dt, int* status, void* stream);
+
 /* ------------------------------------------------------------------------ *
  * Collapsed (single-state) selective scan, fp32, layout (B, L, d)
  * ------------------------------------------------------------------------ */

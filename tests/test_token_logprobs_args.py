@@ -96,3 +96,52 @@ def test_rows_that_are_copied():
         assert rows == want.shape[0]
         for r, o in enumerate(offs):
             assert torch.equal(torch.as_strided(t, (x.shape[-1],), (1,), t.storage_offset() + o), want[r])
+
+
+@pytest.mark.parametrize("bad,err", [
+    (dict(h=torch.zeros(2, 16)), TypeError),
+    (dict(h=torch.zeros(2, 12, dtype=torch.bfloat16), w=torch.zeros(9, 12)), ValueError),
+    (dict(h=torch.zeros(2, 0, dtype=torch.bfloat16), w=torch.zeros(9, 0)), ValueError),
+    (dict(w=torch.zeros(9, 24)), ValueError), (dict(w=torch.zeros(16)), ValueError),
+    (dict(w=torch.zeros(0, 16)), ValueError), (dict(w=torch.zeros(9, 16, dtype=torch.float64)), TypeError),
+    (dict(t=torch.zeros(3, dtype=torch.long)), ValueError), (dict(t=torch.zeros(2)), TypeError),
+    (dict(temperature=0.0), ValueError), (dict(softcap=-2.0), ValueError)])
+def test_linear_refusals(monkeypatch, bad, err):
+    on_gpu(monkeypatch)
+    args = dict(h=torch.zeros(2, 16, dtype=torch.bfloat16), w=torch.zeros(9, 16), t=torch.zeros(2, dtype=torch.long))
+    args.update(bad)
+    with pytest.raises(err):
+        TL.linear_token_logprobs(args.pop("h"), args.pop("w"), args.pop("t"), **args)
+
+
+def test_linear_library_refusals():
+    lib = _ak.lib()
+    fake = ctypes.c_void_p(256)  # never dereferenced: each call fails its checks first
+    n = ctypes.c_size_t(0)
+    assert lib.ak_linear_logprobs_workspace_size(8, 64, 100, 0, None) == 1
+    assert lib.ak_linear_logprobs_workspace_size(8, 0, 100, 0, ctypes.byref(n)) == 3
+    assert lib.ak_linear_logprobs_workspace_size(8, 64, 100, 0, ctypes.byref(n)) == 0 and n.value > 8 * 2 * 12
+    fwd_ws = n.value
+    assert lib.ak_linear_logprobs_workspace_size(8, 64, 100, 1, ctypes.byref(n)) == 0 and n.value > 8 * 104 * 2
+    bwd_ws = n.value
+
+    def fwd(H=fake, lse=fake, lp=fake, t=fake, N=8, D=64, V=100, T=1.0, cap=0.0, dt=1, ws=fwd_ws):
+        return lib.ak_linear_logprobs_fwd(lp, None, lse, None, fake, ws, H, fake, t, N, D, V, T, cap, -100, dt, None,
+                                          None)
+
+    assert fwd(dt=0) == 2
+    for kw in (dict(D=12), dict(D=0), dict(V=0), dict(N=-1), dict(V=1 << 31)):
+        assert fwd(**kw) == 3, kw
+    for kw in (dict(H=None), dict(H=ctypes.c_void_p(258)), dict(lse=None), dict(t=None), dict(T=0.0), dict(cap=-1.0)):
+        assert fwd(**kw) == 1, kw
+    assert fwd(ws=fwd_ws - 1) == 6
+    assert fwd(N=0) == 0
+
+    def bwd(dH=fake, stats=fake, t=fake, ent=fake, gl=fake, ge=fake, ws=bwd_ws, N=8):
+        return lib.ak_linear_logprobs_bwd(dH, fake, fake, ws, fake, fake, t, stats, ent, gl, ge, N, 64, 100, 1.0, 0.0,
+                                          -100, 1, None, None)
+
+    for kw in (dict(dH=ctypes.c_void_p(258)), dict(stats=None), dict(t=None), dict(ent=None)):
+        assert bwd(**kw) == 1, kw
+    assert bwd(ws=bwd_ws - 1) == 6
+    assert bwd(N=0) == 0
