@@ -87,7 +87,7 @@ struct Prob {
   const float* add_f32;     // nullable, same layout as C
   const float* scale;       // nullable device scalar multiplying acc (before add_f32 / accumulate)
   int c_f32, accumulate;
-  // EPI_LOGP: part (largest logit, S), partw (sum of e * argument; nullable) and tlogit.
+  // EPI_LOGP: part (largest logit, S), partw (the entropy's sum; nullable) and tlogit.
   // EPI_LOGP_GRAD: C (ldc) = gradient of the logits / *scale, from the rows' statistics
   float* partw;             // [M][kEpiGroups * ntiles]
   const float2* stats;      // [M] (mu, log S)
@@ -1016,7 +1016,7 @@ logp_rows_reduce(float* __restrict__ logprobs, float* __restrict__ entropy, floa
     }
     logprobs[row] = lp;
   }
-  if (entropy) entropy[row] = (ignored || st.s == 0.f) ? 0.f : logs - kLn2 * (st.w / st.s);
+  if (entropy) entropy[row] = (ignored || st.s == 0.f) ? 0.f : logs - (st.w / st.s) * q.inv_t;
   lse[row] = st.mu * q.inv_t + logs;
   if (stats) stats[row] = make_float2(st.mu, logs);
 }

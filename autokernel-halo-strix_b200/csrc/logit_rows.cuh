@@ -4,6 +4,8 @@
 
 #include "ak_common.cuh"
 
+#include <type_traits>
+
 namespace ak {
 
 // Rows of logits: row r is (outer, inner) = (r / inner, r % inner) and starts at
@@ -150,15 +152,87 @@ __device__ __forceinline__ void store_group(T* p, const float (&x)[kGroup], bool
 }
 
 // ---------------------------------------------------------------------------
+// Values as they lie in memory: words of two 16-bit elements, or of one fp32
+// ---------------------------------------------------------------------------
+template <typename T>
+__host__ __device__ constexpr int elems_per_word() { return 4 / (int)sizeof(T); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, const __nv_bfloat16*) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, const __half*) {
+  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, const float*) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+__device__ __forceinline__ uint32_t word_max_nan(uint32_t a, uint32_t b, const __nv_bfloat16*) {
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t word_max_nan(uint32_t a, uint32_t b, const __half*) {
+  const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t word_max_nan(uint32_t a, uint32_t b, const float*) {
+  return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+}
+
+// Largest value of NW words; NaN is passed over (all NaN: NaN).
+template <typename T, int NW>
+__device__ __forceinline__ float words_max(const uint32_t (&w)[NW]) {
+  uint32_t m = w[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) m = word_max(m, w[i], (const T*)nullptr);
+  if constexpr (sizeof(T) == 4) return __uint_as_float(m);
+  else {
+    const float2 v = unpack2(m, (const T*)nullptr);
+    return fmaxf(v.x, v.y);
+  }
+}
+
+// Pairs of values: pair i of NW words (16-bit: word i; fp32: words 2 i and 2 i + 1).
+template <typename T, int NW>
+__device__ __forceinline__ float2 word_pair(const uint32_t (&w)[NW], int i) {
+  if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  else return unpack2(w[i], (const T*)nullptr);
+}
+
+// Where a product of e = 2^(kl (x - mu)) with x - mu is formed, -inf has to be raised to a finite
+// value whose e is still 0: to `floor`, which the type represents.  Holds where mu lies far enough
+// above it (and below what a difference could overflow from); elsewhere the terms are cut off one
+// by one.
+template <typename T>
+__device__ __forceinline__ float raise_floor() {
+  return sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? -65504.f : -1.0e30f;
+}
+template <typename T>
+__device__ __forceinline__ bool can_raise(float mu, const Squash& q) {
+  return (mu - raise_floor<T>()) * q.kl > 200.f && mu < 1e30f;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t floor_word() {
+  if constexpr (sizeof(T) == 4) return __float_as_uint(raise_floor<T>());
+  else return pack2(raise_floor<T>(), raise_floor<T>(), (const T*)nullptr);
+}
+
+// ---------------------------------------------------------------------------
 // Running softmax statistics of a set of logits
 // ---------------------------------------------------------------------------
 //   m   largest x (before squash; -inf for an empty set, NaN is passed over)
 //   mu  what exponents are taken against: squash(m), or 0 where m is -inf
 //   s   sum of e = 2^(kl (y - mu))
-//   w   sum of e * kl (y - mu)    (entropy only)
+//   w   sum of e * (y - mu)    (entropy only)
 // y - mu is formed before the scaling: the product with kl of a number near the type's lowest
-// value would overflow, and a fused x * kl - mu * kl would turn that into NaN.  A -inf logit
-// adds nothing (its term of w is cut off at a finite exponent); a NaN reaches s.
+// value would overflow, and a fused x * kl - mu * kl would turn that into NaN (and rounds mu * kl,
+// an error that every term shares).  A -inf logit adds nothing; a NaN reaches s.
 template <bool CAP, bool ENT>
 struct RowStats {
   float m, mu, s, w;
@@ -174,8 +248,8 @@ struct RowStats {
   __device__ __forceinline__ void rebase(float mn, const Squash& q) {
     const float nu = CAP ? squash<CAP>(mn, q) : mn;
     if (m != -INFINITY) {  // there s is 0 or NaN
-      const float d = fmaxf((mu - nu) * q.kl, -1e30f);
-      const float f = ex2(d);
+      const float d = fmaxf(mu - nu, -1e30f);
+      const float f = ex2(d * q.kl);
       if constexpr (ENT) w = f * fmaf(d, s, w);
       s *= f;
     }
@@ -197,24 +271,59 @@ struct RowStats {
     static_assert(N % 2 == 0 || N == 1, "pairs");
     if (lm > m) rebase(lm, q);
     if constexpr (N == 1) {
-      const float d = (squash<CAP>(x[0], q) - mu) * q.kl;
-      const float e = ex2(d);
+      const float d = squash<CAP>(x[0], q) - mu;
+      const float e = ex2(d * q.kl);
       s += e;
-      if constexpr (ENT) w = fmaf(e, fmaxf(d, -1e4f), w);
+      if constexpr (ENT) w = fmaf(e, fmaxf(d, -1e30f), w);
     } else {
       const float2 nmu = make_float2(-mu, -mu), kl = make_float2(q.kl, q.kl);
       float2 s2 = make_float2(s, 0.f), w2 = make_float2(w, 0.f);
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
         const float2 y = make_float2(squash<CAP>(x[i], q), squash<CAP>(x[i + 1], q));
-        const float2 d = __fmul2_rn(__fadd2_rn(y, nmu), kl);
-        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+        const float2 d = __fadd2_rn(y, nmu);
+        const float2 a = __fmul2_rn(d, kl);
+        const float2 e = make_float2(ex2(a.x), ex2(a.y));
         s2 = __fadd2_rn(s2, e);
-        if constexpr (ENT) w2 = __ffma2_rn(e, make_float2(fmaxf(d.x, -1e4f), fmaxf(d.y, -1e4f)), w2);
+        if constexpr (ENT) w2 = __ffma2_rn(e, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), w2);
       }
       s = s2.x + s2.y;
       if constexpr (ENT) w = w2.x + w2.y;
     }
+  }
+
+  // NW words as they lie in memory, lm their largest value.  Two elements at a time: 4 (with the
+  // entropy 5) instructions an element for 16-bit types.
+  template <typename T, int NW>
+  __device__ __forceinline__ void add_words(const uint32_t (&w_)[NW], float lm, const Squash& q) {
+    constexpr int P = NW * elems_per_word<T>() / 2;
+    if (CAP || (ENT && !can_raise<T>(fmaxf(m, lm), q))) {
+      float x[2 * P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float2 v = word_pair<T>(w_, i);
+        x[2 * i] = v.x;
+        x[2 * i + 1] = v.y;
+      }
+      add(x, lm, q);
+      return;
+    }
+    if (lm > m) rebase(lm, q);
+    const float2 nmu = make_float2(-mu, -mu), kl = make_float2(q.kl, q.kl);
+    float2 s2 = make_float2(s, 0.f), w2 = make_float2(w, 0.f);
+    uint32_t x[NW];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) x[i] = ENT ? word_max_nan(w_[i], floor_word<T>(), (const T*)nullptr) : w_[i];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float2 d = __fadd2_rn(word_pair<T>(x, i), nmu);
+      const float2 a = __fmul2_rn(d, kl);
+      const float2 e = make_float2(ex2(a.x), ex2(a.y));
+      s2 = __fadd2_rn(s2, e);
+      if constexpr (ENT) w2 = __ffma2_rn(e, d, w2);
+    }
+    s = s2.x + s2.y;
+    if constexpr (ENT) w = w2.x + w2.y;
   }
 
   // Adds the statistics of another set.

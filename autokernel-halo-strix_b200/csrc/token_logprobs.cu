@@ -25,7 +25,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 128;         // alternatives
 constexpr int kMaxCluster = 8;       // the portable cluster size
-constexpr int kMaxGroupKeys = 8194;  // group maxima of one CTA's share (32 KB), head and tail included
+constexpr int kMaxGroupMax = 8194;  // group maxima of one CTA's share (32 KB), head and tail included
 constexpr int kCandGroups = 512;     // candidates of the short way through the selection
 constexpr int kCandElems = 768;
 
@@ -68,17 +68,18 @@ struct SelectScratch {
   uint32_t ngroups, nelems;
 };
 
-// The first k of n keys in the order (key descending, position ascending): their positions,
-// ascending, in out.  Needs n >= k.  A binary search over the key's bits for the k-th largest,
+// The first k of the n keys key(0 .. n - 1) in the order (key descending, position ascending):
+// their positions, ascending, in out.  Needs n >= k.  A binary search over the key's bits for the k-th largest,
 // then everything above it and the first of those equal to it.
-__device__ void select_exact(const uint32_t* keys, int n, int k, uint32_t* out, SelectScratch& sc) {
+template <typename Key>
+__device__ void select_exact(Key key_at, int n, int k, uint32_t* out, SelectScratch& sc) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t t = 0;
   int above = 0;  // number of keys > t, known at the end
   for (int bit = 31; bit >= -1; --bit) {
     const uint32_t probe = bit >= 0 ? (t | (1u << bit)) : t;
     int c = 0;
-    for (int i = tid; i < n; i += kThreads) c += bit >= 0 ? (keys[i] >= probe) : (keys[i] > probe);
+    for (int i = tid; i < n; i += kThreads) c += bit >= 0 ? (key_at(i) >= probe) : (key_at(i) > probe);
     c = __reduce_add_sync(0xffffffffu, c);
     if (lane == 0) sc.warp_n[0][warp] = (uint32_t)c;
     __syncthreads();
@@ -93,7 +94,7 @@ __device__ void select_exact(const uint32_t* keys, int n, int k, uint32_t* out, 
   int taken = 0, equal_seen = 0;
   for (int i0 = 0; i0 < n; i0 += kThreads) {
     const int i = i0 + tid;
-    const uint32_t key = i < n ? keys[i] : 0u;
+    const uint32_t key = i < n ? key_at(i) : 0u;
     const bool eq = i < n && key == t;
     const uint32_t eq_ballot = __ballot_sync(0xffffffffu, eq);
     if (lane == 0) sc.warp_n[0][warp] = __popc(eq_ballot);
@@ -127,31 +128,33 @@ __device__ __forceinline__ uint64_t entry(uint32_t key, int index) {
   return ((uint64_t)key << 32) | (uint32_t)(~(uint32_t)index);
 }
 
-// The k best elements of the share, best first, in top[0 .. k).  gkeys holds the n + 2 group
-// maxima (a barrier has passed since they were written), mine the largest key this thread wrote.
+// The k best elements of the share, best first, in top[0 .. k).  gmax holds the n + 2 group maxima
+// (a barrier has passed since they were written), mine the largest element this thread has seen.
 template <typename T>
-__device__ void select_top(uint64_t* top, const Share<T>& sh, const uint32_t* gkeys, uint32_t mine, int k,
+__device__ void select_top(uint64_t* top, const Share<T>& sh, const float* gmax, float mine, int k,
                            SelectScratch& sc) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // A lower bound of the k-th best group: each warp's j-th largest thread maximum, j = ceil(k /
-  // warps), and the smallest of these; at least warps * j >= k groups reach it.
+  // A lower bound of the k-th best element: each warp's j-th largest thread maximum, j = ceil(k /
+  // warps), and the smallest of these; at least warps * j >= k elements reach it.
   const int j = (k + kWarps - 1) / kWarps;
-  uint32_t v = mine, bound = 0;
+  uint32_t v = order_key(mine), bkey = 0;
   for (int i = 0; i < j; ++i) {
-    bound = __reduce_max_sync(0xffffffffu, v);
-    const uint32_t at = __ballot_sync(0xffffffffu, v == bound);
+    bkey = __reduce_max_sync(0xffffffffu, v);
+    const uint32_t at = __ballot_sync(0xffffffffu, v == bkey);
     if (lane == __ffs(at) - 1) v = 0;
   }
-  if (lane == 0) sc.warp_n[0][warp] = bound;
+  if (lane == 0) sc.warp_n[0][warp] = bkey;
   if (tid == 0) { sc.ngroups = 0; sc.nelems = 0; }
   __syncthreads();
-  bound = sc.warp_n[0][0];
+  bkey = sc.warp_n[0][0];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) bound = min(bound, sc.warp_n[0][w]);
-  bound = max(bound, 1u);  // key 0 is no value
+  for (int w = 1; w < kWarps; ++w) bkey = min(bkey, sc.warp_n[0][w]);
+  // -inf is also what a thread has that saw no number: then every element is a candidate
+  const bool all = bkey <= order_key(-INFINITY);
+  const float bound = key_value(bkey);
   const int ng = sh.n + 2;
   for (int i = tid; i < ng; i += kThreads) {
-    if (gkeys[i] >= bound) {
+    if (gmax[i] >= bound || all) {
       const uint32_t at = atomicAdd(&sc.ngroups, 1u);
       if (at < kCandGroups) sc.cand.groups[at] = (uint32_t)i;
     }
@@ -160,26 +163,37 @@ __device__ void select_top(uint64_t* top, const Share<T>& sh, const uint32_t* gk
   const uint32_t ncg = sc.ngroups;
   bool exact = ncg > kCandGroups;
   if (!exact) {
-    for (int i = tid; i < (int)ncg * kGroup; i += kThreads) {
-      const int g = (int)sc.cand.groups[i / kGroup], e = i % kGroup;
-      if (e < sh.size(g)) {
-        const int idx = sh.start(g) + e;
-        const uint32_t key = order_key(to_f<T>(sh.row[idx]));
-        if (key >= bound) {
+    for (int i = tid; i < (int)ncg; i += kThreads) {
+      const int g = (int)sc.cand.groups[i], first = sh.start(g);
+      auto offer = [&](float x, int idx) {
+        if (x >= bound || all) {
           const uint32_t at = atomicAdd(&sc.nelems, 1u);
-          if (at < kCandElems) sc.cand.elems[at] = entry(key, idx);
+          if (at < kCandElems) sc.cand.elems[at] = entry(order_key(x), idx);
         }
+      };
+      if (g >= 1 && g <= sh.n) {
+        float x[kGroup];
+        unpack_group<T>(x, load_group<T>(sh.row + first));
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) offer(x[e], first + e);
+      } else {
+        for (int e = 0; e < sh.size(g); ++e) offer(to_f<T>(sh.row[first + e]), first + e);
       }
     }
     __syncthreads();
     exact = sc.nelems > kCandElems;
   }
   if (!exact) {
+    // the position of each candidate is the number of better ones
     const int ne = (int)sc.nelems;
     for (int i = tid; i < ne; i += kThreads) {
       const uint64_t e = sc.cand.elems[i];
-      int rank = 0;
-      for (int o = 0; o < ne; ++o) rank += sc.cand.elems[o] > e;
+      int rank = 0, o = 0;
+      for (; o + 4 <= ne; o += 4) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) rank += sc.cand.elems[o + u] > e;
+      }
+      for (; o < ne; ++o) rank += sc.cand.elems[o] > e;
       if (rank < k) top[rank] = e;
     }
     __syncthreads();
@@ -188,7 +202,7 @@ __device__ void select_top(uint64_t* top, const Share<T>& sh, const uint32_t* gk
   // Many equal values (masked or constant rows): choose the k groups, then the k elements, exactly.
   __syncthreads();
   const int kg = min(k, ng);
-  select_exact(gkeys, ng, kg, sc.chosen, sc);
+  select_exact([&](int i) { return sh.size(i) ? order_key(gmax[i]) : 0u; }, ng, kg, sc.chosen, sc);
   for (int i = tid; i < kg * kGroup; i += kThreads) {
     const int g = (int)sc.chosen[i / kGroup], e = i % kGroup;
     sc.keys[i] = e < sh.size(g) ? order_key(to_f<T>(sh.row[sh.start(g) + e])) : 0u;
@@ -198,19 +212,19 @@ __device__ void select_top(uint64_t* top, const Share<T>& sh, const uint32_t* gk
   __shared__ uint32_t groups[kMaxTop];
   for (int i = tid; i < kg; i += kThreads) groups[i] = sc.chosen[i];
   __syncthreads();
-  select_exact(sc.keys, kg * kGroup, k, sc.chosen, sc);
+  select_exact([&](int i) { return sc.keys[i]; }, kg * kGroup, k, sc.chosen, sc);
   uint64_t e = 0;
   if (tid < k) {
     const int at = (int)sc.chosen[tid], g = (int)groups[at / kGroup];
     e = entry(sc.keys[at], sh.start(g) + at % kGroup);
   }
   __syncthreads();
-  uint64_t* all = sc.cand.elems;  // the keys have been read
-  if (tid < k) all[tid] = e;
+  uint64_t* list = sc.cand.elems;  // the keys have been read
+  if (tid < k) list[tid] = e;
   __syncthreads();
   if (tid < k) {
     int rank = 0;
-    for (int o = 0; o < k; ++o) rank += all[o] > e;
+    for (int o = 0; o < k; ++o) rank += list[o] > e;
     top[rank] = e;
   }
   __syncthreads();
@@ -236,8 +250,9 @@ template <typename T, bool CAP, bool ENT, bool TOP>
 __global__ void __launch_bounds__(kThreads)
 token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
   using Stats = RowStats<CAP, ENT>;
-  extern __shared__ uint32_t gkeys[];  // TOP: group maxima
+  extern __shared__ float gmax[];      // TOP: group maxima
   __shared__ Stats s_warp[kWarps];
+  __shared__ Stats s_cta;
   __shared__ float s_share[4];         // this CTA's statistics, read by the others of the cluster
   __shared__ uint64_t s_top[TOP ? kMaxTop : 1];
   __shared__ __align__(8) unsigned char s_scratch[TOP ? sizeof(SelectScratch) : 8];
@@ -260,41 +275,23 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
 
   Stats st;
   st.init();
-  uint32_t mine = 0;
   const T* body = row + cut.head + (int64_t)sh.g0 * kGroup;
+  auto group = [&](const RawGroup<T>& raw, int g) {
+    float lm = words_max<T>(raw.r[0].w);
+    if constexpr (sizeof(T) == 4) lm = fmaxf(lm, words_max<T>(raw.r[1].w));
+    if constexpr (TOP) gmax[1 + g] = lm;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) st.template add_words<T>(raw.r[i].w, lm, q);
+  };
   int g = tid;
   for (; g + (kBatch - 1) * kThreads < sh.n; g += kBatch * kThreads) {
     RawGroup<T> raw[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) raw[u] = load_group<T>(body + (int64_t)(g + u * kThreads) * kGroup);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      float x[kGroup];
-      unpack_group<T>(x, raw[u]);
-      float lm = x[0];
-#pragma unroll
-      for (int i = 1; i < kGroup; ++i) lm = fmaxf(lm, x[i]);
-      if constexpr (TOP) {
-        const uint32_t key = order_key(lm);
-        gkeys[1 + g + u * kThreads] = key;
-        mine = max(mine, key);
-      }
-      st.add(x, lm, q);
-    }
+    for (int u = 0; u < kBatch; ++u) group(raw[u], g + u * kThreads);
   }
-  for (; g < sh.n; g += kThreads) {
-    float x[kGroup];
-    unpack_group<T>(x, load_group<T>(body + (int64_t)g * kGroup));
-    float lm = x[0];
-#pragma unroll
-    for (int i = 1; i < kGroup; ++i) lm = fmaxf(lm, x[i]);
-    if constexpr (TOP) {
-      const uint32_t key = order_key(lm);
-      gkeys[1 + g] = key;
-      mine = max(mine, key);
-    }
-    st.add(x, lm, q);
-  }
+  for (; g < sh.n; g += kThreads) group(load_group<T>(body + (int64_t)g * kGroup), g);
   // head and tail: one element a lane of the first and the last warp
   if (warp == 0 || warp == kWarps - 1) {
     const bool first = warp == 0;
@@ -307,21 +304,26 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
     }
     if constexpr (TOP) {
       const uint32_t best = __reduce_max_sync(0xffffffffu, key);
-      if (lane == 0) {
-        gkeys[first ? 0 : sh.n + 1] = best;
-        mine = max(mine, best);
-      }
+      if (lane == 0) gmax[first ? 0 : sh.n + 1] = key_value(best);
     }
   }
+  const float mine = st.m;
   st.warp_merge(q);
   if (lane == 0) s_warp[warp] = st;
   __syncthreads();
-  st = s_warp[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) st.merge(s_warp[w], q);
+  if (warp == 0) {
+    st.init();
+    if (lane < kWarps) st = s_warp[lane];
+    st.warp_merge(q);
+    if (lane == 0) s_cta = st;
+  }
+  if (TOP || cs > 1) {
+    __syncthreads();
+    st = s_cta;
+  }
   const int kl = TOP ? min(a.k, sh.elems()) : 0;
   if constexpr (TOP)
-    if (kl > 0) select_top<T>(s_top, sh, gkeys, mine, kl, *reinterpret_cast<SelectScratch*>(s_scratch));
+    if (kl > 0) select_top<T>(s_top, sh, gmax, mine, kl, *reinterpret_cast<SelectScratch*>(s_scratch));
   if (cs > 1) {
     if (tid == 0) {
       s_share[0] = st.m;
@@ -378,7 +380,7 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
       a.logprobs[r] = lp;
     }
     if constexpr (ENT)
-      a.entropy[r] = (ignored || st.s == 0.f) ? 0.f : logs - kLn2 * (st.w / st.s);
+      a.entropy[r] = (ignored || st.s == 0.f) ? 0.f : logs - (st.w / st.s) * q.inv_t;
     if (a.lse) a.lse[r] = st.mu * q.inv_t + logs;
     if (a.stats) a.stats[r] = make_float2(st.mu, logs);
   }
@@ -419,18 +421,23 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
   float gl = (a.targets && a.g_lp) ? a.g_lp[r] : 0.f;
   if (a.targets && !none && (t < 0 || t >= a.V)) gl = NAN;
   const float ge = ENT ? a.g_ent[r] : 0.f, H = ENT ? a.entropy[r] : 0.f;
-  // d = (y - mu) kl - log2 S; p = 2^d; dx = p (c0 + c1 d) (+ gl at the target), all times 1 / T
+  // d = y - mu, p = 2^(d kl - log2 S), log p = d / T - log S:
+  // dx = p (c0 + c1 d) (+ gl / T at the target), times the softcap's slope
   const float l2s = ml.y * kLog2e;
-  const float c0 = -(gl + ge * H) * q.inv_t, c1 = -ge * kLn2 * q.inv_t, ct = gl * q.inv_t;
+  const float c0 = (ge * (ml.y - H) - gl) * q.inv_t, c1 = -ge * q.inv_t * q.inv_t, ct = gl * q.inv_t;
+  const int ti = (a.targets && t >= 0 && t < a.V) ? (int)t : -1;
 
   auto one = [&](float x, int i) {
     const float y = squash<CAP>(x, q);
-    const float d = (y - ml.x) * q.kl - l2s;
-    float o = ex2(d);
-    o *= ENT ? fmaf(c1, fmaxf(d, -1e4f), c0) : c0;
-    if (i == (int)t) o += ct;
+    const float d = y - ml.x;
+    float o = ex2(fmaf(d, q.kl, -l2s));
+    o *= ENT ? fmaf(c1, fmaxf(d, -1e30f), c0) : c0;
+    if (i == ti) o += ct;
     return o * squash_slope<CAP>(y, q);
   };
+  const bool quick = !CAP && (!ENT || can_raise<T>(ml.x, q));
+  const float2 nmu = make_float2(-ml.x, -ml.x), kl = make_float2(q.kl, q.kl), nl2s = make_float2(-l2s, -l2s);
+  const float2 c02 = make_float2(c0, c0), c12 = make_float2(c1, c1);
 
   const int gbeg = seg * kBwdGroups;
   const T* body = row + cut.head;
@@ -446,9 +453,37 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
     const int g = gbeg + u * kThreads + tid;
     if (g < cut.groups) {
       float x[kGroup];
-      unpack_group<T>(x, raw[u]);
+      if (none) {
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) x[i] = none ? 0.f : one(x[i], cut.head + g * kGroup + i);
+        for (int i = 0; i < kGroup; ++i) x[i] = 0.f;
+      } else if (quick) {
+        constexpr int W = 8, P = W * elems_per_word<T>() / 2;  // pairs of one 32-byte piece
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+          uint32_t w[W];
+#pragma unroll
+          for (int i = 0; i < W; ++i)
+            w[i] = ENT ? word_max_nan(raw[u].r[h].w[i], floor_word<T>(), (const T*)nullptr) : raw[u].r[h].w[i];
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const float2 d = __fadd2_rn(word_pair<T>(w, i), nmu);
+            const float2 e = __ffma2_rn(d, kl, nl2s);
+            const float2 o = __fmul2_rn(make_float2(ex2(e.x), ex2(e.y)), ENT ? __ffma2_rn(c12, d, c02) : c02);
+            x[h * 2 * P + 2 * i] = o.x;
+            x[h * 2 * P + 2 * i + 1] = o.y;
+          }
+        }
+        const int at = ti - (cut.head + g * kGroup);
+        if ((unsigned)at < (unsigned)kGroup) {
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i)
+            if (i == at) x[i] += ct;
+        }
+      } else {
+        unpack_group<T>(x, raw[u]);
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) x[i] = one(x[i], cut.head + g * kGroup + i);
+      }
       store_group<T>(gbody + (int64_t)g * kGroup, x, vec);
     }
   }
@@ -464,7 +499,7 @@ int cluster_for(int64_t rows, int64_t V, bool top) {
   int cs = 1;
   while (cs < kMaxCluster && rows * cs * 2 <= sm_count() * 2 && V / (2 * cs) >= kThreads * kGroup / 2) cs *= 2;
   if (top)
-    while (cs < kMaxCluster && (V / kGroup) / cs + 2 > kMaxGroupKeys - 2) cs *= 2;
+    while (cs < kMaxCluster && (V / kGroup) / cs + 2 > kMaxGroupMax - 2) cs *= 2;
   return cs;
 }
 
@@ -510,7 +545,7 @@ extern "C" int ak_token_logprobs_fwd(float* logprobs, float* entropy, float* lse
   if (rc) return rc;
   AK_REQUIRE(k >= 0 && k <= kMaxTop && k <= V, AK_ERR_SHAPE,
              "ak_token_logprobs_fwd: top_k %lld must be at most %d and at most the vocabulary", (long long)k, kMaxTop);
-  AK_REQUIRE(k == 0 || V <= (int64_t)kMaxCluster * kGroup * (kMaxGroupKeys - 4), AK_ERR_SHAPE,
+  AK_REQUIRE(k == 0 || V <= (int64_t)kMaxCluster * kGroup * (kMaxGroupMax - 4), AK_ERR_SHAPE,
              "ak_token_logprobs_fwd: vocabulary of %lld too large for top_k", (long long)V);
   if (rows == 0) return AK_OK;
   AK_REQUIRE((k == 0) || (top_lp && top_idx), AK_ERR_ARG, "ak_token_logprobs_fwd: null top_lp or top_idx");

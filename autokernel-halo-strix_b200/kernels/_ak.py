@@ -9,6 +9,7 @@ and the shared library must be present, otherwise the call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from pathlib import Path
 from typing import Optional, Sequence
@@ -110,7 +111,7 @@ def lib() -> ctypes.CDLL:
 
 
 def call(name: str, *args) -> None:
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
         msg = lib().ak_last_error().decode(errors="replace")
         raise AkError(f"{name} failed (status {rc}): {msg}")
@@ -124,11 +125,12 @@ def dtype_code(t: torch.Tensor) -> int:
 
 
 def ptr(t: Optional[torch.Tensor]):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()  # ctypes converts an int to the declared void pointer
 
 
 def stream(device: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """PyTorch's current stream of `device`: the raw handle, without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
 
 
 def require_cuda(*tensors: Optional[torch.Tensor]) -> torch.device:
@@ -151,6 +153,7 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
 
 
+@functools.lru_cache(maxsize=1024)
 def _size_query(name: str, *dims: int) -> int:
     out = ctypes.c_size_t(0)
     call(name, *dims, ctypes.byref(out))
@@ -177,6 +180,7 @@ class _StatusWords:
         with torch.cuda.device(device):
             call("ak_status_device_pointer", ctypes.c_void_p(self.host.data_ptr()), ctypes.byref(dev_ptr))
         self.base = int(dev_ptr.value)
+        self.words = (ctypes.c_int32 * len(STATUS_SLOTS)).from_address(self.host.data_ptr())  # the same memory
 
     def raise_if_set(self, slots) -> None:
         for i in slots:
@@ -206,8 +210,9 @@ def status_ptr(device: torch.device, slot: str):
     family reported a timeout."""
     sw = _status_words(device)
     i = STATUS_SLOTS.index(slot)
-    sw.raise_if_set((i,))
-    return ctypes.c_void_p(sw.base + 4 * i)
+    if sw.words[i]:
+        sw.raise_if_set((i,))
+    return sw.base + 4 * i
 
 
 def check_status(device: Optional[torch.device] = None, synchronize: bool = True) -> None:
@@ -592,7 +597,7 @@ def ce_inv_valid(targets: torch.Tensor, ignore_index: int = -100) -> torch.Tenso
 # ---------------------------------------------------------------------------
 def call_on(device: torch.device, name: str, *args) -> None:
     """`call` with `device` current, which a launch on one of its streams needs."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == torch._C._cuda_getDevice():
         call(name, *args)
     else:
         with torch.cuda.device(device):
