@@ -49,34 +49,34 @@ struct DistillArgs {
   int* status;
 };
 
-// Sum over the CTA in a fixed order, the same on every thread.
-__device__ __forceinline__ float block_sum(float v, float* s_red) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) t += s_red[w];
-  return t;
-}
-__device__ __forceinline__ float block_max(float v, float* s_red) {
-  v = warp_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = s_red[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) t = fmaxf(t, s_red[w]);
-  return t;
-}
-
 // The gradient at a logit outside the teacher's tokens.  c = 0 gives 0 whatever x is.
 template <bool CAP>
 __device__ __forceinline__ float rest_grad(float x, float mu, float c, const Squash& q) {
   if (c == 0.f) return 0.f;
   const float y = squash<CAP>(x, q);
   return ex2((y - mu) * q.kl) * c * squash_slope<CAP>(y, q);
+}
+
+// The same for the values of NW words, two at a time without softcap.
+template <typename T, bool CAP, int NW>
+__device__ __forceinline__ void rest_grads(float* x, const uint32_t (&w)[NW], float mu, float c, const Squash& q) {
+  constexpr int P = NW * elems_per_word<T>() / 2;
+  const float2 nmu = make_float2(-mu, -mu), kl = make_float2(q.kl, q.kl), c2 = make_float2(c, c);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const float2 v = word_pair<T>(w, i);
+    float2 o;
+    if constexpr (CAP) {
+      o = make_float2(rest_grad<CAP>(v.x, mu, c, q), rest_grad<CAP>(v.y, mu, c, q));
+    } else if (c == 0.f) {
+      o = make_float2(0.f, 0.f);
+    } else {
+      const float2 d = __fmul2_rn(__fadd2_rn(v, nmu), kl);
+      o = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), c2);
+    }
+    x[2 * i] = o.x;
+    x[2 * i + 1] = o.y;
+  }
 }
 
 template <typename T, bool CAP, bool GRAD>
@@ -88,8 +88,8 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
   T* s_row = reinterpret_cast<T*>(s_row_raw);
   __shared__ __align__(8) uint64_t s_bar;
   __shared__ Stats s_warp[kWarps];
-  __shared__ float s_red[kWarps];
-  __shared__ float s_share[2];
+  __shared__ float s_share[2];     // this CTA's statistics, read by the others of the cluster
+  __shared__ float s_out[2];       // (mu_rest, c * scale) for the gradient
   __shared__ float s_edge[2][32];  // head and tail of the row
   __shared__ int s_idx[kMaxK];
   __shared__ float s_q[kMaxK];
@@ -140,92 +140,134 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
     for (uint32_t o = 0; o < bytes; o += kCopyBytes)
       bulk_g2s(s_row_raw + o, src + o, min(kCopyBytes, bytes - o), &s_bar);
   }
-  if (warp == 0 && lane < head_here) s_edge[0][lane] = to_f<T>(row[lane]);
-  if (warp == 1 && lane < tail_here) s_edge[1][lane] = to_f<T>(row[tail0 + lane]);
+  if (warp == 1 && lane < head_here) s_edge[0][lane] = to_f<T>(row[lane]);
+  if (warp == 2 && lane < tail_here) s_edge[1][lane] = to_f<T>(row[tail0 + lane]);
+  __syncthreads();
 
-  // ---- the teacher's entries: one a thread.  A negative index is padding.
-  int idx = -1;
-  float t = -INFINITY, yk = -INFINITY;
-  bool bad = false;
-  if (tid < a.K) {
-    const int64_t i = a.idx[r * a.K + tid];
-    bad = i >= a.V;
-    if (i >= 0 && !bad) {
-      idx = (int)i;
-      t = a.tlp[r * a.K + tid];
-      yk = squash<CAP>(to_f<T>(row[idx]), q);
-    }
-    s_idx[tid] = idx;
-  }
-  bad = __syncthreads_or(bad) != 0;
-  const bool any = __syncthreads_or(idx >= 0) != 0;
-  float qk, logq;
-  if (a.tail) {
-    qk = idx >= 0 ? expf(t) : 0.f;
-    logq = t;
-  } else {
-    const float tm = block_max(t, s_red);
-    const float e = (idx >= 0 && tm != -INFINITY) ? expf(t - tm) : 0.f;
-    const float z = block_sum(e, s_red);
-    qk = z == 0.f ? 0.f : e / z;  // z: 0 without entries, NaN kept
-    logq = t - tm - logf(z);
-  }
-  if (tid < a.K) s_q[tid] = qk;
-  const float qsum = block_sum(qk, s_red);
-  const bool none = a.tail ? !any : qsum == 0.f;  // no teacher: loss 0, no gradient
-  const float rest = a.tail ? fmaxf(1.f - qsum, 0.f) : 0.f;
-  // entries of one token: its logit counts once, their masses add up
-  bool first = idx >= 0;
-  float mass = 0.f;
-  if (idx >= 0) {
-    for (int j = 0; j < a.K; ++j) {
-      if (s_idx[j] == idx) {
-        if (j < tid) first = false;
-        mass += s_q[j];
+  // ---- the teacher's entries, all on the first warp: entry 32 j + lane in slot j.  A negative
+  // index is padding.
+  constexpr int S = kMaxK / 32;
+  int idx[S];
+  float yk[S], qk[S], logq[S], mass[S];
+  Stats top;  // the teacher's tokens
+  top.init();
+  bool bad = false, none = false;
+  float rest = 0.f;
+  if (warp == 0) {
+    float t[S], xk[S];
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      const int k = 32 * j + lane;
+      idx[j] = -1;
+      t[j] = yk[j] = xk[j] = -INFINITY;
+      if (k < a.K) {
+        const int64_t i = a.idx[r * a.K + k];
+        bad |= i >= a.V;
+        if (i >= 0 && i < a.V) {
+          idx[j] = (int)i;
+          t[j] = a.tlp[r * a.K + k];
+          xk[j] = to_f<T>(row[i]);
+          yk[j] = squash<CAP>(xk[j], q);
+          any = true;
+        }
       }
     }
-  }
-  Stats top;
-  top.init();
-  if (first) {
-    const float x[1] = {to_f<T>(row[idx])};
-    top.add(x, q);
-  }
-  top.warp_merge(q);
-  if (lane == 0) s_warp[warp] = top;
-  __syncthreads();
-  top = s_warp[0];
+    bad = __any_sync(0xffffffffu, bad);
+    any = __any_sync(0xffffffffu, any);
+    float qsum = 0.f;
+    if (a.tail) {
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) top.merge(s_warp[w], q);
+      for (int j = 0; j < S; ++j) {
+        qk[j] = idx[j] >= 0 ? expf(t[j]) : 0.f;
+        logq[j] = t[j];
+        qsum += qk[j];
+      }
+      qsum = warp_sum(qsum);
+    } else {
+      float tm = t[0], z = 0.f;
+#pragma unroll
+      for (int j = 1; j < S; ++j) tm = fmaxf(tm, t[j]);
+      tm = warp_max(tm);
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        qk[j] = (idx[j] >= 0 && tm != -INFINITY) ? expf(t[j] - tm) : 0.f;
+        z += qk[j];
+      }
+      z = warp_sum(z);
+      const float logz = logf(z);
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        qk[j] = z == 0.f ? 0.f : qk[j] / z;  // z: 0 without entries, NaN kept
+        logq[j] = t[j] - tm - logz;
+        qsum += qk[j];
+      }
+      qsum = warp_sum(qsum);
+    }
+    none = a.tail ? !any : qsum == 0.f;  // no teacher: loss 0, no gradient
+    rest = a.tail ? fmaxf(1.f - qsum, 0.f) : 0.f;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      mass[j] = 0.f;
+      s_idx[32 * j + lane] = idx[j];
+      s_q[32 * j + lane] = qk[j];
+    }
+    __syncwarp();
+    // entries of one token: its logit counts once, at the first of them; their masses add up
+    uint32_t later = 0;
+    for (int m = 0; m < a.K; ++m) {
+      const int im = s_idx[m];
+      const float qm = s_q[m];
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        if (32 * j < a.K && idx[j] == im) {
+          mass[j] += qm;
+          if (m < 32 * j + lane) later |= 1u << j;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      if (idx[j] >= 0 && !(later >> j & 1u)) {
+        const float x[1] = {xk[j]};
+        top.add(x, q);
+      }
+    }
+    top.warp_merge(q);
+    // out of the row, once it is here
+    mbar_wait_bounded(&s_bar, 0u, a.status);
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      const int i = idx[j];
+      if (i < 0) continue;
+      if (i >= body0 && i < body0 + n) s_row[i - body0] = from_f<T>(-INFINITY);
+      else if (i < head_here) s_edge[0][i] = -INFINITY;
+      else if (i >= tail0 && i - tail0 < tail_here) s_edge[1][i - tail0] = -INFINITY;
+    }
+  }
+  __syncthreads();
 
   // ---- the rest of the row
-  mbar_wait_bounded(&s_bar, 0u, a.status);
-  if (idx >= 0) {
-    if (idx >= body0 && idx < body0 + n) s_row[idx - body0] = from_f<T>(-INFINITY);
-    else if (idx < head_here) s_edge[0][idx] = -INFINITY;
-    else if (idx >= tail0 && idx - tail0 < tail_here) s_edge[1][idx - tail0] = -INFINITY;
-  }
-  __syncthreads();
+  mbar_wait_bounded(&s_bar, 0u, a.status);  // complete: makes the copies visible to each thread
   Stats st;
   st.init();
-  constexpr int U = 4;
+  constexpr int U = 2;  // 16-byte pieces at a time
   const int nv = n / VEC;
+  const uint4* s_vec = reinterpret_cast<const uint4*>(s_row_raw);
   int v = tid;
   for (; v + (U - 1) * kThreads < nv; v += U * kThreads) {
-    float x[U * VEC];
+    uint32_t w[4 * U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float f[VEC];
-      load_frag<T, VEC>(f, s_row + (v + u * kThreads) * VEC);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[u * VEC + i] = f[i];
+      const uint4 f = s_vec[v + u * kThreads];
+      w[4 * u] = f.x; w[4 * u + 1] = f.y; w[4 * u + 2] = f.z; w[4 * u + 3] = f.w;
     }
-    st.add(x, q);
+    st.template add_words<T>(w, words_max<T>(w), q);
   }
   for (; v < nv; v += kThreads) {
-    float x[VEC];
-    load_frag<T, VEC>(x, s_row + v * VEC);
-    st.add(x, q);
+    const uint4 f = s_vec[v];
+    const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+    st.template add_words<T>(w, words_max<T>(w), q);
   }
   if (warp < 2 && lane < (warp == 0 ? head_here : tail_here)) {
     const float x[1] = {s_edge[warp][lane]};
@@ -234,55 +276,75 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
   st.warp_merge(q);
   if (lane == 0) s_warp[warp] = st;
   __syncthreads();
-  st = s_warp[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) st.merge(s_warp[w], q);
-  if (cs > 1) {
-    if (tid == 0) { s_share[0] = st.m; s_share[1] = st.s; }
-    row_cluster_sync();
+  if (warp == 0) {
     st.init();
-    for (int c = 0; c < cs; ++c) {  // the same order in every CTA
-      Stats o;
-      o.init();
-      const float m = __uint_as_float(ld_cluster_u32(&s_share[0], c));
-      if (m != -INFINITY) { o.m = m; o.mu = squash<CAP>(m, q); }
-      o.s = __uint_as_float(ld_cluster_u32(&s_share[1], c));
-      st.merge(o, q);
+    if (lane < kWarps) st = s_warp[lane];
+    st.warp_merge(q);
+    if (lane == 0) { s_share[0] = st.m; s_share[1] = st.s; }
+  }
+  if (cs > 1) {
+    row_cluster_sync();
+    if (warp == 0) {
+      st.init();
+      if (lane < cs) {  // every CTA joins them in the same way
+        const float m = __uint_as_float(ld_cluster_u32(&s_share[0], lane));
+        st.s = __uint_as_float(ld_cluster_u32(&s_share[1], lane));
+        if (m != -INFINITY) { st.m = m; st.mu = squash<CAP>(m, q); }
+      }
+      st.warp_merge(q);
     }
   }
 
   // ---- loss and coefficients
-  Stats all = st;
-  all.merge(top, q);
-  const float logs = logf(all.s);
-  const bool empty = all.s == 0.f;  // every logit is -inf: no distribution, no gradient
-  const float lpk = (empty || yk == -INFINITY) ? -INFINITY : (yk - all.mu) * q.inv_t - logs;
-  float term = (idx >= 0 && qk != 0.f) ? qk * (logq - lpk) : 0.f;
-  float loss = block_sum(term, s_red);
-  // the scale of p in units of e: p = e 2^(kl (mu_rest - mu)) / S
-  float c = (none || st.s == 0.f) ? 0.f : ex2((st.mu - all.mu) * q.kl) / all.s;
-  // The rest is left out where the student has masked it: no logit outside the teacher's tokens
-  // above -inf, or none within kMasked of the largest (a mask of the type's lowest value).
-  if (rest > 0.f && st.s != 0.f && !none && !(st.mu - all.mu < -kMasked)) {
-    loss += rest * (logf(rest) - ((st.mu - all.mu) * q.inv_t + logf(st.s) - logs));
-    c -= rest / st.s;
+  const float scale = GRAD ? (a.inv_n ? a.scale * *a.inv_n : a.scale) : 1.f;
+  float gk[S];
+  if (warp == 0) {
+    Stats all = st;
+    all.merge(top, q);
+    const float logs = logf(all.s);
+    const bool empty = all.s == 0.f;  // every logit is -inf: no distribution, no gradient
+    float loss = 0.f;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      const float lpk = (empty || yk[j] == -INFINITY) ? -INFINITY : (yk[j] - all.mu) * q.inv_t - logs;
+      if (idx[j] >= 0 && qk[j] != 0.f) loss += qk[j] * (logq[j] - lpk);
+      gk[j] = 0.f;
+      if (idx[j] >= 0 && !none && !empty) gk[j] = (expf(lpk) - mass[j]) * squash_slope<CAP>(yk[j], q);
+      if (bad) gk[j] = NAN;
+    }
+    loss = warp_sum(loss);
+    // the scale of p in units of e: p = e 2^(kl (mu_rest - mu)) / S
+    float c = (none || st.s == 0.f) ? 0.f : ex2((st.mu - all.mu) * q.kl) / all.s;
+    // The rest is left out where the student has masked it: no logit outside the teacher's tokens
+    // above -inf, or none within kMasked of the largest (a mask of the type's lowest value).
+    if (rest > 0.f && st.s != 0.f && !none && !(st.mu - all.mu < -kMasked)) {
+      loss += rest * (logf(rest) - ((st.mu - all.mu) * q.inv_t + logf(st.s) - logs));
+      c -= rest / st.s;
+    }
+    if (bad) { loss = NAN; c = NAN; }
+    if (lane == 0) {
+      if (rank == 0) a.losses[r] = loss;
+      s_out[0] = st.mu;
+      s_out[1] = c * scale;
+      if (!GRAD && rank == 0 && a.rest) a.rest[r] = make_float2(st.mu, c);
+    }
+    if (!GRAD && rank == 0 && a.gk) {
+#pragma unroll
+      for (int j = 0; j < S; ++j)
+        if (32 * j + lane < a.K) a.gk[r * a.K + 32 * j + lane] = gk[j];
+    }
   }
-  if (bad) { loss = NAN; c = NAN; }
-  float gk = 0.f;
-  if (idx >= 0 && !none && !empty) gk = (expf(lpk) - mass) * squash_slope<CAP>(yk, q);
-  if (bad) gk = NAN;
-  if (rank == 0 && tid == 0) a.losses[r] = loss;
 
   if constexpr (GRAD) {
-    const float scale = a.inv_n ? a.scale * *a.inv_n : a.scale;
-    const float cg = c * scale, mu = st.mu;
-    int v2 = tid;
-    for (; v2 < nv; v2 += kThreads) {
+    __syncthreads();
+    if (cs > 1) row_cluster_arrive_relaxed();  // this CTA has read the others' statistics
+    const float mu = s_out[0], cg = s_out[1];
+    for (int u = tid; u < nv; u += kThreads) {
+      const uint4 f = s_vec[u];
+      const uint32_t w[4] = {f.x, f.y, f.z, f.w};
       float x[VEC];
-      load_frag<T, VEC>(x, s_row + v2 * VEC);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] = rest_grad<CAP>(x[i], mu, cg, q);
-      T* out = grow + body0 + v2 * VEC;
+      rest_grads<T, CAP>(x, w, mu, cg, q);
+      T* out = grow + body0 + u * VEC;
       if (vec) store_frag<T, VEC>(out, x);
       else
         for (int i = 0; i < VEC; ++i) out[i] = from_f<T>(x[i]);
@@ -290,14 +352,18 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
     if (warp < 2 && lane < (warp == 0 ? head_here : tail_here))
       grow[(warp == 0 ? 0 : tail0) + lane] = from_f<T>(rest_grad<CAP>(s_edge[warp][lane], mu, cg, q));
     __syncthreads();  // the teacher's tokens over what was written for them
-    const bool mine = idx >= 0 && ((idx >= body0 && idx < body0 + n) || idx < head_here ||
-                                   (idx >= tail0 && idx - tail0 < tail_here));
-    if (mine) grow[idx] = from_f<T>(gk * scale);
-  } else if (rank == 0) {
-    if (tid == 0 && a.rest) a.rest[r] = make_float2(st.mu, c);
-    if (tid < a.K && a.gk) a.gk[r * a.K + tid] = gk;
+    if (warp == 0) {
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        const int i = idx[j];
+        if (i >= 0 && ((i >= body0 && i < body0 + n) || i < head_here || (i >= tail0 && i - tail0 < tail_here)))
+          grow[i] = from_f<T>(gk[j] * scale);
+      }
+    }
+  } else if (cs > 1) {
+    row_cluster_arrive_relaxed();
   }
-  if (cs > 1) row_cluster_sync();  // the other CTAs have read this one's statistics
+  if (cs > 1) row_cluster_wait();  // the others have read this one's
 }
 
 struct DistillBwdArgs {
@@ -322,8 +388,9 @@ template <typename T, bool CAP>
 __global__ void __launch_bounds__(kThreads)
 distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const DistillBwdArgs a) {
   const int tid = threadIdx.x;
-  const int64_t r = blockIdx.x / a.segs;
-  const int seg = (int)(blockIdx.x - r * a.segs);
+  const uint32_t r32 = blockIdx.x / (uint32_t)a.segs;
+  const int64_t r = r32;
+  const int seg = (int)(blockIdx.x - r32 * (uint32_t)a.segs);
   const Squash q = a.q;
   const T* row = logits + a.addr.off(r);
   T* grow = grad + r * a.V;
@@ -332,7 +399,7 @@ distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Dis
   const bool live = a.mask == nullptr || a.mask[r] != 0;
   const float scale = a.scale * (a.inv_n ? *a.inv_n : 1.f) * *a.g_loss;
   const float2 rc = a.rest[r];
-  const float mu = rc.x, c = rc.y * scale;
+  const float mu = rc.x, c = live ? rc.y * scale : 0.f;  // c = 0: zeros, whatever the row holds
   const int gbeg = seg * kBwdGroups;
   const T* body = row + cut.head;
   T* gbody = grow + cut.head;
@@ -347,17 +414,17 @@ distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Dis
     const int g = gbeg + u * kThreads + tid;
     if (g < cut.groups) {
       float x[kGroup];
-      unpack_group<T>(x, raw[u]);
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) x[i] = live ? rest_grad<CAP>(x[i], mu, c, q) : 0.f;
+      for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+        rest_grads<T, CAP>(x + h * 16 / ((int)sizeof(T) / 2), raw[u].r[h].w, mu, c, q);
       store_group<T>(gbody + (int64_t)g * kGroup, x, vec);
     }
   }
   const int tail0 = cut.head + cut.groups * kGroup;
   const bool first = seg == 0, last = seg == a.segs - 1;
-  if (first && tid < cut.head) grow[tid] = from_f<T>(live ? rest_grad<CAP>(to_f<T>(row[tid]), mu, c, q) : 0.f);
+  if (first && tid < cut.head) grow[tid] = from_f<T>(rest_grad<CAP>(to_f<T>(row[tid]), mu, c, q));
   if (last && tid < cut.tail)
-    grow[tail0 + tid] = from_f<T>(live ? rest_grad<CAP>(to_f<T>(row[tail0 + tid]), mu, c, q) : 0.f);
+    grow[tail0 + tid] = from_f<T>(rest_grad<CAP>(to_f<T>(row[tail0 + tid]), mu, c, q));
   if (!live) return;
   __syncthreads();
   if (tid < a.K) {

@@ -14,8 +14,9 @@ namespace ak {
 struct RowAddr {
   int64_t inner, s_outer, s_inner;
   __host__ __device__ __forceinline__ int64_t off(int64_t r) const {
-    const int64_t o = r / inner;
-    return o * s_outer + (r - o * inner) * s_inner;
+    if (r < inner) return r * s_inner;
+    const uint32_t o = (uint32_t)r / (uint32_t)inner;  // fewer than 2^27 rows
+    return (int64_t)o * s_outer + (int64_t)((uint32_t)r - o * (uint32_t)inner) * s_inner;
   }
 };
 
@@ -24,21 +25,28 @@ struct RowAddr {
 // -inf stays -inf under softcap: a masked token has no probability there either.
 struct Squash {
   float cap, inv_cap, inv_t, kl;
+  float kc;  // -2 log2(e) / cap
 };
 
 inline Squash make_squash(float temperature, float softcap) {
   Squash q;
   q.cap = softcap > 0.f ? softcap : 0.f;
   q.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
+  q.kc = softcap > 0.f ? (float)(-2.0 * 1.4426950408889634 / (double)softcap) : 0.f;
   q.inv_t = 1.f / temperature;
   q.kl = (float)(1.4426950408889634 / (double)temperature);
   return q;
 }
 
+// cap tanh(x / cap) = cap (1 - E) / (1 + E) with E = e^(-2 |x| / cap) and x's sign: two special-unit
+// operations.  With u = 2^-24, E's argument is off by 2 u relative and the hardware's exponential
+// by 4 u, which reaches tanh as 2 E / (1 + E)^2 (4 |x / cap| + 4) u <= 2.4 u; the difference, the sum
+// and the quick division add 6 u of tanh itself: at most 8 u absolute.
 template <bool CAP>
 __device__ __forceinline__ float squash(float x, const Squash& q) {
   if constexpr (!CAP) return x;
-  const float y = q.cap * tanhf(x * q.inv_cap);
+  const float e = ex2(fabsf(x) * q.kc);
+  const float y = copysignf(q.cap * __fdividef(1.f - e, 1.f + e), x);
   return x == -INFINITY ? x : y;
 }
 
@@ -355,6 +363,13 @@ __device__ __forceinline__ void row_cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// For a CTA that leaves once the others have read its shared memory: arrive after the last read of
+// theirs, without ordering any memory, and wait before the end.
+__device__ __forceinline__ void row_cluster_arrive_relaxed() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void row_cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
 // A word at the same shared-memory offset in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t ld_cluster_u32(const void* p, uint32_t rank) {
   uint32_t a, v;

@@ -28,6 +28,7 @@ constexpr int kMaxCluster = 8;       // the portable cluster size
 constexpr int kMaxGroupMax = 8194;  // group maxima of one CTA's share (32 KB), head and tail included
 constexpr int kCandGroups = 512;     // candidates of the short way through the selection
 constexpr int kCandElems = 768;
+constexpr int kBisect = 16;          // steps towards the bound at most
 
 // Unsigned keys in the order of the values: -0 and +0 are equal, NaN is below every number, 0 is
 // no value at all.
@@ -62,6 +63,10 @@ struct SelectScratch {
       uint64_t elems[kCandElems];
     } cand;
     uint32_t keys[kMaxTop * kGroup];  // the exact way: elements of the chosen groups
+    struct {                          // clusters: the lists of all CTAs, and places in the joined one
+      uint64_t lists[kMaxTop * kMaxCluster];
+      int place[kMaxTop];
+    };
   };
   uint32_t chosen[kMaxTop];  // groups, then elements, in order of position
   uint32_t warp_n[2][kWarps];
@@ -134,54 +139,74 @@ template <typename T>
 __device__ void select_top(uint64_t* top, const Share<T>& sh, const float* gmax, float mine, int k,
                            SelectScratch& sc) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // A lower bound of the k-th best element: each warp's j-th largest thread maximum, j = ceil(k /
-  // warps), and the smallest of these; at least warps * j >= k elements reach it.
-  const int j = (k + kWarps - 1) / kWarps;
-  uint32_t v = order_key(mine), bkey = 0;
-  for (int i = 0; i < j; ++i) {
-    bkey = __reduce_max_sync(0xffffffffu, v);
-    const uint32_t at = __ballot_sync(0xffffffffu, v == bkey);
-    if (lane == __ffs(at) - 1) v = 0;
-  }
-  if (lane == 0) sc.warp_n[0][warp] = bkey;
+  // A lower bound of the k-th best element: a key that at least k threads' largest elements reach,
+  // found by bisection between the smallest and the largest of those; it ends early where not many
+  // more than k do.
+  const uint32_t key = order_key(mine);
+  uint32_t lo = __reduce_min_sync(0xffffffffu, key), hi = __reduce_max_sync(0xffffffffu, key);
+  if (lane == 0) { sc.warp_n[0][warp] = lo; sc.warp_n[1][warp] = hi; }
   if (tid == 0) { sc.ngroups = 0; sc.nelems = 0; }
   __syncthreads();
-  bkey = sc.warp_n[0][0];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) bkey = min(bkey, sc.warp_n[0][w]);
+  for (int w = 0; w < kWarps; ++w) {
+    lo = min(lo, sc.warp_n[0][w]);
+    hi = max(hi, sc.warp_n[1][w]);
+  }
+  for (int i = 0; i < kBisect && lo < hi; ++i) {
+    const uint32_t probe = lo + (hi - lo + 1) / 2;
+    const int c = __syncthreads_count(key >= probe);
+    if (c < k) {
+      hi = probe - 1;
+    } else {
+      lo = probe;
+      if (c <= k + k / 8 + 2) break;
+    }
+  }
   // -inf is also what a thread has that saw no number: then every element is a candidate
-  const bool all = bkey <= order_key(-INFINITY);
-  const float bound = key_value(bkey);
+  const bool all = lo <= order_key(-INFINITY);
+  const float bound = key_value(lo);
+  // candidates: the groups that reach the bound (four maxima at a time), then their elements
   const int ng = sh.n + 2;
-  for (int i = tid; i < ng; i += kThreads) {
-    if (gmax[i] >= bound || all) {
-      const uint32_t at = atomicAdd(&sc.ngroups, 1u);
-      if (at < kCandGroups) sc.cand.groups[at] = (uint32_t)i;
+  for (int i = 4 * tid; i < ng; i += 4 * kThreads) {
+    const float4 m = *reinterpret_cast<const float4*>(gmax + i);  // past the end: padding of the buffer
+    const bool c0 = m.x >= bound || all, c1 = (m.y >= bound || all) && i + 1 < ng,
+               c2 = (m.z >= bound || all) && i + 2 < ng, c3 = (m.w >= bound || all) && i + 3 < ng;
+    if (c0 || c1 || c2 || c3) {
+      uint32_t at = atomicAdd(&sc.ngroups, (uint32_t)(c0 + c1 + c2 + c3));
+      if (at + 4 <= kCandGroups) {
+        if (c0) sc.cand.groups[at++] = (uint32_t)i;
+        if (c1) sc.cand.groups[at++] = (uint32_t)i + 1;
+        if (c2) sc.cand.groups[at++] = (uint32_t)i + 2;
+        if (c3) sc.cand.groups[at] = (uint32_t)i + 3;
+      }
     }
   }
   __syncthreads();
   const uint32_t ncg = sc.ngroups;
-  bool exact = ncg > kCandGroups;
+  bool exact = ncg > kCandGroups - 4;
   if (!exact) {
     for (int i = tid; i < (int)ncg; i += kThreads) {
-      const int g = (int)sc.cand.groups[i], first = sh.start(g);
-      auto offer = [&](float x, int idx) {
-        if (x >= bound || all) {
-          const uint32_t at = atomicAdd(&sc.nelems, 1u);
-          if (at < kCandElems) sc.cand.elems[at] = entry(order_key(x), idx);
-        }
-      };
+      const int g = (int)sc.cand.groups[i], first = sh.start(g), size = sh.size(g);
+      float x[kGroup];
       if (g >= 1 && g <= sh.n) {
-        float x[kGroup];
         unpack_group<T>(x, load_group<T>(sh.row + first));
-#pragma unroll
-        for (int e = 0; e < kGroup; ++e) offer(x[e], first + e);
       } else {
-        for (int e = 0; e < sh.size(g); ++e) offer(to_f<T>(sh.row[first + e]), first + e);
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) x[e] = e < size ? to_f<T>(sh.row[first + e]) : 0.f;
+      }
+      uint32_t take = 0;
+#pragma unroll
+      for (int e = 0; e < kGroup; ++e) take |= (x[e] >= bound || all) ? 1u << e : 0u;
+      take &= (1u << size) - 1u;
+      uint32_t at = atomicAdd(&sc.nelems, (uint32_t)__popc(take));
+      if (at + kGroup <= kCandElems) {
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e)
+          if (take >> e & 1u) sc.cand.elems[at++] = entry(order_key(x[e]), first + e);
       }
     }
     __syncthreads();
-    exact = sc.nelems > kCandElems;
+    exact = sc.nelems > kCandElems - kGroup;
   }
   if (!exact) {
     // the position of each candidate is the number of better ones
@@ -190,8 +215,9 @@ __device__ void select_top(uint64_t* top, const Share<T>& sh, const float* gmax,
       const uint64_t e = sc.cand.elems[i];
       int rank = 0, o = 0;
       for (; o + 4 <= ne; o += 4) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) rank += sc.cand.elems[o + u] > e;
+        const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sc.cand.elems + o);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sc.cand.elems + o + 2);
+        rank += (a.x > e) + (a.y > e) + (b.x > e) + (b.y > e);
       }
       for (; o < ne; ++o) rank += sc.cand.elems[o] > e;
       if (rank < k) top[rank] = e;
@@ -245,17 +271,21 @@ struct FwdArgs {
 };
 
 constexpr int kBatch = 2;  // groups of a thread in flight
+// CTAs on an SM: 16-bit groups take 32 registers a thread with two in flight, which hides the
+// row's start and end behind seven other rows; fp32 groups are twice as large
+template <typename T, bool CAP>
+constexpr int resident() { return sizeof(T) == 4 ? 4 : (CAP ? 5 : 8); }
 
 template <typename T, bool CAP, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, (resident<T, CAP>()))
 token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
   using Stats = RowStats<CAP, ENT>;
-  extern __shared__ float gmax[];      // TOP: group maxima
+  extern __shared__ __align__(16) float gmax[];  // TOP: group maxima
   __shared__ Stats s_warp[kWarps];
   __shared__ Stats s_cta;
   __shared__ float s_share[4];         // this CTA's statistics, read by the others of the cluster
   __shared__ uint64_t s_top[TOP ? kMaxTop : 1];
-  __shared__ __align__(8) unsigned char s_scratch[TOP ? sizeof(SelectScratch) : 8];
+  __shared__ __align__(16) unsigned char s_scratch[TOP ? sizeof(SelectScratch) : 8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cs = a.cs;
   const int64_t r = cs > 1 ? blockIdx.x / cs : blockIdx.x;
@@ -333,33 +363,45 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
     }
     row_cluster_sync();
     st.init();
-    for (int c = 0; c < cs; ++c) {  // the same order in every CTA
-      Stats o;
-      o.init();
-      const float m = __uint_as_float(ld_cluster_u32(&s_share[0], c));
-      if (m != -INFINITY) { o.m = m; o.mu = squash<CAP>(m, q); }
-      o.s = __uint_as_float(ld_cluster_u32(&s_share[1], c));
-      o.w = __uint_as_float(ld_cluster_u32(&s_share[2], c));
-      st.merge(o, q);
+    if (lane < cs) {  // every warp of every CTA joins them in the same way
+      const float m = __uint_as_float(ld_cluster_u32(&s_share[0], lane));
+      st.s = __uint_as_float(ld_cluster_u32(&s_share[1], lane));
+      st.w = __uint_as_float(ld_cluster_u32(&s_share[2], lane));
+      if (m != -INFINITY) { st.m = m; st.mu = squash<CAP>(m, q); }
     }
+    st.warp_merge(q);
   }
   // S = 0: every logit is -inf and the row has no distribution: log-probabilities -inf, entropy 0
   const float logs = logf(st.s);
   if constexpr (TOP) {
-    for (int i = tid; i < kl; i += kThreads) {
-      const uint64_t e = s_top[i];
-      int pos = i;
-      for (int c = 0; c < cs; ++c) {
+    // An entry's position in the row's list: its own in this CTA's list and the number of better
+    // entries in each other list, all sorted.  The other lists are copied here first.
+    SelectScratch& sc = *reinterpret_cast<SelectScratch*>(s_scratch);
+    if (cs > 1) {
+      __syncthreads();  // the selection is done with its scratch
+      for (int i = tid; i < cs * a.k; i += kThreads) {  // 0 from the end of a shorter list on
+        const int c = i / a.k, o = i - c * a.k;
+        sc.lists[i] = o < (int)ld_cluster_u32(&s_share[3], c) ? ld_cluster_u64(&s_top[o], c) : 0ull;
+      }
+      for (int i = tid; i < kl; i += kThreads) sc.place[i] = i;
+      __syncthreads();
+      for (int i = tid; i < cs * kl; i += kThreads) {
+        const int c = i / kl, o = i - c * kl;
         if (c == rank) continue;
-        // entries of the other list that are better: it is sorted
-        int lo = 0, hi = __float_as_int(__uint_as_float(ld_cluster_u32(&s_share[3], c)));
+        const uint64_t e = s_top[o];
+        int lo = 0, hi = a.k;
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;
-          if (ld_cluster_u64(&s_top[mid], c) > e) lo = mid + 1;
+          if (sc.lists[c * a.k + mid] > e) lo = mid + 1;
           else hi = mid;
         }
-        pos += lo;
+        if (lo) atomicAdd(&sc.place[o], lo);
       }
+      __syncthreads();
+    }
+    for (int i = tid; i < kl; i += kThreads) {
+      const uint64_t e = s_top[i];
+      const int pos = cs > 1 ? sc.place[i] : i;
       if (pos < a.k) {
         const float x = key_value((uint32_t)(e >> 32));
         a.top_idx[r * a.k + pos] = (int64_t)(uint32_t)~(uint32_t)e;
@@ -384,7 +426,10 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
     if (a.lse) a.lse[r] = st.mu * q.inv_t + logs;
     if (a.stats) a.stats[r] = make_float2(st.mu, logs);
   }
-  if (cs > 1) row_cluster_sync();  // the other CTAs have read this one's shared memory
+  if (cs > 1) {  // the other CTAs have read this one's shared memory
+    row_cluster_arrive_relaxed();
+    row_cluster_wait();
+  }
 }
 
 struct BwdArgs {
@@ -407,8 +452,9 @@ template <typename T, bool CAP, bool ENT>
 __global__ void __launch_bounds__(kThreads)
 token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const BwdArgs a) {
   const int tid = threadIdx.x;
-  const int64_t r = blockIdx.x / a.segs;
-  const int seg = (int)(blockIdx.x - r * a.segs);
+  const uint32_t r32 = blockIdx.x / (uint32_t)a.segs;
+  const int64_t r = r32;
+  const int seg = (int)(blockIdx.x - r32 * (uint32_t)a.segs);
   const Squash q = a.q;
   const T* row = logits + a.addr.off(r);
   T* grow = grad + r * a.V;
@@ -526,7 +572,7 @@ int launch_fwd(const T* logits, const FwdArgs& a, int64_t rows, cudaStream_t st)
   AK_PICK(false, false, false) AK_PICK(false, false, true) AK_PICK(false, true, false) AK_PICK(false, true, true)
   AK_PICK(true, false, false) AK_PICK(true, false, true) AK_PICK(true, true, false) AK_PICK(true, true, true)
 #undef AK_PICK
-  const size_t smem = top ? ((size_t)(a.V / kGroup) / a.cs + 4) * 4 : 0;
+  const size_t smem = top ? ((size_t)(a.V / kGroup) / a.cs + 3 + 4) * 4 : 0;  // read four at a time
   AK_CUDA_TRY(launch_rows(kern, rows * a.cs, kThreads, a.cs, smem, st, logits, a), "ak_token_logprobs_fwd");
   return AK_OK;
 }

@@ -8,12 +8,16 @@ difference, the product with log2(e) / T and that constant are each off by u rel
 argument a (in powers of 2) is off by at most 3 u |a| and e by 3 u |a| ln 2, plus 2^-22 for the
 hardware's exponential.  A sum of n terms added one after the other, all positive, is off by n u
 relative; a thread adds V / 512 of them into each of two sums, and 32 more join threads and CTAs.
-With softcap, tanhf is off by 2 units in the last place: 4 u c in y, twice in a difference.
+With softcap c, y is formed as c (1 - E) / (1 + E), E = e^(-2 |x| / c): E's argument is off by 2 u
+relative, the exponential by 4 u, so tanh by 2 E / (1 + E)^2 (4 |x / c| + 4) u <= 2.4 u; the
+difference, the sum, a quotient of 2 units in the last place and the product add 6 u of tanh: 9 u c
+at most, twice in a difference (CAP).
 """
 import torch
 
 U = 2.0 ** -24
 LN2 = 0.6931471805599453
+CAP = 18  # of a difference of two squashed logits, in u * softcap
 
 
 def squash(x, temperature=1.0, softcap=0.0):
@@ -43,7 +47,7 @@ def token_logprobs(x, targets=None, ignore_index=-100, temperature=1.0, softcap=
     # bounds
     a = torch.where(p == 0, torch.zeros_like(p), d / LN2).abs()
     adds = v / 512 + 32
-    cap_err = 8 * U * softcap / temperature
+    cap_err = CAP * U * softcap / temperature
     a1, a2 = (p * a).sum(1), (p * a * a).sum(1)
     tol_s = 3 * U * LN2 * a1 + 4 * U + adds * U + cap_err
     tol_logs = tol_s + 2 * U * torch.log(s)[:, 0].abs()
@@ -93,7 +97,7 @@ def token_logprobs_grad(x, targets, g_lp, g_ent, ignore_index=-100, temperature=
     y, dy = squash(x, temperature, softcap)
     none = (ign | r["empty"])[:, None]
     tol_logs, tol_h = r["tol_logs"][:, None], r["tol_entropy"][:, None]
-    cap_err = 8 * U * softcap / temperature
+    cap_err = CAP * U * softcap / temperature
     # p = 2^d, d = (y - M) kl - log2 S: both parts are at most |log p| + log V, three and two
     # roundings, and one of the difference
     logv = torch.log(torch.tensor(v + 1.0, dtype=torch.float64)).item()
@@ -101,8 +105,8 @@ def token_logprobs_grad(x, targets, g_lp, g_ent, ignore_index=-100, temperature=
     mag = gl.abs() + ge.abs() * (lgp.abs() + H)
     tol = p * (rel * mag + ge.abs() * (tol_h + rel) + 6 * U * mag) + 4 * U * (g.abs() + hot * gl.abs())
     tol = tol * dy.abs()
-    if softcap > 0:  # the slope 1 - t^2, t = tanh off by 6 u
-        tol = tol + g.abs() * (16 * U) / temperature
+    if softcap > 0:  # the slope 1 - t^2, t = tanh off by 9 u
+        tol = tol + g.abs() * (20 * U) / temperature
     g = torch.where(none, torch.zeros_like(g), g * dy)
     return g, torch.where(none, torch.zeros_like(tol), tol)
 
@@ -169,11 +173,11 @@ def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=Fals
     dr = (k + 6) * U
     tail_term = torch.where(has_rest & (rest > 0), rest * (torch.log(rest) - logpr), torch.zeros_like(rest))
     losses = terms.sum(1) + tail_term
-    tol_lp = r["tol_logs"][:, None] + 8 * U * (lpk.abs().nan_to_num(0, 0, 0) + torch.log(torch.tensor(v + 1.0)).item()) + 8 * U * softcap / temperature
+    tol_lp = r["tol_logs"][:, None] + 8 * U * (lpk.abs().nan_to_num(0, 0, 0) + torch.log(torch.tensor(v + 1.0)).item()) + CAP * U * softcap / temperature
     absl = torch.where(q > 0, logq.abs(), 0.0)
     tol = (q * (rel_q * diff.abs().nan_to_num(0, 0, 0) + tol_lp + (4 + k) * U * (absl + 1))).sum(1)
     tol = tol + torch.where(has_rest, dr * (3 + torch.log(rest + dr).abs() + logpr.abs().nan_to_num(0, 0, 0))
-                            + rest * (2 * r["tol_logs"] + 12 * U * (1 + logpr.abs().nan_to_num(0, 0, 0)) + 16 * U * softcap / temperature),
+                            + rest * (2 * r["tol_logs"] + 12 * U * (1 + logpr.abs().nan_to_num(0, 0, 0)) + 2 * CAP * U * softcap / temperature),
                             torch.zeros_like(rest))
     tol = tol + 24 * U * (terms.abs().nan_to_num(0, 0, 0).sum(1) + tail_term.abs())
     losses = torch.where(none, torch.zeros_like(losses), losses)
@@ -189,10 +193,10 @@ def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=Fals
     logv = torch.log(torch.tensor(v + 1.0)).item()
     lgp = torch.where(p > 0, logp, torch.zeros_like(p))
     lpr = torch.where(has_rest, logpr, torch.zeros_like(rest)).abs()[:, None]
-    rel = 10 * U + (4 * lgp.abs() + 6 * logv + 6 * lpr) * U + 2 * r["tol_logs"][:, None] + 16 * U * softcap / temperature
+    rel = 10 * U + (4 * lgp.abs() + 6 * logv + 6 * lpr) * U + 2 * r["tol_logs"][:, None] + 2 * CAP * U * softcap / temperature
     relm = torch.zeros_like(p).scatter_add_(1, at, torch.where(used, q * (rel_q + k * U), torch.zeros_like(q)))
     tg = torch.where(inside, p * rel + relm, p * rel + cond * (rest[:, None] * rel + dr)) + 6 * U * g.abs()
-    tg = tg * dy.abs() + (g.abs() * 16 * U / temperature if softcap > 0 else 0.0)
+    tg = tg * dy.abs() + (g.abs() * 20 * U / temperature if softcap > 0 else 0.0)
     off = (none | empty | ~live)[:, None]
     g, tg = torch.where(off, torch.zeros_like(g), g * dy), torch.where(off, torch.zeros_like(tg), tg)
     g = torch.where((bad & live)[:, None], torch.full_like(g, torch.nan), g)
