@@ -12,11 +12,17 @@
 // p_r = 1 - sum_k p_{i_k} would cancel where the student agrees with the teacher, so the rest is
 // summed by itself, with a maximum of its own: the teacher's tokens are taken out of the row as it
 // lies in shared memory (-inf), and join with the statistics of those K logits afterwards.
-// A gradient outside the K tokens is e c with e = 2^(kl (y - mu_rest)) and the row's
+// A gradient outside the K tokens is e c with e = 2^d against the rest's reference and the row's
 // c = (share of p) / S - r / S_rest, which neither over- nor underflows where p_r does.
 //
 // One read of the logits: a CTA, or the CTAs of a cluster, bring the row into shared memory by
-// bulk copies, form the statistics, and write the gradient from shared memory.
+// bulk copies, form the statistics, and write the gradient from shared memory.  The kernel is
+// persistent and its warps have roles, so that a row's long chain of small steps (its indices, the
+// K logits they point at, the masses of repeated tokens) runs while the row before it is worked on:
+//   loader    copies the next row piece by piece, each as soon as compute has left that piece
+//   teacher   the K entries of the next row; takes their tokens out of it when it has arrived
+//   compute   statistics of the rest, then the gradient from them
+//   finisher  the row's loss, and the gradient at the teacher's tokens over what compute wrote
 #include "logit_rows.cuh"
 
 #include <algorithm>
@@ -24,350 +30,614 @@
 namespace ak {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 256;    // of the backward kernel
+constexpr int kRoles = 3;        // loader, teacher, finisher
+// Compute warps: kWide of them with two CTAs on an SM, which a long row (100 KB of shared memory)
+// allows anyhow; kNarrow with six CTAs for shares up to kShareNarrow, where what counts is how many
+// rows are under way at once.
+constexpr int kWide = 11, kNarrow = 2;
+constexpr int kShareNarrow = 16 * 1024;
 constexpr int kMaxK = 128;       // teacher entries
+constexpr int kSlots = kMaxK / 32;
 constexpr int kMaxCluster = 8;   // the portable cluster size
-constexpr int kShareWanted = 56 * 1024;  // row bytes per CTA: four CTAs on an SM
-constexpr int kShareMost = 216 * 1024;
+constexpr int kShareWanted = 101 * 1024;  // bytes of one row in one CTA: two CTAs fit an SM
+constexpr int kShareMost = 208 * 1024;    // of a row too long for that in eight CTAs
+constexpr int kPieces = 8;                // a buffer is handed back in pieces
 constexpr float kMasked = 30000.f;
-constexpr uint32_t kCopyBytes = 8192;    // of one bulk copy
 
 struct DistillArgs {
   float* losses;        // [rows]
   void* grad;           // GRAD: [rows][V]
-  float2* rest;         // !GRAD, nullable: (mu_rest, c) of each row, for the backward
+  float4* rest;         // !GRAD, nullable: (reference, c) of each row's rest, for the backward
   float* gk;            // !GRAD, nullable: [rows][K] T dL/dx at the teacher's tokens
   const int64_t* idx;   // [rows][K]
   const float* tlp;     // [rows][K]
   const uint8_t* mask;  // nullable [rows]
   const float* inv_n;   // GRAD, nullable: 1 / rows that count (host value in scale otherwise)
   RowAddr addr;
+  int64_t rows;
   float scale;          // GRAD: T, times 1 / rows without inv_n
-  int V, K, cs, tail;
+  int V, K, log_cs, tail;
+  uint32_t piece;       // bytes of a piece of the row buffer
   Squash q;
   int* status;
 };
 
 // The gradient at a logit outside the teacher's tokens.  c = 0 gives 0 whatever x is.
 template <bool CAP>
-__device__ __forceinline__ float rest_grad(float x, float mu, float c, const Squash& q) {
+__device__ __forceinline__ float rest_grad(float x, const Ref& ref, float c, const Squash& q) {
   if (c == 0.f) return 0.f;
   const float y = squash<CAP>(x, q);
-  return ex2((y - mu) * q.kl) * c * squash_slope<CAP>(y, q);
+  return ex2(exponent(y, ref, q)) * c * squash_slope<CAP>(y, q);
 }
 
-// The same for the values of NW words, two at a time without softcap.
+// The same for the values of NW words, two at a time where it can.
 template <typename T, bool CAP, int NW>
-__device__ __forceinline__ void rest_grads(float* x, const uint32_t (&w)[NW], float mu, float c, const Squash& q) {
+__device__ __forceinline__ void rest_grads(float* x, const uint32_t (&w)[NW], const Ref& ref, float c, const Squash& q) {
   constexpr int P = NW * elems_per_word<T>() / 2;
-  const float2 nmu = make_float2(-mu, -mu), kl = make_float2(q.kl, q.kl), c2 = make_float2(c, c);
+  const float2 kl = make_float2(q.kl, q.kl), nk = make_float2(-ref.k, -ref.k), c2 = make_float2(c, c);
+  if (!CAP && ref.sh == 0.f && c != 0.f) {
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const float2 v = word_pair<T>(w, i);
-    float2 o;
-    if constexpr (CAP) {
-      o = make_float2(rest_grad<CAP>(v.x, mu, c, q), rest_grad<CAP>(v.y, mu, c, q));
-    } else if (c == 0.f) {
-      o = make_float2(0.f, 0.f);
-    } else {
-      const float2 d = __fmul2_rn(__fadd2_rn(v, nmu), kl);
-      o = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), c2);
+    for (int i = 0; i < P; ++i) {
+      const float2 d = __ffma2_rn(word_pair<T>(w, i), kl, nk);
+      const float2 o = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), c2);
+      x[2 * i] = o.x;
+      x[2 * i + 1] = o.y;
     }
-    x[2 * i] = o.x;
-    x[2 * i + 1] = o.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float2 v = word_pair<T>(w, i);
+      x[2 * i] = rest_grad<CAP>(v.x, ref, c, q);
+      x[2 * i + 1] = rest_grad<CAP>(v.y, ref, c, q);
+    }
   }
 }
 
-template <typename T, bool CAP, bool GRAD>
-__global__ void __launch_bounds__(kThreads)
-distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
-  using Stats = RowStats<CAP, false>;
+// The gradients of one 16-byte vector, rounded to T and stored.
+template <typename T, bool CAP>
+__device__ __forceinline__ void store_grads(T* out, const uint4& f, const Ref& ref, float c, const Squash& q, bool vec) {
   constexpr int VEC = 16 / sizeof(T);
-  extern __shared__ __align__(128) unsigned char s_row_raw[];  // this CTA's share of the row's groups
-  T* s_row = reinterpret_cast<T*>(s_row_raw);
-  __shared__ __align__(8) uint64_t s_bar;
-  __shared__ Stats s_warp[kWarps];
-  __shared__ float s_share[2];     // this CTA's statistics, read by the others of the cluster
-  __shared__ float s_out[2];       // (mu_rest, c * scale) for the gradient
-  __shared__ float s_edge[2][32];  // head and tail of the row
-  __shared__ int s_idx[kMaxK];
-  __shared__ float s_q[kMaxK];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int cs = a.cs;
-  const int64_t r = cs > 1 ? blockIdx.x / cs : blockIdx.x;
-  const int rank = cs > 1 ? (int)row_cluster_rank() : 0;
+  const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+  float x[VEC];
+  rest_grads<T, CAP>(x, w, ref, c, q);
+  if (vec) {
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) o[i] = __float_as_uint(x[i]);
+      else o[i] = pack2(x[2 * i], x[2 * i + 1], (const T*)nullptr);
+    }
+    *reinterpret_cast<uint4*>(out) = make_uint4(o[0], o[1], o[2], o[3]);
+  } else {
+    for (int i = 0; i < VEC; ++i) out[i] = from_f<T>(x[i]);
+  }
+}
+
+// One CTA's share of a row: n elements from body0 in its buffer, and the row's head (first CTA) or
+// tail (last CTA) as loose elements.
+template <typename T>
+struct Share {
+  const T* row;
+  int body0, n, tail0, head_here, tail_here;
+  __device__ __forceinline__ Share(const T* row_, int V, int rank, int log_cs) : row(row_) {
+    const RowCut cut = cut_row(row_, V);
+    const int g0 = (int)(((int64_t)cut.groups * rank) >> log_cs);
+    n = ((int)(((int64_t)cut.groups * (rank + 1)) >> log_cs) - g0) * kGroup;
+    body0 = cut.head + g0 * kGroup;
+    tail0 = cut.head + cut.groups * kGroup;
+    head_here = rank == 0 ? cut.head : 0;
+    tail_here = rank == (1 << log_cs) - 1 ? cut.tail : 0;
+  }
+  __device__ __forceinline__ bool has(int i) const {
+    return (i >= body0 && i < body0 + n) || i < head_here || (i >= tail0 && i - tail0 < tail_here);
+  }
+};
+
+// What the teacher's warp hands on with a row.
+struct TeacherRow {
+  float m, lim, s;  // statistics of the teacher's tokens, each once
+  Ref r;
+  float rest;      // r
+  int none, bad;
+  int idx[kMaxK];  // -1: no entry
+  float q[kMaxK], logq[kMaxK], y[kMaxK], mass[kMaxK];
+};
+
+// What compute hands to the finisher.
+struct FinishRow {
+  Ref all, rest;
+  float logs, tail_loss, c;
+  int empty;
+};
+
+// Bounded waits.  The first that runs out reports AK_ERR_TIMEOUT and raises the CTA's abort flag;
+// the later ones return at once, so the kernel runs to its end without waiting (every role passes
+// the same barriers as ever) and its outputs are invalid.
+struct Waits {
+  int* status;
+  volatile int* abort;
+  template <bool kCluster>
+  __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) const {
+    if (*abort) return;
+    for (uint32_t i = 0; i < kMaxSpins; ++i) {
+      uint32_t ok;
+      if constexpr (kCluster) {
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+            " selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+      } else {
+        ok = mbar_try_wait(bar, parity);
+      }
+      if (ok) return;
+      if (i > 64) __nanosleep(32);
+      if ((i & 255u) == 255u && *abort) return;
+    }
+    *abort = 1;
+    report_status(status, (int)AK_ERR_TIMEOUT);
+  }
+};
+
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Named barriers; the warp is whole again first, after waits that its lanes left one by one.
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void named_arrive(int id, int threads) {
+  __syncwarp();
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// A row's K entries as they lie in memory, entry 32 j + lane in slot j of the teacher's warp.
+struct Entries {
+  int64_t i[kSlots];
+  float t[kSlots];
+  __device__ __forceinline__ void load(const DistillArgs& a, int64_t r) {
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      const int k = 32 * j + (int)(threadIdx.x & 31);
+      i[j] = k < a.K ? a.idx[r * a.K + k] : -1;
+      t[j] = k < a.K ? a.tlp[r * a.K + k] : 0.f;
+    }
+  }
+};
+
+constexpr int kTags = 2048;
+__device__ __forceinline__ int mix_bits(int i) { return (int)(((uint32_t)i * 2654435761u) >> 21); }  // 11 bits
+
+// A row's teacher: everything that needs only its K entries and their logits.  s_idx, s_q and s_tag
+// are the warp's scratch.
+template <typename T, bool CAP>
+__device__ __forceinline__ void teacher_row(TeacherRow& out_head, int (&idx)[kSlots], float (&qk)[kSlots],
+                                            float (&logq)[kSlots], float (&yk)[kSlots], float (&mass)[kSlots],
+                                            const Entries& e, const T* row, const DistillArgs& a, int* s_idx,
+                                            float* s_q, uint8_t (*s_tag)[kTags]) {
+  const int lane = threadIdx.x & 31;
   const Squash q = a.q;
-  const T* row = logits + a.addr.off(r);
-  const RowCut cut = cut_row(row, a.V);
-  const int g0 = (int)((int64_t)cut.groups * rank / cs);
-  const int n = ((int)((int64_t)cut.groups * (rank + 1) / cs) - g0) * kGroup;  // elements in s_row
-  const int body0 = cut.head + g0 * kGroup;                                   // the first of them
-  const int tail0 = cut.head + cut.groups * kGroup;
-  const int head_here = rank == 0 ? cut.head : 0, tail_here = rank == cs - 1 ? cut.tail : 0;
-  T* grow = GRAD ? reinterpret_cast<T*>(a.grad) + r * a.V : nullptr;
-  const bool vec = GRAD && (reinterpret_cast<uintptr_t>(grow + body0) & 15u) == 0;
-  const bool live = a.mask == nullptr || a.mask[r] != 0;
-
-  if (!live) {  // the same in every CTA of the row; what the row holds is not looked at
-    if constexpr (GRAD) {
-      const float zero[VEC] = {};
-      for (int v = tid; v < n / VEC; v += kThreads) {
-        if (vec) store_frag<T, VEC>(grow + body0 + v * VEC, zero);
-        else
-          for (int i = 0; i < VEC; ++i) grow[body0 + v * VEC + i] = from_f<T>(0.f);
-      }
-      if (tid < head_here) grow[tid] = from_f<T>(0.f);
-      if (tid < tail_here) grow[tail0 + tid] = from_f<T>(0.f);
-    }
-    if (rank == 0) {
-      if (tid == 0) {
-        a.losses[r] = 0.f;
-        if (!GRAD && a.rest) a.rest[r] = make_float2(0.f, 0.f);
-      }
-      if (!GRAD && a.gk && tid < a.K) a.gk[r * a.K + tid] = 0.f;
-    }
-    return;
-  }
-
-  // ---- the row on its way into shared memory
-  if (tid == 0) {
-    mbar_init(&s_bar, 1);
-    mbar_fence_init();
-    const uint32_t bytes = (uint32_t)(n * sizeof(T));
-    mbar_arrive_expect_tx(&s_bar, bytes);
-    const char* src = reinterpret_cast<const char*>(row + body0);
-    for (uint32_t o = 0; o < bytes; o += kCopyBytes)
-      bulk_g2s(s_row_raw + o, src + o, min(kCopyBytes, bytes - o), &s_bar);
-  }
-  if (warp == 1 && lane < head_here) s_edge[0][lane] = to_f<T>(row[lane]);
-  if (warp == 2 && lane < tail_here) s_edge[1][lane] = to_f<T>(row[tail0 + lane]);
-  __syncthreads();
-
-  // ---- the teacher's entries, all on the first warp: entry 32 j + lane in slot j.  A negative
-  // index is padding.
-  constexpr int S = kMaxK / 32;
-  int idx[S];
-  float yk[S], qk[S], logq[S], mass[S];
-  Stats top;  // the teacher's tokens
-  top.init();
-  bool bad = false, none = false;
-  float rest = 0.f;
-  if (warp == 0) {
-    float t[S], xk[S];
-    bool any = false;
+  float t[kSlots], xk[kSlots];
+  bool any = false, bad = false;
 #pragma unroll
-    for (int j = 0; j < S; ++j) {
-      const int k = 32 * j + lane;
-      idx[j] = -1;
-      t[j] = yk[j] = xk[j] = -INFINITY;
-      if (k < a.K) {
-        const int64_t i = a.idx[r * a.K + k];
-        bad |= i >= a.V;
-        if (i >= 0 && i < a.V) {
-          idx[j] = (int)i;
-          t[j] = a.tlp[r * a.K + k];
-          xk[j] = to_f<T>(row[i]);
-          yk[j] = squash<CAP>(xk[j], q);
-          any = true;
-        }
+  for (int j = 0; j < kSlots; ++j) {
+    idx[j] = -1;
+    t[j] = xk[j] = -INFINITY;
+    if (32 * j < a.K) {
+      bad |= e.i[j] >= a.V;
+      const bool ok = e.i[j] >= 0 && e.i[j] < a.V;
+      any |= ok;
+      if (ok) {
+        idx[j] = (int)e.i[j];
+        t[j] = e.t[j];
+        xk[j] = to_f<T>(row[idx[j]]);
       }
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    any = __any_sync(0xffffffffu, any);
-    float qsum = 0.f;
-    if (a.tail) {
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        qk[j] = idx[j] >= 0 ? expf(t[j]) : 0.f;
-        logq[j] = t[j];
-        qsum += qk[j];
-      }
-      qsum = warp_sum(qsum);
-    } else {
-      float tm = t[0], z = 0.f;
-#pragma unroll
-      for (int j = 1; j < S; ++j) tm = fmaxf(tm, t[j]);
-      tm = warp_max(tm);
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        qk[j] = (idx[j] >= 0 && tm != -INFINITY) ? expf(t[j] - tm) : 0.f;
-        z += qk[j];
-      }
-      z = warp_sum(z);
-      const float logz = logf(z);
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        qk[j] = z == 0.f ? 0.f : qk[j] / z;  // z: 0 without entries, NaN kept
-        logq[j] = t[j] - tm - logz;
-        qsum += qk[j];
-      }
-      qsum = warp_sum(qsum);
-    }
-    none = a.tail ? !any : qsum == 0.f;  // no teacher: loss 0, no gradient
-    rest = a.tail ? fmaxf(1.f - qsum, 0.f) : 0.f;
-#pragma unroll
-    for (int j = 0; j < S; ++j) {
-      mass[j] = 0.f;
       s_idx[32 * j + lane] = idx[j];
-      s_q[32 * j + lane] = qk[j];
+      // two tables of who came last to a place that the token's low and mixed bits name
+      if (ok) {
+        s_tag[0][idx[j] & (kTags - 1)] = (uint8_t)(32 * j + lane);
+        s_tag[1][mix_bits(idx[j])] = (uint8_t)(32 * j + lane);
+      }
     }
+  }
+  __syncwarp();
+  // a token that comes twice is not the last in either table at one of its entries; so, rarely, is
+  // one that shares its places with others, which costs the comparison below
+  bool twice = false;
+#pragma unroll
+  for (int j = 0; j < kSlots; ++j)
+    if (idx[j] >= 0)
+      twice |= s_tag[0][idx[j] & (kTags - 1)] != (uint8_t)(32 * j + lane) &&
+               s_tag[1][mix_bits(idx[j])] != (uint8_t)(32 * j + lane);
+  twice = __any_sync(0xffffffffu, twice);
+  bad = __any_sync(0xffffffffu, bad);
+  any = __any_sync(0xffffffffu, any);
+  float qsum = 0.f;
+  if (a.tail) {
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      qk[j] = 0.f;
+      logq[j] = t[j];
+      if (32 * j < a.K) qsum += qk[j] = idx[j] >= 0 ? expf(t[j]) : 0.f;
+    }
+  } else {
+    float tm = t[0], z = 0.f;
+#pragma unroll
+    for (int j = 1; j < kSlots; ++j) tm = fmaxf(tm, t[j]);
+    tm = redux_max(tm);
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      qk[j] = 0.f;
+      if (32 * j < a.K) z += qk[j] = (idx[j] >= 0 && tm != -INFINITY) ? expf(t[j] - tm) : 0.f;
+    }
+    z = warp_sum(z);
+    const float logz = logf(z);
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      qk[j] = z == 0.f ? 0.f : qk[j] / z;  // z: 0 without entries, NaN kept
+      logq[j] = t[j] - tm - logz;
+      qsum += qk[j];
+    }
+  }
+  qsum = warp_sum(qsum);
+  // entries of one token: its logit counts once, at the first of them; their masses add up
+  uint32_t later = 0;
+#pragma unroll
+  for (int j = 0; j < kSlots; ++j) mass[j] = twice ? 0.f : qk[j];
+  if (twice) {
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) s_q[32 * j + lane] = qk[j];
     __syncwarp();
-    // entries of one token: its logit counts once, at the first of them; their masses add up
-    uint32_t later = 0;
     for (int m = 0; m < a.K; ++m) {
       const int im = s_idx[m];
       const float qm = s_q[m];
 #pragma unroll
-      for (int j = 0; j < S; ++j) {
-        if (32 * j < a.K && idx[j] == im) {
+      for (int j = 0; j < kSlots; ++j) {
+        if (idx[j] == im) {
           mass[j] += qm;
           if (m < 32 * j + lane) later |= 1u << j;
         }
       }
     }
+  }
+  __syncwarp();  // the scratch is free for the next row
+  RowStats<CAP, false> top;
+  top.init();
+  uint32_t w[kSlots];
 #pragma unroll
-    for (int j = 0; j < S; ++j) {
-      if (idx[j] >= 0 && !(later >> j & 1u)) {
-        const float x[1] = {xk[j]};
-        top.add(x, q);
-      }
+  for (int j = 0; j < kSlots; ++j) {
+    yk[j] = squash<CAP>(xk[j], q);
+    w[j] = __float_as_uint((idx[j] < 0 || (later >> j & 1u)) ? -INFINITY : xk[j]);
+  }
+  top.template add_words<float>(w, words_max<float>(w), q);
+  top.warp_merge(q);
+  out_head.m = top.m;
+  out_head.lim = top.lim;
+  out_head.s = top.s;
+  out_head.r = top.r;
+  out_head.rest = a.tail ? fmaxf(1.f - qsum, 0.f) : 0.f;
+  out_head.none = a.tail ? !any : qsum == 0.f;  // no teacher: loss 0, no gradient
+  out_head.bad = bad;
+}
+
+template <typename T, bool CAP, bool GRAD, int W>
+__global__ void __launch_bounds__(32 * (W + kRoles), W == kWide ? 2 : 6)
+distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
+  using Stats = RowStats<CAP, false>;
+  constexpr int VEC = 16 / sizeof(T), kCompute = 32 * W;
+  constexpr int U = W == kWide ? 4 : 2;  // 16-byte vectors that a compute thread works on at a time
+  extern __shared__ __align__(128) unsigned char s_row[];  // this CTA's share of a row
+  __shared__ __align__(8) uint64_t full;                   // the row has arrived
+  __shared__ __align__(8) uint64_t left[kPieces];          // compute has left the piece
+  __shared__ __align__(8) uint64_t ready[2], done[2];      // s_teacher, s_edge: written, read
+  __shared__ __align__(8) uint64_t joined[2];
+  __shared__ TeacherRow s_teacher[2];
+  __shared__ FinishRow s_fin[2];
+  __shared__ Stats s_warp[2][W];
+  __shared__ __align__(16) float4 s_joined[2][kMaxCluster];  // statistics of the cluster's CTAs
+  __shared__ float s_edge[2][2][32];                         // head and tail of the row
+  __shared__ int s_idx[kMaxK];
+  __shared__ float s_q[kMaxK];
+  __shared__ uint8_t s_tag[2][kTags];
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cs = 1 << a.log_cs;
+  const int64_t first = blockIdx.x >> a.log_cs, step = gridDim.x >> a.log_cs;
+  const int rank = cs > 1 ? (int)row_cluster_rank() : 0;
+  const Squash q = a.q;
+  const Waits wait{a.status, &s_abort};
+  if (tid == 0) {
+    s_abort = 0;
+    mbar_init(&full, 1);
+    for (int c = 0; c < kPieces; ++c) mbar_init(&left[c], W);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ready[b], 1);
+      mbar_init(&done[b], W + 1);
+      mbar_init(&joined[b], cs);
     }
-    top.warp_merge(q);
-    // out of the row, once it is here
-    mbar_wait_bounded(&s_bar, 0u, a.status);
-#pragma unroll
-    for (int j = 0; j < S; ++j) {
-      const int i = idx[j];
-      if (i < 0) continue;
-      if (i >= body0 && i < body0 + n) s_row[i - body0] = from_f<T>(-INFINITY);
-      else if (i < head_here) s_edge[0][i] = -INFINITY;
-      else if (i >= tail0 && i - tail0 < tail_here) s_edge[1][i - tail0] = -INFINITY;
-    }
+    mbar_fence_init();
   }
   __syncthreads();
+  if (cs > 1) row_cluster_sync();  // the barriers of every CTA are initialised
 
-  // ---- the rest of the row
-  mbar_wait_bounded(&s_bar, 0u, a.status);  // complete: makes the copies visible to each thread
-  Stats st;
-  st.init();
-  constexpr int U = 2;  // 16-byte pieces at a time
-  const int nv = n / VEC;
-  const uint4* s_vec = reinterpret_cast<const uint4*>(s_row_raw);
-  int v = tid;
-  for (; v + (U - 1) * kThreads < nv; v += U * kThreads) {
-    uint32_t w[4 * U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint4 f = s_vec[v + u * kThreads];
-      w[4 * u] = f.x; w[4 * u + 1] = f.y; w[4 * u + 2] = f.z; w[4 * u + 3] = f.w;
-    }
-    st.template add_words<T>(w, words_max<T>(w), q);
-  }
-  for (; v < nv; v += kThreads) {
-    const uint4 f = s_vec[v];
-    const uint32_t w[4] = {f.x, f.y, f.z, f.w};
-    st.template add_words<T>(w, words_max<T>(w), q);
-  }
-  if (warp < 2 && lane < (warp == 0 ? head_here : tail_here)) {
-    const float x[1] = {s_edge[warp][lane]};
-    st.add(x, q);
-  }
-  st.warp_merge(q);
-  if (lane == 0) s_warp[warp] = st;
-  __syncthreads();
   if (warp == 0) {
-    st.init();
-    if (lane < kWarps) st = s_warp[lane];
-    st.warp_merge(q);
-    if (lane == 0) { s_share[0] = st.m; s_share[1] = st.s; }
-  }
-  if (cs > 1) {
-    row_cluster_sync();
-    if (warp == 0) {
-      st.init();
-      if (lane < cs) {  // every CTA joins them in the same way
-        const float m = __uint_as_float(ld_cluster_u32(&s_share[0], lane));
-        st.s = __uint_as_float(ld_cluster_u32(&s_share[1], lane));
-        if (m != -INFINITY) { st.m = m; st.mu = squash<CAP>(m, q); }
-      }
-      st.warp_merge(q);
-    }
-  }
-
-  // ---- loss and coefficients
-  const float scale = GRAD ? (a.inv_n ? a.scale * *a.inv_n : a.scale) : 1.f;
-  float gk[S];
-  if (warp == 0) {
-    Stats all = st;
-    all.merge(top, q);
-    const float logs = logf(all.s);
-    const bool empty = all.s == 0.f;  // every logit is -inf: no distribution, no gradient
-    float loss = 0.f;
-#pragma unroll
-    for (int j = 0; j < S; ++j) {
-      const float lpk = (empty || yk[j] == -INFINITY) ? -INFINITY : (yk[j] - all.mu) * q.inv_t - logs;
-      if (idx[j] >= 0 && qk[j] != 0.f) loss += qk[j] * (logq[j] - lpk);
-      gk[j] = 0.f;
-      if (idx[j] >= 0 && !none && !empty) gk[j] = (expf(lpk) - mass[j]) * squash_slope<CAP>(yk[j], q);
-      if (bad) gk[j] = NAN;
-    }
-    loss = warp_sum(loss);
-    // the scale of p in units of e: p = e 2^(kl (mu_rest - mu)) / S
-    float c = (none || st.s == 0.f) ? 0.f : ex2((st.mu - all.mu) * q.kl) / all.s;
-    // The rest is left out where the student has masked it: no logit outside the teacher's tokens
-    // above -inf, or none within kMasked of the largest (a mask of the type's lowest value).
-    if (rest > 0.f && st.s != 0.f && !none && !(st.mu - all.mu < -kMasked)) {
-      loss += rest * (logf(rest) - ((st.mu - all.mu) * q.inv_t + logf(st.s) - logs));
-      c -= rest / st.s;
-    }
-    if (bad) { loss = NAN; c = NAN; }
+    // ---------------- loader
     if (lane == 0) {
-      if (rank == 0) a.losses[r] = loss;
-      s_out[0] = st.mu;
-      s_out[1] = c * scale;
-      if (!GRAD && rank == 0 && a.rest) a.rest[r] = make_float2(st.mu, c);
-    }
-    if (!GRAD && rank == 0 && a.gk) {
-#pragma unroll
-      for (int j = 0; j < S; ++j)
-        if (32 * j + lane < a.K) a.gk[r * a.K + 32 * j + lane] = gk[j];
-    }
-  }
-
-  if constexpr (GRAD) {
-    __syncthreads();
-    if (cs > 1) row_cluster_arrive_relaxed();  // this CTA has read the others' statistics
-    const float mu = s_out[0], cg = s_out[1];
-    for (int u = tid; u < nv; u += kThreads) {
-      const uint4 f = s_vec[u];
-      const uint32_t w[4] = {f.x, f.y, f.z, f.w};
-      float x[VEC];
-      rest_grads<T, CAP>(x, w, mu, cg, q);
-      T* out = grow + body0 + u * VEC;
-      if (vec) store_frag<T, VEC>(out, x);
-      else
-        for (int i = 0; i < VEC; ++i) out[i] = from_f<T>(x[i]);
-    }
-    if (warp < 2 && lane < (warp == 0 ? head_here : tail_here))
-      grow[(warp == 0 ? 0 : tail0) + lane] = from_f<T>(rest_grad<CAP>(s_edge[warp][lane], mu, cg, q));
-    __syncthreads();  // the teacher's tokens over what was written for them
-    if (warp == 0) {
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        const int i = idx[j];
-        if (i >= 0 && ((i >= body0 && i < body0 + n) || i < head_here || (i >= tail0 && i - tail0 < tail_here)))
-          grow[i] = from_f<T>(gk[j] * scale);
+      uint32_t ph = 0;
+      for (int64_t r = first; r < a.rows; r += step, ph ^= 1u) {
+        const bool live = a.mask == nullptr || a.mask[r] != 0;
+        const Share<T> sh(logits + a.addr.off(r), a.V, rank, a.log_cs);
+        const uint32_t bytes = live ? (uint32_t)(sh.n * sizeof(T)) : 0u;
+        const char* src = reinterpret_cast<const char*>(sh.row + sh.body0);
+        for (int c = 0; c < kPieces; ++c) {
+          wait.operator()<false>(&left[c], ph ^ 1u);
+          if (*wait.abort) break;
+          if (c == 0) mbar_expect_tx(&full, bytes);
+          // the generic accesses to the piece (the teacher's writes among them) before the copy
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          const uint32_t o = c * a.piece;
+          if (o < bytes) bulk_g2s(s_row + o, src + o, min(a.piece, bytes - o), &full);
+        }
+        // last: until now the row is not complete, so nobody can leave a piece for the second time
+        // before this warp has seen the first
+        if (!*wait.abort) mbar_arrive(&full);
       }
     }
-  } else if (cs > 1) {
-    row_cluster_arrive_relaxed();
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- teacher
+    Entries entries;  // of the next row, on their way while this one is worked on
+    if (first < a.rows) entries.load(a, first);
+    int it = 0;
+    for (int64_t r = first; r < a.rows; r += step, ++it) {
+      const int b = it & 1;
+      const bool live = a.mask == nullptr || a.mask[r] != 0;
+      const Share<T> sh(logits + a.addr.off(r), a.V, rank, a.log_cs);
+      TeacherRow& out = s_teacher[b];
+      TeacherRow head;
+      int idx[kSlots];
+      float qk[kSlots], logq[kSlots], yk[kSlots], mass[kSlots], e0 = 0.f, e1 = 0.f;
+      const Entries now = entries;
+      if (r + step < a.rows) entries.load(a, r + step);
+      if (live) {  // all that needs no shared row
+        if (lane < sh.head_here) e0 = to_f<T>(sh.row[lane]);
+        if (lane < sh.tail_here) e1 = to_f<T>(sh.row[sh.tail0 + lane]);
+        teacher_row<T, CAP>(head, idx, qk, logq, yk, mass, now, sh.row, a, s_idx, s_q, s_tag);
+      }
+      wait.operator()<false>(&done[b], ((uint32_t)(it >> 1) & 1u) ^ 1u);
+      wait.operator()<false>(&full, (uint32_t)it & 1u);
+      if (live) {
+        s_edge[b][0][lane] = e0;
+        s_edge[b][1][lane] = e1;
+        __syncwarp();
+        T* buf = reinterpret_cast<T*>(s_row);
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) {
+          if (32 * j >= a.K) break;
+          const int k = 32 * j + lane, i = idx[j];
+          out.idx[k] = i;
+          out.q[k] = qk[j];
+          out.logq[k] = logq[j];
+          out.y[k] = yk[j];
+          out.mass[k] = mass[j];
+          if (i < 0) continue;
+          if (i >= sh.body0 && i < sh.body0 + sh.n) buf[i - sh.body0] = from_f<T>(-INFINITY);
+          else if (i < sh.head_here) s_edge[b][0][i] = -INFINITY;
+          else if (i >= sh.tail0 && i - sh.tail0 < sh.tail_here) s_edge[b][1][i - sh.tail0] = -INFINITY;
+        }
+        if (lane == 0) {
+          out.m = head.m;
+          out.lim = head.lim;
+          out.s = head.s;
+          out.r = head.r;
+          out.rest = head.rest;
+          out.none = head.none;
+          out.bad = head.bad;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ready[b]);
+    }
+  } else if (warp == 2) {
+    // ---------------- finisher
+    const float scale = GRAD ? (a.inv_n ? a.scale * *a.inv_n : a.scale) : 1.f;
+    int it = 0;
+    for (int64_t r = first; r < a.rows; r += step, ++it) {
+      const int b = it & 1;
+      const bool live = a.mask == nullptr || a.mask[r] != 0;
+      // for a masked row too: no second arrival on done[b] before its phase has ended
+      wait.operator()<false>(&ready[b], (uint32_t)(it >> 1) & 1u);
+      if (live) {
+        named_sync(2, kCompute + 32);  // compute is done with the row
+        const TeacherRow& tr = s_teacher[b];
+        const FinishRow fin = s_fin[b];
+        const Share<T> sh(logits + a.addr.off(r), a.V, rank, a.log_cs);
+        T* grow = GRAD ? reinterpret_cast<T*>(a.grad) + r * a.V : nullptr;
+        float loss = 0.f;
+        for (int k = lane; k < a.K; k += 32) {
+          const int i = tr.idx[k];
+          const float qk = tr.q[k], yk = tr.y[k];
+          const float lpk = (fin.empty || yk == -INFINITY) ? -INFINITY : log_prob(yk, fin.all, fin.logs, q);
+          if (i >= 0 && qk != 0.f) loss += qk * (tr.logq[k] - lpk);
+          float gk = 0.f;
+          if (i >= 0 && !tr.none && !fin.empty) gk = (expf(lpk) - tr.mass[k]) * squash_slope<CAP>(yk, q);
+          if (tr.bad) gk = NAN;
+          if constexpr (GRAD) {
+            if (i >= 0 && sh.has(i)) grow[i] = from_f<T>(gk * scale);
+          } else {
+            if (rank == 0 && a.gk) a.gk[r * a.K + k] = gk;
+          }
+        }
+        loss = warp_sum(loss) + fin.tail_loss;
+        if (rank == 0 && lane == 0) {
+          a.losses[r] = tr.bad ? NAN : loss;
+          if (!GRAD && a.rest) a.rest[r] = make_float4(fin.rest.sh, fin.rest.k, fin.c, 0.f);
+        }
+      } else if (rank == 0) {
+        if (lane == 0) {
+          a.losses[r] = 0.f;
+          if (!GRAD && a.rest) a.rest[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (!GRAD && a.gk)
+          for (int k = lane; k < a.K; k += 32) a.gk[r * a.K + k] = 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&done[b]);
+    }
+  } else {
+    // ---------------- compute
+    const int cw = warp - kRoles, ct = tid - 32 * kRoles;
+    const float scale = GRAD ? (a.inv_n ? a.scale * *a.inv_n : a.scale) : 1.f;
+    const uint4* s_vec = reinterpret_cast<const uint4*>(s_row);
+    const int pv = (int)(a.piece / 16);
+    int it = 0, nlive = 0;
+    for (int64_t r = first; r < a.rows; r += step, ++it) {
+      const int b = it & 1;
+      const bool live = a.mask == nullptr || a.mask[r] != 0;
+      const Share<T> sh(logits + a.addr.off(r), a.V, rank, a.log_cs);
+      const int nv = sh.n / VEC;
+      T* grow = GRAD ? reinterpret_cast<T*>(a.grad) + r * a.V : nullptr;
+      const bool vec = GRAD && (reinterpret_cast<uintptr_t>(grow + sh.body0) & 15u) == 0;
+      // hands back the pieces before this warp's next 16 bytes, v (of its first lane)
+      int piece = 0;
+      auto leave = [&](int v) {
+        while (piece < kPieces && v >= (piece + 1) * pv) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&left[piece]);
+          ++piece;
+        }
+      };
+      Ref rest_ref{0.f, 0.f};
+      float cg = 0.f;  // a masked row: zeros, whatever it holds
+      wait.operator()<false>(&ready[b], (uint32_t)(it >> 1) & 1u);
+      if (live) {
+        wait.operator()<false>(&full, (uint32_t)it & 1u);  // complete: makes the copies visible to this thread
+        const int lb = nlive & 1;
+        const uint32_t lph = (uint32_t)(nlive >> 1) & 1u;
+        ++nlive;
+        Stats st;
+        st.init();
+        int v = ct;
+        for (; v + (U - 1) * kCompute < nv; v += U * kCompute) {
+          uint32_t w[4 * U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const uint4 f = s_vec[v + u * kCompute];
+            w[4 * u] = f.x; w[4 * u + 1] = f.y; w[4 * u + 2] = f.z; w[4 * u + 3] = f.w;
+          }
+          st.template add_words<T>(w, words_max<T>(w), q);
+          if constexpr (!GRAD) leave(v - lane + U * kCompute);
+        }
+        for (; v < nv; v += kCompute) {
+          const uint4 f = s_vec[v];
+          const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+          st.template add_words<T>(w, words_max<T>(w), q);
+        }
+        if constexpr (!GRAD) leave(kPieces * pv);
+        const int e = cw * 32 + lane;  // head and tail: loose elements 0 .. 31, 32 .. 63
+        for (int i = e; i < 64; i += kCompute)
+          if ((i & 31) < (i < 32 ? sh.head_here : sh.tail_here)) st.add1(s_edge[b][i >> 5][i & 31], q);
+        st.warp_merge(q);
+        if (lane == 0) s_warp[lb][cw] = st;
+        named_sync(1, kCompute);
+        st.init();
+        if (lane < W) st = s_warp[lb][lane];
+        st.warp_merge(q);
+        if (cs > 1) {
+          if (cw == 0 && lane < cs) {  // to every CTA of the cluster
+            uint32_t at, bar;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&s_joined[lb][rank])), "r"(lane));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&joined[lb])), "r"(lane));
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(st.m), "f"(st.r.sh),
+                         "f"(st.r.k), "f"(st.s)
+                         : "memory");
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+          }
+          wait.operator()<true>(&joined[lb], lph);
+          st.init();
+          if (lane < cs) {  // every warp of every CTA joins them in the same way
+            const float4 o = s_joined[lb][lane];
+            st.m = o.x;
+            st.r = Ref{o.y, o.z};
+            st.s = o.w;
+            if (o.w > 0.f) st.lim = 0.f;  // something was seen
+          }
+          st.warp_merge(q);
+        }
+        const TeacherRow& tr = s_teacher[b];
+        Stats all = st, top;
+        top.m = tr.m;
+        top.lim = tr.lim;
+        top.s = tr.s;
+        top.r = tr.r;
+        all.merge(top, q);
+        all.center();
+        const float logs = logf(all.s);
+        // the scale of p in units of e: p = e 2^(rest's reference - the row's) / S
+        const float below = ref_diff(st.r, all.r, q);
+        float c = (tr.none || st.s == 0.f) ? 0.f : ex2(below) / all.s;
+        // The rest is left out where the student has masked it: no logit outside the teacher's
+        // tokens above -inf, or none within kMasked of the largest (a mask of the type's lowest value).
+        const float rest = tr.rest;
+        float tail_loss = 0.f;
+        if (rest > 0.f && st.s != 0.f && !tr.none && !(squash<CAP>(st.m, q) - squash<CAP>(all.m, q) < -kMasked)) {
+          tail_loss = rest * (logf(rest) - (fmaf(below, kLn2, logf(st.s)) - logs));
+          c -= rest / st.s;
+        }
+        if (tr.bad) c = NAN;
+        if (cw == 0 && lane == 0) {
+          FinishRow f;
+          f.all = all.r;
+          f.rest = st.r;
+          f.logs = logs;
+          f.tail_loss = tail_loss;
+          f.c = c;
+          f.empty = all.s == 0.f;  // every logit is -inf: no distribution, no gradient
+          s_fin[b] = f;
+        }
+        rest_ref = st.r;
+        cg = c * scale;
+      }
+      if constexpr (GRAD) {
+        T* gbody = grow + sh.body0;
+        int u = ct;
+        for (; u + (U - 1) * kCompute < nv; u += U * kCompute) {
+          uint4 f[U];
+#pragma unroll
+          for (int j = 0; j < U; ++j) f[j] = s_vec[u + j * kCompute];
+#pragma unroll
+          for (int j = 0; j < U; ++j)
+            store_grads<T, CAP>(gbody + (u + j * kCompute) * VEC, f[j], rest_ref, cg, q, vec);
+          leave(u - lane + U * kCompute);
+        }
+        for (; u < nv; u += kCompute) store_grads<T, CAP>(gbody + u * VEC, s_vec[u], rest_ref, cg, q, vec);
+        const int e = cw * 32 + lane;
+        for (int i = e; i < 64; i += kCompute)
+          if ((i & 31) < (i < 32 ? sh.head_here : sh.tail_here))
+            grow[(i < 32 ? 0 : sh.tail0) + (i & 31)] =
+                from_f<T>(rest_grad<CAP>(s_edge[b][i >> 5][i & 31], rest_ref, cg, q));
+      }
+      leave(kPieces * pv);
+      if (live) named_arrive(2, kCompute + 32);  // the finisher writes over what was stored here
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&done[b]);
+    }
   }
-  if (cs > 1) row_cluster_wait();  // the others have read this one's
+  __syncthreads();
+  if (s_abort) {  // a copy may still be on its way into this CTA's shared memory
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+  if (cs > 1) row_cluster_sync();  // no more statistics from the other CTAs
 }
 
 struct DistillBwdArgs {
-  const float2* rest;
+  const float4* rest;
   const float* gk;
   const int64_t* idx;
   const uint8_t* mask;
@@ -382,7 +652,7 @@ struct DistillBwdArgs {
 constexpr int kBwdBatch = 2;
 constexpr int kBwdGroups = kThreads * kBwdBatch;
 
-// The gradient from the forward's (mu_rest, c) and K numbers a row: each CTA takes one segment of a
+// The gradient from the forward's reference, c and K numbers a row: each CTA takes one segment of a
 // row, then writes those of the teacher's tokens that lie in it.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kThreads)
@@ -398,8 +668,9 @@ distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Dis
   const bool vec = (reinterpret_cast<uintptr_t>(grow + cut.head) & 31u) == 0;
   const bool live = a.mask == nullptr || a.mask[r] != 0;
   const float scale = a.scale * (a.inv_n ? *a.inv_n : 1.f) * *a.g_loss;
-  const float2 rc = a.rest[r];
-  const float mu = rc.x, c = live ? rc.y * scale : 0.f;  // c = 0: zeros, whatever the row holds
+  const float4 rc = a.rest[r];
+  const Ref ref{rc.x, rc.y};
+  const float c = live ? rc.z * scale : 0.f;  // c = 0: zeros, whatever the row holds
   const int gbeg = seg * kBwdGroups;
   const T* body = row + cut.head;
   T* gbody = grow + cut.head;
@@ -416,15 +687,15 @@ distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Dis
       float x[kGroup];
 #pragma unroll
       for (int h = 0; h < (int)sizeof(T) / 2; ++h)
-        rest_grads<T, CAP>(x + h * 16 / ((int)sizeof(T) / 2), raw[u].r[h].w, mu, c, q);
+        rest_grads<T, CAP>(x + h * 16 / ((int)sizeof(T) / 2), raw[u].r[h].w, ref, c, q);
       store_group<T>(gbody + (int64_t)g * kGroup, x, vec);
     }
   }
   const int tail0 = cut.head + cut.groups * kGroup;
   const bool first = seg == 0, last = seg == a.segs - 1;
-  if (first && tid < cut.head) grow[tid] = from_f<T>(rest_grad<CAP>(to_f<T>(row[tid]), mu, c, q));
+  if (first && tid < cut.head) grow[tid] = from_f<T>(rest_grad<CAP>(to_f<T>(row[tid]), ref, c, q));
   if (last && tid < cut.tail)
-    grow[tail0 + tid] = from_f<T>(rest_grad<CAP>(to_f<T>(row[tail0 + tid]), mu, c, q));
+    grow[tail0 + tid] = from_f<T>(rest_grad<CAP>(to_f<T>(row[tail0 + tid]), ref, c, q));
   if (!live) return;
   __syncthreads();
   if (tid < a.K) {
@@ -470,13 +741,13 @@ distill_mean(float* __restrict__ loss, const float* __restrict__ losses, const f
 
 int64_t share_bytes(int64_t V, int cs, int es) { return ((V / kGroup + cs - 1) / cs) * kGroup * es; }
 
-// CTAs per row: as many as bring the share to kShareWanted, and more while the rows leave SMs
-// without a CTA and each CTA keeps half a group per thread.
-int cluster_for(int64_t rows, int64_t V, int es) {
-  int cs = 1;
-  while (cs < kMaxCluster && share_bytes(V, cs, es) > kShareWanted) cs *= 2;
-  while (cs < kMaxCluster && rows * cs * 2 <= sm_count() * 2 && V / (2 * cs) >= kThreads * kGroup / 2) cs *= 2;
-  return cs;
+// log2 of the CTAs per row: as many as let two CTAs' shares fit an SM, and more while the rows leave
+// SMs without a CTA and each CTA keeps half a group per thread.
+int log_cluster_for(int64_t rows, int64_t V, int es) {
+  int l = 0;
+  while ((1 << l) < kMaxCluster && share_bytes(V, 1 << l, es) > kShareWanted) ++l;
+  while ((1 << l) < kMaxCluster && (rows << (l + 1)) <= sm_count() && (V >> (l + 1)) >= 32 * kWide * kGroup / 2) ++l;
+  return l;
 }
 
 int check_args(const char* what, const void* logits, int64_t rows, int64_t inner, int64_t V, int64_t K,
@@ -497,16 +768,29 @@ int check_args(const char* what, const void* logits, int64_t rows, int64_t inner
   return AK_OK;
 }
 
-template <typename T>
-int launch_fwd(const T* logits, const DistillArgs& a, int64_t rows, cudaStream_t st) {
+template <typename T, int W>
+int launch_width(const T* logits, DistillArgs& a, int64_t share, cudaStream_t st) {
   const bool cap = a.q.cap > 0.f;
-  auto kern = a.grad ? (cap ? distill_fwd_kernel<T, true, true> : distill_fwd_kernel<T, false, true>)
-                     : (cap ? distill_fwd_kernel<T, true, false> : distill_fwd_kernel<T, false, false>);
-  const size_t smem = (size_t)share_bytes(a.V, a.cs, sizeof(T)) + 16;
+  auto kern = a.grad ? (cap ? distill_fwd_kernel<T, true, true, W> : distill_fwd_kernel<T, false, true, W>)
+                     : (cap ? distill_fwd_kernel<T, true, false, W> : distill_fwd_kernel<T, false, false, W>);
+  const int cs = 1 << a.log_cs;
+  a.piece = (uint32_t)((share + kPieces * 16 - 1) / (kPieces * 16) * 16);
+  const size_t smem = (size_t)std::max<int64_t>(share, 16);
   AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
               "ak_distill_topk_fwd: shared memory");
-  AK_CUDA_TRY(launch_rows(kern, rows * a.cs, kThreads, a.cs, smem, st, logits, a), "ak_distill_topk_fwd");
+  int clusters = 0;
+  AK_CUDA_TRY(resident_clusters(kern, 32 * (W + kRoles), cs, smem, &clusters), "ak_distill_topk_fwd: occupancy");
+  const int64_t grid = std::min<int64_t>(a.rows, clusters) * cs;
+  AK_CUDA_TRY(launch_rows(kern, grid, 32 * (W + kRoles), cs, smem, st, logits, (const DistillArgs&)a),
+              "ak_distill_topk_fwd");
   return AK_OK;
+}
+
+template <typename T>
+int launch_fwd(const T* logits, DistillArgs& a, cudaStream_t st) {
+  const int64_t share = share_bytes(a.V, 1 << a.log_cs, sizeof(T));
+  return share <= kShareNarrow ? launch_width<T, kNarrow>(logits, a, share, st)
+                               : launch_width<T, kWide>(logits, a, share, st);
 }
 
 }  // namespace
@@ -525,6 +809,7 @@ extern "C" int ak_distill_topk_fwd(float* loss, float* losses, float* inv_n, voi
   AK_REQUIRE(loss, AK_ERR_ARG, "ak_distill_topk_fwd: null pointer");
   AK_REQUIRE(rows == 0 || (losses && teacher_idx && teacher_lp && (!mask || inv_n)), AK_ERR_ARG,
              "ak_distill_topk_fwd: null pointer");
+  AK_REQUIRE(aligned16(rest_stats), AK_ERR_ARG, "ak_distill_topk_fwd: rest_stats not 16-byte aligned");
   AK_REQUIRE(!grad || (!rest_stats && !gk), AK_ERR_ARG,
              "ak_distill_topk_fwd: the gradient, or what its kernel needs, not both");
   AK_REQUIRE((reinterpret_cast<uintptr_t>(grad) % elem_size(dt)) == 0, AK_ERR_ARG,
@@ -537,15 +822,15 @@ extern "C" int ak_distill_topk_fwd(float* loss, float* losses, float* inv_n, voi
     }
     DistillArgs a{};
     a.losses = losses; a.grad = grad;
-    a.rest = reinterpret_cast<float2*>(rest_stats);
+    a.rest = reinterpret_cast<float4*>(rest_stats);
     a.gk = gk; a.idx = teacher_idx; a.tlp = teacher_lp; a.mask = mask;
     a.inv_n = mask ? inv_n : nullptr;
     a.addr = RowAddr{inner, stride_outer, stride_inner};
     a.scale = mask ? temperature : temperature / (float)rows;
-    a.V = (int)V; a.K = (int)K; a.cs = cluster_for(rows, V, elem_size(dt)); a.tail = tail != 0;
+    a.rows = rows; a.V = (int)V; a.K = (int)K; a.log_cs = log_cluster_for(rows, V, elem_size(dt)); a.tail = tail != 0;
     a.q = make_squash(temperature, softcap);
     a.status = status;
-    AK_DISPATCH_DTYPE(dt, T, rc = launch_fwd<T>((const T*)logits, a, rows, st));
+    AK_DISPATCH_DTYPE(dt, T, rc = launch_fwd<T>((const T*)logits, a, st));
     if (rc) return rc;
   }
   distill_mean<<<1, 1024, 0, st>>>(loss, losses, (mask && rows > 0) ? inv_n : nullptr,
@@ -563,12 +848,12 @@ extern "C" int ak_distill_topk_bwd(void* grad, const void* logits, const int64_t
   int rc = check_args("ak_distill_topk_bwd", logits, rows, inner, V, K, temperature, softcap, dt);
   if (rc) return rc;
   if (rows == 0) return AK_OK;
-  AK_REQUIRE(grad && teacher_idx && rest_stats && gk && g_loss && (!mask || inv_n), AK_ERR_ARG,
-             "ak_distill_topk_bwd: null pointer");
+  AK_REQUIRE(grad && teacher_idx && rest_stats && aligned16(rest_stats) && gk && g_loss && (!mask || inv_n), AK_ERR_ARG,
+             "ak_distill_topk_bwd: null pointer, or rest_stats not 16-byte aligned");
   AK_REQUIRE((reinterpret_cast<uintptr_t>(grad) % elem_size(dt)) == 0, AK_ERR_ARG,
              "ak_distill_topk_bwd: grad not aligned to its type");
   DistillBwdArgs a{};
-  a.rest = reinterpret_cast<const float2*>(rest_stats);
+  a.rest = reinterpret_cast<const float4*>(rest_stats);
   a.gk = gk; a.idx = teacher_idx; a.mask = mask; a.inv_n = mask ? inv_n : nullptr; a.g_loss = g_loss;
   a.addr = RowAddr{inner, stride_outer, stride_inner};
   a.scale = mask ? temperature : temperature / (float)rows;

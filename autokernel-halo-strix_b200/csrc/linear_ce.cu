@@ -87,11 +87,11 @@ struct Prob {
   const float* add_f32;     // nullable, same layout as C
   const float* scale;       // nullable device scalar multiplying acc (before add_f32 / accumulate)
   int c_f32, accumulate;
-  // EPI_LOGP: part (largest logit, S), partw (the entropy's sum; nullable) and tlogit.
+  // EPI_LOGP: lpart (reference, S, the entropy's sum if want_ent) and tlogit.
   // EPI_LOGP_GRAD: C (ldc) = gradient of the logits / *scale, from the rows' statistics
-  float* partw;             // [M][kEpiGroups * ntiles]
-  const float2* stats;      // [M] (mu, log S)
-  const float* entropy;     // [M], with g_ent
+  float4* lpart;            // [M][kEpiGroups * ntiles]
+  int want_ent;
+  const float4* stats;      // [M] (reference, log S, entropy)
   const float* g_lp;        // nullable [M]
   const float* g_ent;       // nullable [M]
   Squash q;
@@ -560,16 +560,16 @@ __device__ __forceinline__ void epi_store(const Prob& P, uint32_t tbase, int row
 
 // One 32-column chunk into a row's statistics; columns from P.N on hold nothing.
 template <bool CAP, bool ENT>
-__device__ __forceinline__ void logp_chunk(const float (&v)[32], RowStats<true, true>& st, const Squash& q) {
+__device__ __forceinline__ void logp_chunk(const uint32_t (&v)[32], RowStats<true, true>& st, const Squash& q) {
   RowStats<CAP, ENT> a;
-  a.m = st.m; a.mu = st.mu; a.s = st.s;
+  a.m = st.m; a.lim = st.lim; a.s = st.s; a.r = st.r;
   if constexpr (ENT) a.w = st.w;
-  a.add(v, q);
-  st.m = a.m; st.mu = a.mu; st.s = a.s;
+  a.template add_words<float>(v, words_max<float>(v), q);
+  st.m = a.m; st.lim = a.lim; st.s = a.s; st.r = a.r;
   if constexpr (ENT) st.w = a.w;
 }
 
-// Per-row softmax statistics of this warpgroup's 128 columns, with the entropy's sum if P.partw,
+// Per-row softmax statistics of this warpgroup's 128 columns, with the entropy's sum if asked for,
 // and the target logit.  Nothing else is stored.
 template <typename T>
 __device__ __forceinline__ void epi_logp(const Prob& P, uint32_t tbase, int row0, int lane, int64_t lab, int col0,
@@ -577,7 +577,7 @@ __device__ __forceinline__ void epi_logp(const Prob& P, uint32_t tbase, int row0
   const int row = row0 + lane;
   const int c0 = eg * kGroupCols;
   const Squash q = P.q;
-  const bool cap = q.cap > 0.f, ent = P.partw != nullptr;
+  const bool cap = q.cap > 0.f, ent = P.want_ent != 0;
   RowStats<true, true> st;
   st.init();
   Tm32 buf[2];
@@ -587,20 +587,20 @@ __device__ __forceinline__ void epi_logp(const Prob& P, uint32_t tbase, int row0
 #pragma unroll
   for (int k = 0; k < kGroupCols / 32; ++k) {
     if (k + 1 < kGroupCols / 32) tmem_ld_issue(tbase + (uint32_t)(c0 + 32 * (k + 1)), buf[(k + 1) & 1]);
-    float v[32];
+    uint32_t v[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[k & 1].r[j]);
+    for (int j = 0; j < 32; ++j) v[j] = buf[k & 1].r[j];
     const int cbase = col0 + c0 + 32 * k;
     const int rel = (int)(lab - cbase);  // lab is -1 where the row has no target (or is no row)
     if ((unsigned)rel < 32u) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (j == rel) P.tlogit[row] = v[j];
+        if (j == rel) P.tlogit[row] = __uint_as_float(v[j]);
     }
     if (cbase + 32 > P.N) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (cbase + j >= P.N) v[j] = -INFINITY;
+        if (cbase + j >= P.N) v[j] = __float_as_uint(-INFINITY);
     }
     if (!cap && ent) logp_chunk<false, true>(v, st, q);
     else if (!cap) logp_chunk<false, false>(v, st, q);
@@ -608,17 +608,16 @@ __device__ __forceinline__ void epi_logp(const Prob& P, uint32_t tbase, int row0
     else logp_chunk<true, false>(v, st, q);
     if (k + 1 < kGroupCols / 32) tmem_ld_wait(buf[(k + 1) & 1]);
   }
-  if (row < P.M) {
-    const int64_t at = (int64_t)row * (kEpiGroups * P.ntiles) + kEpiGroups * (col0 / BN) + eg;
-    P.part[at] = make_float2(st.m, st.s);
-    if (ent) P.partw[at] = st.w;
-  }
+  if (row < P.M)
+    P.lpart[(int64_t)row * (kEpiGroups * P.ntiles) + kEpiGroups * (col0 / BN) + eg] =
+        make_float4(st.r.sh, st.r.k, st.s, st.w);
 }
 
-// What a lane needs to turn its row's logits into their gradient: with d = (y - mu) kl - log2 S and
-// p = 2^d, dx = (p (c0 + c1 d) [+ ct at the target]) * slope of the softcap.
+// What a lane needs to turn its row's logits into their gradient: with e = 2^d against the row's
+// reference, dx = (e (c0 + c1 d) [+ ct at the target]) * slope of the softcap.
 struct LogpRow {
-  float mu, l2s, c0, c1, ct;
+  Ref ref;
+  float c0, c1, ct;
   int t;      // target column, or -1
   bool none;  // no gradient: ignored, no distribution, or no such row
 };
@@ -629,17 +628,17 @@ __device__ __forceinline__ LogpRow load_logp_row(const Prob& P, int row) {
   r.none = true;
   if (row >= P.M) return r;
   const int64_t lab = P.labels ? P.labels[row] : -1;
-  const float2 ml = P.stats[row];
-  r.none = (P.labels && lab == P.ignore_index) || ml.y == -INFINITY;
+  const float4 st = P.stats[row];
+  const float logs = st.z, H = st.w;
+  r.none = (P.labels && lab == P.ignore_index) || logs == -INFINITY;
   float gl = (P.labels && P.g_lp) ? P.g_lp[row] : 0.f;
   if (P.labels && !r.none && (lab < 0 || lab >= P.N)) gl = NAN;
   else r.t = (int)lab;
-  const float ge = P.g_ent ? P.g_ent[row] : 0.f, H = P.g_ent ? P.entropy[row] : 0.f;
-  const float f = P.q.inv_t / (P.scale ? *P.scale : 1.f);
-  r.mu = ml.x;
-  r.l2s = ml.y * kLog2e;
-  r.c0 = -(gl + ge * H) * f;
-  r.c1 = -ge * kLn2 * f;
+  const float ge = P.g_ent ? P.g_ent[row] : 0.f;
+  const float f = P.q.inv_t / (P.scale ? *P.scale : 1.f), fs = f * expf(-logs);
+  r.ref = Ref{st.x, st.y};
+  r.c0 = (ge * (logs - H) - gl) * fs;
+  r.c1 = -ge * kLn2 * fs;
   r.ct = gl * f;
   return r;
 }
@@ -672,7 +671,7 @@ __device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int
     } else if (!cap) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        const float d = (v[j] - lr.mu) * q.kl - lr.l2s;
+        const float d = exponent(v[j], lr.ref, q);
         float o = ex2(d) * fmaf(lr.c1, fmaxf(d, -1e4f), lr.c0);
         if (j == rel) o += lr.ct;
         v[j] = o;
@@ -681,7 +680,7 @@ __device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         const float y = squash<true>(v[j], q);
-        const float d = (y - lr.mu) * q.kl - lr.l2s;
+        const float d = exponent(y, lr.ref, q);
         float o = ex2(d) * fmaf(lr.c1, fmaxf(d, -1e4f), lr.c0);
         if (j == rel) o += lr.ct;
         v[j] = o * squash_slope<true>(y, q);
@@ -986,23 +985,24 @@ lce_grad_inplace(T* __restrict__ L, const float* __restrict__ lse, const int64_t
 template <bool CAP>
 __global__ void __launch_bounds__(256)
 logp_rows_reduce(float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ lse,
-                 float2* __restrict__ stats, const float2* __restrict__ part, const float* __restrict__ partw,
-                 const float* __restrict__ tlogit, const int64_t* __restrict__ labels, int M, int V, int nparts,
-                 int64_t ignore_index, const Squash q) {
+                 float4* __restrict__ stats, const float4* __restrict__ part, const float* __restrict__ tlogit,
+                 const int64_t* __restrict__ labels, int M, int V, int nparts, int64_t ignore_index, const Squash q) {
   const int row = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
   if (row >= M) return;
   RowStats<CAP, true> st;
   st.init();
   for (int t = lane; t < nparts; t += 32) {
-    const float2 p = part[(int64_t)row * nparts + t];
+    const float4 p = part[(int64_t)row * nparts + t];
     RowStats<CAP, true> o;
     o.init();
-    if (p.x != -INFINITY) { o.m = p.x; o.mu = squash<CAP>(p.x, q); }
-    o.s = p.y;
-    o.w = partw ? partw[(int64_t)row * nparts + t] : 0.f;
+    o.r = Ref{p.x, p.y};
+    o.s = p.z;
+    o.w = p.w;
+    if (o.s > 0.f) o.lim = 0.f;  // something was seen
     st.merge(o, q);
   }
   st.warp_merge(q);
+  st.center();
   if (lane != 0) return;
   const float logs = logf(st.s);
   const int64_t t = labels ? labels[row] : -1;
@@ -1012,13 +1012,14 @@ logp_rows_reduce(float* __restrict__ logprobs, float* __restrict__ entropy, floa
     if (!ignored) {
       if (t < 0 || t >= V) lp = NAN;  // not a token
       else if (st.s == 0.f) lp = -INFINITY;
-      else lp = (squash<CAP>(tlogit[row], q) - st.mu) * q.inv_t - logs;
+      else lp = log_prob(squash<CAP>(tlogit[row], q), st.r, logs, q);
     }
     logprobs[row] = lp;
   }
-  if (entropy) entropy[row] = (ignored || st.s == 0.f) ? 0.f : logs - (st.w / st.s) * q.inv_t;
-  lse[row] = st.mu * q.inv_t + logs;
-  if (stats) stats[row] = make_float2(st.mu, logs);
+  const float H = (ignored || st.s == 0.f) ? 0.f : fmaf(-kLn2, st.w / st.s, logs);
+  if (entropy) entropy[row] = H;
+  lse[row] = ref_lse(st.r, logs, q);
+  if (stats) stats[row] = make_float4(st.r.sh, st.r.k, logs, H);
 }
 
 // scale[0] = largest |g_lp| + |g_ent| over the rows (1 where that is 0 or not finite): divides the
@@ -1290,8 +1291,7 @@ int run(float* loss, float* lse, void* dH, void* dW, const Ws& w, const void* H,
 // Token log-probabilities.  Workspace: the tiles' statistics of one chunk (forward), or the chunk's
 // 16-bit gradient of the logits, rows padded to 8 elements, and the fp32 dW accumulator (backward).
 struct LogpWs {
-  float2* part;
-  float* partw;
+  float4* part;
   float* tlogit;
   void* G;
   float* scale;
@@ -1314,8 +1314,7 @@ LogpWs carve_logp(void* base, int64_t N, int64_t D, int64_t V, bool backward) {
     w.scale = reinterpret_cast<float*>(take(4));
     w.dWacc = N > Nc ? reinterpret_cast<float*>(take((size_t)V * D * 4)) : nullptr;
   } else {
-    w.part = reinterpret_cast<float2*>(take((size_t)Nc * nparts * sizeof(float2)));
-    w.partw = reinterpret_cast<float*>(take((size_t)Nc * nparts * 4));
+    w.part = reinterpret_cast<float4*>(take((size_t)Nc * nparts * sizeof(float4)));
     w.tlogit = reinterpret_cast<float*>(take((size_t)Nc * 4));
   }
   w.bytes = off + 256;
@@ -1323,7 +1322,7 @@ LogpWs carve_logp(void* base, int64_t N, int64_t D, int64_t V, bool backward) {
 }
 
 template <typename T>
-int logp_fwd(float* logprobs, float* entropy, float* lse, float2* stats, const LogpWs& w, const void* H,
+int logp_fwd(float* logprobs, float* entropy, float* lse, float4* stats, const LogpWs& w, const void* H,
              const void* W, const int64_t* labels, int64_t N, int64_t D, int64_t V, const Squash& q,
              int64_t ignore_index, int* status, cudaStream_t st) {
   const int64_t Nc = chunk_rows(N);
@@ -1338,7 +1337,7 @@ int logp_fwd(float* logprobs, float* entropy, float* lse, float2* stats, const L
     Prob& P = g.p[0];
     P.M = (int)nr; P.N = (int)V; P.K = (int)D;
     P.epi = EPI_LOGP;
-    P.part = w.part; P.partw = entropy ? w.partw : nullptr; P.tlogit = w.tlogit;
+    P.lpart = w.part; P.want_ent = entropy != nullptr; P.tlogit = w.tlogit;
     P.labels = labels ? labels + r0 : nullptr; P.ignore_index = ignore_index;
     P.q = q;
     const int rc = launch_group<T>(A, B, g, st);
@@ -1346,7 +1345,7 @@ int logp_fwd(float* logprobs, float* entropy, float* lse, float2* stats, const L
     auto kern = q.cap > 0.f ? logp_rows_reduce<true> : logp_rows_reduce<false>;
     kern<<<(unsigned)((nr * 32 + 255) / 256), 256, 0, st>>>(
         logprobs ? logprobs + r0 : nullptr, entropy ? entropy + r0 : nullptr, lse + r0, stats ? stats + r0 : nullptr,
-        w.part, P.partw, w.tlogit, P.labels, (int)nr, (int)V, nparts, ignore_index, q);
+        w.part, w.tlogit, P.labels, (int)nr, (int)V, nparts, ignore_index, q);
     AK_CHECK_LAUNCH("ak_linear_logprobs_fwd: rows");
   }
   return AK_OK;
@@ -1354,8 +1353,8 @@ int logp_fwd(float* logprobs, float* entropy, float* lse, float2* stats, const L
 
 template <typename T>
 int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, const int64_t* labels,
-             const float2* stats, const float* entropy, const float* g_lp, const float* g_ent, int64_t N, int64_t D,
-             int64_t V, const Squash& q, int64_t ignore_index, int* status, cudaStream_t st) {
+             const float4* stats, const float* g_lp, const float* g_ent, int64_t N, int64_t D, int64_t V,
+             const Squash& q, int64_t ignore_index, int* status, cudaStream_t st) {
   const int64_t Nc = chunk_rows(N), ldg = (V + 7) / 8 * 8;
   // bf16 has fp32's range; only fp16 is scaled
   const float* scale = nullptr;
@@ -1379,7 +1378,7 @@ int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, 
     L.epi = EPI_LOGP_GRAD;
     L.C = w.G; L.ldc = ldg;
     L.labels = labels ? labels + r0 : nullptr; L.ignore_index = ignore_index;
-    L.stats = stats + r0; L.entropy = entropy ? entropy + r0 : nullptr;
+    L.stats = stats + r0;
     L.g_lp = g_lp ? g_lp + r0 : nullptr; L.g_ent = g_ent ? g_ent + r0 : nullptr;
     L.scale = scale; L.q = q;
     if ((rc = launch_group<T>(A, B, g, st))) return rc;
@@ -1560,29 +1559,30 @@ extern "C" int ak_linear_logprobs_fwd(float* logprobs, float* entropy, float* ls
   const int rc = check_logp("ak_linear_logprobs_fwd", H, W, N, D, V, temperature, softcap, dt);
   if (rc) return rc;
   if (N == 0) return AK_OK;
-  AK_REQUIRE(lse && (!logprobs || targets), AK_ERR_ARG, "ak_linear_logprobs_fwd: null pointer");
+  AK_REQUIRE(lse && (!logprobs || targets) && aligned16(row_stats), AK_ERR_ARG,
+             "ak_linear_logprobs_fwd: null pointer, or row_stats not 16-byte aligned");
   AK_REQUIRE(workspace && ws_bytes >= carve_logp(nullptr, N, D, V, false).bytes, AK_ERR_WORKSPACE,
              "ak_linear_logprobs_fwd: workspace too small");
   void* base = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   const LogpWs w = carve_logp(base, N, D, V, false);
   const Squash q = make_squash(temperature, softcap);
   auto fn = dt == AK_BF16 ? logp_fwd<__nv_bfloat16> : logp_fwd<__half>;
-  return fn(logprobs, entropy, lse, reinterpret_cast<float2*>(row_stats), w, H, W, targets, N, D, V, q, ignore_index,
+  return fn(logprobs, entropy, lse, reinterpret_cast<float4*>(row_stats), w, H, W, targets, N, D, V, q, ignore_index,
             status, (cudaStream_t)stream);
 }
 
 extern "C" int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_t ws_bytes, const void* H,
                                       const void* W, const int64_t* targets, const float* row_stats,
-                                      const float* entropy, const float* g_logprobs, const float* g_entropy, int64_t N,
-                                      int64_t D, int64_t V, float temperature, float softcap, int64_t ignore_index,
-                                      int dt, int* status, void* stream) {
+                                      const float* g_logprobs, const float* g_entropy, int64_t N, int64_t D, int64_t V,
+                                      float temperature, float softcap, int64_t ignore_index, int dt, int* status,
+                                      void* stream) {
   clear_error();
   const int rc = check_logp("ak_linear_logprobs_bwd", H, W, N, D, V, temperature, softcap, dt);
   if (rc) return rc;
   if (N == 0 || (!dH && !dW)) return AK_OK;
-  AK_REQUIRE(row_stats, AK_ERR_ARG, "ak_linear_logprobs_bwd: null pointer");
+  AK_REQUIRE(row_stats && aligned16(row_stats), AK_ERR_ARG,
+             "ak_linear_logprobs_bwd: null pointer, or row_stats not 16-byte aligned");
   AK_REQUIRE(!g_logprobs || targets, AK_ERR_ARG, "ak_linear_logprobs_bwd: a gradient of logprobs needs targets");
-  AK_REQUIRE(!g_entropy || entropy, AK_ERR_ARG, "ak_linear_logprobs_bwd: a gradient of the entropy needs the entropy");
   AK_REQUIRE((!dH || aligned16(dH)) && (!dW || aligned16(dW)), AK_ERR_ARG,
              "ak_linear_logprobs_bwd: dH and dW must be 16-byte aligned");
   AK_REQUIRE(workspace && ws_bytes >= carve_logp(nullptr, N, D, V, true).bytes, AK_ERR_WORKSPACE,
@@ -1591,6 +1591,6 @@ extern "C" int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_
   const LogpWs w = carve_logp(base, N, D, V, true);
   const Squash q = make_squash(temperature, softcap);
   auto fn = dt == AK_BF16 ? logp_bwd<__nv_bfloat16> : logp_bwd<__half>;
-  return fn(dH, dW, w, H, W, targets, reinterpret_cast<const float2*>(row_stats), entropy, g_logprobs, g_entropy, N, D,
-            V, q, ignore_index, status, (cudaStream_t)stream);
+  return fn(dH, dW, w, H, W, targets, reinterpret_cast<const float4*>(row_stats), g_logprobs, g_entropy, N, D, V, q,
+            ignore_index, status, (cudaStream_t)stream);
 }

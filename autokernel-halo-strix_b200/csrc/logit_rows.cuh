@@ -4,6 +4,8 @@
 
 #include "ak_common.cuh"
 
+#include <algorithm>
+#include <climits>
 #include <type_traits>
 
 namespace ak {
@@ -25,7 +27,8 @@ struct RowAddr {
 // -inf stays -inf under softcap: a masked token has no probability there either.
 struct Squash {
   float cap, inv_cap, inv_t, kl;
-  float kc;  // -2 log2(e) / cap
+  float rkl;  // 1 / kl
+  float kc;   // -2 log2(e) / cap
 };
 
 inline Squash make_squash(float temperature, float softcap) {
@@ -35,6 +38,7 @@ inline Squash make_squash(float temperature, float softcap) {
   q.kc = softcap > 0.f ? (float)(-2.0 * 1.4426950408889634 / (double)softcap) : 0.f;
   q.inv_t = 1.f / temperature;
   q.kl = (float)(1.4426950408889634 / (double)temperature);
+  q.rkl = 1.f / q.kl;
   return q;
 }
 
@@ -213,17 +217,49 @@ __device__ __forceinline__ float2 word_pair(const uint32_t (&w)[NW], int i) {
   else return unpack2(w[i], (const T*)nullptr);
 }
 
-// Where a product of e = 2^(kl (x - mu)) with x - mu is formed, -inf has to be raised to a finite
-// value whose e is still 0: to `floor`, which the type represents.  Holds where mu lies far enough
-// above it (and below what a difference could overflow from); elsewhere the terms are cut off one
-// by one.
+// ---------------------------------------------------------------------------
+// Running softmax statistics of a set of logits
+// ---------------------------------------------------------------------------
+// Exponents are taken against a reference point given in powers of two: e = 2^d with
+//   d = (y - sh) * kl - k,    k an integer, sh = 0
+// so that a logit costs one fused multiply-add, which rounds once, whatever y is; moving the
+// reference multiplies by an exact power of two.  (kl itself is rounded: all results are those of a
+// temperature off by half a unit in the last place.)  Where |y * kl| reaches 2^22 -- rows that hold
+// nothing but a mask of the type's lowest value, whose product with kl would overflow -- y is
+// subtracted first (sh = y, k = 0).
+struct Ref {
+  float sh, k;
+};
+
+__device__ __forceinline__ float exponent(float y, const Ref& r, const Squash& q) {
+  return fmaf(y - r.sh, q.kl, -r.k);
+}
+
+// 2^d for an integer d <= 0 (0 below the normal numbers).
+__device__ __forceinline__ float pow2i(float d) {
+  return d < -126.f ? 0.f : __int_as_float((127 + (int)d) << 23);
+}
+
+// How far reference a lies above b, in powers of two (at least -1e30), and the factor 2 to that.
+__device__ __forceinline__ float ref_diff(const Ref& a, const Ref& b, const Squash& q) {
+  if (a.sh == b.sh) return a.k - b.k;
+  return fmaxf((a.sh - b.sh) * q.kl + (a.k - b.k), -1e30f);
+}
+__device__ __forceinline__ float ref_scale(const Ref& a, const Ref& b, const Squash& q) {
+  const float d = ref_diff(a, b, q);
+  return a.sh == b.sh && d <= 0.f ? pow2i(d) : ex2(d);
+}
+
+// Where a product of e = 2^d with d is formed, -inf has to be raised to a finite logit whose e is
+// still 0: to `raise_floor`, which the type represents.  Holds for a reference far enough above it;
+// elsewhere the terms are cut off one by one.
 template <typename T>
 __device__ __forceinline__ float raise_floor() {
-  return sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? -65504.f : -1.0e30f;
+  return std::is_same<T, __half>::value ? -65504.f : -1.0e30f;
 }
 template <typename T>
-__device__ __forceinline__ bool can_raise(float mu, const Squash& q) {
-  return (mu - raise_floor<T>()) * q.kl > 200.f && mu < 1e30f;
+__device__ __forceinline__ bool can_raise(const Ref& r, const Squash& q) {
+  return r.sh == 0.f && r.k - raise_floor<T>() * q.kl > 200.f;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t floor_word() {
@@ -231,104 +267,88 @@ __device__ __forceinline__ uint32_t floor_word() {
   else return pack2(raise_floor<T>(), raise_floor<T>(), (const T*)nullptr);
 }
 
-// ---------------------------------------------------------------------------
-// Running softmax statistics of a set of logits
-// ---------------------------------------------------------------------------
-//   m   largest x (before squash; -inf for an empty set, NaN is passed over)
-//   mu  what exponents are taken against: squash(m), or 0 where m is -inf
-//   s   sum of e = 2^(kl (y - mu))
-//   w   sum of e * (y - mu)    (entropy only)
-// y - mu is formed before the scaling: the product with kl of a number near the type's lowest
-// value would overflow, and a fused x * kl - mu * kl would turn that into NaN (and rounds mu * kl,
-// an error that every term shares).  A -inf logit adds nothing; a NaN reaches s.
+__device__ __forceinline__ float redux_max(float v) {  // over the warp; NaN is passed over
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+constexpr float kHugeExponent = 4194304.f;  // 2^22
+constexpr float kSlack = 16.f;              // a maximum this far above the reference moves it
+
+//   m    largest x (before squash; -inf for an empty set, NaN is passed over)
+//   r    the reference;  lim  the y above which it moves (-inf: nothing seen yet)
+//   s    sum of e;  w  sum of e * d (entropy only)
+// A -inf logit adds nothing (its term of w is cut off at a finite d); a NaN reaches s.
 template <bool CAP, bool ENT>
 struct RowStats {
-  float m, mu, s, w;
+  float m, lim, s, w;
+  Ref r;
 
   __device__ __forceinline__ void init() {
-    m = -INFINITY;
-    mu = 0.f;
-    s = 0.f;
-    w = 0.f;
+    m = lim = -INFINITY;
+    s = w = 0.f;
+    r = Ref{0.f, 0.f};
   }
+  __device__ __forceinline__ bool unset() const { return lim == -INFINITY; }  // then s is 0 or NaN
 
-  // Moves the statistics to the larger maximum mn.
-  __device__ __forceinline__ void rebase(float mn, const Squash& q) {
-    const float nu = CAP ? squash<CAP>(mn, q) : mn;
-    if (m != -INFINITY) {  // there s is 0 or NaN
-      const float d = fmaxf(mu - nu, -1e30f);
-      const float f = ex2(d * q.kl);
-      if constexpr (ENT) w = f * fmaf(d, s, w);
+  __device__ __forceinline__ void rebase(const Ref& to, const Squash& q) {
+    if (!unset()) {
+      const float f = ref_scale(r, to, q);
+      if constexpr (ENT) w = f * fmaf(ref_diff(r, to, q), s, w);
       s *= f;
     }
-    m = mn;
-    mu = nu;
+    r = to;
   }
 
-  template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N], const Squash& q) {
-    float lm = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) lm = fmaxf(lm, x[i]);
-    add(x, lm, q);
+  // Takes the reference to the logit y.
+  __device__ __forceinline__ void move(float y, const Squash& q) {
+    const float t = y * q.kl;
+    const bool huge = !(fabsf(t) < kHugeExponent);
+    rebase(huge ? Ref{y, 0.f} : Ref{0.f, rintf(t)}, q);
+    lim = huge ? y : (r.k + kSlack) * q.rkl;
   }
 
-  // lm: the largest of x
-  template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N], float lm, const Squash& q) {
-    static_assert(N % 2 == 0 || N == 1, "pairs");
-    if (lm > m) rebase(lm, q);
-    if constexpr (N == 1) {
-      const float d = squash<CAP>(x[0], q) - mu;
-      const float e = ex2(d * q.kl);
-      s += e;
-      if constexpr (ENT) w = fmaf(e, fmaxf(d, -1e30f), w);
-    } else {
-      const float2 nmu = make_float2(-mu, -mu), kl = make_float2(q.kl, q.kl);
-      float2 s2 = make_float2(s, 0.f), w2 = make_float2(w, 0.f);
-#pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        const float2 y = make_float2(squash<CAP>(x[i], q), squash<CAP>(x[i + 1], q));
-        const float2 d = __fadd2_rn(y, nmu);
-        const float2 a = __fmul2_rn(d, kl);
-        const float2 e = make_float2(ex2(a.x), ex2(a.y));
-        s2 = __fadd2_rn(s2, e);
-        if constexpr (ENT) w2 = __ffma2_rn(e, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), w2);
-      }
-      s = s2.x + s2.y;
-      if constexpr (ENT) w = w2.x + w2.y;
-    }
+  // One logit (a row's head and tail).
+  __device__ __forceinline__ void add1(float x, const Squash& q) {
+    const float y = squash<CAP>(x, q);
+    if (y > lim) move(y, q);
+    m = fmaxf(m, x);
+    const float d = exponent(y, r, q), e = ex2(d);
+    s += e;
+    if constexpr (ENT) w = fmaf(e, fmaxf(d, -1e30f), w);
   }
 
-  // NW words as they lie in memory, lm their largest value.  Two elements at a time: 4 (with the
-  // entropy 5) instructions an element for 16-bit types.
+  // NW words as they lie in memory, lm their largest value.  Two elements at a time: 3.5 (with the
+  // entropy 4.5) instructions an element for 16-bit types.
   template <typename T, int NW>
   __device__ __forceinline__ void add_words(const uint32_t (&w_)[NW], float lm, const Squash& q) {
     constexpr int P = NW * elems_per_word<T>() / 2;
-    if (CAP || (ENT && !can_raise<T>(fmaxf(m, lm), q))) {
-      float x[2 * P];
+    const float ly = squash<CAP>(lm, q);
+    if (ly > lim) move(ly, q);
+    m = fmaxf(m, lm);
+    float2 s2 = make_float2(s, 0.f), w2 = make_float2(w, 0.f);
+    const float2 kl = make_float2(q.kl, q.kl), nk = make_float2(-r.k, -r.k);
+    if (!CAP && (ENT ? can_raise<T>(r, q) : r.sh == 0.f)) {
+      uint32_t x[NW];
+#pragma unroll
+      for (int i = 0; i < NW; ++i) x[i] = ENT ? word_max_nan(w_[i], floor_word<T>(), (const T*)nullptr) : w_[i];
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const float2 v = word_pair<T>(w_, i);
-        x[2 * i] = v.x;
-        x[2 * i + 1] = v.y;
+        const float2 d = __ffma2_rn(word_pair<T>(x, i), kl, nk);
+        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+        s2 = __fadd2_rn(s2, e);
+        if constexpr (ENT) w2 = __ffma2_rn(e, d, w2);
       }
-      add(x, lm, q);
-      return;
-    }
-    if (lm > m) rebase(lm, q);
-    const float2 nmu = make_float2(-mu, -mu), kl = make_float2(q.kl, q.kl);
-    float2 s2 = make_float2(s, 0.f), w2 = make_float2(w, 0.f);
-    uint32_t x[NW];
+    } else {
 #pragma unroll
-    for (int i = 0; i < NW; ++i) x[i] = ENT ? word_max_nan(w_[i], floor_word<T>(), (const T*)nullptr) : w_[i];
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const float2 d = __fadd2_rn(word_pair<T>(x, i), nmu);
-      const float2 a = __fmul2_rn(d, kl);
-      const float2 e = make_float2(ex2(a.x), ex2(a.y));
-      s2 = __fadd2_rn(s2, e);
-      if constexpr (ENT) w2 = __ffma2_rn(e, d, w2);
+      for (int i = 0; i < P; ++i) {
+        const float2 x = word_pair<T>(w_, i);
+        const float2 d = make_float2(exponent(squash<CAP>(x.x, q), r, q), exponent(squash<CAP>(x.y, q), r, q));
+        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+        s2 = __fadd2_rn(s2, e);
+        if constexpr (ENT) w2 = __ffma2_rn(e, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), w2);
+      }
     }
     s = s2.x + s2.y;
     if constexpr (ENT) w = w2.x + w2.y;
@@ -336,20 +356,67 @@ struct RowStats {
 
   // Adds the statistics of another set.
   __device__ __forceinline__ void merge(RowStats o, const Squash& q) {
-    if (o.m > m) rebase(o.m, q);
-    else if (m > o.m) o.rebase(m, q);
+    m = fmaxf(m, o.m);
+    if (!o.unset()) {
+      if (unset() || ref_diff(o.r, r, q) > 0.f) {
+        rebase(o.r, q);
+        lim = o.lim;
+      } else {
+        o.rebase(r, q);
+      }
+    }
     s += o.s;
     if constexpr (ENT) w += o.w;
   }
 
-  // Sums over the warp, the same on every lane.
+  // Joins the sets of the warp's lanes; the same result on every lane.
   __device__ __forceinline__ void warp_merge(const Squash& q) {
-    const float M = warp_max(m);
-    if (M > m) rebase(M, q);
+    m = redux_max(m);
+    if (__any_sync(0xffffffffu, r.sh != 0.f)) {
+#pragma unroll 1
+      for (int o = 16; o > 0; o >>= 1) {
+        RowStats t;
+        t.m = m;
+        t.lim = __shfl_xor_sync(0xffffffffu, lim, o);
+        t.s = __shfl_xor_sync(0xffffffffu, s, o);
+        t.w = ENT ? __shfl_xor_sync(0xffffffffu, w, o) : 0.f;
+        t.r.sh = __shfl_xor_sync(0xffffffffu, r.sh, o);
+        t.r.k = __shfl_xor_sync(0xffffffffu, r.k, o);
+        merge(t, q);
+      }
+      return;
+    }
+    const int top = __reduce_max_sync(0xffffffffu, unset() ? INT_MIN : (int)r.k);
+    if (top != INT_MIN) {
+      rebase(Ref{0.f, (float)top}, q);
+      lim = (r.k + kSlack) * q.rkl;
+    }
     s = warp_sum(s);
     if constexpr (ENT) w = warp_sum(w);
   }
+
+  // Brings S into [1, 2) by moving the reference (exactly), so that log S is small next to it.
+  __device__ __forceinline__ void center() {
+    if (!(s > 0.f && s < INFINITY)) return;
+    const int e = (int)(__float_as_uint(s) >> 23) - 127;
+    const float f = __int_as_float((127 - e) << 23);
+    if constexpr (ENT) w = (w - (float)e * s) * f;
+    s *= f;
+    r.k += (float)e;
+  }
 };
+
+// log-probability of the logit y given a centred reference and log S.
+__device__ __forceinline__ float log_prob(float y, const Ref& r, float logs, const Squash& q) {
+  const float d = exponent(y, r, q);
+  // a logit at the type's lowest value: only its product with kl overflows
+  if (d == -INFINITY) return (y - (r.sh + r.k * q.rkl)) * q.inv_t - logs;
+  return fmaf(d, kLn2, -logs);
+}
+// log sum exp.
+__device__ __forceinline__ float ref_lse(const Ref& r, float logs, const Squash& q) {
+  return fmaf(r.k, kLn2, logs) + r.sh * q.inv_t;
+}
 
 // ---------------------------------------------------------------------------
 // Thread-block clusters: CTAs of one row
@@ -383,6 +450,31 @@ __device__ __forceinline__ uint64_t ld_cluster_u64(const void* p, uint32_t rank)
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
+}
+
+// Clusters of `cs` CTAs of a persistent kernel that the device holds at once.
+template <typename... KArgs>
+inline cudaError_t resident_clusters(void (*kern)(KArgs...), int threads, int cs, size_t smem, int* n) {
+  if (cs == 1) {
+    int per_sm = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
+    *n = std::max(1, per_sm) * sm_count();
+    return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(cs * sm_count()));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cs;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(n, kern, &cfg);
+  *n = std::max(1, *n);
+  return e;
 }
 
 // Launches `kern` with clusters of `cs` CTAs (none for 1).

@@ -260,7 +260,7 @@ struct FwdArgs {
   float* logprobs;      // nullable
   float* entropy;       // nullable
   float* lse;           // nullable
-  float2* stats;        // nullable: (mu, log S) for the backward
+  float4* stats;        // nullable: (reference, log S, entropy) for the backward
   float* top_lp;        // nullable with top_idx
   int64_t* top_idx;
   const int64_t* targets;  // nullable
@@ -283,7 +283,7 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
   extern __shared__ __align__(16) float gmax[];  // TOP: group maxima
   __shared__ Stats s_warp[kWarps];
   __shared__ Stats s_cta;
-  __shared__ float s_share[4];         // this CTA's statistics, read by the others of the cluster
+  __shared__ float s_share[6];         // this CTA's statistics, read by the others of the cluster
   __shared__ uint64_t s_top[TOP ? kMaxTop : 1];
   __shared__ __align__(16) unsigned char s_scratch[TOP ? sizeof(SelectScratch) : 8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -328,9 +328,9 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
     const int n = first ? sh.head_here : sh.tail_here;
     uint32_t key = 0;
     if (lane < n) {
-      const float x[1] = {to_f<T>(row[(first ? 0 : sh.body_end) + lane])};
-      st.add(x, q);
-      key = order_key(x[0]);
+      const float x = to_f<T>(row[(first ? 0 : sh.body_end) + lane]);
+      st.add1(x, q);
+      key = order_key(x);
     }
     if constexpr (TOP) {
       const uint32_t best = __reduce_max_sync(0xffffffffu, key);
@@ -356,21 +356,25 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
     if (kl > 0) select_top<T>(s_top, sh, gmax, mine, kl, *reinterpret_cast<SelectScratch*>(s_scratch));
   if (cs > 1) {
     if (tid == 0) {
-      s_share[0] = st.m;
+      s_share[0] = st.lim;
       s_share[1] = st.s;
       s_share[2] = ENT ? st.w : 0.f;
       s_share[3] = __int_as_float(kl);
+      s_share[4] = st.r.sh;
+      s_share[5] = st.r.k;
     }
     row_cluster_sync();
     st.init();
     if (lane < cs) {  // every warp of every CTA joins them in the same way
-      const float m = __uint_as_float(ld_cluster_u32(&s_share[0], lane));
+      st.lim = __uint_as_float(ld_cluster_u32(&s_share[0], lane));
       st.s = __uint_as_float(ld_cluster_u32(&s_share[1], lane));
       st.w = __uint_as_float(ld_cluster_u32(&s_share[2], lane));
-      if (m != -INFINITY) { st.m = m; st.mu = squash<CAP>(m, q); }
+      st.r.sh = __uint_as_float(ld_cluster_u32(&s_share[4], lane));
+      st.r.k = __uint_as_float(ld_cluster_u32(&s_share[5], lane));
     }
     st.warp_merge(q);
   }
+  st.center();
   // S = 0: every logit is -inf and the row has no distribution: log-probabilities -inf, entropy 0
   const float logs = logf(st.s);
   if constexpr (TOP) {
@@ -405,7 +409,7 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
       if (pos < a.k) {
         const float x = key_value((uint32_t)(e >> 32));
         a.top_idx[r * a.k + pos] = (int64_t)(uint32_t)~(uint32_t)e;
-        a.top_lp[r * a.k + pos] = st.s == 0.f ? -INFINITY : (squash<CAP>(x, q) - st.mu) * q.inv_t - logs;
+        a.top_lp[r * a.k + pos] = st.s == 0.f ? -INFINITY : log_prob(squash<CAP>(x, q), st.r, logs, q);
       }
     }
   }
@@ -417,14 +421,17 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
       if (!ignored) {
         if (t < 0 || t >= a.V) lp = NAN;  // not a token
         else if (st.s == 0.f) lp = -INFINITY;
-        else lp = (squash<CAP>(to_f<T>(row[t]), q) - st.mu) * q.inv_t - logs;
+        else lp = log_prob(squash<CAP>(to_f<T>(row[t]), q), st.r, logs, q);
       }
       a.logprobs[r] = lp;
     }
-    if constexpr (ENT)
-      a.entropy[r] = (ignored || st.s == 0.f) ? 0.f : logs - (st.w / st.s) * q.inv_t;
-    if (a.lse) a.lse[r] = st.mu * q.inv_t + logs;
-    if (a.stats) a.stats[r] = make_float2(st.mu, logs);
+    float H = 0.f;
+    if constexpr (ENT) {
+      if (!ignored && st.s != 0.f) H = fmaf(-kLn2, st.w / st.s, logs);
+      a.entropy[r] = H;
+    }
+    if (a.lse) a.lse[r] = ref_lse(st.r, logs, q);
+    if (a.stats) a.stats[r] = make_float4(st.r.sh, st.r.k, logs, H);
   }
   if (cs > 1) {  // the other CTAs have read this one's shared memory
     row_cluster_arrive_relaxed();
@@ -433,8 +440,7 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
 }
 
 struct BwdArgs {
-  const float2* stats;
-  const float* entropy;    // nullable with g_ent
+  const float4* stats;
   const float* g_lp;       // nullable
   const float* g_ent;      // nullable
   const int64_t* targets;  // nullable
@@ -444,10 +450,10 @@ struct BwdArgs {
   Squash q;
 };
 
-constexpr int kBwdBatch = 2;
+constexpr int kBwdBatch = 4;
 constexpr int kBwdGroups = kThreads * kBwdBatch;  // groups of one CTA
 
-// Elementwise from the saved (mu, log S, H): each CTA takes one segment of a row.
+// Elementwise from the forward's numbers: each CTA takes one segment of a row.
 template <typename T, bool CAP, bool ENT>
 __global__ void __launch_bounds__(kThreads)
 token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const BwdArgs a) {
@@ -461,28 +467,30 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
   const RowCut cut = cut_row(row, a.V);
   const bool vec = (reinterpret_cast<uintptr_t>(grow + cut.head) & 31u) == 0;
   const int64_t t = a.targets ? a.targets[r] : -1;
-  const float2 ml = a.stats[r];
+  const float4 st = a.stats[r];
+  const Ref ref{st.x, st.y};
+  const float logs = st.z, H = st.w;
   // rows without a gradient: ignored ones, and those whose every logit is -inf (S = 0)
-  const bool none = (a.targets && t == a.ignore_index) || ml.y == -INFINITY;
+  const bool none = (a.targets && t == a.ignore_index) || logs == -INFINITY;
   float gl = (a.targets && a.g_lp) ? a.g_lp[r] : 0.f;
   if (a.targets && !none && (t < 0 || t >= a.V)) gl = NAN;
-  const float ge = ENT ? a.g_ent[r] : 0.f, H = ENT ? a.entropy[r] : 0.f;
-  // d = y - mu, p = 2^(d kl - log2 S), log p = d / T - log S:
-  // dx = p (c0 + c1 d) (+ gl / T at the target), times the softcap's slope
-  const float l2s = ml.y * kLog2e;
-  const float c0 = (ge * (ml.y - H) - gl) * q.inv_t, c1 = -ge * q.inv_t * q.inv_t, ct = gl * q.inv_t;
+  const float ge = ENT ? a.g_ent[r] : 0.f;
+  // e = 2^d, p = e / S, log p = d ln 2 - log S:
+  // dx = e (c0 + c1 d) (+ gl / T at the target), times the softcap's slope
+  const float f = q.inv_t * expf(-logs);
+  const float c0 = (ge * (logs - H) - gl) * f, c1 = -ge * kLn2 * f, ct = gl * q.inv_t;
   const int ti = (a.targets && t >= 0 && t < a.V) ? (int)t : -1;
 
   auto one = [&](float x, int i) {
     const float y = squash<CAP>(x, q);
-    const float d = y - ml.x;
-    float o = ex2(fmaf(d, q.kl, -l2s));
+    const float d = exponent(y, ref, q);
+    float o = ex2(d);
     o *= ENT ? fmaf(c1, fmaxf(d, -1e30f), c0) : c0;
     if (i == ti) o += ct;
     return o * squash_slope<CAP>(y, q);
   };
-  const bool quick = !CAP && (!ENT || can_raise<T>(ml.x, q));
-  const float2 nmu = make_float2(-ml.x, -ml.x), kl = make_float2(q.kl, q.kl), nl2s = make_float2(-l2s, -l2s);
+  const bool quick = !CAP && (ENT ? can_raise<T>(ref, q) : ref.sh == 0.f);
+  const float2 kl = make_float2(q.kl, q.kl), nk = make_float2(-ref.k, -ref.k);
   const float2 c02 = make_float2(c0, c0), c12 = make_float2(c1, c1);
 
   const int gbeg = seg * kBwdGroups;
@@ -512,9 +520,8 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
             w[i] = ENT ? word_max_nan(raw[u].r[h].w[i], floor_word<T>(), (const T*)nullptr) : raw[u].r[h].w[i];
 #pragma unroll
           for (int i = 0; i < P; ++i) {
-            const float2 d = __fadd2_rn(word_pair<T>(w, i), nmu);
-            const float2 e = __ffma2_rn(d, kl, nl2s);
-            const float2 o = __fmul2_rn(make_float2(ex2(e.x), ex2(e.y)), ENT ? __ffma2_rn(c12, d, c02) : c02);
+            const float2 d = __ffma2_rn(word_pair<T>(w, i), kl, nk);
+            const float2 o = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), ENT ? __ffma2_rn(c12, d, c02) : c02);
             x[h * 2 * P + 2 * i] = o.x;
             x[h * 2 * P + 2 * i + 1] = o.y;
           }
@@ -596,9 +603,10 @@ extern "C" int ak_token_logprobs_fwd(float* logprobs, float* entropy, float* lse
   if (rows == 0) return AK_OK;
   AK_REQUIRE((k == 0) || (top_lp && top_idx), AK_ERR_ARG, "ak_token_logprobs_fwd: null top_lp or top_idx");
   AK_REQUIRE(!logprobs || targets, AK_ERR_ARG, "ak_token_logprobs_fwd: logprobs need targets");
+  AK_REQUIRE(aligned16(row_stats), AK_ERR_ARG, "ak_token_logprobs_fwd: row_stats not 16-byte aligned");
   FwdArgs a{};
   a.logprobs = logprobs; a.entropy = entropy; a.lse = lse;
-  a.stats = reinterpret_cast<float2*>(row_stats);
+  a.stats = reinterpret_cast<float4*>(row_stats);
   a.top_lp = top_lp; a.top_idx = top_idx; a.targets = targets;
   a.addr = RowAddr{inner, stride_outer, stride_inner};
   a.ignore_index = ignore_index;
@@ -609,22 +617,21 @@ extern "C" int ak_token_logprobs_fwd(float* logprobs, float* entropy, float* lse
 }
 
 extern "C" int ak_token_logprobs_bwd(void* grad, const void* logits, const int64_t* targets, const float* row_stats,
-                                     const float* entropy, const float* g_logprobs, const float* g_entropy,
-                                     int64_t rows, int64_t inner, int64_t stride_outer, int64_t stride_inner,
-                                     int64_t V, float temperature, float softcap, int64_t ignore_index, int dt,
-                                     void* stream) {
+                                     const float* g_logprobs, const float* g_entropy, int64_t rows, int64_t inner,
+                                     int64_t stride_outer, int64_t stride_inner, int64_t V, float temperature,
+                                     float softcap, int64_t ignore_index, int dt, void* stream) {
   clear_error();
   int rc = check_rows("ak_token_logprobs_bwd", logits, rows, inner, V, temperature, softcap, dt);
   if (rc) return rc;
   if (rows == 0) return AK_OK;
-  AK_REQUIRE(grad && row_stats, AK_ERR_ARG, "ak_token_logprobs_bwd: null pointer");
+  AK_REQUIRE(grad && row_stats && aligned16(row_stats), AK_ERR_ARG,
+             "ak_token_logprobs_bwd: null pointer, or row_stats not 16-byte aligned");
   AK_REQUIRE(!g_logprobs || targets, AK_ERR_ARG, "ak_token_logprobs_bwd: a gradient of logprobs needs targets");
-  AK_REQUIRE(!g_entropy || entropy, AK_ERR_ARG, "ak_token_logprobs_bwd: a gradient of the entropy needs the entropy");
   AK_REQUIRE((reinterpret_cast<uintptr_t>(grad) % elem_size(dt)) == 0, AK_ERR_ARG,
              "ak_token_logprobs_bwd: grad not aligned to its type");
   BwdArgs a{};
-  a.stats = reinterpret_cast<const float2*>(row_stats);
-  a.entropy = entropy; a.g_lp = g_logprobs; a.g_ent = g_entropy; a.targets = targets;
+  a.stats = reinterpret_cast<const float4*>(row_stats);
+  a.g_lp = g_logprobs; a.g_ent = g_entropy; a.targets = targets;
   a.addr = RowAddr{inner, stride_outer, stride_inner};
   a.ignore_index = ignore_index;
   a.V = (int)V;

@@ -49,12 +49,12 @@ SIGNATURES = {
     "ak_ce_rows_reduce": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _vp],
     "ak_ce_inv_valid": [_vp, _vp, _i64, _i64, _vp],
     "ak_token_logprobs_fwd": [_vp] * 8 + [_i64] * 6 + [_f, _f, _i64, _i, _vp],
-    "ak_token_logprobs_bwd": [_vp] * 7 + [_i64] * 5 + [_f, _f, _i64, _i, _vp],
+    "ak_token_logprobs_bwd": [_vp] * 6 + [_i64] * 5 + [_f, _f, _i64, _i, _vp],
     "ak_distill_topk_fwd": [_vp] * 10 + [_i64] * 6 + [_f, _f, _i, _i, _vp, _vp],
     "ak_distill_topk_bwd": [_vp] * 8 + [_i64] * 6 + [_f, _f, _i, _vp],
     "ak_linear_logprobs_workspace_size": [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)],
     "ak_linear_logprobs_fwd": [_vp] * 5 + [_sz] + [_vp] * 3 + [_i64] * 3 + [_f, _f, _i64, _i, _vp, _vp],
-    "ak_linear_logprobs_bwd": [_vp] * 3 + [_sz] + [_vp] * 7 + [_i64] * 3 + [_f, _f, _i64, _i, _vp, _vp],
+    "ak_linear_logprobs_bwd": [_vp] * 3 + [_sz] + [_vp] * 6 + [_i64] * 3 + [_f, _f, _i64, _i, _vp, _vp],
     "ak_linear_ce_logits_grad_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
     "ak_linear_ce_logits_grad": [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp],
     "ak_linear_ce_workspace_size": [_i64, _i64, _i64, ctypes.POINTER(_sz)],
@@ -641,7 +641,7 @@ def token_logprobs_fwd(logits: torch.Tensor, targets: Optional[torch.Tensor], to
     lp = torch.empty(lead, **f32) if targets is not None else None
     ent = torch.empty(lead, **f32) if want_entropy else None
     lse = torch.empty(lead, **f32)
-    stats = torch.empty(rows, 2, **f32) if want_stats else None
+    stats = torch.empty(rows, 4, **f32) if want_stats else None
     top_lp = torch.empty(*lead, top_k, **f32) if top_k else None
     top_idx = torch.empty(*lead, top_k, dtype=torch.int64, device=dev) if top_k else None
     call_on(dev, "ak_token_logprobs_fwd", ptr(lp), ptr(ent), ptr(lse), ptr(stats), ptr(top_lp), ptr(top_idx), ptr(x),
@@ -651,16 +651,15 @@ def token_logprobs_fwd(logits: torch.Tensor, targets: Optional[torch.Tensor], to
 
 
 def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], row_stats: torch.Tensor,
-                       entropy: Optional[torch.Tensor], g_logprobs: Optional[torch.Tensor],
-                       g_entropy: Optional[torch.Tensor], temperature: float = 1.0, softcap: float = 0.0,
+                       g_logprobs: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor], temperature: float = 1.0, softcap: float = 0.0,
                        ignore_index: int = -100) -> torch.Tensor:
     """Gradient of the logits (dense, their dtype) from those of logprobs and entropy (either may be None)."""
-    dev = require_cuda(logits, targets, row_stats, entropy, g_logprobs, g_entropy)
+    dev = require_cuda(logits, targets, row_stats, g_logprobs, g_entropy)
     x, rows, inner, so, si = logit_rows(logits)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
     glp = g_logprobs.to(torch.float32).contiguous() if g_logprobs is not None else None
     gent = g_entropy.to(torch.float32).contiguous() if g_entropy is not None else None
-    call_on(dev, "ak_token_logprobs_bwd", ptr(grad), ptr(x), ptr(targets), ptr(row_stats), ptr(entropy), ptr(glp),
+    call_on(dev, "ak_token_logprobs_bwd", ptr(grad), ptr(x), ptr(targets), ptr(row_stats), ptr(glp),
             ptr(gent), rows, inner, so, si, logits.shape[-1], temperature, softcap, ignore_index,
             dtype_code(logits), stream(dev))
     return grad
@@ -682,7 +681,7 @@ def distill_topk_fwd(logits: torch.Tensor, teacher_idx: torch.Tensor, teacher_lp
     losses = torch.empty(logits.shape[:-1], **f32)
     inv_n = torch.empty((), **f32) if mask is not None else None
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
-    rest = torch.empty(rows, 2, **f32) if want_stats else None
+    rest = torch.empty(rows, 4, **f32) if want_stats else None
     gk = torch.empty(rows, K, **f32) if want_stats else None
     call_on(dev, "ak_distill_topk_fwd", ptr(loss), ptr(losses), ptr(inv_n), ptr(grad), ptr(rest), ptr(gk), ptr(x),
             ptr(teacher_idx), ptr(teacher_lp), ptr(mask), rows, inner, so, si, logits.shape[-1], K, temperature,
@@ -765,7 +764,7 @@ def linear_logprobs_fwd(hidden, weight, targets, temperature=1.0, softcap=0.0, i
     lp = torch.empty(N, **f32) if targets is not None else None
     ent = torch.empty(N, **f32) if want_entropy else None
     lse = torch.empty(N, **f32)
-    stats = torch.empty(N, 2, **f32) if want_stats else None
+    stats = torch.empty(N, 4, **f32) if want_stats else None
     ws_bytes = _size_query("ak_linear_logprobs_workspace_size", N, D, V, 0)
     ws = workspace(ws_bytes, dev)
     call_on(dev, "ak_linear_logprobs_fwd", ptr(lp), ptr(ent), ptr(lse), ptr(stats), ptr(ws), ws_bytes, ptr(hidden),
@@ -774,10 +773,10 @@ def linear_logprobs_fwd(hidden, weight, targets, temperature=1.0, softcap=0.0, i
     return [lp, ent, lse, stats]
 
 
-def linear_logprobs_bwd(hidden, weight, targets, row_stats, entropy, g_logprobs, g_entropy, temperature=1.0,
+def linear_logprobs_bwd(hidden, weight, targets, row_stats, g_logprobs, g_entropy, temperature=1.0,
                         softcap=0.0, ignore_index=-100, need_dh=True, need_dw=True):
     """Returns (dH or None, dW or None) from the gradients of logprobs and entropy (either may be None)."""
-    dev = require_cuda(hidden, weight, targets, row_stats, entropy, g_logprobs, g_entropy)
+    dev = require_cuda(hidden, weight, targets, row_stats, g_logprobs, g_entropy)
     N, D = hidden.shape
     V = weight.shape[0]
     dH = torch.empty_like(hidden) if need_dh else None
@@ -787,7 +786,7 @@ def linear_logprobs_bwd(hidden, weight, targets, row_stats, entropy, g_logprobs,
     ws_bytes = _size_query("ak_linear_logprobs_workspace_size", N, D, V, 1)
     ws = workspace(ws_bytes, dev)
     call_on(dev, "ak_linear_logprobs_bwd", ptr(dH), ptr(dW), ptr(ws), ws_bytes, ptr(hidden), ptr(weight),
-            ptr(targets), ptr(row_stats), ptr(entropy), ptr(glp), ptr(gent), N, D, V, temperature, softcap,
+            ptr(targets), ptr(row_stats), ptr(glp), ptr(gent), N, D, V, temperature, softcap,
             ignore_index, dtype_code(hidden), status_ptr(dev, "linear_logprobs"), stream(dev))
     return dH, dW
 

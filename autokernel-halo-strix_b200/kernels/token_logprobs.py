@@ -36,13 +36,13 @@ class TokenLogprobs(NamedTuple):
 
 
 class _TokenLogprobs(torch.autograd.Function):
-    """Saves the logits and two numbers a row; the backward recomputes the softmax from them."""
+    """Saves the logits and four numbers a row; the backward recomputes the softmax from them."""
 
     @staticmethod
     def forward(ctx, logits, targets, top_k, temperature, softcap, ignore_index, entropy):
         lp, ent, lse, top_lp, top_idx, stats = _ak.token_logprobs_fwd(
             logits, targets, top_k, temperature, softcap, ignore_index, want_entropy=entropy, want_stats=True)
-        ctx.save_for_backward(logits, targets, stats, ent)
+        ctx.save_for_backward(logits, targets, stats)
         ctx.args = (temperature, softcap, ignore_index)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*(t for t in (lse, top_lp, top_idx) if t is not None))
@@ -53,8 +53,8 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_lp, g_ent, *rest):
         if g_lp is None and g_ent is None:
             return (None,) * 7
-        logits, targets, stats, ent = ctx.saved_tensors
-        grad = _ak.token_logprobs_bwd(logits, targets, stats, ent, g_lp, g_ent, *ctx.args)
+        logits, targets, stats = ctx.saved_tensors
+        grad = _ak.token_logprobs_bwd(logits, targets, stats, g_lp, g_ent, *ctx.args)
         return (grad,) + (None,) * 6
 
 
@@ -113,14 +113,14 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
 
 
 class _LinearTokenLogprobs(torch.autograd.Function):
-    """Saves its operands and two numbers a row; the backward forms the logits again, chunk by chunk."""
+    """Saves its operands and four numbers a row; the backward forms the logits again, chunk by chunk."""
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, temperature, softcap, ignore_index, entropy):
         w = weight.to(hidden.dtype)
         lp, ent, lse, stats = _ak.linear_logprobs_fwd(hidden, w, targets, temperature, softcap, ignore_index,
                                                       want_entropy=entropy, want_stats=True)
-        ctx.save_for_backward(hidden, w, targets, stats, ent)
+        ctx.save_for_backward(hidden, w, targets, stats)
         ctx.args, ctx.weight_dtype = (temperature, softcap, ignore_index), weight.dtype
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(lse)
@@ -131,8 +131,8 @@ class _LinearTokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_lp, g_ent, *rest):
         if g_lp is None and g_ent is None:
             return (None,) * 7
-        hidden, w, targets, stats, ent = ctx.saved_tensors
-        dh, dw = _ak.linear_logprobs_bwd(hidden, w, targets, stats, ent, g_lp, g_ent, *ctx.args,
+        hidden, w, targets, stats = ctx.saved_tensors
+        dh, dw = _ak.linear_logprobs_bwd(hidden, w, targets, stats, g_lp, g_ent, *ctx.args,
                                          need_dh=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
         return (dh, dw.to(ctx.weight_dtype) if dw is not None else None) + (None,) * 5
 

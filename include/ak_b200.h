@@ -184,7 +184,8 @@ AK_API int ak_scale_by_device_scalar(void* x, int64_t n, const float* scale, int
  *   logprobs[rows]  y_target - lse; 0 where target == ignore_index, NaN where it is no token
  *   entropy[rows]   -sum p log p; 0 where target == ignore_index
  *   lse[rows]
- *   row_stats[rows][2]  what ak_token_logprobs_bwd needs
+ *   row_stats[rows][4]  what ak_token_logprobs_bwd needs (16-byte aligned; with entropy != NULL if
+ *                   a gradient of the entropy will be given)
  *   top_lp / top_idx[rows][k]  log-probability and index of the k largest logits, largest first,
  *                   equal ones by lowest index; 0 <= k <= min(128, V), V <= 1048320 for k > 0
  * Each output is fp32 (top_idx int64) and nullable; logprobs needs targets (int64, nullable).
@@ -204,14 +205,14 @@ AK_API int ak_token_logprobs_fwd(float* logprobs, float* entropy, float* lse, fl
 /* Gradient of the logits, grad[rows][V] (dt, dense), given those of logprobs (g_logprobs) and
  * entropy (g_entropy), fp32 [rows], each nullable:
  *   dx_i = [ g_lp (1[i = t] - p_i) - g_H p_i (log p_i + H) ] dy_i/dx_i.
- * row_stats and entropy are the forward's, with the same arguments.  Ignored rows and rows of
+ * row_stats is the forward's, with the same arguments.  Ignored rows and rows of
  * -inf get zeros.  Reads the logits once and writes the gradient once. */
 AK_API int ak_token_logprobs_bwd(void* grad, const void* logits, const int64_t* targets,
-                                 const float* row_stats, const float* entropy,
-                                 const float* g_logprobs, const float* g_entropy, int64_t rows,
-                                 int64_t inner, int64_t stride_outer, int64_t stride_inner,
-                                 int64_t V, float temperature, float softcap,
-                                 int64_t ignore_index, int dt, void* stream);
+                                 const float* row_stats, const float* g_logprobs,
+                                 const float* g_entropy, int64_t rows, int64_t inner,
+                                 int64_t stride_outer, int64_t stride_inner, int64_t V,
+                                 float temperature, float softcap, int64_t ignore_index, int dt,
+                                 void* stream);
 
 /* ------------------------------------------------------------------------ *
  * Distillation from a teacher's top-K log-probabilities
@@ -228,10 +229,10 @@ AK_API int ak_token_logprobs_bwd(void* grad, const void* logits, const int64_t* 
  * mean).  An index >= V makes its row's loss and gradient NaN.  Entries of one token add up.
  * losses[rows] fp32: the rows' divergences (0 without mask).  inv_n (needed with a mask): receives
  * 1 / max(1, rows with mask).
- * grad (nullable): d loss / d logits, dense [rows][V] dt.  Without it, rest_stats [rows][2] and
- * gk [rows][K] (both nullable, fp32) receive what ak_distill_topk_bwd needs.
+ * grad (nullable): d loss / d logits, dense [rows][V] dt.  Without it, rest_stats [rows][4] and
+ * gk [rows][K] (both nullable, fp32, rest_stats 16-byte aligned) receive what ak_distill_topk_bwd needs.
  * Rows of logits as in ak_token_logprobs_fwd; a row has to fit the shared memory of 8 CTAs
- * (about 880,000 16-bit or 440,000 fp32 elements).  Reads the logits once.
+ * (851,968 16-bit or 425,984 fp32 elements).  Reads the logits once.
  * No counterpart in the reference, which trains on hard labels only (kernels/ce_fused.py:122-382). */
 AK_API int ak_distill_topk_fwd(float* loss, float* losses, float* inv_n, void* grad,
                                float* rest_stats, float* gk, const void* logits,
@@ -323,17 +324,17 @@ AK_API int ak_linear_logprobs_fwd(float* logprobs, float* entropy, float* lse, f
                                   int* status, void* stream);
 
 /* dH[N, D] and dW[V, D] (dt, each nullable) from the gradients of logprobs and entropy (fp32 [N],
- * each nullable) and the forward's row_stats and entropy.  Per chunk of at most 16384 rows the
+ * each nullable) and the forward's row_stats.  Per chunk of at most 16384 rows the
  * logits are formed again and leave the accumulators as their gradient, rounded to dt once (in
  * fp16 divided by the largest upstream gradient, which the next products' fp32 accumulators
  * restore); then dW += G^T H and dH = G W in one launch.  Ignored rows have G = 0: their hidden
  * states enter dW as 0 * h. */
 AK_API int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_t ws_bytes,
                                   const void* H, const void* W, const int64_t* targets,
-                                  const float* row_stats, const float* entropy,
-                                  const float* g_logprobs, const float* g_entropy, int64_t N,
-                                  int64_t D, int64_t V, float temperature, float softcap,
-                                  int64_t ignore_index, int dt, int* status, void* stream);
+                                  const float* row_stats, const float* g_logprobs,
+                                  const float* g_entropy, int64_t N, int64_t D, int64_t V,
+                                  float temperature, float softcap, int64_t ignore_index, int dt,
+                                  int* status, void* stream);
 
 /* ------------------------------------------------------------------------ *
  * Collapsed (single-state) selective scan, fp32, layout (B, L, d)

@@ -274,3 +274,14 @@ def test_large_offsets():
         O.assert_within(g[-1:], ref["grad"], ref["tol_grad"], "grad")
         assert (g[0] == 0).all() and (g[n // 2] == 0).all()
         del g, loss, leaf
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,k", [(700, 50257, 9), (1201, 4099, 128), (310, 131073, 3), (3, 262147, 40), (450, 15, 2)])
+def test_many_rows_per_cta(n, v, k, dtype):
+    """More rows than the GPU takes at once, so that each CTA (or cluster) walks several, some of
+    them masked; and a row that needs all eight CTAs of a cluster."""
+    x, idx, tlp, mask = problem(n, v, min(k, v), dtype, seed=21)
+    check(x, idx, tlp, mask, tail=True)
+    mask[::2] = False
+    check(x, idx, tlp, mask, tail=False, modes=("fused",))

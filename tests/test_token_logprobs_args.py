@@ -57,11 +57,10 @@ def test_library_refusals():
         assert lib.ak_last_error()
     assert fwd(rows=0) == 0
 
-    def bwd(rows=2, V=64, grad=fake, stats=fake, targets=fake, ent=fake, gl=fake, ge=fake, T=1.0):
-        return lib.ak_token_logprobs_bwd(grad, fake, targets, stats, ent, gl, ge, rows, 2, 0, V, V, T, 0.0, -100, 1,
-                                         None)
+    def bwd(rows=2, V=64, grad=fake, stats=fake, targets=fake, gl=fake, ge=fake, T=1.0):
+        return lib.ak_token_logprobs_bwd(grad, fake, targets, stats, gl, ge, rows, 2, 0, V, V, T, 0.0, -100, 1, None)
 
-    for kw in (dict(grad=None), dict(stats=None), dict(targets=None), dict(ent=None), dict(T=-1.0),
+    for kw in (dict(grad=None), dict(stats=None), dict(targets=None), dict(stats=ctypes.c_void_p(264)), dict(T=-1.0),
                dict(grad=ctypes.c_void_p(257))):
         assert bwd(**kw) == 1, kw
     assert bwd(rows=0) == 0
@@ -137,11 +136,11 @@ def test_linear_library_refusals():
     assert fwd(ws=fwd_ws - 1) == 6
     assert fwd(N=0) == 0
 
-    def bwd(dH=fake, stats=fake, t=fake, ent=fake, gl=fake, ge=fake, ws=bwd_ws, N=8):
-        return lib.ak_linear_logprobs_bwd(dH, fake, fake, ws, fake, fake, t, stats, ent, gl, ge, N, 64, 100, 1.0, 0.0,
-                                          -100, 1, None, None)
+    def bwd(dH=fake, stats=fake, t=fake, gl=fake, ge=fake, ws=bwd_ws, N=8):
+        return lib.ak_linear_logprobs_bwd(dH, fake, fake, ws, fake, fake, t, stats, gl, ge, N, 64, 100, 1.0, 0.0, -100,
+                                          1, None, None)
 
-    for kw in (dict(dH=ctypes.c_void_p(258)), dict(stats=None), dict(t=None), dict(ent=None)):
+    for kw in (dict(dH=ctypes.c_void_p(258)), dict(stats=None), dict(t=None), dict(stats=ctypes.c_void_p(264))):
         assert bwd(**kw) == 1, kw
     assert bwd(ws=bwd_ws - 1) == 6
     assert bwd(N=0) == 0
