@@ -33,10 +33,10 @@ namespace {
 constexpr int kThreads = 256;    // of the backward kernel
 constexpr int kRoles = 3;        // loader, teacher, finisher
 // Compute warps: kWide of them with two CTAs on an SM, which a long row (100 KB of shared memory)
-// allows anyhow; kNarrow with six CTAs for shares up to kShareNarrow, where what counts is how many
+// allows anyhow; kNarrow with four CTAs for shares up to kShareNarrow, where what counts is how many
 // rows are under way at once.
-constexpr int kWide = 11, kNarrow = 2;
-constexpr int kShareNarrow = 16 * 1024;
+constexpr int kWide = 11, kNarrow = 5;
+constexpr int kShareNarrow = 44 * 1024;
 constexpr int kMaxK = 128;       // teacher entries
 constexpr int kSlots = kMaxK / 32;
 constexpr int kMaxCluster = 8;   // the portable cluster size
@@ -211,123 +211,177 @@ struct Entries {
   }
 };
 
-constexpr int kTags = 2048;
-__device__ __forceinline__ int mix_bits(int i) { return (int)(((uint32_t)i * 2654435761u) >> 21); }  // 11 bits
-
-// A row's teacher: everything that needs only its K entries and their logits.  s_idx, s_q and s_tag
-// are the warp's scratch.
-template <typename T, bool CAP>
-__device__ __forceinline__ void teacher_row(TeacherRow& out_head, int (&idx)[kSlots], float (&qk)[kSlots],
-                                            float (&logq)[kSlots], float (&yk)[kSlots], float (&mass)[kSlots],
-                                            const Entries& e, const T* row, const DistillArgs& a, int* s_idx,
-                                            float* s_q, uint8_t (*s_tag)[kTags]) {
-  const int lane = threadIdx.x & 31;
-  const Squash q = a.q;
-  float t[kSlots], xk[kSlots];
-  bool any = false, bad = false;
+// The valid entries: token (or -1), log-probability and the student's logit.
+struct Picked {
+  int idx[kSlots];
+  float t[kSlots], x[kSlots];
+  bool any, bad;
+  // logit(i): the student's logit of token i
+  template <typename F>
+  __device__ __forceinline__ void pick(const Entries& e, const DistillArgs& a, F logit) {
+    any = bad = false;
 #pragma unroll
-  for (int j = 0; j < kSlots; ++j) {
-    idx[j] = -1;
-    t[j] = xk[j] = -INFINITY;
-    if (32 * j < a.K) {
-      bad |= e.i[j] >= a.V;
-      const bool ok = e.i[j] >= 0 && e.i[j] < a.V;
-      any |= ok;
-      if (ok) {
-        idx[j] = (int)e.i[j];
-        t[j] = e.t[j];
-        xk[j] = to_f<T>(row[idx[j]]);
-      }
-      s_idx[32 * j + lane] = idx[j];
-      // two tables of who came last to a place that the token's low and mixed bits name
-      if (ok) {
-        s_tag[0][idx[j] & (kTags - 1)] = (uint8_t)(32 * j + lane);
-        s_tag[1][mix_bits(idx[j])] = (uint8_t)(32 * j + lane);
+    for (int j = 0; j < kSlots; ++j) {
+      idx[j] = -1;
+      t[j] = x[j] = -INFINITY;
+      if (32 * j < a.K) {
+        bad |= e.i[j] >= a.V;
+        if (e.i[j] >= 0 && e.i[j] < a.V) {
+          any = true;
+          idx[j] = (int)e.i[j];
+          t[j] = e.t[j];
+          x[j] = logit(idx[j]);
+        }
       }
     }
   }
+};
+
+constexpr int kTags = 2048;
+__device__ __forceinline__ int mix_bits(int i) { return (int)(((uint32_t)i * 2654435761u) >> 21); }  // 11 bits
+
+// Whether a token may come twice: two tables of who came last to a place that its low and its mixed
+// bits name.  One that comes twice is not the last in either table at one of its entries; so,
+// rarely, is one that shares its places with others, which costs a comparison of all with all.
+__device__ __forceinline__ bool maybe_twice(const Picked& p, uint8_t (*tag)[kTags]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < kSlots; ++j) {
+    if (p.idx[j] >= 0) {
+      tag[0][p.idx[j] & (kTags - 1)] = (uint8_t)(32 * j + lane);
+      tag[1][mix_bits(p.idx[j])] = (uint8_t)(32 * j + lane);
+    }
+  }
   __syncwarp();
-  // a token that comes twice is not the last in either table at one of its entries; so, rarely, is
-  // one that shares its places with others, which costs the comparison below
   bool twice = false;
 #pragma unroll
   for (int j = 0; j < kSlots; ++j)
-    if (idx[j] >= 0)
-      twice |= s_tag[0][idx[j] & (kTags - 1)] != (uint8_t)(32 * j + lane) &&
-               s_tag[1][mix_bits(idx[j])] != (uint8_t)(32 * j + lane);
-  twice = __any_sync(0xffffffffu, twice);
-  bad = __any_sync(0xffffffffu, bad);
-  any = __any_sync(0xffffffffu, any);
+    if (p.idx[j] >= 0)
+      twice |= tag[0][p.idx[j] & (kTags - 1)] != (uint8_t)(32 * j + lane) &&
+               tag[1][mix_bits(p.idx[j])] != (uint8_t)(32 * j + lane);
+  return __any_sync(0xffffffffu, twice);
+}
+
+// What a row's teacher says, on one warp.  s_idx and s_q are its scratch (twice only).
+struct Teacher {
+  float q[kSlots], logq[kSlots], y[kSlots], mass[kSlots];
+  float rest;
+  bool none, bad;
+  template <bool CAP>
+  __device__ __forceinline__ void work(RowStats<CAP, false>& top, Picked& p, bool twice, const DistillArgs& a, int* s_idx,
+                                       float* s_q);
+};
+
+template <bool CAP>
+__device__ __forceinline__ void Teacher::work(RowStats<CAP, false>& top, Picked& p, bool twice, const DistillArgs& a,
+                                              int* s_idx, float* s_q) {
+  const int lane = threadIdx.x & 31;
+  const Squash sq = a.q;
+  bad = __any_sync(0xffffffffu, p.bad);
+  const bool any = __any_sync(0xffffffffu, p.any);
   float qsum = 0.f;
   if (a.tail) {
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
-      qk[j] = 0.f;
-      logq[j] = t[j];
-      if (32 * j < a.K) qsum += qk[j] = idx[j] >= 0 ? expf(t[j]) : 0.f;
+      q[j] = 0.f;
+      logq[j] = p.t[j];
+      if (32 * j < a.K) qsum += q[j] = p.idx[j] >= 0 ? expf(p.t[j]) : 0.f;
     }
   } else {
-    float tm = t[0], z = 0.f;
+    float tm = p.t[0], z = 0.f;
 #pragma unroll
-    for (int j = 1; j < kSlots; ++j) tm = fmaxf(tm, t[j]);
+    for (int j = 1; j < kSlots; ++j) tm = fmaxf(tm, p.t[j]);
     tm = redux_max(tm);
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
-      qk[j] = 0.f;
-      if (32 * j < a.K) z += qk[j] = (idx[j] >= 0 && tm != -INFINITY) ? expf(t[j] - tm) : 0.f;
+      q[j] = 0.f;
+      if (32 * j < a.K) z += q[j] = (p.idx[j] >= 0 && tm != -INFINITY) ? expf(p.t[j] - tm) : 0.f;
     }
     z = warp_sum(z);
     const float logz = logf(z);
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
-      qk[j] = z == 0.f ? 0.f : qk[j] / z;  // z: 0 without entries, NaN kept
-      logq[j] = t[j] - tm - logz;
-      qsum += qk[j];
+      q[j] = z == 0.f ? 0.f : q[j] / z;  // z: 0 without entries, NaN kept
+      logq[j] = p.t[j] - tm - logz;
+      qsum += q[j];
     }
   }
   qsum = warp_sum(qsum);
+  none = a.tail ? !any : qsum == 0.f;  // no teacher: loss 0, no gradient
+  rest = a.tail ? fmaxf(1.f - qsum, 0.f) : 0.f;
   // entries of one token: its logit counts once, at the first of them; their masses add up
   uint32_t later = 0;
 #pragma unroll
-  for (int j = 0; j < kSlots; ++j) mass[j] = twice ? 0.f : qk[j];
+  for (int j = 0; j < kSlots; ++j) mass[j] = twice ? 0.f : q[j];
   if (twice) {
 #pragma unroll
-    for (int j = 0; j < kSlots; ++j) s_q[32 * j + lane] = qk[j];
+    for (int j = 0; j < kSlots; ++j) {
+      s_idx[32 * j + lane] = p.idx[j];
+      s_q[32 * j + lane] = q[j];
+    }
     __syncwarp();
     for (int m = 0; m < a.K; ++m) {
       const int im = s_idx[m];
       const float qm = s_q[m];
 #pragma unroll
       for (int j = 0; j < kSlots; ++j) {
-        if (idx[j] == im) {
+        if (p.idx[j] == im) {
           mass[j] += qm;
           if (m < 32 * j + lane) later |= 1u << j;
         }
       }
     }
+    __syncwarp();  // the scratch is free for the next row
   }
-  __syncwarp();  // the scratch is free for the next row
-  RowStats<CAP, false> top;
   top.init();
   uint32_t w[kSlots];
 #pragma unroll
   for (int j = 0; j < kSlots; ++j) {
-    yk[j] = squash<CAP>(xk[j], q);
-    w[j] = __float_as_uint((idx[j] < 0 || (later >> j & 1u)) ? -INFINITY : xk[j]);
+    y[j] = squash<CAP>(p.x[j], sq);
+    w[j] = __float_as_uint((p.idx[j] < 0 || (later >> j & 1u)) ? -INFINITY : p.x[j]);
   }
-  top.template add_words<float>(w, words_max<float>(w), q);
-  top.warp_merge(q);
-  out_head.m = top.m;
-  out_head.lim = top.lim;
-  out_head.s = top.s;
-  out_head.r = top.r;
-  out_head.rest = a.tail ? fmaxf(1.f - qsum, 0.f) : 0.f;
-  out_head.none = a.tail ? !any : qsum == 0.f;  // no teacher: loss 0, no gradient
-  out_head.bad = bad;
+  top.template add_words<float>(w, words_max<float>(w), sq);
+  top.warp_merge(sq);
+}
+
+// A row's coefficients from the statistics of the rest and of the teacher's tokens.
+template <bool CAP>
+__device__ __forceinline__ FinishRow coefficients(const RowStats<CAP, false>& st, const RowStats<CAP, false>& top,
+                                                  float rest, bool none, bool bad, const Squash& q) {
+  RowStats<CAP, false> all = st;
+  all.merge(top, q);
+  all.center();
+  FinishRow f;
+  f.all = all.r;
+  f.rest = st.r;
+  f.logs = logf(all.s);
+  f.empty = all.s == 0.f;  // every logit is -inf: no distribution, no gradient
+  f.tail_loss = 0.f;
+  // the scale of p in units of e: p = e 2^(rest's reference - the row's) / S
+  const float below = ref_diff(st.r, all.r, q);
+  f.c = (none || st.s == 0.f) ? 0.f : ex2(below) / all.s;
+  // The rest is left out where the student has masked it: no logit outside the teacher's tokens
+  // above -inf, or none within kMasked of the largest (a mask of the type's lowest value).
+  if (rest > 0.f && st.s != 0.f && !none && !(squash<CAP>(st.m, q) - squash<CAP>(all.m, q) < -kMasked)) {
+    f.tail_loss = rest * (logf(rest) - (fmaf(below, kLn2, logf(st.s)) - f.logs));
+    f.c -= rest / st.s;
+  }
+  if (bad) f.c = NAN;
+  return f;
+}
+
+// One entry's term of the loss, added to it, and its token's gradient before the scale.
+template <bool CAP>
+__device__ __forceinline__ float entry_grad(float& loss, int idx, float qk, float logq, float y, float mass,
+                                            const FinishRow& f, bool none, bool bad, const Squash& q) {
+  const float lpk = (f.empty || y == -INFINITY) ? -INFINITY : log_prob(y, f.all, f.logs, q);
+  if (idx >= 0 && qk != 0.f) loss += qk * (logq - lpk);
+  if (bad) return NAN;
+  return (idx >= 0 && !none && !f.empty) ? (expf(lpk) - mass) * squash_slope<CAP>(y, q) : 0.f;
 }
 
 template <typename T, bool CAP, bool GRAD, int W>
-__global__ void __launch_bounds__(32 * (W + kRoles), W == kWide ? 2 : 6)
+__global__ void __launch_bounds__(32 * (W + kRoles), W == kWide ? 2 : 4)
 distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
   using Stats = RowStats<CAP, false>;
   constexpr int VEC = 16 / sizeof(T), kCompute = 32 * W;
@@ -400,15 +454,18 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
       const bool live = a.mask == nullptr || a.mask[r] != 0;
       const Share<T> sh(logits + a.addr.off(r), a.V, rank, a.log_cs);
       TeacherRow& out = s_teacher[b];
-      TeacherRow head;
-      int idx[kSlots];
-      float qk[kSlots], logq[kSlots], yk[kSlots], mass[kSlots], e0 = 0.f, e1 = 0.f;
+      Picked p;
+      Teacher te;
+      Stats top;
+      float e0 = 0.f, e1 = 0.f;
       const Entries now = entries;
       if (r + step < a.rows) entries.load(a, r + step);
       if (live) {  // all that needs no shared row
         if (lane < sh.head_here) e0 = to_f<T>(sh.row[lane]);
         if (lane < sh.tail_here) e1 = to_f<T>(sh.row[sh.tail0 + lane]);
-        teacher_row<T, CAP>(head, idx, qk, logq, yk, mass, now, sh.row, a, s_idx, s_q, s_tag);
+        p.pick(now, a, [&](int i) { return to_f<T>(sh.row[i]); });
+        const bool twice = maybe_twice(p, s_tag);
+        te.template work<CAP>(top, p, twice, a, s_idx, s_q);
       }
       wait.operator()<false>(&done[b], ((uint32_t)(it >> 1) & 1u) ^ 1u);
       wait.operator()<false>(&full, (uint32_t)it & 1u);
@@ -420,25 +477,25 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
           if (32 * j >= a.K) break;
-          const int k = 32 * j + lane, i = idx[j];
+          const int k = 32 * j + lane, i = p.idx[j];
           out.idx[k] = i;
-          out.q[k] = qk[j];
-          out.logq[k] = logq[j];
-          out.y[k] = yk[j];
-          out.mass[k] = mass[j];
+          out.q[k] = te.q[j];
+          out.logq[k] = te.logq[j];
+          out.y[k] = te.y[j];
+          out.mass[k] = te.mass[j];
           if (i < 0) continue;
           if (i >= sh.body0 && i < sh.body0 + sh.n) buf[i - sh.body0] = from_f<T>(-INFINITY);
           else if (i < sh.head_here) s_edge[b][0][i] = -INFINITY;
           else if (i >= sh.tail0 && i - sh.tail0 < sh.tail_here) s_edge[b][1][i - sh.tail0] = -INFINITY;
         }
         if (lane == 0) {
-          out.m = head.m;
-          out.lim = head.lim;
-          out.s = head.s;
-          out.r = head.r;
-          out.rest = head.rest;
-          out.none = head.none;
-          out.bad = head.bad;
+          out.m = top.m;
+          out.lim = top.lim;
+          out.s = top.s;
+          out.r = top.r;
+          out.rest = te.rest;
+          out.none = te.none;
+          out.bad = te.bad;
         }
       }
       __syncwarp();
@@ -462,12 +519,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
         float loss = 0.f;
         for (int k = lane; k < a.K; k += 32) {
           const int i = tr.idx[k];
-          const float qk = tr.q[k], yk = tr.y[k];
-          const float lpk = (fin.empty || yk == -INFINITY) ? -INFINITY : log_prob(yk, fin.all, fin.logs, q);
-          if (i >= 0 && qk != 0.f) loss += qk * (tr.logq[k] - lpk);
-          float gk = 0.f;
-          if (i >= 0 && !tr.none && !fin.empty) gk = (expf(lpk) - tr.mass[k]) * squash_slope<CAP>(yk, q);
-          if (tr.bad) gk = NAN;
+          const float gk = entry_grad<CAP>(loss, i, tr.q[k], tr.logq[k], tr.y[k], tr.mass[k], fin, tr.none, tr.bad, q);
           if constexpr (GRAD) {
             if (i >= 0 && sh.has(i)) grow[i] = from_f<T>(gk * scale);
           } else {
@@ -571,38 +623,15 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
           st.warp_merge(q);
         }
         const TeacherRow& tr = s_teacher[b];
-        Stats all = st, top;
+        Stats top;
         top.m = tr.m;
         top.lim = tr.lim;
         top.s = tr.s;
         top.r = tr.r;
-        all.merge(top, q);
-        all.center();
-        const float logs = logf(all.s);
-        // the scale of p in units of e: p = e 2^(rest's reference - the row's) / S
-        const float below = ref_diff(st.r, all.r, q);
-        float c = (tr.none || st.s == 0.f) ? 0.f : ex2(below) / all.s;
-        // The rest is left out where the student has masked it: no logit outside the teacher's
-        // tokens above -inf, or none within kMasked of the largest (a mask of the type's lowest value).
-        const float rest = tr.rest;
-        float tail_loss = 0.f;
-        if (rest > 0.f && st.s != 0.f && !tr.none && !(squash<CAP>(st.m, q) - squash<CAP>(all.m, q) < -kMasked)) {
-          tail_loss = rest * (logf(rest) - (fmaf(below, kLn2, logf(st.s)) - logs));
-          c -= rest / st.s;
-        }
-        if (tr.bad) c = NAN;
-        if (cw == 0 && lane == 0) {
-          FinishRow f;
-          f.all = all.r;
-          f.rest = st.r;
-          f.logs = logs;
-          f.tail_loss = tail_loss;
-          f.c = c;
-          f.empty = all.s == 0.f;  // every logit is -inf: no distribution, no gradient
-          s_fin[b] = f;
-        }
-        rest_ref = st.r;
-        cg = c * scale;
+        const FinishRow f = coefficients<CAP>(st, top, tr.rest, tr.none, tr.bad, q);
+        if (cw == 0 && lane == 0) s_fin[b] = f;
+        rest_ref = f.rest;
+        cg = f.c * scale;
       }
       if constexpr (GRAD) {
         T* gbody = grow + sh.body0;
@@ -636,6 +665,141 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
   if (cs > 1) row_cluster_sync();  // no more statistics from the other CTAs
 }
 
+// Short rows: one warp a row does it all, so that the steps of many rows overlap.
+constexpr int kShortBytes = 8192;  // of a row at most
+constexpr int kRowWarps = 8;
+
+__host__ __device__ constexpr int warp_row_bytes(int bytes) { return (bytes + 15) / 16 * 16; }
+
+template <typename T, bool CAP, bool GRAD>
+__global__ void __launch_bounds__(32 * kRowWarps, 3)
+distill_warp_kernel(const T* __restrict__ logits, const DistillArgs a) {
+  using Stats = RowStats<CAP, false>;
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ __align__(128) unsigned char s_rows[];
+  __shared__ float s_edges[kRowWarps][2][32];
+  __shared__ int s_idxs[kRowWarps][kMaxK];
+  __shared__ float s_qs[kRowWarps][kMaxK];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r = (int64_t)blockIdx.x * kRowWarps + warp;
+  if (r >= a.rows) return;
+  const Squash q = a.q;
+  const Share<T> sh(logits + a.addr.off(r), a.V, 0, 0);
+  const int nv = sh.n / VEC;
+  T* buf = reinterpret_cast<T*>(s_rows + warp * warp_row_bytes(a.V * (int)sizeof(T)));
+  float (*edge)[32] = s_edges[warp];
+  T* grow = GRAD ? reinterpret_cast<T*>(a.grad) + r * a.V : nullptr;
+  const bool vec = GRAD && (reinterpret_cast<uintptr_t>(grow + sh.body0) & 15u) == 0;
+  const bool live = a.mask == nullptr || a.mask[r] != 0;
+  const uint4* s_vec = reinterpret_cast<const uint4*>(buf);
+  Ref rest_ref{0.f, 0.f};
+  float cg = 0.f;
+  if (live) {
+    Entries e;
+    e.load(a, r);
+    for (int v = lane; v < nv; v += 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(buf + v * VEC)), "l"(sh.row + sh.body0 + v * VEC)
+                   : "memory");
+    if (lane < sh.head_here) edge[0][lane] = to_f<T>(sh.row[lane]);
+    if (lane < sh.tail_here) edge[1][lane] = to_f<T>(sh.row[sh.tail0 + lane]);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    Picked p;
+    p.pick(e, a, [&](int i) {
+      return i < sh.body0 ? edge[0][i] : (i < sh.tail0 ? to_f<T>(buf[i - sh.body0]) : edge[1][i - sh.tail0]);
+    });
+    __syncwarp();
+    // the row itself tells whether a token comes twice: each entry leaves its number there
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      const int i = p.idx[j];
+      if (i < 0) continue;
+      if (i < sh.body0) edge[0][i] = (float)(32 * j + lane);
+      else if (i < sh.tail0) buf[i - sh.body0] = from_f<T>((float)(32 * j + lane));
+      else edge[1][i - sh.tail0] = (float)(32 * j + lane);
+    }
+    __syncwarp();
+    bool twice = false;
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      const int i = p.idx[j];
+      if (i < 0) continue;
+      const float who = i < sh.body0 ? edge[0][i] : (i < sh.tail0 ? to_f<T>(buf[i - sh.body0]) : edge[1][i - sh.tail0]);
+      twice |= who != (float)(32 * j + lane);
+    }
+    twice = __any_sync(0xffffffffu, twice);
+    // ... and gives way to a logit without probability
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      const int i = p.idx[j];
+      if (i < 0) continue;
+      if (i < sh.body0) edge[0][i] = -INFINITY;
+      else if (i < sh.tail0) buf[i - sh.body0] = from_f<T>(-INFINITY);
+      else edge[1][i - sh.tail0] = -INFINITY;
+    }
+    __syncwarp();
+    Teacher te;
+    Stats top, st;
+    te.template work<CAP>(top, p, twice, a, s_idxs[warp], s_qs[warp]);
+    st.init();
+    int v = lane;
+    for (; v + 32 < nv; v += 64) {
+      const uint4 f = s_vec[v], h = s_vec[v + 32];
+      const uint32_t w[8] = {f.x, f.y, f.z, f.w, h.x, h.y, h.z, h.w};
+      st.template add_words<T>(w, words_max<T>(w), q);
+    }
+    if (v < nv) {
+      const uint4 f = s_vec[v];
+      const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+      st.template add_words<T>(w, words_max<T>(w), q);
+    }
+    if (lane < sh.head_here) st.add1(edge[0][lane], q);
+    if (lane < sh.tail_here) st.add1(edge[1][lane], q);
+    st.warp_merge(q);
+    const FinishRow f = coefficients<CAP>(st, top, te.rest, te.none, te.bad, q);
+    const float scale = GRAD ? (a.inv_n ? a.scale * *a.inv_n : a.scale) : 1.f;
+    float loss = 0.f, gk[kSlots];
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      gk[j] = 0.f;
+      if (32 * j < a.K)
+        gk[j] = entry_grad<CAP>(loss, p.idx[j], te.q[j], te.logq[j], te.y[j], te.mass[j], f, te.none, te.bad, q);
+    }
+    loss = warp_sum(loss) + f.tail_loss;
+    if (lane == 0) a.losses[r] = te.bad ? NAN : loss;
+    if constexpr (GRAD) {
+      rest_ref = f.rest;
+      cg = f.c * scale;
+      for (int u = lane; u < nv; u += 32) store_grads<T, CAP>(grow + sh.body0 + u * VEC, s_vec[u], rest_ref, cg, q, vec);
+      if (lane < sh.head_here) grow[lane] = from_f<T>(rest_grad<CAP>(edge[0][lane], rest_ref, cg, q));
+      if (lane < sh.tail_here) grow[sh.tail0 + lane] = from_f<T>(rest_grad<CAP>(edge[1][lane], rest_ref, cg, q));
+      __syncwarp();  // the teacher's tokens over what was written for them
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j)
+        if (p.idx[j] >= 0) grow[p.idx[j]] = from_f<T>(gk[j] * scale);
+    } else {
+      if (lane == 0 && a.rest) a.rest[r] = make_float4(f.rest.sh, f.rest.k, f.c, 0.f);
+      if (a.gk) {
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j)
+          if (32 * j + lane < a.K) a.gk[r * a.K + 32 * j + lane] = gk[j];
+      }
+    }
+  } else {  // what the row holds is not looked at
+    if (lane == 0) a.losses[r] = 0.f;
+    if constexpr (GRAD) {
+      const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+      for (int u = lane; u < nv; u += 32) store_grads<T, CAP>(grow + sh.body0 + u * VEC, none, rest_ref, 0.f, q, vec);
+      if (lane < sh.head_here) grow[lane] = from_f<T>(0.f);
+      if (lane < sh.tail_here) grow[sh.tail0 + lane] = from_f<T>(0.f);
+    } else {
+      if (lane == 0 && a.rest) a.rest[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (a.gk)
+        for (int k = lane; k < a.K; k += 32) a.gk[r * a.K + k] = 0.f;
+    }
+  }
+}
+
 struct DistillBwdArgs {
   const float4* rest;
   const float* gk;
@@ -644,23 +808,25 @@ struct DistillBwdArgs {
   const float* inv_n;
   const float* g_loss;
   RowAddr addr;
+  int64_t rows;
   float scale;
   int V, K, segs;
   Squash q;
 };
 
-constexpr int kBwdBatch = 2;
-constexpr int kBwdGroups = kThreads * kBwdBatch;
+constexpr int kBwdBatch = 4;
+constexpr int kBwdGroups = 32 * kBwdBatch;  // groups of one warp
 
-// The gradient from the forward's reference, c and K numbers a row: each CTA takes one segment of a
+// The gradient from the forward's reference, c and K numbers a row: each warp takes one segment of a
 // row, then writes those of the teacher's tokens that lie in it.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kThreads)
 distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const DistillBwdArgs a) {
-  const int tid = threadIdx.x;
-  const uint32_t r32 = blockIdx.x / (uint32_t)a.segs;
+  const int tid = threadIdx.x & 31;
+  const uint32_t at = blockIdx.x * (uint32_t)(kThreads / 32) + (threadIdx.x >> 5), r32 = at / (uint32_t)a.segs;
   const int64_t r = r32;
-  const int seg = (int)(blockIdx.x - r32 * (uint32_t)a.segs);
+  const int seg = (int)(at - r32 * (uint32_t)a.segs);
+  if (r >= a.rows) return;
   const Squash q = a.q;
   const T* row = logits + a.addr.off(r);
   T* grow = grad + r * a.V;
@@ -677,12 +843,12 @@ distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Dis
   RawGroup<T> raw[kBwdBatch];
 #pragma unroll
   for (int u = 0; u < kBwdBatch; ++u) {
-    const int g = gbeg + u * kThreads + tid;
+    const int g = gbeg + u * 32 + tid;
     if (g < cut.groups) raw[u] = load_group<T>(body + (int64_t)g * kGroup);
   }
 #pragma unroll
   for (int u = 0; u < kBwdBatch; ++u) {
-    const int g = gbeg + u * kThreads + tid;
+    const int g = gbeg + u * 32 + tid;
     if (g < cut.groups) {
       float x[kGroup];
 #pragma unroll
@@ -697,12 +863,12 @@ distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Dis
   if (last && tid < cut.tail)
     grow[tail0 + tid] = from_f<T>(rest_grad<CAP>(to_f<T>(row[tail0 + tid]), ref, c, q));
   if (!live) return;
-  __syncthreads();
-  if (tid < a.K) {
-    const int64_t i = a.idx[r * a.K + tid];
+  __syncwarp();
+  for (int k = tid; k < a.K; k += 32) {
+    const int64_t i = a.idx[r * a.K + k];
     const int64_t lo = first ? 0 : cut.head + (int64_t)gbeg * kGroup;
     const int64_t hi = last ? a.V : cut.head + (int64_t)(gbeg + kBwdGroups) * kGroup;
-    if (i >= lo && i < hi && i < a.V) grow[i] = from_f<T>(a.gk[r * a.K + tid] * scale);
+    if (i >= lo && i < hi && i < a.V) grow[i] = from_f<T>(a.gk[r * a.K + k] * scale);
   }
 }
 
@@ -788,6 +954,18 @@ int launch_width(const T* logits, DistillArgs& a, int64_t share, cudaStream_t st
 
 template <typename T>
 int launch_fwd(const T* logits, DistillArgs& a, cudaStream_t st) {
+  const bool cap = a.q.cap > 0.f;
+  if ((int64_t)a.V * (int64_t)sizeof(T) <= kShortBytes && a.rows >= 4 * sm_count()) {
+    auto kern = a.grad ? (cap ? distill_warp_kernel<T, true, true> : distill_warp_kernel<T, false, true>)
+                       : (cap ? distill_warp_kernel<T, true, false> : distill_warp_kernel<T, false, false>);
+    const size_t smem = (size_t)kRowWarps * warp_row_bytes(a.V * (int)sizeof(T));
+    AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                "ak_distill_topk_fwd: shared memory");
+    AK_CUDA_TRY(launch_rows(kern, (a.rows + kRowWarps - 1) / kRowWarps, 32 * kRowWarps, 1, smem, st, logits,
+                            (const DistillArgs&)a),
+                "ak_distill_topk_fwd");
+    return AK_OK;
+  }
   const int64_t share = share_bytes(a.V, 1 << a.log_cs, sizeof(T));
   return share <= kShareNarrow ? launch_width<T, kNarrow>(logits, a, share, st)
                                : launch_width<T, kWide>(logits, a, share, st);
@@ -857,14 +1035,15 @@ extern "C" int ak_distill_topk_bwd(void* grad, const void* logits, const int64_t
   a.gk = gk; a.idx = teacher_idx; a.mask = mask; a.inv_n = mask ? inv_n : nullptr; a.g_loss = g_loss;
   a.addr = RowAddr{inner, stride_outer, stride_inner};
   a.scale = mask ? temperature : temperature / (float)rows;
-  a.V = (int)V; a.K = (int)K;
+  a.rows = rows; a.V = (int)V; a.K = (int)K;
   a.segs = (int)std::max<int64_t>(1, (V / kGroup + kBwdGroups - 1) / kBwdGroups);
   a.q = make_squash(temperature, softcap);
-  AK_REQUIRE(rows * a.segs < (1LL << 31), AK_ERR_SHAPE, "ak_distill_topk_bwd: too many rows");
+  AK_REQUIRE(rows * a.segs < (1LL << 32) - 8, AK_ERR_SHAPE, "ak_distill_topk_bwd: too many rows");
   const bool cap = a.q.cap > 0.f;
   AK_DISPATCH_DTYPE(dt, T, {
     auto kern = cap ? distill_bwd_kernel<T, true> : distill_bwd_kernel<T, false>;
-    kern<<<(unsigned)(rows * a.segs), kThreads, 0, (cudaStream_t)stream>>>((T*)grad, (const T*)logits, a);
+    kern<<<(unsigned)((rows * a.segs + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, (cudaStream_t)stream>>>(
+        (T*)grad, (const T*)logits, a);
   });
   AK_CHECK_LAUNCH("ak_distill_topk_bwd");
   return AK_OK;

@@ -21,8 +21,8 @@
 namespace ak {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 256;       // of a CTA; kFew where a row has no work for that many
+constexpr int kFew = 128;
 constexpr int kMaxTop = 128;         // alternatives
 constexpr int kMaxCluster = 8;       // the portable cluster size
 constexpr int kMaxGroupMax = 8194;  // group maxima of one CTA's share (32 KB), head and tail included
@@ -56,6 +56,7 @@ struct Share {
   __device__ __forceinline__ int elems() const { return head_here + n * kGroup + tail_here; }
 };
 
+template <int NT>
 struct SelectScratch {
   union {
     struct {
@@ -69,22 +70,23 @@ struct SelectScratch {
     };
   };
   uint32_t chosen[kMaxTop];  // groups, then elements, in order of position
-  uint32_t warp_n[2][kWarps];
+  uint32_t warp_n[2][NT / 32];
   uint32_t ngroups, nelems;
 };
 
 // The first k of the n keys key(0 .. n - 1) in the order (key descending, position ascending):
 // their positions, ascending, in out.  Needs n >= k.  A binary search over the key's bits for the k-th largest,
 // then everything above it and the first of those equal to it.
-template <typename Key>
-__device__ void select_exact(Key key_at, int n, int k, uint32_t* out, SelectScratch& sc) {
+template <int NT, typename Key>
+__device__ void select_exact(Key key_at, int n, int k, uint32_t* out, SelectScratch<NT>& sc) {
+  constexpr int kWarps = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t t = 0;
   int above = 0;  // number of keys > t, known at the end
   for (int bit = 31; bit >= -1; --bit) {
     const uint32_t probe = bit >= 0 ? (t | (1u << bit)) : t;
     int c = 0;
-    for (int i = tid; i < n; i += kThreads) c += bit >= 0 ? (key_at(i) >= probe) : (key_at(i) > probe);
+    for (int i = tid; i < n; i += NT) c += bit >= 0 ? (key_at(i) >= probe) : (key_at(i) > probe);
     c = __reduce_add_sync(0xffffffffu, c);
     if (lane == 0) sc.warp_n[0][warp] = (uint32_t)c;
     __syncthreads();
@@ -97,7 +99,7 @@ __device__ void select_exact(Key key_at, int n, int k, uint32_t* out, SelectScra
   }
   const int equal_wanted = k - above;
   int taken = 0, equal_seen = 0;
-  for (int i0 = 0; i0 < n; i0 += kThreads) {
+  for (int i0 = 0; i0 < n; i0 += NT) {
     const int i = i0 + tid;
     const uint32_t key = i < n ? key_at(i) : 0u;
     const bool eq = i < n && key == t;
@@ -135,9 +137,10 @@ __device__ __forceinline__ uint64_t entry(uint32_t key, int index) {
 
 // The k best elements of the share, best first, in top[0 .. k).  gmax holds the n + 2 group maxima
 // (a barrier has passed since they were written), mine the largest element this thread has seen.
-template <typename T>
+template <typename T, int NT>
 __device__ void select_top(uint64_t* top, const Share<T>& sh, const float* gmax, float mine, int k,
-                           SelectScratch& sc) {
+                           SelectScratch<NT>& sc) {
+  constexpr int kWarps = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // A lower bound of the k-th best element: a key that at least k threads' largest elements reach,
   // found by bisection between the smallest and the largest of those; it ends early where not many
@@ -167,7 +170,7 @@ __device__ void select_top(uint64_t* top, const Share<T>& sh, const float* gmax,
   const float bound = key_value(lo);
   // candidates: the groups that reach the bound (four maxima at a time), then their elements
   const int ng = sh.n + 2;
-  for (int i = 4 * tid; i < ng; i += 4 * kThreads) {
+  for (int i = 4 * tid; i < ng; i += 4 * NT) {
     const float4 m = *reinterpret_cast<const float4*>(gmax + i);  // past the end: padding of the buffer
     const bool c0 = m.x >= bound || all, c1 = (m.y >= bound || all) && i + 1 < ng,
                c2 = (m.z >= bound || all) && i + 2 < ng, c3 = (m.w >= bound || all) && i + 3 < ng;
@@ -185,7 +188,7 @@ __device__ void select_top(uint64_t* top, const Share<T>& sh, const float* gmax,
   const uint32_t ncg = sc.ngroups;
   bool exact = ncg > kCandGroups - 4;
   if (!exact) {
-    for (int i = tid; i < (int)ncg; i += kThreads) {
+    for (int i = tid; i < (int)ncg; i += NT) {
       const int g = (int)sc.cand.groups[i], first = sh.start(g), size = sh.size(g);
       float x[kGroup];
       if (g >= 1 && g <= sh.n) {
@@ -211,7 +214,7 @@ __device__ void select_top(uint64_t* top, const Share<T>& sh, const float* gmax,
   if (!exact) {
     // the position of each candidate is the number of better ones
     const int ne = (int)sc.nelems;
-    for (int i = tid; i < ne; i += kThreads) {
+    for (int i = tid; i < ne; i += NT) {
       const uint64_t e = sc.cand.elems[i];
       int rank = 0, o = 0;
       for (; o + 4 <= ne; o += 4) {
@@ -228,17 +231,17 @@ __device__ void select_top(uint64_t* top, const Share<T>& sh, const float* gmax,
   // Many equal values (masked or constant rows): choose the k groups, then the k elements, exactly.
   __syncthreads();
   const int kg = min(k, ng);
-  select_exact([&](int i) { return sh.size(i) ? order_key(gmax[i]) : 0u; }, ng, kg, sc.chosen, sc);
-  for (int i = tid; i < kg * kGroup; i += kThreads) {
+  select_exact<NT>([&](int i) { return sh.size(i) ? order_key(gmax[i]) : 0u; }, ng, kg, sc.chosen, sc);
+  for (int i = tid; i < kg * kGroup; i += NT) {
     const int g = (int)sc.chosen[i / kGroup], e = i % kGroup;
     sc.keys[i] = e < sh.size(g) ? order_key(to_f<T>(sh.row[sh.start(g) + e])) : 0u;
   }
   __syncthreads();
   // positions in the list of chosen groups ascend with the position in the row
   __shared__ uint32_t groups[kMaxTop];
-  for (int i = tid; i < kg; i += kThreads) groups[i] = sc.chosen[i];
+  for (int i = tid; i < kg; i += NT) groups[i] = sc.chosen[i];
   __syncthreads();
-  select_exact([&](int i) { return sc.keys[i]; }, kg * kGroup, k, sc.chosen, sc);
+  select_exact<NT>([&](int i) { return sc.keys[i]; }, kg * kGroup, k, sc.chosen, sc);
   uint64_t e = 0;
   if (tid < k) {
     const int at = (int)sc.chosen[tid], g = (int)groups[at / kGroup];
@@ -273,19 +276,44 @@ struct FwdArgs {
 constexpr int kBatch = 2;  // groups of a thread in flight
 // CTAs on an SM: 16-bit groups take 32 registers a thread with two in flight, which hides the
 // row's start and end behind seven other rows; fp32 groups are twice as large
-template <typename T, bool CAP>
-constexpr int resident() { return sizeof(T) == 4 ? 4 : (CAP ? 5 : 8); }
+template <typename T, bool CAP, int NT>
+constexpr int resident() { return (sizeof(T) == 4 ? 4 : (CAP ? 5 : 8)) * (kThreads / NT); }
 
-template <typename T, bool CAP, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kThreads, (resident<T, CAP>()))
+// A row's results from its joined and centred statistics.
+template <typename T, bool CAP, bool ENT>
+__device__ __forceinline__ void write_row(const FwdArgs& a, int64_t r, const T* row, const RowStats<CAP, ENT>& st,
+                                          float logs) {
+  const int64_t t = a.targets ? a.targets[r] : 0;
+  const bool ignored = a.targets && t == a.ignore_index;
+  if (a.logprobs) {
+    float lp = 0.f;
+    if (!ignored) {
+      if (t < 0 || t >= a.V) lp = NAN;  // not a token
+      else if (st.s == 0.f) lp = -INFINITY;
+      else lp = log_prob(squash<CAP>(to_f<T>(row[t]), a.q), st.r, logs, a.q);
+    }
+    a.logprobs[r] = lp;
+  }
+  float H = 0.f;
+  if constexpr (ENT) {
+    if (!ignored && st.s != 0.f) H = fmaf(-kLn2, st.w / st.s, logs);
+    a.entropy[r] = H;
+  }
+  if (a.lse) a.lse[r] = ref_lse(st.r, logs, a.q);
+  if (a.stats) a.stats[r] = make_float4(st.r.sh, st.r.k, logs, H);
+}
+
+template <typename T, bool CAP, bool ENT, bool TOP, int NT>
+__global__ void __launch_bounds__(NT, (resident<T, CAP, NT>()))
 token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
+  constexpr int kWarps = NT / 32;
   using Stats = RowStats<CAP, ENT>;
   extern __shared__ __align__(16) float gmax[];  // TOP: group maxima
   __shared__ Stats s_warp[kWarps];
   __shared__ Stats s_cta;
   __shared__ float s_share[6];         // this CTA's statistics, read by the others of the cluster
   __shared__ uint64_t s_top[TOP ? kMaxTop : 1];
-  __shared__ __align__(16) unsigned char s_scratch[TOP ? sizeof(SelectScratch) : 8];
+  __shared__ __align__(16) unsigned char s_scratch[TOP ? sizeof(SelectScratch<NT>) : 8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cs = a.cs;
   const int64_t r = cs > 1 ? blockIdx.x / cs : blockIdx.x;
@@ -314,14 +342,14 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) st.template add_words<T>(raw.r[i].w, lm, q);
   };
   int g = tid;
-  for (; g + (kBatch - 1) * kThreads < sh.n; g += kBatch * kThreads) {
+  for (; g + (kBatch - 1) * NT < sh.n; g += kBatch * NT) {
     RawGroup<T> raw[kBatch];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) raw[u] = load_group<T>(body + (int64_t)(g + u * kThreads) * kGroup);
+    for (int u = 0; u < kBatch; ++u) raw[u] = load_group<T>(body + (int64_t)(g + u * NT) * kGroup);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) group(raw[u], g + u * kThreads);
+    for (int u = 0; u < kBatch; ++u) group(raw[u], g + u * NT);
   }
-  for (; g < sh.n; g += kThreads) group(load_group<T>(body + (int64_t)g * kGroup), g);
+  for (; g < sh.n; g += NT) group(load_group<T>(body + (int64_t)g * kGroup), g);
   // head and tail: one element a lane of the first and the last warp
   if (warp == 0 || warp == kWarps - 1) {
     const bool first = warp == 0;
@@ -353,7 +381,7 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
   }
   const int kl = TOP ? min(a.k, sh.elems()) : 0;
   if constexpr (TOP)
-    if (kl > 0) select_top<T>(s_top, sh, gmax, mine, kl, *reinterpret_cast<SelectScratch*>(s_scratch));
+    if (kl > 0) select_top<T>(s_top, sh, gmax, mine, kl, *reinterpret_cast<SelectScratch<NT>*>(s_scratch));
   if (cs > 1) {
     if (tid == 0) {
       s_share[0] = st.lim;
@@ -380,16 +408,16 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
   if constexpr (TOP) {
     // An entry's position in the row's list: its own in this CTA's list and the number of better
     // entries in each other list, all sorted.  The other lists are copied here first.
-    SelectScratch& sc = *reinterpret_cast<SelectScratch*>(s_scratch);
+    SelectScratch<NT>& sc = *reinterpret_cast<SelectScratch<NT>*>(s_scratch);
     if (cs > 1) {
       __syncthreads();  // the selection is done with its scratch
-      for (int i = tid; i < cs * a.k; i += kThreads) {  // 0 from the end of a shorter list on
+      for (int i = tid; i < cs * a.k; i += NT) {  // 0 from the end of a shorter list on
         const int c = i / a.k, o = i - c * a.k;
         sc.lists[i] = o < (int)ld_cluster_u32(&s_share[3], c) ? ld_cluster_u64(&s_top[o], c) : 0ull;
       }
-      for (int i = tid; i < kl; i += kThreads) sc.place[i] = i;
+      for (int i = tid; i < kl; i += NT) sc.place[i] = i;
       __syncthreads();
-      for (int i = tid; i < cs * kl; i += kThreads) {
+      for (int i = tid; i < cs * kl; i += NT) {
         const int c = i / kl, o = i - c * kl;
         if (c == rank) continue;
         const uint64_t e = s_top[o];
@@ -403,7 +431,7 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
       }
       __syncthreads();
     }
-    for (int i = tid; i < kl; i += kThreads) {
+    for (int i = tid; i < kl; i += NT) {
       const uint64_t e = s_top[i];
       const int pos = cs > 1 ? sc.place[i] : i;
       if (pos < a.k) {
@@ -413,30 +441,47 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
       }
     }
   }
-  if (rank == 0 && tid == 0) {
-    const int64_t t = a.targets ? a.targets[r] : 0;
-    const bool ignored = a.targets && t == a.ignore_index;
-    if (a.logprobs) {
-      float lp = 0.f;
-      if (!ignored) {
-        if (t < 0 || t >= a.V) lp = NAN;  // not a token
-        else if (st.s == 0.f) lp = -INFINITY;
-        else lp = log_prob(squash<CAP>(to_f<T>(row[t]), q), st.r, logs, q);
-      }
-      a.logprobs[r] = lp;
-    }
-    float H = 0.f;
-    if constexpr (ENT) {
-      if (!ignored && st.s != 0.f) H = fmaf(-kLn2, st.w / st.s, logs);
-      a.entropy[r] = H;
-    }
-    if (a.lse) a.lse[r] = ref_lse(st.r, logs, q);
-    if (a.stats) a.stats[r] = make_float4(st.r.sh, st.r.k, logs, H);
-  }
+  if (rank == 0 && tid == 0) write_row<T, CAP, ENT>(a, r, row, st, logs);
   if (cs > 1) {  // the other CTAs have read this one's shared memory
     row_cluster_arrive_relaxed();
     row_cluster_wait();
   }
+}
+
+// Many short rows: one warp a row, nothing shared.
+template <typename T, bool CAP, bool ENT>
+__global__ void __launch_bounds__(kThreads)
+token_logprobs_warp_kernel(const T* __restrict__ logits, const FwdArgs a, int64_t rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const Squash q = a.q;
+  const T* row = logits + a.addr.off(r);
+  const RowCut cut = cut_row(row, a.V);
+  RowStats<CAP, ENT> st;
+  st.init();
+  const T* body = row + cut.head;
+  auto group = [&](const RawGroup<T>& raw) {
+    float lm = words_max<T>(raw.r[0].w);
+    if constexpr (sizeof(T) == 4) lm = fmaxf(lm, words_max<T>(raw.r[1].w));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) st.template add_words<T>(raw.r[i].w, lm, q);
+  };
+  int g = lane;
+  for (; g + (kBatch - 1) * 32 < cut.groups; g += kBatch * 32) {
+    RawGroup<T> raw[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) raw[u] = load_group<T>(body + (int64_t)(g + u * 32) * kGroup);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) group(raw[u]);
+  }
+  for (; g < cut.groups; g += 32) group(load_group<T>(body + (int64_t)g * kGroup));
+  if (lane < cut.head) st.add1(to_f<T>(row[lane]), q);
+  if (lane < cut.tail) st.add1(to_f<T>(row[cut.head + cut.groups * kGroup + lane]), q);
+  st.warp_merge(q);
+  st.center();
+  const float logs = logf(st.s);
+  if (lane == 0) write_row<T, CAP, ENT>(a, r, row, st, logs);
 }
 
 struct BwdArgs {
@@ -445,22 +490,23 @@ struct BwdArgs {
   const float* g_ent;      // nullable
   const int64_t* targets;  // nullable
   RowAddr addr;
-  int64_t ignore_index;
+  int64_t rows, ignore_index;
   int V, segs;
   Squash q;
 };
 
 constexpr int kBwdBatch = 4;
-constexpr int kBwdGroups = kThreads * kBwdBatch;  // groups of one CTA
+constexpr int kBwdGroups = 32 * kBwdBatch;  // groups of one warp
 
-// Elementwise from the forward's numbers: each CTA takes one segment of a row.
+// Elementwise from the forward's numbers: each warp takes one segment of a row.
 template <typename T, bool CAP, bool ENT>
 __global__ void __launch_bounds__(kThreads)
 token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const BwdArgs a) {
-  const int tid = threadIdx.x;
-  const uint32_t r32 = blockIdx.x / (uint32_t)a.segs;
+  const int tid = threadIdx.x & 31;
+  const uint32_t at = blockIdx.x * (uint32_t)(kThreads / 32) + (threadIdx.x >> 5), r32 = at / (uint32_t)a.segs;
   const int64_t r = r32;
-  const int seg = (int)(blockIdx.x - r32 * (uint32_t)a.segs);
+  const int seg = (int)(at - r32 * (uint32_t)a.segs);
+  if (r >= a.rows) return;
   const Squash q = a.q;
   const T* row = logits + a.addr.off(r);
   T* grow = grad + r * a.V;
@@ -499,12 +545,12 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
   RawGroup<T> raw[kBwdBatch];
 #pragma unroll
   for (int u = 0; u < kBwdBatch; ++u) {
-    const int g = gbeg + u * kThreads + tid;
+    const int g = gbeg + u * 32 + tid;
     if (g < cut.groups) raw[u] = load_group<T>(body + (int64_t)g * kGroup);
   }
 #pragma unroll
   for (int u = 0; u < kBwdBatch; ++u) {
-    const int g = gbeg + u * kThreads + tid;
+    const int g = gbeg + u * 32 + tid;
     if (g < cut.groups) {
       float x[kGroup];
       if (none) {
@@ -526,11 +572,11 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
             x[h * 2 * P + 2 * i + 1] = o.y;
           }
         }
-        const int at = ti - (cut.head + g * kGroup);
-        if ((unsigned)at < (unsigned)kGroup) {
+        const int ta = ti - (cut.head + g * kGroup);
+        if ((unsigned)ta < (unsigned)kGroup) {
 #pragma unroll
           for (int i = 0; i < kGroup; ++i)
-            if (i == at) x[i] += ct;
+            if (i == ta) x[i] += ct;
         }
       } else {
         unpack_group<T>(x, raw[u]);
@@ -570,17 +616,36 @@ int check_rows(const char* what, const void* logits, int64_t rows, int64_t inner
   return AK_OK;
 }
 
+// Rows up to kShortRow elements: a warp each where there are enough of them to fill the GPU with
+// warps (100000 rows of 1500 bf16 values: 60 us, a CTA each 262 us), else, and where alternatives
+// are wanted, a CTA of 128 threads.
+constexpr int64_t kShortRow = 4096, kSmallRow = 8192;
+
+template <typename T, int NT>
+void (*pick_fwd(bool cap, bool ent, bool top))(const T*, FwdArgs) {
+#define AK_PICK(C, E, P) \
+  if (cap == C && ent == E && top == P) return token_logprobs_fwd_kernel<T, C, E, P, NT>;
+  AK_PICK(false, false, false) AK_PICK(false, false, true) AK_PICK(false, true, false) AK_PICK(false, true, true)
+  AK_PICK(true, false, false) AK_PICK(true, false, true) AK_PICK(true, true, false)
+#undef AK_PICK
+  return token_logprobs_fwd_kernel<T, true, true, true, NT>;
+}
+
 template <typename T>
 int launch_fwd(const T* logits, const FwdArgs& a, int64_t rows, cudaStream_t st) {
   const bool cap = a.q.cap > 0.f, ent = a.entropy != nullptr, top = a.k > 0;
-  void (*kern)(const T*, FwdArgs) = nullptr;
-#define AK_PICK(C, E, P) \
-  if (cap == C && ent == E && top == P) kern = token_logprobs_fwd_kernel<T, C, E, P>;
-  AK_PICK(false, false, false) AK_PICK(false, false, true) AK_PICK(false, true, false) AK_PICK(false, true, true)
-  AK_PICK(true, false, false) AK_PICK(true, false, true) AK_PICK(true, true, false) AK_PICK(true, true, true)
-#undef AK_PICK
+  if (!top && a.V <= kShortRow && rows >= 4 * sm_count()) {
+    auto kern = cap ? (ent ? token_logprobs_warp_kernel<T, true, true> : token_logprobs_warp_kernel<T, true, false>)
+                    : (ent ? token_logprobs_warp_kernel<T, false, true> : token_logprobs_warp_kernel<T, false, false>);
+    const int64_t grid = (rows + kThreads / 32 - 1) / (kThreads / 32);
+    AK_CUDA_TRY(launch_rows(kern, grid, kThreads, 1, 0, st, logits, a, rows), "ak_token_logprobs_fwd");
+    return AK_OK;
+  }
+  const bool few = a.V <= kSmallRow && a.cs == 1;
+  const int nt = few ? kFew : kThreads;
+  auto kern = few ? pick_fwd<T, kFew>(cap, ent, top) : pick_fwd<T, kThreads>(cap, ent, top);
   const size_t smem = top ? ((size_t)(a.V / kGroup) / a.cs + 3 + 4) * 4 : 0;  // read four at a time
-  AK_CUDA_TRY(launch_rows(kern, rows * a.cs, kThreads, a.cs, smem, st, logits, a), "ak_token_logprobs_fwd");
+  AK_CUDA_TRY(launch_rows(kern, rows * a.cs, nt, a.cs, smem, st, logits, a), "ak_token_logprobs_fwd");
   return AK_OK;
 }
 
@@ -634,15 +699,17 @@ extern "C" int ak_token_logprobs_bwd(void* grad, const void* logits, const int64
   a.g_lp = g_logprobs; a.g_ent = g_entropy; a.targets = targets;
   a.addr = RowAddr{inner, stride_outer, stride_inner};
   a.ignore_index = ignore_index;
+  a.rows = rows;
   a.V = (int)V;
   a.segs = (int)std::max<int64_t>(1, (V / kGroup + kBwdGroups - 1) / kBwdGroups);
   a.q = make_squash(temperature, softcap);
-  AK_REQUIRE(rows * a.segs < (1LL << 31), AK_ERR_SHAPE, "ak_token_logprobs_bwd: too many rows");
+  AK_REQUIRE(rows * a.segs < (1LL << 32) - 8, AK_ERR_SHAPE, "ak_token_logprobs_bwd: too many rows");
   const bool cap = a.q.cap > 0.f, ent = g_entropy != nullptr;
   AK_DISPATCH_DTYPE(dt, T, {
     auto kern = cap ? (ent ? token_logprobs_bwd_kernel<T, true, true> : token_logprobs_bwd_kernel<T, true, false>)
                     : (ent ? token_logprobs_bwd_kernel<T, false, true> : token_logprobs_bwd_kernel<T, false, false>);
-    kern<<<(unsigned)(rows * a.segs), kThreads, 0, (cudaStream_t)stream>>>((T*)grad, (const T*)logits, a);
+    kern<<<(unsigned)((rows * a.segs + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, (cudaStream_t)stream>>>(
+        (T*)grad, (const T*)logits, a);
   });
   AK_CHECK_LAUNCH("ak_token_logprobs_bwd");
   return AK_OK;

@@ -285,3 +285,14 @@ def test_many_rows_per_cta(n, v, k, dtype):
     check(x, idx, tlp, mask, tail=True)
     mask[::2] = False
     check(x, idx, tlp, mask, tail=False, modes=("fused",))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,k", [(1000, 1, 1), (700, 13, 5), (900, 1500, 128), (1300, 2048, 9), (601, 2047, 33)])
+def test_many_short_rows(n, v, k, dtype):
+    x, idx, tlp, mask = problem(n, v, min(k, v), dtype, seed=22)
+    idx[5, -1] = idx[5, 0]
+    idx[6, 0] = -1
+    idx[7] = -1
+    check(x, idx, tlp, mask, tail=True)
+    check(x, idx, tlp, None, tail=False, softcap=5.0, temperature=1.3)

@@ -306,3 +306,23 @@ def test_large_offsets():
     g, = torch.autograd.grad(token_logprobs(xg, t).logprobs, xg, torch.ones(n, device=DEV))
     ref, tol = O.token_logprobs_grad(x[-1:].detach().double().cpu(), t[-1:].cpu(), torch.ones(1), None)
     O.assert_within(g[-1:], ref, tol, "grad")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v", [(1000, 1), (700, 13), (900, 1500), (801, 4095), (650, 4097), (601, 8192)])
+def test_many_short_rows(n, v, dtype):
+    from kernels.token_logprobs import token_logprobs
+    x, t = rows(n, v, dtype, seed=13)
+    x[3] = -torch.inf
+    x[4] = torch.finfo(dtype).min
+    x[5, v // 2:] = -torch.inf
+    x[6] = 1.5
+    for k in sorted({0, min(3, v), min(128, v)}):
+        check(x, t, token_logprobs(x, t, top_k=k, entropy=True), top_k=k)
+    check(x, t, token_logprobs(x, t, softcap=7.0), entropy=False, softcap=7.0)
+    gl = torch.randn(n, generator=torch.Generator().manual_seed(1))
+    xg = x.clone().requires_grad_(True)
+    r = token_logprobs(xg, t, entropy=True)
+    g, = torch.autograd.grad([r.logprobs, r.entropy], xg, [gl.to(DEV), gl.to(DEV)])
+    ref, tol = O.token_logprobs_grad(x.double().cpu(), t.cpu(), gl, gl)
+    O.assert_within(g, ref, tol, "grad")
