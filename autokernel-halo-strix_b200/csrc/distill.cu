@@ -44,6 +44,7 @@ constexpr int kShareWanted = 101 * 1024;  // bytes of one row in one CTA: two CT
 constexpr int kShareMost = 208 * 1024;    // of a row too long for that in eight CTAs
 constexpr int kPieces = 8;                // a buffer is handed back in pieces
 constexpr float kMasked = 30000.f;
+constexpr int64_t kCountRows = 1024;      // rows up to which every warp counts the mask
 
 struct DistillArgs {
   float* losses;        // [rows]
@@ -53,15 +54,26 @@ struct DistillArgs {
   const int64_t* idx;   // [rows][K]
   const float* tlp;     // [rows][K]
   const uint8_t* mask;  // nullable [rows]
-  const float* inv_n;   // GRAD, nullable: 1 / rows that count (host value in scale otherwise)
+  const float* inv_n;   // GRAD, nullable: 1 / rows that count (else each warp counts the mask itself)
   RowAddr addr;
   int64_t rows;
-  float scale;          // GRAD: T, times 1 / rows without inv_n
+  float scale;          // GRAD: T, times 1 / rows without a mask
   int V, K, log_cs, tail;
   uint32_t piece;       // bytes of a piece of the row buffer
   Squash q;
   int* status;
 };
+
+// 1 / max(1, rows whose mask is set), counted by one warp.
+__device__ __forceinline__ float count_rows(const uint8_t* mask, int64_t rows) {
+  int c = 0;
+  for (int64_t i = threadIdx.x & 31; i < rows; i += 32) c += mask[i] != 0;
+  return 1.f / (float)max(__reduce_add_sync(0xffffffffu, c), 1);
+}
+__device__ __forceinline__ float grad_scale(const DistillArgs& a) {
+  if (a.mask == nullptr) return a.scale;
+  return a.scale * (a.inv_n ? *a.inv_n : count_rows(a.mask, a.rows));
+}
 
 // The gradient at a logit outside the teacher's tokens.  c = 0 gives 0 whatever x is.
 template <bool CAP>
@@ -503,7 +515,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
     }
   } else if (warp == 2) {
     // ---------------- finisher
-    const float scale = GRAD ? (a.inv_n ? a.scale * *a.inv_n : a.scale) : 1.f;
+    const float scale = GRAD ? grad_scale(a) : 1.f;
     int it = 0;
     for (int64_t r = first; r < a.rows; r += step, ++it) {
       const int b = it & 1;
@@ -545,7 +557,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
   } else {
     // ---------------- compute
     const int cw = warp - kRoles, ct = tid - 32 * kRoles;
-    const float scale = GRAD ? (a.inv_n ? a.scale * *a.inv_n : a.scale) : 1.f;
+    const float scale = GRAD ? grad_scale(a) : 1.f;
     const uint4* s_vec = reinterpret_cast<const uint4*>(s_row);
     const int pv = (int)(a.piece / 16);
     int it = 0, nlive = 0;
@@ -757,7 +769,7 @@ distill_warp_kernel(const T* __restrict__ logits, const DistillArgs a) {
     if (lane < sh.tail_here) st.add1(edge[1][lane], q);
     st.warp_merge(q);
     const FinishRow f = coefficients<CAP>(st, top, te.rest, te.none, te.bad, q);
-    const float scale = GRAD ? (a.inv_n ? a.scale * *a.inv_n : a.scale) : 1.f;
+    const float scale = GRAD ? grad_scale(a) : 1.f;
     float loss = 0.f, gk[kSlots];
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
@@ -888,20 +900,30 @@ distill_inv_rows(float* __restrict__ inv_n, const uint8_t* __restrict__ mask, in
   }
 }
 
-// loss[0] = mult * inv_n * sum of the rows' losses, in a fixed order.
+// loss[0] = mult / rows that count * sum of the rows' losses, in a fixed order; inv_n (with a mask)
+// receives that quotient of 1.
 __global__ void __launch_bounds__(1024)
-distill_mean(float* __restrict__ loss, const float* __restrict__ losses, const float* __restrict__ inv_n,
-             float mult, int64_t rows) {
+distill_mean(float* __restrict__ loss, float* __restrict__ inv_n, const float* __restrict__ losses,
+             const uint8_t* __restrict__ mask, float mult, int64_t rows) {
   __shared__ float s[32];
+  __shared__ int n[32];
   float v = 0.f;
-  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) v += losses[i];
+  int c = 0;
+  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) {
+    v += losses[i];
+    if (mask) c += mask[i] != 0;
+  }
   v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  c = __reduce_add_sync(0xffffffffu, c);
+  if ((threadIdx.x & 31) == 0) { s[threadIdx.x >> 5] = v; n[threadIdx.x >> 5] = c; }
   __syncthreads();
   if (threadIdx.x == 0) {
     float t = 0.f;
-    for (int i = 0; i < 32; ++i) t += s[i];
-    loss[0] = t * mult * (inv_n ? *inv_n : 1.f);
+    int k = 0;
+    for (int i = 0; i < 32; ++i) { t += s[i]; k += n[i]; }
+    const float inv = mask ? 1.f / (float)max(k, 1) : 1.f;
+    loss[0] = t * mult * inv;
+    if (inv_n) inv_n[0] = inv;
   }
 }
 
@@ -994,7 +1016,9 @@ extern "C" int ak_distill_topk_fwd(float* loss, float* losses, float* inv_n, voi
              "ak_distill_topk_fwd: grad not aligned to its type");
   cudaStream_t st = (cudaStream_t)stream;
   if (rows > 0) {
-    if (mask) {
+    // few rows: each warp counts them, which costs less than a launch
+    const bool count = mask && grad && rows > kCountRows;
+    if (count) {
       distill_inv_rows<<<1, 1024, 0, st>>>(inv_n, mask, rows);
       AK_CHECK_LAUNCH("ak_distill_topk_fwd");
     }
@@ -1002,7 +1026,7 @@ extern "C" int ak_distill_topk_fwd(float* loss, float* losses, float* inv_n, voi
     a.losses = losses; a.grad = grad;
     a.rest = reinterpret_cast<float4*>(rest_stats);
     a.gk = gk; a.idx = teacher_idx; a.tlp = teacher_lp; a.mask = mask;
-    a.inv_n = mask ? inv_n : nullptr;
+    a.inv_n = count ? inv_n : nullptr;
     a.addr = RowAddr{inner, stride_outer, stride_inner};
     a.scale = mask ? temperature : temperature / (float)rows;
     a.rows = rows; a.V = (int)V; a.K = (int)K; a.log_cs = log_cluster_for(rows, V, elem_size(dt)); a.tail = tail != 0;
@@ -1011,7 +1035,7 @@ extern "C" int ak_distill_topk_fwd(float* loss, float* losses, float* inv_n, voi
     AK_DISPATCH_DTYPE(dt, T, rc = launch_fwd<T>((const T*)logits, a, st));
     if (rc) return rc;
   }
-  distill_mean<<<1, 1024, 0, st>>>(loss, losses, (mask && rows > 0) ? inv_n : nullptr,
+  distill_mean<<<1, 1024, 0, st>>>(loss, rows > 0 ? inv_n : nullptr, losses, mask,
                                    temperature * temperature / ((mask || rows == 0) ? 1.f : (float)rows), rows);
   AK_CHECK_LAUNCH("ak_distill_topk_fwd");
   return AK_OK;

@@ -68,6 +68,7 @@ constexpr int64_t kChunkRows = 16384;
 constexpr int kTileOverheadK = 4;  // per-tile cost beyond its K blocks, in K blocks (list schedule)
 
 // EPI_NONE: accumulate only (timing)
+enum Mode : int { kGemm = 0, kLogpFwd = 1, kLogpBwd = 2 };
 enum Epi : int { EPI_STATS = 0, EPI_STORE = 1, EPI_NONE = 2, EPI_LOGP = 3, EPI_LOGP_GRAD = 4 };
 
 struct Prob {
@@ -95,6 +96,11 @@ struct Prob {
   const float* g_lp;        // nullable [M]
   const float* g_ent;       // nullable [M]
   Squash q;
+  // launches of the kLogpBwd instance only.  two: operand A is the sum of two matrices (the second
+  // problem's map).  The K blocks (of both) are cut into ksplits runs of kper; run r's fp32 result
+  // lies r * M * ldc elements into C.  C2 (EPI_LOGP_GRAD, nullable): what rounding C left over.
+  int two, ksplits, kper;
+  void* C2;
 };
 
 // Two problems whose tiles differ in K (dW's short-K tiles and dH's long-K ones)
@@ -374,6 +380,26 @@ __device__ __forceinline__ int sched_tile(const Group& g, int pair, int npairs, 
   return g.lp == 0 ? g.p[0].tiles + (int)sidx : (int)sidx;
 }
 
+// kLogpBwd launches hold one problem whose tiles may each be cut into runs of K blocks: takes the
+// run out of the tile's number.
+template <bool kCut>
+__device__ __forceinline__ int split_tile(const Group& g, int& t) {
+  if constexpr (!kCut) return 0;
+  const int run = t / g.p[0].tiles;
+  t -= run * g.p[0].tiles;
+  return run;
+}
+// K blocks [kbeg, kend) of a run; kend comes in as the blocks of one A matrix.
+__device__ __forceinline__ void k_run(const Prob& P, int run, int& kbeg, int& kend) {
+  const int all = P.two ? 2 * kend : kend;
+  kbeg = 0;
+  kend = all;
+  if (P.ksplits > 1) {
+    kbeg = run * P.kper;
+    kend = min(all, kbeg + P.kper);
+  }
+}
+
 // This pair's tile after `prev` (its k-th turn).  kList = false: plain round robin,
 // the loop the single-class launches compile to; true: sched_tile.
 template <bool kList>
@@ -490,7 +516,7 @@ __device__ __forceinline__ void epi_stats(const Prob& P, uint32_t tbase, int row
 // C = acc * scale (+ add_f32) (+ C if accumulate), fp32 or 16-bit (staged rows).
 template <typename T>
 __device__ __forceinline__ void epi_store(const Prob& P, uint32_t tbase, int row0, int lane, int col0, int eg,
-                                          uint32_t stg) {
+                                          uint32_t stg, int64_t c_f32_off = 0) {
   const int row = row0 + lane;
   const bool rv = row < P.M;
   const int nrows = min(32, P.M - row0);
@@ -524,7 +550,7 @@ __device__ __forceinline__ void epi_store(const Prob& P, uint32_t tbase, int row
     }
     if (P.c_f32) {
       if (rv) {
-        float* crow = reinterpret_cast<float*>(P.C) + off;
+        float* crow = reinterpret_cast<float*>(P.C) + off + c_f32_off;
         if (full) {
 #pragma unroll
           for (int q = 0; q < 32; q += 4) {
@@ -686,6 +712,12 @@ __device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int
         v[j] = o * squash_slope<true>(y, q);
       }
     }
+    if (P.C2 != nullptr && row < P.M) {
+      T* lo = reinterpret_cast<T*>(P.C2) + (int64_t)row * P.ldc + cbase;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (cbase + j < P.N) lo[j] = from_f<T>(v[j] - to_f<T>(from_f<T>(v[j])));
+    }
     if (col0 + c0 + 32 * (k | 1) + 32 <= P.N) {
       stage_put<T>(stg, lane, k & 1, v);
       if (k & 1) {
@@ -706,8 +738,10 @@ __device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int
 // ---------------------------------------------------------------------------
 // The GEMM kernel (clusters of 2 CTAs)
 // ---------------------------------------------------------------------------
-// kLogp: the log-probability epilogues, kept out of the instances that the other launches use.
-template <typename T, bool kList, bool kLogp>
+// kMode keeps what the log-probabilities need out of the instances that the other launches use:
+// kGemm as before, kLogpFwd with EPI_LOGP alone, kLogpBwd with EPI_LOGP_GRAD and the products of two
+// matrices or of a cut K.
+template <typename T, bool kList, int kMode>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 tc_gemm2_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tB0,
                 const __grid_constant__ CUtensorMap tA1, const __grid_constant__ CUtensorMap tB1,
@@ -753,21 +787,30 @@ tc_gemm2_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__
       bool live = true;
       for (int k = 0, t = -1; live && (t = next_tile<kList>(g, pair, npairs, k, t)) >= 0; ++k) {
         int pi, mt, nt;
-        decode_tile(g, t, pi, mt, nt);
+        int tile = t;
+        [[maybe_unused]] const int run = split_tile<kMode == kLogpBwd>(g, tile);
+        decode_tile(g, tile, pi, mt, nt);
         const Prob& P = pi ? g.p[1] : g.p[0];
         const CUtensorMap* mA = pi ? &tA1 : &tA0;
         const CUtensorMap* mB = pi ? &tB1 : &tB0;
         const int m0 = mt * (2 * BM) + (int)rank * BM;
         const int n0 = nt * BN + (int)rank * (BN / 2);
-        const int ktiles = (P.K + BK - 1) / BK;  // the K tail is zero-filled by TMA in both operands
-        for (int kb = 0; kb < ktiles; ++kb, ++it) {
+        int ktiles = (P.K + BK - 1) / BK;  // the K tail is zero-filled by TMA in both operands
+        [[maybe_unused]] const int kone = ktiles;
+        int kbeg = 0;
+        if constexpr (kMode == kLogpBwd) k_run(P, run, kbeg, ktiles);
+        for (int kb = kbeg; kb < ktiles; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (uint32_t)(it / STAGES) & 1u;
           if (!wait_bar<false>(&empty[s], ph ^ 1u, wt)) { live = false; break; }  // issue no more loads
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
           const uint32_t bar = full0 + (uint32_t)(s * 8);
           const uint32_t st = smem_u32(tiles + s * STAGE_BYTES);
-          const int k0 = kb * BK;
+          int k0 = kb * BK;
+          if constexpr (kMode == kLogpBwd) {
+            if (P.two) mA = kb >= kone ? &tA1 : &tA0;
+            if (kb >= kone) k0 = (kb - kone) * BK;
+          }
           if (P.a_mn) {
             tma_load_2d(st, mA, m0, k0, bar);
             tma_load_2d(st + A_BYTES / 2, mA, m0 + 64, k0, bar);
@@ -795,7 +838,9 @@ tc_gemm2_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__
       bool live = true;
       for (int t = -1; live && (t = next_tile<kList>(g, pair, npairs, local, t)) >= 0; ++local) {
         int pi, mt, nt;
-        decode_tile(g, t, pi, mt, nt);
+        int tile = t;
+        [[maybe_unused]] const int run = split_tile<kMode == kLogpBwd>(g, tile);
+        decode_tile(g, tile, pi, mt, nt);
         const Prob& P = pi ? g.p[1] : g.p[0];
         const uint32_t idesc = make_idesc(kBf16, 2 * BM, BN, P.a_mn, P.b_mn);
         // K = 16 steps inside a 64-deep stage: 32 B along a K-major row, or two
@@ -805,8 +850,10 @@ tc_gemm2_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__
         if (!wait_bar<true>(&tempty[acc], ((uint32_t)(local >> 1) & 1u) ^ 1u, wt)) { live = false; break; }
         tc_fence_after();
         const uint32_t dcol = tmem_base + (uint32_t)(acc * BN);
-        const int ktiles = (P.K + BK - 1) / BK;
-        for (int kb = 0; kb < ktiles; ++kb, ++it) {
+        int ktiles = (P.K + BK - 1) / BK;
+        int kbeg = 0;
+        if constexpr (kMode == kLogpBwd) k_run(P, run, kbeg, ktiles);
+        for (int kb = 0; kb < ktiles - kbeg; ++kb, ++it) {
           const int s = it % STAGES;
           if (!wait_bar<false>(&full[s], (uint32_t)(it / STAGES) & 1u, wt)) { live = false; break; }
           tc_fence_after();
@@ -838,7 +885,9 @@ tc_gemm2_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__
     int local = 0;
     for (int t = -1; (t = next_tile<kList>(g, pair, npairs, local, t)) >= 0; ++local) {
       int pi, mt, nt;
-      decode_tile(g, t, pi, mt, nt);
+      int tile = t;
+      [[maybe_unused]] const int run = split_tile<kMode == kLogpBwd>(g, tile);
+      decode_tile(g, tile, pi, mt, nt);
       const Prob& P = pi ? g.p[1] : g.p[0];
       const int acc = local & 1;
       const int row0 = mt * (2 * BM) + (int)rank * BM + quad * 32;  // this warp's 32 rows
@@ -846,22 +895,22 @@ tc_gemm2_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__
       // behind the MMAs
       int64_t lab = -1;
       [[maybe_unused]] LogpRow lr;
-      if constexpr (kLogp) {
-        if (P.epi == EPI_LOGP) {
-          if (P.labels && row0 + lane < P.M) lab = P.labels[row0 + lane];
-          if (lab < 0 || lab >= P.N) lab = -1;
-        } else {
-          lr = load_logp_row(P, row0 + lane);
-        }
+      if constexpr (kMode == kLogpFwd) {
+        if (P.labels && row0 + lane < P.M) lab = P.labels[row0 + lane];
+        if (lab < 0 || lab >= P.N) lab = -1;
+      } else if constexpr (kMode == kLogpBwd) {
+        if (P.epi == EPI_LOGP_GRAD) lr = load_logp_row(P, row0 + lane);
       } else {
         lab = (P.epi == EPI_STATS && row0 + lane < P.M) ? P.labels[row0 + lane] : -1;
       }
       if (!wait_bar<false>(&tfull[acc], (uint32_t)(local >> 1) & 1u, wt)) break;  // no accumulator to read
       tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
-      if constexpr (kLogp) {
-        if (P.epi == EPI_LOGP) epi_logp<T>(P, tbase, row0, lane, lab, nt * BN, eg);
-        else epi_logp_grad<T>(P, tbase, row0, lane, lr, nt * BN, eg, stg);
+      if constexpr (kMode == kLogpFwd) {
+        epi_logp<T>(P, tbase, row0, lane, lab, nt * BN, eg);
+      } else if constexpr (kMode == kLogpBwd) {
+        if (P.epi == EPI_LOGP_GRAD) epi_logp_grad<T>(P, tbase, row0, lane, lr, nt * BN, eg, stg);
+        else epi_store<T>(P, tbase, row0, lane, nt * BN, eg, stg, (int64_t)run * P.M * P.ldc);
       } else {
         if (P.epi == EPI_STATS) epi_stats<T>(P, tbase, row0, lane, lab, nt * BN, eg, stg);
         else if (P.epi == EPI_STORE) epi_store<T>(P, tbase, row0, lane, nt * BN, eg, stg);
@@ -1022,6 +1071,22 @@ logp_rows_reduce(float* __restrict__ logprobs, float* __restrict__ entropy, floa
   if (stats) stats[row] = make_float4(st.r.sh, st.r.k, logs, H);
 }
 
+// out[i] = sum of the `runs` fp32 arrays of n elements, rounded once.  n is a multiple of 8.
+template <typename T>
+__global__ void __launch_bounds__(256)
+logp_sum_runs(T* __restrict__ out, const float* __restrict__ part, int runs, int64_t n) {
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int r = 0; r < runs; ++r) {
+      const float4 p = *reinterpret_cast<const float4*>(part + r * n + i);
+      s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+    }
+    const float o[4] = {s.x, s.y, s.z, s.w};
+    store_frag<T, 4>(out + i, o);
+  }
+}
+
 // scale[0] = largest |g_lp| + |g_ent| over the rows (1 where that is 0 or not finite): divides the
 // 16-bit gradient of the logits, so that small upstream gradients do not underflow in fp16.
 __global__ void __launch_bounds__(1024)
@@ -1101,7 +1166,7 @@ int resident_pairs() {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmem;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, tc_gemm2_kernel<T, false, false>, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, tc_gemm2_kernel<T, false, kGemm>, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
       n = sm_count() / 2;
     }
@@ -1111,16 +1176,17 @@ int resident_pairs() {
 }
 
 template <typename T>
-int launch_group(const Operand* A, const Operand* B, Group& g, cudaStream_t st) {
+int launch_group(const Operand* A, const Operand* B, Group& g, cudaStream_t st, const Operand* A2 = nullptr) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   // before the tensor maps: the runtime call binds the device's context to this thread, which the
   // driver's encoder needs (an autograd worker may come here with none bound yet)
   auto prepare = [](auto kern) {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   };
-  const bool logp = g.p[0].epi == EPI_LOGP || g.p[0].epi == EPI_LOGP_GRAD;
-  AK_CUDA_TRY(logp ? prepare(tc_gemm2_kernel<T, false, true>) : prepare(tc_gemm2_kernel<T, false, false>),
-              "linear_ce: smem attribute");
+  auto kern = tc_gemm2_kernel<T, false, kGemm>;
+  if (g.p[0].epi == EPI_LOGP) kern = tc_gemm2_kernel<T, false, kLogpFwd>;
+  else if (g.p[0].epi == EPI_LOGP_GRAD || g.p[0].ksplits > 0) kern = tc_gemm2_kernel<T, false, kLogpBwd>;
+  AK_CUDA_TRY(prepare(kern), "linear_ce: smem attribute");
   CUtensorMap maps[4];
   int rc;
   for (int i = 0; i < g.nprob; ++i) {
@@ -1134,7 +1200,10 @@ int launch_group(const Operand* A, const Operand* B, Group& g, cudaStream_t st) 
     finish_prob(g.p[i]);
   }
   if (g.nprob == 1) { maps[2] = maps[0]; maps[3] = maps[1]; }
-  g.total = g.p[0].tiles + (g.nprob > 1 ? g.p[1].tiles : 0);
+  if (A2 != nullptr &&
+      (rc = make_tmap(&maps[2], A2->base, A2->rows, A2->cols, A2->ld ? A2->ld : A2->cols, A2->mn, bf16)))
+    return rc;
+  g.total = g.p[0].tiles * std::max(1, g.p[0].ksplits) + (g.nprob > 1 ? g.p[1].tiles : 0);
   g.lp = -1;
   if (g.nprob == 2 && g.p[0].tiles > 0 && g.p[1].tiles > 0) {
     const int k0 = (g.p[0].K + BK - 1) / BK, k1 = (g.p[1].K + BK - 1) / BK;
@@ -1147,9 +1216,8 @@ int launch_group(const Operand* A, const Operand* B, Group& g, cudaStream_t st) 
     }
   }
   if (g.total == 0) return AK_OK;
-  auto kern = logp ? tc_gemm2_kernel<T, false, true> : tc_gemm2_kernel<T, false, false>;
   if (g.lp >= 0) {
-    kern = tc_gemm2_kernel<T, true, false>;
+    kern = tc_gemm2_kernel<T, true, kGemm>;
     AK_CUDA_TRY(prepare(kern), "linear_ce: smem attribute");
   }
   const int pairs = std::max(1, std::min(g.total, resident_pairs<T>()));
@@ -1291,6 +1359,8 @@ int run(float* loss, float* lse, void* dH, void* dW, const Ws& w, const void* H,
 // Token log-probabilities.  Workspace: the tiles' statistics of one chunk (forward), or the chunk's
 // 16-bit gradient of the logits, rows padded to 8 elements, and the fp32 dW accumulator (backward).
 struct LogpWs {
+  void* G2;      // few rows: what rounding G left over
+  float* runs;   // fp32 partial products of dH, when its long K is cut
   float4* part;
   float* tlogit;
   void* G;
@@ -1298,6 +1368,34 @@ struct LogpWs {
   float* dWacc;
   size_t bytes;
 };
+
+// The backward's plan for a chunk of nr rows.
+struct LogpPlan {
+  int two;         // G in two 16-bit matrices: few rows have few roundings to average over
+  int dh_splits;   // runs that dH's K (the vocabulary) is cut into; 1: one launch with dW
+};
+
+constexpr int64_t kFewRows = 256;
+constexpr int64_t kRunRows = 160 * 2 * BM;  // tiles * runs <= CTA pairs (fewer than 160) of 256 rows each
+constexpr int kMostRuns = 64;
+
+// dH has few tiles of a long K (786 K blocks for a vocabulary of 50304) where the rows are few, and
+// one CTA pair per tile would take longer than all others together: 1 row of 200 hidden units took
+// 320 us there.  Then the K is cut so that every pair has a run of at least 8 blocks.
+LogpPlan plan_logp(int64_t nr, int64_t D, int64_t V, int pairs) {
+  LogpPlan p;
+  p.two = nr <= kFewRows;
+  const int64_t tiles = ((nr + 2 * BM - 1) / (2 * BM)) * ((D + BN - 1) / BN);
+  const int64_t kall = ((V + BK - 1) / BK) * (1 + p.two);
+  const int64_t dw = ((V + 2 * BM - 1) / (2 * BM)) * ((D + BN - 1) / BN) * ((nr + BK - 1) / BK);
+  p.dh_splits = 1;
+  if (p.two || kall * pairs > tiles * kall + dw) {
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({(int64_t)pairs / tiles, kall / 8, (int64_t)kMostRuns}));
+    const int64_t kper = (kall + splits - 1) / splits;
+    p.dh_splits = (int)((kall + kper - 1) / kper);
+  }
+  return p;
+}
 
 LogpWs carve_logp(void* base, int64_t N, int64_t D, int64_t V, bool backward) {
   LogpWs w{};
@@ -1311,6 +1409,11 @@ LogpWs carve_logp(void* base, int64_t N, int64_t D, int64_t V, bool backward) {
   };
   if (backward) {
     w.G = take((size_t)Nc * ((V + 7) / 8 * 8) * 2);
+    // the last chunk may be the one with few rows, and each has its own number of runs: at most as
+    // many as leave tiles * runs within the CTA pairs of any device this is built for
+    w.G2 = take((size_t)std::min(Nc, kFewRows) * ((V + 7) / 8 * 8) * 2);
+    w.runs = reinterpret_cast<float*>(take((size_t)std::min<int64_t>(
+                 (int64_t)kMostRuns * Nc, (int64_t)kRunRows) * D * 4));
     w.scale = reinterpret_cast<float*>(take(4));
     w.dWacc = N > Nc ? reinterpret_cast<float*>(take((size_t)V * D * 4)) : nullptr;
   } else {
@@ -1367,12 +1470,11 @@ int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, 
   for (int64_t r0 = 0; r0 < N; r0 += Nc) {
     const int64_t nr = std::min(Nc, N - r0);
     const bool first = r0 == 0, last = r0 + nr >= N;
-    Operand A[2], B[2];
+    const LogpPlan plan = plan_logp(nr, D, V, std::min(resident_pairs<T>(), 159));
+    Operand Ah{static_cast<const T*>(H) + r0 * D, nr, D, 0}, Bw{W, V, D, 0};
     Group g{};
     g.status = status;
     g.nprob = 1;
-    A[0] = {static_cast<const T*>(H) + r0 * D, nr, D, 0};
-    B[0] = {W, V, D, 0};
     Prob& L = g.p[0];
     L.M = (int)nr; L.N = (int)V; L.K = (int)D;
     L.epi = EPI_LOGP_GRAD;
@@ -1381,13 +1483,17 @@ int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, 
     L.stats = stats + r0;
     L.g_lp = g_lp ? g_lp + r0 : nullptr; L.g_ent = g_ent ? g_ent + r0 : nullptr;
     L.scale = scale; L.q = q;
-    if ((rc = launch_group<T>(A, B, g, st))) return rc;
-    // dW (+)= G^T H_c and dH_c = G W in one launch, as in the linear + CE
+    L.C2 = plan.two ? w.G2 : nullptr;
+    if ((rc = launch_group<T>(&Ah, &Bw, g, st))) return rc;
+    Operand G{w.G, nr, V, 0, ldg}, G2{w.G2, nr, V, 0, ldg};
+    const bool apart = plan.two || (dH && plan.dh_splits > 1);
+    Operand A[2], B[2];
     g = Group{};
     g.status = status;
     int np = 0;
     if (dW) {
-      A[np] = {w.G, nr, V, 1, ldg};
+      A[np] = G;
+      A[np].mn = 1;
       B[np] = {static_cast<const T*>(H) + r0 * D, nr, D, 1};
       Prob& P = g.p[np++];
       P.M = (int)V; P.N = (int)D; P.K = (int)nr;
@@ -1401,9 +1507,40 @@ int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, 
       } else {
         P.C = dW; P.add_f32 = w.dWacc;
       }
+      if (apart) {
+        if (plan.two) { P.two = 1; P.ksplits = 1; }
+        Operand A2 = G2;
+        A2.mn = 1;
+        g.nprob = 1;
+        if ((rc = launch_group<T>(A, B, g, st, plan.two ? &A2 : nullptr))) return rc;
+      }
     }
-    if (dH) {
-      A[np] = {w.G, nr, V, 0, ldg};
+    if (dH && apart) {
+      Group h{};
+      h.status = status;
+      h.nprob = 1;
+      Operand Bh{W, V, D, 1};
+      Prob& P = h.p[0];
+      P.M = (int)nr; P.N = (int)D; P.K = (int)V;
+      P.epi = EPI_STORE;
+      P.ldc = D;
+      P.scale = scale;
+      P.two = plan.two;
+      P.ksplits = plan.dh_splits;
+      const int64_t kall = ((V + BK - 1) / BK) * (1 + plan.two);
+      P.kper = (int)((kall + plan.dh_splits - 1) / plan.dh_splits);
+      T* out = static_cast<T*>(dH) + r0 * D;
+      if (plan.dh_splits > 1) { P.C = w.runs; P.c_f32 = 1; }
+      else P.C = out;
+      if ((rc = launch_group<T>(&G, &Bh, h, st, plan.two ? &G2 : nullptr))) return rc;
+      if (plan.dh_splits > 1) {
+        const int64_t n = nr * D;
+        const unsigned grid = (unsigned)std::min<int64_t>((n + 1023) / 1024, (int64_t)sm_count() * 8);
+        logp_sum_runs<T><<<grid, 256, 0, st>>>(out, w.runs, plan.dh_splits, n);
+        AK_CHECK_LAUNCH("ak_linear_logprobs_bwd: dH");
+      }
+    } else if (dH) {
+      A[np] = G;
       B[np] = {W, V, D, 1};
       Prob& P = g.p[np++];
       P.M = (int)nr; P.N = (int)D; P.K = (int)V;
@@ -1411,8 +1548,10 @@ int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, 
       P.C = static_cast<T*>(dH) + r0 * D; P.ldc = D;
       P.scale = scale;
     }
-    g.nprob = np;
-    if ((rc = launch_group<T>(A, B, g, st))) return rc;
+    if (!apart) {  // dW (+)= G^T H_c and dH_c = G W in one launch, as in the linear + CE
+      g.nprob = np;
+      if ((rc = launch_group<T>(A, B, g, st))) return rc;
+    }
   }
   return AK_OK;
 }

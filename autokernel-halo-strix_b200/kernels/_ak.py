@@ -450,9 +450,9 @@ def scale_by_device_scalar_(x: torch.Tensor, scale: torch.Tensor) -> torch.Tenso
     dev = require_cuda(x, scale)
     if not x.is_contiguous():
         raise ValueError("scale_by_device_scalar_: x must be contiguous")
-    s = scale.reshape(1).to(torch.float32)
+    s = f32_dense(scale)
     if x.numel():
-        call("ak_scale_by_device_scalar", ptr(x), x.numel(), ptr(s), dtype_code(x), stream(dev))
+        call_on(dev, "ak_scale_by_device_scalar", ptr(x), x.numel(), ptr(s), dtype_code(x), stream(dev))
     return x
 
 
@@ -604,6 +604,13 @@ def call_on(device: torch.device, name: str, *args) -> None:
             call(name, *args)
 
 
+def f32_dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t as a contiguous fp32 tensor (itself where it is one)."""
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
+
+
 def logit_rows(logits: torch.Tensor):
     """(tensor, rows, inner, stride_outer, stride_inner): the rows of logits (..., V) as the library
     addresses them.  A view whose leading dimensions are at most two runs of evenly spaced rows
@@ -657,8 +664,7 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], ro
     dev = require_cuda(logits, targets, row_stats, g_logprobs, g_entropy)
     x, rows, inner, so, si = logit_rows(logits)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    glp = g_logprobs.to(torch.float32).contiguous() if g_logprobs is not None else None
-    gent = g_entropy.to(torch.float32).contiguous() if g_entropy is not None else None
+    glp, gent = f32_dense(g_logprobs), f32_dense(g_entropy)
     call_on(dev, "ak_token_logprobs_bwd", ptr(grad), ptr(x), ptr(targets), ptr(row_stats), ptr(glp),
             ptr(gent), rows, inner, so, si, logits.shape[-1], temperature, softcap, ignore_index,
             dtype_code(logits), stream(dev))
@@ -695,7 +701,7 @@ def distill_topk_bwd(logits: torch.Tensor, teacher_idx: torch.Tensor, rest_stats
     dev = require_cuda(logits, teacher_idx, rest_stats, gk, mask, inv_n, g_loss)
     x, rows, inner, so, si = logit_rows(logits)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    g = g_loss.reshape(1).to(torch.float32)
+    g = f32_dense(g_loss)
     call_on(dev, "ak_distill_topk_bwd", ptr(grad), ptr(x), ptr(teacher_idx), ptr(rest_stats), ptr(gk), ptr(mask),
             ptr(inv_n), ptr(g), rows, inner, so, si, logits.shape[-1], teacher_idx.shape[-1], temperature, softcap,
             dtype_code(logits), stream(dev))
@@ -781,8 +787,7 @@ def linear_logprobs_bwd(hidden, weight, targets, row_stats, g_logprobs, g_entrop
     V = weight.shape[0]
     dH = torch.empty_like(hidden) if need_dh else None
     dW = (torch.empty_like(weight) if N else torch.zeros_like(weight)) if need_dw else None
-    glp = g_logprobs.to(torch.float32).contiguous() if g_logprobs is not None else None
-    gent = g_entropy.to(torch.float32).contiguous() if g_entropy is not None else None
+    glp, gent = f32_dense(g_logprobs), f32_dense(g_entropy)
     ws_bytes = _size_query("ak_linear_logprobs_workspace_size", N, D, V, 1)
     ws = workspace(ws_bytes, dev)
     call_on(dev, "ak_linear_logprobs_bwd", ptr(dH), ptr(dW), ptr(ws), ws_bytes, ptr(hidden), ptr(weight),

@@ -10,15 +10,28 @@ The reference trains on hard labels only (kernels/ce_fused.py:557-785).
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from kernels import _ak
-from kernels.token_logprobs import check_scales
+from kernels.token_logprobs import check_scales, once
 
 KERNEL_TYPE = "distill_topk"
 BACKEND = "cuda_sm100a"
 
 MAX_TOP_K = 128
+
+
+def _distill_backward(ctx, g_loss):
+    if ctx.fused:
+        if ctx.consumed:
+            raise RuntimeError("distill_topk: backward through the same graph twice needs mode='tiny' (the "
+                               "gradient made in the forward is consumed by the first backward)")
+        ctx.consumed = True
+        (grad,) = ctx.saved_tensors
+        _ak.scale_by_device_scalar_(grad, g_loss)
+    else:
+        logits, idx, rest, gk, mask, inv_n = ctx.saved_tensors
+        grad = _ak.distill_topk_bwd(logits, idx, rest, gk, mask, inv_n, g_loss, *ctx.args)
+    return (grad,) + (None,) * 7
 
 
 class _DistillTopK(torch.autograd.Function):
@@ -37,20 +50,8 @@ class _DistillTopK(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_loss):
-        if ctx.fused:
-            if ctx.consumed:
-                raise RuntimeError("distill_topk: backward through the same graph twice needs mode='tiny' (the "
-                                   "gradient made in the forward is consumed by the first backward)")
-            ctx.consumed = True
-            (grad,) = ctx.saved_tensors
-            with torch.cuda.device(grad.device):
-                _ak.scale_by_device_scalar_(grad, g_loss)
-        else:
-            logits, idx, rest, gk, mask, inv_n = ctx.saved_tensors
-            grad = _ak.distill_topk_bwd(logits, idx, rest, gk, mask, inv_n, g_loss, *ctx.args)
-        return (grad,) + (None,) * 7
+        return once(_distill_backward, ctx, g_loss)
 
 
 def distill_topk(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_logprobs: torch.Tensor, *,
@@ -99,7 +100,7 @@ def distill_topk(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_lo
     if mode not in (None, "fused", "tiny"):
         raise ValueError(f"{what}: mode must be 'fused' or 'tiny', got {mode!r}")
     idx = teacher_indices.to(torch.int64).contiguous()
-    lp = teacher_logprobs.to(torch.float32).contiguous()
+    lp = _ak.f32_dense(teacher_logprobs)
     if logits.requires_grad and torch.is_grad_enabled():
         fused = mode == "fused" or (mode is None and logits.dtype != torch.float16)
         return _DistillTopK.apply(logits, idx, lp, mask, temperature, softcap, bool(tail), fused)

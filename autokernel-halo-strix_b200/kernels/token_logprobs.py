@@ -35,6 +35,21 @@ class TokenLogprobs(NamedTuple):
     top_indices: Optional[torch.Tensor] = None
 
 
+def once(backward, ctx, *grads):
+    """`backward(ctx, *grads)` as torch's `once_differentiable` runs it; its bookkeeping (several
+    microseconds) is only needed where a graph of the backward is built."""
+    if torch.is_grad_enabled():
+        return once_differentiable(backward)(ctx, *grads)
+    return backward(ctx, *grads)
+
+
+def _token_logprobs_backward(ctx, g_lp, g_ent):
+    if g_lp is None and g_ent is None:
+        return (None,) * 7
+    logits, targets, stats = ctx.saved_tensors
+    return (_ak.token_logprobs_bwd(logits, targets, stats, g_lp, g_ent, *ctx.args),) + (None,) * 6
+
+
 class _TokenLogprobs(torch.autograd.Function):
     """Saves the logits and four numbers a row; the backward recomputes the softmax from them."""
 
@@ -49,13 +64,8 @@ class _TokenLogprobs(torch.autograd.Function):
         return lp, ent, lse, top_lp, top_idx
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_lp, g_ent, *rest):
-        if g_lp is None and g_ent is None:
-            return (None,) * 7
-        logits, targets, stats = ctx.saved_tensors
-        grad = _ak.token_logprobs_bwd(logits, targets, stats, g_lp, g_ent, *ctx.args)
-        return (grad,) + (None,) * 6
+        return once(_token_logprobs_backward, ctx, g_lp, g_ent)
 
 
 def check_scales(what: str, temperature: float, softcap: float):
@@ -72,6 +82,8 @@ def check_targets(what: str, targets: torch.Tensor, lead) -> torch.Tensor:
         raise TypeError(f"{what}: targets must be int64 or int32, got {targets.dtype}")
     if targets.shape != lead:
         raise ValueError(f"{what}: targets {tuple(targets.shape)} do not match the rows {tuple(lead)}")
+    if targets.dtype is torch.int64 and targets.is_contiguous():
+        return targets
     return targets.to(torch.int64).contiguous()
 
 
@@ -112,6 +124,15 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
                                                  want_entropy=bool(entropy))[:5])
 
 
+def _linear_token_logprobs_backward(ctx, g_lp, g_ent):
+    if g_lp is None and g_ent is None:
+        return (None,) * 7
+    hidden, w, targets, stats = ctx.saved_tensors
+    dh, dw = _ak.linear_logprobs_bwd(hidden, w, targets, stats, g_lp, g_ent, *ctx.args,
+                                     need_dh=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
+    return (dh, dw.to(ctx.weight_dtype) if dw is not None else None) + (None,) * 5
+
+
 class _LinearTokenLogprobs(torch.autograd.Function):
     """Saves its operands and four numbers a row; the backward forms the logits again, chunk by chunk."""
 
@@ -127,14 +148,8 @@ class _LinearTokenLogprobs(torch.autograd.Function):
         return lp, ent, lse
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_lp, g_ent, *rest):
-        if g_lp is None and g_ent is None:
-            return (None,) * 7
-        hidden, w, targets, stats = ctx.saved_tensors
-        dh, dw = _ak.linear_logprobs_bwd(hidden, w, targets, stats, g_lp, g_ent, *ctx.args,
-                                         need_dh=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
-        return (dh, dw.to(ctx.weight_dtype) if dw is not None else None) + (None,) * 5
+        return once(_linear_token_logprobs_backward, ctx, g_lp, g_ent)
 
 
 def _dense16(t: torch.Tensor) -> torch.Tensor:

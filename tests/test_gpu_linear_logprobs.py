@@ -55,9 +55,10 @@ def test_forward(n, d, v, dtype):
         check(h, w, t, linear_token_logprobs(h, w, t, **kw), entropy=False, **kw)
 
 
-def grad_reference(h, w, t, gl, ge, **kw):
+def grad_reference(h, w, t, gl, ge, two=False, **kw):
     """(dH, dW) in 64 bits and their bounds: G is off by its fp32 bound, the accumulators' error and
-    one rounding to 16 bits; the two products add (N or V + 1) u of their absolute sums."""
+    one rounding to 16 bits (two: the rounding's rest is rounded again and kept); the two products
+    add (N or V + 1) u of their absolute sums."""
     x = h.double().cpu() @ w.double().cpu().T
     G, tol = O.token_logprobs_grad(x, t.cpu(), gl, ge, **kw)
     r = O.token_logprobs(x, t.cpu(), **kw)
@@ -68,7 +69,8 @@ def grad_reference(h, w, t, gl, ge, **kw):
     scale = 1.0 if h.dtype == torch.bfloat16 else float(((0 if gl is None else gl.abs()) + (0 if ge is None else ge.abs())).max())
     live = (t.cpu() != -100).double()[:, None]
     tol = tol + (4 * e * r["p"] * mag / kw.get("temperature", 1.0)) * live
-    tol = tol + (G.abs() + tol) * info.eps / 2 + scale * info.smallest_normal * info.eps / 2
+    half = info.eps / 2
+    tol = tol + (G.abs() + tol) * (half * half if two else half) + scale * info.smallest_normal * half
     W, H = w.double().cpu(), h.double().cpu()
     dH, dW = G @ W, G.T @ H
     tH = tol @ W.abs() + (G.abs() @ W.abs()) * (W.shape[0] + 1) * O.U
@@ -193,3 +195,24 @@ def test_streams_and_graph():
         assert torch.equal(r.logprobs, e.logprobs) and torch.equal(r.entropy, e.entropy)
         assert torch.equal(grads[0], eg[0]) and torch.equal(grads[1], eg[1])
     _ak.check_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,v", [(1, 200, 20011), (1, 8, 9001), (40, 768, 30001), (256, 136, 12000), (700, 520, 9000),
+                                   (16384 + 5, 64, 515)])
+def test_long_vocabulary_few_rows(n, d, v, dtype):
+    """dH's vocabulary is cut into runs; up to 256 rows the logits' gradient is kept in two matrices,
+    so that what it loses is below a 16-bit rounding of its rounding."""
+    from kernels.token_logprobs import linear_token_logprobs
+    h, w, t = problem(n, d, v, dtype, seed=12)
+    g = torch.Generator().manual_seed(n)
+    gl, ge = torch.randn(n, generator=g), torch.randn(n, generator=g) * 0.2
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    r = linear_token_logprobs(hg, wg, t, entropy=True)
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [hg, wg], [gl.to(DEV), ge.to(DEV)])
+    rh, th, rw, tw = grad_reference(h, w, t, gl, ge, two=n <= 256)
+    O.assert_within(dh, rh, th, "dH")
+    O.assert_within(dw, rw, tw, "dW")
+    only, = torch.autograd.grad(linear_token_logprobs(hg, w, t).logprobs, hg, gl.to(DEV))
+    rh, th, _, _ = grad_reference(h, w, t, gl, None, two=n <= 256)
+    O.assert_within(only, rh, th, "dH alone")
