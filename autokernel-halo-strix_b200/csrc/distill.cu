@@ -889,6 +889,7 @@ __global__ void __launch_bounds__(1024)
 distill_inv_rows(float* __restrict__ inv_n, const uint8_t* __restrict__ mask, int64_t rows) {
   __shared__ int s[32];
   int c = 0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) c += mask[i] != 0;
   c = __reduce_add_sync(0xffffffffu, c);
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = c;
@@ -909,6 +910,7 @@ distill_mean(float* __restrict__ loss, float* __restrict__ inv_n, const float* _
   __shared__ int n[32];
   float v = 0.f;
   int c = 0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) {
     v += losses[i];
     if (mask) c += mask[i] != 0;

@@ -1030,26 +1030,41 @@ lce_grad_inplace(T* __restrict__ L, const float* __restrict__ lse, const int64_t
   }
 }
 
-// Merge the per-tile partials of a row (one warp each) into its log-probability, entropy and lse.
+// Merge the per-tile partials of a row (one CTA each) into its log-probability, entropy and lse.
+constexpr int kRowThreads = 128;
+
 template <bool CAP>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kRowThreads)
 logp_rows_reduce(float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ lse,
                  float4* __restrict__ stats, const float4* __restrict__ part, const float* __restrict__ tlogit,
-                 const int64_t* __restrict__ labels, int M, int V, int nparts, int64_t ignore_index, const Squash q) {
-  const int row = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
-  if (row >= M) return;
+                 const int64_t* __restrict__ labels, int V, int nparts, int64_t ignore_index, const Squash q) {
+  __shared__ RowStats<CAP, true> s_warp[kRowThreads / 32];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+  const float4* p = part + (int64_t)row * nparts;
+  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
   RowStats<CAP, true> st;
   st.init();
-  for (int t = lane; t < nparts; t += 32) {
-    const float4 p = part[(int64_t)row * nparts + t];
-    RowStats<CAP, true> o;
-    o.init();
-    o.r = Ref{p.x, p.y};
-    o.s = p.z;
-    o.w = p.w;
-    if (o.s > 0.f) o.lim = 0.f;  // something was seen
-    st.merge(o, q);
+  for (int t0 = tid; t0 < nparts; t0 += 4 * kRowThreads) {
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = t0 + u * kRowThreads < nparts ? p[t0 + u * kRowThreads] : none;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      RowStats<CAP, true> o;
+      o.init();
+      o.r = Ref{v[u].x, v[u].y};
+      o.s = v[u].z;
+      o.w = v[u].w;
+      if (o.s > 0.f) o.lim = 0.f;  // something was seen
+      st.merge(o, q);
+    }
   }
+  st.warp_merge(q);
+  if (lane == 0) s_warp[tid >> 5] = st;
+  __syncthreads();
+  if (tid >= 32) return;
+  st.init();
+  if (lane < kRowThreads / 32) st = s_warp[lane];
   st.warp_merge(q);
   st.center();
   if (lane != 0) return;
@@ -1446,9 +1461,9 @@ int logp_fwd(float* logprobs, float* entropy, float* lse, float4* stats, const L
     const int rc = launch_group<T>(A, B, g, st);
     if (rc) return rc;
     auto kern = q.cap > 0.f ? logp_rows_reduce<true> : logp_rows_reduce<false>;
-    kern<<<(unsigned)((nr * 32 + 255) / 256), 256, 0, st>>>(
+    kern<<<(unsigned)nr, kRowThreads, 0, st>>>(
         logprobs ? logprobs + r0 : nullptr, entropy ? entropy + r0 : nullptr, lse + r0, stats ? stats + r0 : nullptr,
-        w.part, w.tlogit, P.labels, (int)nr, (int)V, nparts, ignore_index, q);
+        w.part, w.tlogit, P.labels, (int)V, nparts, ignore_index, q);
     AK_CHECK_LAUNCH("ak_linear_logprobs_fwd: rows");
   }
   return AK_OK;

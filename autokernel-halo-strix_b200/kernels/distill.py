@@ -75,7 +75,6 @@ def distill_topk(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_lo
     a loss scale reaches it, else "fused".
     """
     what = "distill_topk"
-    _ak.require_cuda(logits, teacher_indices, teacher_logprobs, mask)
     _ak.dtype_code(logits)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"{what}: logits must be (..., V) with V >= 1, got {tuple(logits.shape)}")

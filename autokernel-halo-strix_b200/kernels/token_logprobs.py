@@ -69,6 +69,8 @@ class _TokenLogprobs(torch.autograd.Function):
 
 
 def check_scales(what: str, temperature: float, softcap: float):
+    if temperature == 1.0 and softcap == 0.0:
+        return 1.0, 0.0
     temperature, softcap = float(temperature), float(softcap)
     if not (temperature > 0.0 and math.isfinite(temperature)):
         raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
@@ -106,15 +108,17 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     entropy 0 and no gradient; a row with NaN is NaN.
     """
     what = "token_logprobs"
-    _ak.require_cuda(logits, targets)
     _ak.dtype_code(logits)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"{what}: logits must be (..., V) with V >= 1, got {tuple(logits.shape)}")
     if targets is not None:
         targets = check_targets(what, targets, logits.shape[:-1])
-    top_k = int(top_k)
-    if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
-        raise ValueError(f"{what}: top_k must be in 0..{min(MAX_TOP_K, logits.shape[-1])}, got {top_k}")
+    if top_k:
+        top_k = int(top_k)
+        if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
+            raise ValueError(f"{what}: top_k must be in 0..{min(MAX_TOP_K, logits.shape[-1])}, got {top_k}")
+    else:
+        top_k = 0
     temperature, softcap = check_scales(what, temperature, softcap)
     ignore_index = int(ignore_index)
     if logits.requires_grad and torch.is_grad_enabled():
@@ -170,7 +174,6 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: O
     finite where a gradient of weight is wanted (they enter it times 0).
     """
     what = "linear_token_logprobs"
-    _ak.require_cuda(hidden, weight, targets)
     if hidden.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"{what}: hidden must be bfloat16 or float16, got {hidden.dtype}")
     _ak.dtype_code(weight)
