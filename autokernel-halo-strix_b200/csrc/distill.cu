@@ -87,7 +87,7 @@ __device__ __forceinline__ float rest_grad(float x, const Ref& ref, float c, con
 template <typename T, bool CAP, int NW>
 __device__ __forceinline__ void rest_grads(float* x, const uint32_t (&w)[NW], const Ref& ref, float c, const Squash& q) {
   constexpr int P = NW * elems_per_word<T>() / 2;
-  const float2 kl = make_float2(q.kl, q.kl), nk = make_float2(-ref.k, -ref.k), c2 = make_float2(c, c);
+  const float2 kl = both(q.kl), nk = both(-ref.k), c2 = both(c);
   if (!CAP && ref.sh == 0.f && c != 0.f) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -185,7 +185,7 @@ struct Waits {
         ok = mbar_try_wait(bar, parity);
       }
       if (ok) return;
-      if (i > 64) __nanosleep(32);
+      if (i > 1) __nanosleep(100);  // three of the roles wait most of the time
       if ((i & 255u) == 255u && *abort) return;
     }
     *abort = 1;

@@ -217,6 +217,15 @@ __device__ __forceinline__ float2 word_pair(const uint32_t (&w)[NW], int i) {
   else return unpack2(w[i], (const T*)nullptr);
 }
 
+// The same value twice, as an operand of paired arithmetic in plain registers: where the compiler
+// knows that a value is the same in the whole warp it keeps it in uniform registers, and each paired
+// instruction then costs moves.
+__device__ __forceinline__ float2 both(float v) {
+  float2 r = make_float2(v, v);
+  asm volatile("" : "+f"(r.x), "+f"(r.y));
+  return r;
+}
+
 // ---------------------------------------------------------------------------
 // Running softmax statistics of a set of logits
 // ---------------------------------------------------------------------------
@@ -328,7 +337,7 @@ struct RowStats {
     if (ly > lim) move(ly, q);
     m = fmaxf(m, lm);
     float2 s2 = make_float2(s, 0.f), w2 = make_float2(w, 0.f);
-    const float2 kl = make_float2(q.kl, q.kl), nk = make_float2(-r.k, -r.k);
+    const float2 kl = both(q.kl), nk = both(-r.k);
     if (!CAP && (ENT ? can_raise<T>(r, q) : r.sh == 0.f)) {
       uint32_t x[NW];
 #pragma unroll

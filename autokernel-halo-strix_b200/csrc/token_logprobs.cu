@@ -536,8 +536,7 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
     return o * squash_slope<CAP>(y, q);
   };
   const bool quick = !CAP && (ENT ? can_raise<T>(ref, q) : ref.sh == 0.f);
-  const float2 kl = make_float2(q.kl, q.kl), nk = make_float2(-ref.k, -ref.k);
-  const float2 c02 = make_float2(c0, c0), c12 = make_float2(c1, c1);
+  const float2 kl = both(q.kl), nk = both(-ref.k), c02 = both(c0), c12 = both(c1);
 
   const int gbeg = seg * kBwdGroups;
   const T* body = row + cut.head;
