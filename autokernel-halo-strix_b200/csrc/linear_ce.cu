@@ -40,7 +40,10 @@
 // The same GEMM also answers token log-probabilities from hidden states (EPI_LOGP: each tile is
 // reduced to per-row softmax statistics with the sums the entropy needs, nothing is stored) and
 // their gradients (EPI_LOGP_GRAD: the logits are formed again and leave the accumulators as
-// dL/dlogits in 16 bits, from the forward's statistics; then the grouped dW / dH launch).
+// dL/dlogits in 16 bits, from the forward's statistics; then the grouped dW / dH launch).  Measured:
+// 4096 x 768 x 50304 bf16 270-320 us forward (1.0-1.2 PFLOP/s, tensor cores; clocks under the power
+// cap) and 840-900 us backward (three products and the logits again); 2001 x 1536 x 32000 fp16 172 us
+// forward; 8 x 768 x 50304 bf16 27 us, floor 12 (the weight once): 2.7 rounds of tiles and the row join.
 #include "logit_rows.cuh"
 
 #include <cuda.h>
