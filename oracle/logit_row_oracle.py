@@ -16,6 +16,7 @@ at most, twice in a difference (CAP).
 import torch
 
 U = 2.0 ** -24
+FLUSH = 2.0 ** -125  # the hardware's exponential gives 0 below 2^-126 (S is in [1, 2))
 LN2 = 0.6931471805599453
 CAP = 18  # of a difference of two squashed logits, in u * softcap
 
@@ -104,6 +105,7 @@ def token_logprobs_grad(x, targets, g_lp, g_ent, ignore_index=-100, temperature=
     rel = 4 * U + (4 * lgp.abs() + 5 * logv) * U + tol_logs + cap_err
     mag = gl.abs() + ge.abs() * (lgp.abs() + H)
     tol = p * (rel * mag + ge.abs() * (tol_h + rel) + 6 * U * mag) + 4 * U * (g.abs() + hot * gl.abs())
+    tol = tol + FLUSH * mag
     tol = tol * dy.abs()
     if softcap > 0:  # the slope 1 - t^2, t = tanh off by 9 u
         tol = tol + g.abs() * (20 * U) / temperature
@@ -195,7 +197,7 @@ def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=Fals
     lpr = torch.where(has_rest, logpr, torch.zeros_like(rest)).abs()[:, None]
     rel = 10 * U + (4 * lgp.abs() + 6 * logv + 6 * lpr) * U + 2 * r["tol_logs"][:, None] + 2 * CAP * U * softcap / temperature
     relm = torch.zeros_like(p).scatter_add_(1, at, torch.where(used, q * (rel_q + k * U), torch.zeros_like(q)))
-    tg = torch.where(inside, p * rel + relm, p * rel + cond * (rest[:, None] * rel + dr)) + 6 * U * g.abs()
+    tg = torch.where(inside, p * rel + relm, p * rel + cond * (rest[:, None] * rel + dr)) + 6 * U * g.abs() + 2 * FLUSH
     tg = tg * dy.abs() + (g.abs() * 20 * U / temperature if softcap > 0 else 0.0)
     off = (none | empty | ~live)[:, None]
     g, tg = torch.where(off, torch.zeros_like(g), g * dy), torch.where(off, torch.zeros_like(tg), tg)

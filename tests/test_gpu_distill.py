@@ -296,3 +296,35 @@ def test_many_short_rows(n, v, k, dtype):
     idx[7] = -1
     check(x, idx, tlp, mask, tail=True)
     check(x, idx, tlp, None, tail=False, softcap=5.0, temperature=1.3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_short_strided_rows(dtype):
+    B, T, V, K = 60, 13, 1003, 6
+    g = torch.Generator().manual_seed(5)
+    full = torch.randn(B, T, V + 5, generator=g).to(dtype).to(DEV)
+    for x in (full[:, :-1], full[..., 2:V + 1], full[:, 1:, :V]):
+        idx = torch.randint(-1, x.shape[-1], (*x.shape[:-1], K), generator=g).to(DEV)
+        tlp = (torch.log_softmax(torch.randn(*x.shape[:-1], K, generator=g), -1) - 0.2).to(DEV)
+        mask = (torch.rand(x.shape[:-1], generator=g) < 0.7).to(DEV)
+        check(x, idx, tlp, mask, tail=True)
+
+
+@pytest.mark.parametrize("v,copies", [(37, 1), (5003, 1), (900, 200)])
+def test_huge_logits(v, copies):
+    g = torch.Generator().manual_seed(v)
+    base = torch.randn(4, v, generator=g)
+    x = base * torch.tensor([1e7, 1.0, 1e12, 1.0])[:, None]
+    x[1, 0] = 5e8
+    x[3] = -1e8 + base[3] * 100.0
+    x = x.repeat(copies, 1).to(DEV)
+    top = torch.topk(x, 3, dim=1).indices            # teacher's tokens the student's own
+    tlp = torch.log(torch.tensor([0.7, 0.2, 0.1])).expand(x.shape[0], 3).contiguous().to(DEV)
+    from kernels.distill import distill_topk
+    ref = O.distill_topk(x.double().cpu(), top.cpu(), tlp.cpu(), tail=False)
+    for mode in ("fused", "tiny"):
+        leaf = x.clone().requires_grad_(True)
+        loss = distill_topk(leaf, top, tlp, mode=mode)
+        got, = torch.autograd.grad(loss, leaf)
+        O.assert_within(loss, ref["loss"], ref["tol_loss"] + ref["loss"].abs() * 8 * O.U, "loss")
+        O.assert_within(got, ref["grad"], ref["tol_grad"], "grad")

@@ -216,3 +216,38 @@ def test_long_vocabulary_few_rows(n, d, v, dtype):
     only, = torch.autograd.grad(linear_token_logprobs(hg, w, t).logprobs, hg, gl.to(DEV))
     rh, th, _, _ = grad_reference(h, w, t, gl, None, two=n <= 256)
     O.assert_within(only, rh, th, "dH alone")
+
+
+def test_policy_step_from_rows_and_from_hidden_states():
+    """A policy-gradient loss with an entropy bonus both ways: stored bf16 logits, and none."""
+    from kernels.token_logprobs import linear_token_logprobs, token_logprobs
+    h, w, t = problem(96, 128, 2003, torch.bfloat16, seed=15)
+    adv = torch.randn(96, generator=torch.Generator().manual_seed(4)).to(DEV)
+    live = t != -100
+
+    def loss(r):
+        return -(adv * r.logprobs + 0.01 * r.entropy)[live].mean()
+
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss(linear_token_logprobs(hg, wg, t, entropy=True)).backward()
+    h2, w2 = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss(token_logprobs(torch.nn.functional.linear(h2.float(), w2.float()), t, entropy=True)).backward()
+    # the same gradients up to bf16 roundings of the results (and of G, kept in two parts here)
+    for a, b in ((hg.grad, h2.grad), (wg.grad, w2.grad)):
+        assert (a.double() - b.double()).norm() <= 2 * 2.0 ** -8 * b.double().norm()
+
+
+def test_huge_and_broken_hidden_states():
+    from kernels.token_logprobs import linear_token_logprobs
+    h, w, t = problem(70, 64, 900, torch.bfloat16, seed=16)
+    h[:35] *= 1e6                                     # one token takes all
+    x = h.double().cpu() @ w.double().cpu().T
+    ref = O.token_logprobs(x, t.cpu())
+    r = linear_token_logprobs(h, w, t, entropy=True)
+    e = logit_bound(h, w)
+    O.assert_within(r.logprobs, ref["logprobs"], ref["tol_logprobs"] + 2 * e, "logprobs")
+    h[3, 5] = torch.nan
+    h[4, 6] = torch.inf
+    r = linear_token_logprobs(h, w, t, entropy=True)
+    assert torch.isnan(r.logprobs[3]) and torch.isnan(r.entropy[3]) and torch.isfinite(r.logprobs[5:]).all()
+    assert not torch.isfinite(r.logprobs[4])

@@ -326,3 +326,71 @@ def test_many_short_rows(n, v, dtype):
     g, = torch.autograd.grad([r.logprobs, r.entropy], xg, [gl.to(DEV), gl.to(DEV)])
     ref, tol = O.token_logprobs_grad(x.double().cpu(), t.cpu(), gl, gl)
     O.assert_within(g, ref, tol, "grad")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v,copies", [(37, 1), (5003, 1), (5003, 200), (900, 400)])
+def test_huge_logits(v, copies, dtype):
+    """Exponents beyond 2^22 are taken after a subtraction; rows that go from ordinary to huge logits
+    and back change their reference on the way."""
+    from kernels.token_logprobs import token_logprobs
+    g = torch.Generator().manual_seed(v)
+    base = torch.randn(6, v, generator=g)
+    x = base * torch.tensor([1e7, 1e12, 3e30, 1.0, 1.0, 1e5])[:, None]
+    x[3, v // 2] = 5e8                       # one huge logit among ordinary ones
+    x[4, : v // 2] = -1e9                    # huge and negative first
+    x[5] = -1e8 + base[5] * 100.0            # far from zero, close together (in fp32)
+    x = x.to(dtype).repeat(copies, 1).to(DEV)
+    t = torch.arange(x.shape[0], device=DEV) % v
+    ref = O.token_logprobs(x[:6].double().cpu(), t[:6].cpu(), top_k=min(9, v))
+    r = token_logprobs(x, t, top_k=min(9, v), entropy=True)
+    assert torch.equal(r.top_indices[:6].cpu(), ref["top_indices"])
+    for i in range(6):
+        lp = r.logprobs[i::6][t[i::6] == t[i]]
+        O.assert_within(lp, ref["logprobs"][i].expand(lp.shape[0]), ref["tol_logprobs"][i], f"logprobs {i}")
+        n = r.entropy[i::6]
+        O.assert_within(n, ref["entropy"][i].expand(n.shape[0]), ref["tol_entropy"][i], f"entropy {i}")
+    gl, ge = torch.ones(6), torch.full((6,), 0.5)
+    xg = x[:6].clone().requires_grad_(True)
+    q = token_logprobs(xg, t[:6], entropy=True)
+    got, = torch.autograd.grad([q.logprobs, q.entropy], xg, [gl.to(DEV), ge.to(DEV)])
+    want, tol = O.token_logprobs_grad(x[:6].double().cpu(), t[:6].cpu(), gl, ge)
+    O.assert_within(got, want, tol, "grad")
+
+
+def test_graphs_of_the_backward_and_inference_mode():
+    from kernels.token_logprobs import token_logprobs
+    x, t = rows(4, 300, torch.float32)
+    x.requires_grad_(True)
+    lp = token_logprobs(x, t).logprobs
+    g, = torch.autograd.grad(lp.sum(), x, create_graph=True, retain_graph=True)
+    with pytest.raises(RuntimeError):  # a gradient is a constant to what comes after it
+        torch.autograd.grad(g.sum(), x)
+    u = torch.ones(4, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(lp, x, u, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    with torch.inference_mode():
+        r = token_logprobs(x, t, top_k=3, entropy=True)
+    assert torch.equal(r.logprobs, lp.detach())
+
+
+def test_two_streams_at_once():
+    from kernels.distill import distill_topk
+    from kernels.token_logprobs import token_logprobs
+    a, t = rows(700, 20011, torch.bfloat16, seed=31)
+    b, _ = rows(700, 20011, torch.bfloat16, seed=32)
+    idx = torch.topk(a, 16, dim=1).indices
+    lp = torch.log_softmax(torch.randn(700, 16, generator=torch.Generator().manual_seed(1)), 1).to(DEV)
+    want = [(token_logprobs(x, t, top_k=16, entropy=True), distill_topk(x, idx, lp, tail=True)) for x in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for s, x, out in zip(streams, (a, b), got):
+            with torch.cuda.stream(s):
+                out.append((token_logprobs(x, t, top_k=16, entropy=True), distill_topk(x, idx, lp, tail=True)))
+    torch.cuda.synchronize()
+    for w, out in zip(want, got):
+        for r, loss in out:
+            assert torch.equal(loss, w[1]) and all(torch.equal(p, q) for p, q in zip(r, w[0]))
