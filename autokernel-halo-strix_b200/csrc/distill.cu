@@ -981,9 +981,12 @@ int launch_width(const T* logits, DistillArgs& a, int64_t share, cudaStream_t st
   const size_t smem = (size_t)std::max<int64_t>(share, 16);
   AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
               "ak_distill_topk_fwd: shared memory");
-  int clusters = 0;
-  AK_CUDA_TRY(resident_clusters(kern, 32 * (W + kRoles), cs, smem, &clusters), "ak_distill_topk_fwd: occupancy");
-  const int64_t grid = std::min<int64_t>(a.rows, clusters) * cs;
+  int64_t grid = a.rows * cs;
+  if (grid > sm_count()) {  // fewer have an SM each
+    int clusters = 0;
+    AK_CUDA_TRY(resident_clusters(kern, 32 * (W + kRoles), cs, smem, &clusters), "ak_distill_topk_fwd: occupancy");
+    grid = std::min<int64_t>(a.rows, clusters) * cs;
+  }
   AK_CUDA_TRY(launch_rows(kern, grid, 32 * (W + kRoles), cs, smem, st, logits, (const DistillArgs&)a),
               "ak_distill_topk_fwd");
   return AK_OK;

@@ -100,7 +100,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     targets (...): the tokens whose `logprobs` are wanted, or None.  Where a target is `ignore_index`
     its log-probability and entropy are 0 and its row gets no gradient, whatever the row holds; a
     target outside the vocabulary gives NaN.
-    top_k: alternatives per row, at most 128: `top_logprobs` and `top_indices` (..., top_k), most
+    top_k: alternatives per row, at most 128 (of at most 1,048,320 tokens): `top_logprobs` and `top_indices` (..., top_k), most
     likely first, equal logits by lowest index.  They and `lse` carry no gradient.
     entropy: whether to compute the entropy (nats).
 
@@ -188,7 +188,7 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: O
         targets = check_targets(what, targets, lead).view(-1)
     temperature, softcap = check_scales(what, temperature, softcap)
     ignore_index = int(ignore_index)
-    h = _dense16(hidden.reshape(-1, D))
+    h = _dense16(hidden if hidden.dim() == 2 else hidden.reshape(-1, D))
     w = _dense16(weight)
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         lp, ent, lse = _LinearTokenLogprobs.apply(h, w, targets, temperature, softcap, ignore_index, bool(entropy))
