@@ -46,6 +46,7 @@
 // forward; 8 x 768 x 50304 bf16 27 us, floor 12 (the weight once): 2.7 rounds of tiles and the row join.
 #include "logit_rows.cuh"
 
+#include <cfloat>
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -1105,20 +1106,26 @@ logp_sum_runs(T* __restrict__ out, const float* __restrict__ part, int runs, int
   }
 }
 
-// scale[0] = largest |g_lp| + |g_ent| over the rows (1 where that is 0 or not finite): divides the
-// 16-bit gradient of the logits, so that small upstream gradients do not underflow in fp16.
+// scale[0] = largest |g_lp| + |g_ent| over the rows that count (1 where that is 0 or not finite): divides
+// the 16-bit gradient of the logits, so that small upstream gradients do not underflow in fp16.  Divided
+// by it an element is at most 1/T (1 + max p |H + log p|) < 16/T, so temperatures below 1/256, which
+// could leave fp16's range, are taken into the scale too.
 __global__ void __launch_bounds__(1024)
-logp_grad_scale(float* __restrict__ scale, const float* __restrict__ g_lp, const float* __restrict__ g_ent, int64_t M) {
+logp_grad_scale(float* __restrict__ scale, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
+                const int64_t* __restrict__ labels, int64_t ignore_index, float inv_t, int64_t M) {
   __shared__ float s[32];
   float m = 0.f;
-  for (int64_t i = threadIdx.x; i < M; i += blockDim.x)
+  for (int64_t i = threadIdx.x; i < M; i += blockDim.x) {
+    if (labels && labels[i] == ignore_index) continue;
     m = fmaxf(m, (g_lp ? fabsf(g_lp[i]) : 0.f) + (g_ent ? fabsf(g_ent[i]) : 0.f));
+  }
   m = warp_max(m);
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 32; ++i) m = fmaxf(m, s[i]);
-    scale[0] = (m > 0.f && m < INFINITY) ? m : 1.f;
+    if (!(m > 0.f && m < INFINITY)) m = 1.f;
+    scale[0] = fminf(m * fmaxf(inv_t * (1.f / 256.f), 1.f), FLT_MAX);
   }
 }
 
@@ -1480,7 +1487,7 @@ int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, 
   // bf16 has fp32's range; only fp16 is scaled
   const float* scale = nullptr;
   if (std::is_same<T, __half>::value) {
-    logp_grad_scale<<<1, 1024, 0, st>>>(w.scale, g_lp, g_ent, N);
+    logp_grad_scale<<<1, 1024, 0, st>>>(w.scale, g_lp, g_ent, labels, ignore_index, q.inv_t, N);
     AK_CHECK_LAUNCH("ak_linear_logprobs_bwd: scale");
     scale = w.scale;
   }

@@ -69,9 +69,10 @@ def distill_topk(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_lo
     are and compares the rest of both distributions as one bucket, left out where the student has
     masked it (no logit outside the teacher's tokens within 30000 of its largest).
     mask (...), bool: rows that count; the others have no gradient, whatever they hold.
-    mode: "fused" writes the gradient in the forward (one read of the logits, one write); "tiny" keeps
-    the logits and recomputes in the backward, which rounds once whatever the upstream gradient is
-    and can run twice.  Default: "tiny" for fp16, whose gradient of a mean would underflow before
+    mode: "fused" writes the gradient in the forward (one read of the logits, one write) and its
+    backward scales it in place, once per forward (a graph of the backward alone is replayed once per
+    replay of the forward); "tiny" keeps the logits and recomputes in the backward, which rounds once
+    whatever the upstream gradient is and can run twice.  Default: "tiny" for fp16, whose gradient of a mean would underflow before
     a loss scale reaches it, else "fused".
     """
     what = "distill_topk"

@@ -251,3 +251,44 @@ def test_huge_and_broken_hidden_states():
     r = linear_token_logprobs(h, w, t, entropy=True)
     assert torch.isnan(r.logprobs[3]) and torch.isnan(r.entropy[3]) and torch.isfinite(r.logprobs[5:]).all()
     assert not torch.isfinite(r.logprobs[4])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_low_temperature_gradients(dtype):
+    """1/T = 2^17 is beyond fp16's range, the gradients of hidden and weight are not.  Every logit is an
+    exact sum (multiples of 2^-12 below 2^-5), so only the roundings of G and of the products count."""
+    from kernels.token_logprobs import linear_token_logprobs
+    n, d, v, T = 5, 8, 300, 2.0 ** -17
+    g = torch.Generator().manual_seed(21)
+    h = (torch.randint(-2, 3, (n, d), generator=g) * 2.0 ** -6).to(dtype)
+    w = (torch.randint(-2, 3, (v, d), generator=g) * 2.0 ** -6).to(dtype)
+    t = torch.randint(0, v, (n,), generator=g)
+    gl, ge = torch.tensor([1.0, -0.5, 0.25, 1.0, -1.0]), torch.tensor([0.5, 0.25, -0.5, 0.0, 1.0])
+    hg, wg = h.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    r = linear_token_logprobs(hg, wg, t.to(DEV), temperature=T, entropy=True)
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [hg, wg], [gl.to(DEV), ge.to(DEV)])
+    W, H = w.double(), h.double()
+    G, tol = O.token_logprobs_grad(H @ W.T, t, gl, ge, temperature=T)
+    info = torch.finfo(dtype)
+    half = info.eps / 2
+    # two 16-bit parts of G; subnormal steps count times the scale, at most (1 + 1) * 2^17 / 2^8
+    tol = tol + (G.abs() + tol) * half * half + 2.0 ** 10 * info.smallest_normal * half
+    tH = tol @ W.abs() + (G.abs() @ W.abs()) * (v + 1) * O.U
+    tW = tol.T @ H.abs() + (G.abs().T @ H.abs()) * (n + 1) * O.U
+    O.assert_within(dh, G @ W, tH, "dH")
+    O.assert_within(dw, G.T @ H, tW, "dW")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_upstream_of_ignored_rows_does_not_count(dtype):
+    from kernels.token_logprobs import linear_token_logprobs
+    h, w, t = problem(9, 64, 515, dtype, seed=22)     # row 1 is ignored
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    got = []
+    for other in (0.0, 1e30):
+        gl = torch.ones(9)
+        gl[1] = other
+        r = linear_token_logprobs(hg, wg, t)
+        got.append(torch.autograd.grad(r.logprobs, [hg, wg], gl.to(DEV)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
