@@ -92,7 +92,7 @@ __device__ __forceinline__ float grad_scale(const DistillArgs& a) {
 template <bool CAP>
 __device__ __forceinline__ float rest_grad(float x, const Ref& ref, float c, const Squash& q) {
   if (c == 0.f) return 0.f;
-  const float y = squash<CAP>(x, q);
+  const float y = CAP ? squash_far(x, q) : x;
   return ex2(exponent(y, ref, q)) * c * squash_slope<CAP>(y, q);
 }
 
@@ -106,6 +106,15 @@ __device__ __forceinline__ void rest_grads(float* x, const uint32_t (&w)[NW], co
     for (int i = 0; i < P; ++i) {
       const float2 d = __ffma2_rn(word_pair<T>(w, i), kl, nk);
       const float2 o = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), c2);
+      x[2 * i] = o.x;
+      x[2 * i + 1] = o.y;
+    }
+  } else if (CAP && ref.sh == 0.f && c != 0.f && all_near<T>(w, words_max<T>(w), q)) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float2 y = squash_near(word_pair<T>(w, i), q);
+      const float2 d = __ffma2_rn(y, kl, nk);
+      const float2 o = __fmul2_rn(__fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), c2), squash_slope_near(y, q));
       x[2 * i] = o.x;
       x[2 * i + 1] = o.y;
     }

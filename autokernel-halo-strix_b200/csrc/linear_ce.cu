@@ -695,6 +695,7 @@ __device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[k & 1].r[j]);
     const int cbase = col0 + c0 + 32 * k;
     const int rel = lr.t - cbase;
+    const bool near = cap && all_near<float>(buf[k & 1].r, words_max<float>(buf[k & 1].r), q);
     if (lr.none) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = 0.f;
@@ -706,10 +707,19 @@ __device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int
         if (j == rel) o += lr.ct;
         v[j] = o;
       }
+    } else if (near) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float y = squash_near(v[j], q);
+        const float d = exponent(y, lr.ref, q);
+        float o = ex2(d) * fmaf(lr.c1, fmaxf(d, -1e4f), lr.c0);
+        if (j == rel) o += lr.ct;
+        v[j] = o * squash_slope<true>(y, q);
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        const float y = squash<true>(v[j], q);
+        const float y = squash_far(v[j], q);
         const float d = exponent(y, lr.ref, q);
         float o = ex2(d) * fmaf(lr.c1, fmaxf(d, -1e4f), lr.c0);
         if (j == rel) o += lr.ct;

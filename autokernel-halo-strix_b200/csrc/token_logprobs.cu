@@ -21,7 +21,7 @@
 //   4096 x 32768 fp16, entropy   48.5 us = 5.5 TB/s
 //   8192 x 50304 bf16, top 64    163 us: the selection costs 35 us (its barriers and a few hundred
 //                                instructions a warp; ranking by counting among the ~75 candidates)
-//   64 x 131072 fp32, softcap    18 us, floor 5.1 us: tanh takes two more special-unit operations
+//   64 x 131072 fp32, softcap    17 us, floor 5.1 us (18.4 with the softcap by special units alone)
 //   1 x 50304 bf16, top 20       9.5 us: latency of one cluster (load, two reductions, selection, join)
 //   backward 8192 x 50304 bf16   237 us = 6.95 TB/s: HBM
 #include "logit_rows.cuh"
@@ -538,14 +538,14 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
   const int ti = (a.targets && t >= 0 && t < a.V) ? (int)t : -1;
 
   auto one = [&](float x, int i) {
-    const float y = squash<CAP>(x, q);
+    const float y = CAP ? squash_far(x, q) : x;
     const float d = exponent(y, ref, q);
     float o = ex2(d);
     o *= ENT ? fmaf(c1, fmaxf(d, -1e30f), c0) : c0;
     if (i == ti) o += ct;
     return o * squash_slope<CAP>(y, q);
   };
-  const bool quick = !CAP && (ENT ? can_raise<T>(ref, q) : ref.sh == 0.f);
+  const bool quick = CAP ? ref.sh == 0.f : ENT ? can_raise<T>(ref, q) : ref.sh == 0.f;
   const float2 kl = both(q.kl), nk = both(-ref.k), c02 = both(c0), c12 = both(c1);
 
   const int gbeg = seg * kBwdGroups;
@@ -572,20 +572,34 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
           uint32_t w[W];
 #pragma unroll
           for (int i = 0; i < W; ++i)
-            w[i] = ENT ? word_max_nan(raw[u].r[h].w[i], floor_word<T>(), (const T*)nullptr) : raw[u].r[h].w[i];
+            w[i] = ENT && !CAP ? word_max_nan(raw[u].r[h].w[i], floor_word<T>(), (const T*)nullptr) : raw[u].r[h].w[i];
+          if (CAP && !all_near<T>(w, words_max<T>(w), q)) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              const float2 v = word_pair<T>(w, i);
+              x[h * 2 * P + 2 * i] = one(v.x, -2);  // the target's part follows
+              x[h * 2 * P + 2 * i + 1] = one(v.y, -2);
+            }
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < P; ++i) {
-            const float2 d = __ffma2_rn(word_pair<T>(w, i), kl, nk);
-            const float2 o = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), ENT ? __ffma2_rn(c12, d, c02) : c02);
+            float2 y = word_pair<T>(w, i);
+            if constexpr (CAP) y = squash_near(y, q);
+            float2 d = __ffma2_rn(y, kl, nk);
+            if constexpr (CAP && ENT) d = make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f));
+            float2 o = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), ENT ? __ffma2_rn(c12, d, c02) : c02);
+            if constexpr (CAP) o = __fmul2_rn(o, squash_slope_near(y, q));
             x[h * 2 * P + 2 * i] = o.x;
             x[h * 2 * P + 2 * i + 1] = o.y;
           }
         }
         const int ta = ti - (cut.head + g * kGroup);
         if ((unsigned)ta < (unsigned)kGroup) {
+          const float add = CAP ? ct * squash_slope<CAP>(squash<CAP>(to_f<T>(row[ti]), q), q) : ct;
 #pragma unroll
           for (int i = 0; i < kGroup; ++i)
-            if (i == ta) x[i] += ct;
+            if (i == ta) x[i] += add;
         }
       } else {
         unpack_group<T>(x, raw[u]);

@@ -328,3 +328,16 @@ def test_huge_logits(v, copies):
         got, = torch.autograd.grad(loss, leaf)
         O.assert_within(loss, ref["loss"], ref["tol_loss"] + ref["loss"].abs() * 8 * O.U, "loss")
         O.assert_within(got, ref["grad"], ref["tol_grad"], "grad")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,k", [(5, 5003, 40), (64, 1500, 7)])
+def test_softcap_with_masked_and_far_logits(n, v, k, dtype):
+    x, idx, tlp, _ = problem(n, v, k, dtype, seed=41)
+    holes = torch.rand(n, v, generator=torch.Generator().manual_seed(42)) < 0.05
+    holes.scatter_(1, idx.cpu().clamp(min=0), False)
+    x[holes.to(DEV)] = -torch.inf
+    x[1, 64:128] *= 9.0
+    for tail in (False, True):
+        check(x, idx, tlp, tail=tail, softcap=10.0)
+        check(x, idx, tlp, tail=tail, softcap=30.0, temperature=1.4)

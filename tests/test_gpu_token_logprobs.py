@@ -394,3 +394,47 @@ def test_two_streams_at_once():
     for w, out in zip(want, got):
         for r, loss in out:
             assert torch.equal(loss, w[1]) and all(torch.equal(p, q) for p, q in zip(r, w[0]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_softcap(dtype):
+    """Under a cap far above the logits their small differences count: each capped logit is within
+    8 u of its own value (5 by the polynomial's bound), not of the cap."""
+    from kernels.token_logprobs import token_logprobs
+    cap = 2.0e4
+    for n, v in ((3, 4001), (40, 1500)):
+        x, t = rows(n, v, dtype, seed=31, std=6.0)
+        ref = O.token_logprobs(x.double().cpu(), t.cpu(), softcap=cap)
+        plain = O.token_logprobs(x.double().cpu(), t.cpu())  # the bounds without a cap
+        e = 8 * O.U * x.double().abs().amax(1).cpu()
+        r = token_logprobs(x, t, entropy=True, softcap=cap)
+        O.assert_within(r.lse, ref["lse"], plain["tol_lse"] + e, "lse")
+        O.assert_within(r.logprobs, ref["logprobs"], plain["tol_logprobs"] + 2 * e, "logprobs")
+        O.assert_within(r.entropy, ref["entropy"], plain["tol_entropy"] + 2 * e * (1 + 2 * ref["entropy"].abs()), "entropy")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_softcap_with_masked_and_far_logits(dtype):
+    """Groups of logits within the cap, with -inf among them, beyond the cap, and of the lowest value."""
+    from kernels.token_logprobs import token_logprobs
+    g = torch.Generator().manual_seed(32)
+    for n, v in ((6, 2051), (200, 515)):
+        x, t = rows(n, v, dtype, seed=33)
+        holes = torch.rand(n, v, generator=g) < 0.1
+        holes[:, ::64] = True
+        x[holes.to(DEV)] = -torch.inf
+        x[1, 100:400] = torch.finfo(dtype).min
+        x[2, 37] = 60.0
+        x[3, 200:300] *= 9.0
+        gl, ge = torch.randn(n, generator=g), torch.randn(n, generator=g) * 0.3
+        for kw in (dict(softcap=12.0), dict(softcap=30.0, temperature=0.6)):
+            check(x, t, token_logprobs(x, t, top_k=9, entropy=True, **kw), top_k=9, **kw)
+            check(x, t, token_logprobs(x, t, **kw), entropy=False, **kw)
+            xg = x.clone().requires_grad_(True)
+            r = token_logprobs(xg, t, entropy=True, **kw)
+            got, = torch.autograd.grad([r.logprobs, r.entropy], xg, [gl.to(DEV), ge.to(DEV)])
+            ref, tol = O.token_logprobs_grad(x.double().cpu(), t.cpu(), gl, ge, **kw)
+            O.assert_within(got, ref, tol, "gradient")
+            one, = torch.autograd.grad(token_logprobs(xg, t, **kw).logprobs, xg, gl.to(DEV))
+            ref, tol = O.token_logprobs_grad(x.double().cpu(), t.cpu(), gl, None, **kw)
+            O.assert_within(one, ref, tol, "gradient of the log-probability")
