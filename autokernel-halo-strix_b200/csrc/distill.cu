@@ -186,8 +186,11 @@ struct FinishRow {
 };
 
 // Bounded waits.  The first that runs out reports AK_ERR_TIMEOUT and raises the CTA's abort flag;
-// the later ones return at once, so the kernel runs to its end without waiting (every role passes
-// the same barriers as ever) and its outputs are invalid.
+// the later ones return at once, so the kernel runs to its end without waiting and its outputs are
+// invalid.  Roles hand over to one another by these waits alone: one role may then run any number of
+// rows ahead of another, which a barrier that counts threads would not survive.  The only barriers
+// of that kind are among the compute warps (each passes one a live row, in step or not at all) and
+// at the kernel's end.
 struct Waits {
   int* status;
   volatile int* abort;
@@ -221,14 +224,10 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Named barriers; the warp is whole again first, after waits that its lanes left one by one.
-__device__ __forceinline__ void named_sync(int id, int threads) {
+// The compute warps' barrier; the warp is whole again first, after waits that its lanes left one by one.
+__device__ __forceinline__ void compute_sync(int threads) {
   __syncwarp();
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ void named_arrive(int id, int threads) {
-  __syncwarp();
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+  asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
 }
 
 // A row's K entries as they lie in memory, entry 32 j + lane in slot j of the teacher's warp.
@@ -424,6 +423,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
   __shared__ __align__(8) uint64_t full;                   // the row has arrived
   __shared__ __align__(8) uint64_t left[kPieces];          // compute has left the piece
   __shared__ __align__(8) uint64_t ready[2], done[2];      // s_teacher, s_edge: written, read
+  __shared__ __align__(8) uint64_t stored[2];              // compute is done with the row
   __shared__ __align__(8) uint64_t joined[2];
   __shared__ TeacherRow s_teacher[2];
   __shared__ FinishRow s_fin[2];
@@ -446,7 +446,8 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
     for (int c = 0; c < kPieces; ++c) mbar_init(&left[c], W);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&ready[b], 1);
-      mbar_init(&done[b], W + 1);
+      mbar_init(&done[b], 1);
+      mbar_init(&stored[b], W);
       mbar_init(&joined[b], cs);
     }
     mbar_fence_init();
@@ -542,10 +543,10 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
     for (int64_t r = first; r < a.rows; r += step, ++it) {
       const int b = it & 1;
       const bool live = a.mask == nullptr || a.mask[r] != 0;
-      // for a masked row too: no second arrival on done[b] before its phase has ended
+      // of every row, masked or not, so that no phase of the two is passed over
       wait.operator()<false>(&ready[b], (uint32_t)(it >> 1) & 1u);
+      wait.operator()<false>(&stored[b], (uint32_t)(it >> 1) & 1u);
       if (live) {
-        named_sync(2, kCompute + 32);  // compute is done with the row
         const TeacherRow& tr = s_teacher[b];
         const FinishRow fin = s_fin[b];
         const Share<T> sh(logits + a.addr.off(r), a.V, rank, a.log_cs);
@@ -631,7 +632,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
           if ((i & 31) < (i < 32 ? sh.head_here : sh.tail_here)) st.add1(s_edge[b][i >> 5][i & 31], q);
         st.warp_merge(q);
         if (lane == 0) s_warp[lb][cw] = st;
-        named_sync(1, kCompute);
+        compute_sync(kCompute);
         st.init();
         if (lane < W) st = s_warp[lb][lane];
         st.warp_merge(q);
@@ -687,9 +688,10 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
                 from_f<T>(rest_grad<CAP>(s_edge[b][i >> 5][i & 31], rest_ref, cg, q));
       }
       leave(kPieces * pv);
-      if (live) named_arrive(2, kCompute + 32);  // the finisher writes over what was stored here
+      // The finisher writes over what was stored here, and hands the row back to the teacher.  Row
+      // it + 2 arrives on the same barrier: its ready[b] waits for done[b], so for the finisher.
       __syncwarp();
-      if (lane == 0) mbar_arrive(&done[b]);
+      if (lane == 0) mbar_arrive(&stored[b]);
     }
   }
   __syncthreads();
