@@ -6,8 +6,10 @@
 //                 T dL/dx_i = p_i - q_i
 //   tail:         q_k = exp(t_k), r = max(0, 1 - sum q), p_r = sum of p outside the K tokens
 //                 L = sum_k q_k (log q_k - log p_{i_k}) + r (log r - log p_r)
-//                 T dL/dx_i = p_i - q_i at the teacher's tokens, p_i (1 - r / p_r) elsewhere
-// (q_i: the teacher's mass on token i, entries of one token added up; times the softcap's slope).
+//                 T dL/dx_i = Q p_i - q_i at the teacher's tokens, Q p_i - r p_i / p_r elsewhere
+// (q_i: the teacher's mass on token i, entries of one token added up; Q: the mass of all terms of L,
+// sum q + r; times the softcap's slope).  Where the rest has no term (the student has masked it, or
+// sum q > 1) Q is sum q.
 //
 // p_r = 1 - sum_k p_{i_k} would cancel where the student agrees with the teacher, so the rest is
 // summed by itself, with a maximum of its own: the teacher's tokens are taken out of the row as it
@@ -173,6 +175,7 @@ struct TeacherRow {
   float m, lim, s;  // statistics of the teacher's tokens, each once
   Ref r;
   float rest;      // r
+  float total;     // sum q
   int none, bad;
   int idx[kMaxK];  // -1: no entry
   float q[kMaxK], logq[kMaxK], y[kMaxK], mass[kMaxK];
@@ -181,7 +184,7 @@ struct TeacherRow {
 // What compute hands to the finisher.
 struct FinishRow {
   Ref all, rest;
-  float logs, tail_loss, c;
+  float logs, tail_loss, c, mass;  // mass: Q
   int empty;
 };
 
@@ -298,7 +301,7 @@ __device__ __forceinline__ bool maybe_twice(const Picked& p, uint8_t (*tag)[kTag
 // What a row's teacher says, on one warp.  s_idx and s_q are its scratch (twice only).
 struct Teacher {
   float q[kSlots], logq[kSlots], y[kSlots], mass[kSlots];
-  float rest;
+  float rest, total;
   bool none, bad;
   template <bool CAP>
   __device__ __forceinline__ void work(RowStats<CAP, false>& top, Picked& p, bool twice, const DistillArgs& a, int* s_idx,
@@ -342,6 +345,7 @@ __device__ __forceinline__ void Teacher::work(RowStats<CAP, false>& top, Picked&
   qsum = warp_sum(qsum);
   none = a.tail ? !any : qsum == 0.f;  // no teacher: loss 0, no gradient
   rest = a.tail ? fmaxf(1.f - qsum, 0.f) : 0.f;
+  total = a.tail ? qsum : 1.f;
   // entries of one token: its logit counts once, at the first of them; their masses add up
   uint32_t later = 0;
 #pragma unroll
@@ -380,7 +384,7 @@ __device__ __forceinline__ void Teacher::work(RowStats<CAP, false>& top, Picked&
 // A row's coefficients from the statistics of the rest and of the teacher's tokens.
 template <bool CAP>
 __device__ __forceinline__ FinishRow coefficients(const RowStats<CAP, false>& st, const RowStats<CAP, false>& top,
-                                                  float rest, bool none, bool bad, const Squash& q) {
+                                                  float rest, float total, bool none, bool bad, const Squash& q) {
   RowStats<CAP, false> all = st;
   all.merge(top, q);
   all.center();
@@ -392,10 +396,13 @@ __device__ __forceinline__ FinishRow coefficients(const RowStats<CAP, false>& st
   f.tail_loss = 0.f;
   // the scale of p in units of e: p = e 2^(rest's reference - the row's) / S
   const float below = ref_diff(st.r, all.r, q);
-  f.c = (none || st.s == 0.f) ? 0.f : ex2(below) / all.s;
   // The rest is left out where the student has masked it: no logit outside the teacher's tokens
   // above -inf, or none within kMasked of the largest (a mask of the type's lowest value).
-  if (rest > 0.f && st.s != 0.f && !none && !(squash<CAP>(st.m, q) - squash<CAP>(all.m, q) < -kMasked)) {
+  const bool counts =
+      rest > 0.f && st.s != 0.f && !none && !(squash<CAP>(st.m, q) - squash<CAP>(all.m, q) < -kMasked);
+  f.mass = counts ? 1.f : total;
+  f.c = (none || st.s == 0.f) ? 0.f : f.mass * ex2(below) / all.s;
+  if (counts) {
     f.tail_loss = rest * (logf(rest) - (fmaf(below, kLn2, logf(st.s)) - f.logs));
     f.c -= rest / st.s;
   }
@@ -410,7 +417,7 @@ __device__ __forceinline__ float entry_grad(float& loss, int idx, float qk, floa
   const float lpk = (f.empty || y == -INFINITY) ? -INFINITY : log_prob(y, f.all, f.logs, q);
   if (idx >= 0 && qk != 0.f) loss += qk * (logq - lpk);
   if (bad) return NAN;
-  return (idx >= 0 && !none && !f.empty) ? (expf(lpk) - mass) * squash_slope<CAP>(y, q) : 0.f;
+  return (idx >= 0 && !none && !f.empty) ? fmaf(f.mass, expf(lpk), -mass) * squash_slope<CAP>(y, q) : 0.f;
 }
 
 template <typename T, bool CAP, bool GRAD, int W>
@@ -529,6 +536,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
           out.s = top.s;
           out.r = top.r;
           out.rest = te.rest;
+          out.total = te.total;
           out.none = te.none;
           out.bad = te.bad;
         }
@@ -663,7 +671,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
         top.lim = tr.lim;
         top.s = tr.s;
         top.r = tr.r;
-        const FinishRow f = coefficients<CAP>(st, top, tr.rest, tr.none, tr.bad, q);
+        const FinishRow f = coefficients<CAP>(st, top, tr.rest, tr.total, tr.none, tr.bad, q);
         if (cw == 0 && lane == 0) s_fin[b] = f;
         rest_ref = f.rest;
         cg = f.c * scale;
@@ -792,7 +800,7 @@ distill_warp_kernel(const T* __restrict__ logits, const DistillArgs a) {
     if (lane < sh.head_here) st.add1(edge[0][lane], q);
     if (lane < sh.tail_here) st.add1(edge[1][lane], q);
     st.warp_merge(q);
-    const FinishRow f = coefficients<CAP>(st, top, te.rest, te.none, te.bad, q);
+    const FinishRow f = coefficients<CAP>(st, top, te.rest, te.total, te.none, te.bad, q);
     const float scale = GRAD ? grad_scale(a) : 1.f;
     float loss = 0.f, gk[kSlots];
 #pragma unroll

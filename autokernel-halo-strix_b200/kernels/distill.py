@@ -67,7 +67,8 @@ def distill_topk(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_lo
     of one token add up.
     tail: False renormalises the teacher over its K entries; True takes exp(teacher_logprobs) as they
     are and compares the rest of both distributions as one bucket, left out where the student has
-    masked it (no logit outside the teacher's tokens within 30000 of its largest).
+    masked it (no logit outside the teacher's tokens within 30000 of its largest) and where the
+    entries' mass exceeds 1.  The gradient is that of the terms that are there, whatever mass they have.
     mask (...), bool: rows that count; the others have no gradient, whatever they hold.
     mode: "fused" writes the gradient in the forward (one read of the logits, one write) and its
     backward scales it in place, once per forward (a graph of the backward alone is replayed once per

@@ -224,7 +224,9 @@ AK_API int ak_token_logprobs_bwd(void* grad, const void* logits, const int64_t* 
  *   tail = 0: q = softmax of the entries;   sum_k q_k (log q_k - log p_{i_k})
  *   tail = 1: q_k = exp(lp_k), r = max(0, 1 - sum q);  the same sum + r (log r - log p_r), p_r the
  *             student's probability outside the K tokens (left out where it has no logit there
- *             within 30000 of its largest: -inf or lowest-value masks)
+ *             within 30000 of its largest: -inf or lowest-value masks).  The gradient is that of
+ *             the terms that are there: T dL/dx_i = Q p_i - q_i (- r p_i / p_r outside the K
+ *             tokens), Q = sum q + r, or sum q without the rest's term
  * A negative index is padding; a row of nothing else has loss 0 and no gradient (it counts in the
  * mean).  An index >= V makes its row's loss and gradient NaN.  Entries of one token add up.
  * losses[rows] fp32: the rows' divergences (0 without mask).  inv_n (needed with a mask): receives

@@ -190,14 +190,19 @@ def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=Fals
     # gradient
     mass = torch.zeros_like(p).scatter_add_(1, at, torch.where(used, q, 0.0))
     cond = torch.where(has_rest[:, None] & outside, (logp - logpr[:, None]).exp(), torch.zeros_like(p))  # p_i / p_r
-    g = torch.where(inside, p - mass, p - rest[:, None] * cond)
+    # the mass of all terms of the loss: 1, or the entries' own where the rest has no term
+    counts = has_rest & (rest > 0)
+    total = torch.where(counts, torch.ones_like(rest), q.sum(1))[:, None] if tail else torch.ones_like(rest)[:, None]
+    g = torch.where(inside, total * p - mass, total * p - rest[:, None] * cond)
     _, dy = squash(x, temperature, softcap)
     logv = torch.log(torch.tensor(v + 1.0)).item()
     lgp = torch.where(p > 0, logp, torch.zeros_like(p))
     lpr = torch.where(has_rest, logpr, torch.zeros_like(rest)).abs()[:, None]
     rel = 10 * U + (4 * lgp.abs() + 6 * logv + 6 * lpr) * U + 2 * r["tol_logs"][:, None] + 2 * CAP * U * softcap / temperature
     relm = torch.zeros_like(p).scatter_add_(1, at, torch.where(used, q * (rel_q + k * U), torch.zeros_like(q)))
-    tg = torch.where(inside, p * rel + relm, p * rel + cond * (rest[:, None] * rel + dr)) + 6 * U * g.abs() + 2 * FLUSH
+    rel_t = (q * (rel_q + k * U)).sum(1, keepdim=True)  # of total, absolute
+    tg = p * (total * rel + rel_t) + torch.where(inside, relm, cond * (rest[:, None] * rel + dr))
+    tg = tg + 6 * U * g.abs() + 2 * FLUSH
     tg = tg * dy.abs() + (g.abs() * 20 * U / temperature if softcap > 0 else 0.0)
     off = (none | empty | ~live)[:, None]
     g, tg = torch.where(off, torch.zeros_like(g), g * dy), torch.where(off, torch.zeros_like(tg), tg)

@@ -33,3 +33,61 @@ def test_many_rows_with_a_slow_finish(n, v, k):
     O.assert_within(first[1][at], ref["losses"], ref["tol_losses"], "losses")
     f = max(1, int(mask[at].sum())) / int(mask.sum())  # the mean is over all rows
     O.assert_within(first[3][at], ref["grad"] * f, ref["tol_grad"] * f, "grad")
+
+
+def check(x, idx, tlp, mask=None, modes=("fused", "tiny"), upstream=1.0, **kw):
+    from kernels.distill import distill_topk
+    ref = O.distill_topk(x.double().cpu(), idx.cpu(), tlp.cpu(), None if mask is None else mask.cpu(), g_loss=upstream, **kw)
+    for mode in modes:
+        leaf = x.detach().requires_grad_(True)
+        loss = distill_topk(leaf, idx, tlp, mask=mask, mode=mode, **kw)
+        O.assert_within(loss, ref["loss"], ref["tol_loss"], "loss")
+        g, = torch.autograd.grad(loss, leaf, torch.full((), upstream, device=DEV))
+        O.assert_within(g, ref["grad"], ref["tol_grad"], f"grad {mode} {kw}")
+    return ref
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,v,k", [(9, 300, 7), (700, 520, 40), (5, 50257, 64), (300, 20011, 5)])
+def test_terms_whose_mass_is_not_one(n, v, k, dtype):
+    """The rest masked by the student, or entries whose mass exceeds 1 (rounded log-probabilities,
+    repeated tokens): the gradient is that of the terms left, so it sums to 0 over a row."""
+    x, idx, tlp = rows(n, v, k, dtype, 5, rest=0.3)
+    gone = torch.ones(n, v, dtype=torch.bool, device=DEV).scatter_(1, idx, False)
+    x[1] = torch.where(gone[1], -torch.inf, x[1])
+    x[2] = torch.where(gone[2], torch.finfo(dtype).min, x[2])
+    tlp[3] += 0.5                          # mass 0.7 e^0.5 > 1
+    idx[4, k // 2:] = idx[4, 0]            # one token many times
+    tlp[4] += 0.6
+    if n > 8:
+        x[7] = torch.where(gone[7], -torch.inf, x[7])
+        tlp[7] += 0.9
+        x[8] = torch.where(gone[8], -torch.inf, x[8])
+        idx[8, 1] = idx[8, 0]
+    ref = check(x, idx, tlp, tail=True)
+    total = ref["grad"].sum(1).abs()
+    assert (total <= 1e-12).all()          # of the oracle's, in 64 bits
+    check(x, idx, tlp, tail=True, temperature=1.6)
+    check(x, idx, tlp, tail=True, softcap=12.0, temperature=0.9)
+    check(x, idx, tlp, tail=False)
+
+
+def test_masked_rest_against_differences():
+    """Along d, |d| = 1, as a loss of mass Q <= 2: its third derivative is at most 2 Q, and 4 with the
+    rest's own term."""
+    from kernels.distill import distill_topk
+    n, v, k = 6, 200, 9
+    x, idx, tlp = rows(n, v, k, torch.float32, 6, rest=0.3)
+    gone = torch.ones(n, v, dtype=torch.bool, device=DEV).scatter_(1, idx, False)
+    x[:3] = torch.where(gone[:3], -torch.inf, x[:3])
+    tlp[2:4] += 0.7
+    idx[5, 1] = idx[5, 0]
+    d = torch.randn(n, v, generator=torch.Generator().manual_seed(4), dtype=torch.float64)
+    d /= d.norm()
+    leaf = x.clone().requires_grad_(True)
+    g, = torch.autograd.grad(distill_topk(leaf, idx, tlp, tail=True), leaf)
+    h, args = 1e-4, (idx.cpu(), tlp.cpu())
+    f = [O.distill_topk(x.double().cpu() + s * h * d, *args, tail=True)["loss"] for s in (1, -1)]
+    ref = O.distill_topk(x.double().cpu(), *args, tail=True)
+    bound = h * h / 6 * 8 + ((ref["tol_grad"] + O.U * ref["grad"].abs()) * d.abs()).sum() + 1e-11
+    assert abs((f[0] - f[1]) / (2 * h) - (g.double().cpu() * d).sum()) <= bound
