@@ -1597,8 +1597,8 @@ int check_logp(const char* what, const void* H, const void* W, int64_t N, int64_
   AK_REQUIRE(N >= 0 && D > 0 && V > 0 && D % 8 == 0 && D <= (1 << 20) && N < (1LL << 31) && V < (1LL << 30),
              AK_ERR_SHAPE, "%s: bad shape: %lld x %lld, vocabulary %lld (the hidden size must be a multiple of 8)", what,
              (long long)N, (long long)D, (long long)V);
-  AK_REQUIRE(temperature > 0.f && temperature < INFINITY, AK_ERR_ARG, "%s: temperature must be positive and finite",
-             what);
+  AK_REQUIRE(temperature >= kLowestTemperature && temperature < INFINITY, AK_ERR_ARG,
+             "%s: temperature must be at least 2^-100 and finite", what);
   AK_REQUIRE(softcap >= 0.f && softcap < INFINITY, AK_ERR_ARG, "%s: softcap must be >= 0 and finite", what);
   AK_REQUIRE(N == 0 || (H && W && aligned16(H) && aligned16(W)), AK_ERR_ARG,
              "%s: hidden states and weight must be 16-byte aligned", what);

@@ -25,12 +25,15 @@ struct RowAddr {
 // What a logit x means: y = softcap(x), log-probabilities of y / temperature.
 // kl = log2(e) / temperature turns a difference of y into an exponent of 2.
 // -inf stays -inf under softcap: a masked token has no probability there either.
+// temperature >= kLowestTemperature: its reciprocal and products with raise_floor stay finite.
 struct Squash {
   float cap, inv_cap, inv_t, kl;
   float rkl;   // 1 / kl
   float kc;    // -2 log2(e) / cap
   float near;  // softcap by the polynomial up to this |x|
 };
+
+constexpr float kLowestTemperature = 7.888609052210118e-31f;  // 2^-100
 
 inline Squash make_squash(float temperature, float softcap) {
   Squash q;
@@ -332,21 +335,36 @@ __device__ __forceinline__ float ref_scale(const Ref& a, const Ref& b, const Squ
 }
 
 // Where a product of e = 2^d with d is formed, -inf has to be raised to a finite logit whose e is
-// still 0: to `raise_floor`, which the type represents.  Holds for a reference far enough above it;
-// elsewhere the terms are cut off one by one.
+// still 0: to `raise_floor`, which the type represents, and whose d is finite at the lowest
+// temperature (-2^20 log2(e) 2^100).  Holds for a reference far enough above it, so for rows whose
+// largest logit is above -10^6 up to a temperature of some thousands; elsewhere the terms are cut off
+// one by one.
 template <typename T>
 __device__ __forceinline__ float raise_floor() {
-  return std::is_same<T, __half>::value ? -65504.f : -1.0e30f;
+  return std::is_same<T, __half>::value ? -65504.f : -1048576.f;
 }
 template <typename T>
 __device__ __forceinline__ bool can_raise(const Ref& r, const Squash& q) {
   return r.sh == 0.f && r.k - raise_floor<T>() * q.kl > 200.f;
 }
 template <typename T>
-__device__ __forceinline__ uint32_t floor_word() {
-  if constexpr (sizeof(T) == 4) return __float_as_uint(raise_floor<T>());
-  else return pack2(raise_floor<T>(), raise_floor<T>(), (const T*)nullptr);
+__device__ __forceinline__ uint32_t floor_word(float floor = raise_floor<T>()) {
+  if constexpr (sizeof(T) == 4) return __float_as_uint(floor);
+  else return pack2(floor, floor, (const T*)nullptr);
 }
+
+// A gradient multiplies d by what comes from upstream, which may be large: there -inf is raised no
+// lower than it has to be, about 300 powers of 2 below the reference.  (1/64 of the reference more,
+// so that rounding the logit to T, 2^-9 of it at most, leaves its term 0.)  `floor` receives the
+// logit and the answer is whether its term is 0.
+template <typename T>
+__device__ __forceinline__ bool raise_to(float& floor, const Ref& r, const Squash& q) {
+  const float f = fmaxf((r.k - (300.f + fabsf(r.k) * (1.f / 64.f))) * q.rkl, sizeof(T) == 2 ? -65504.f : -1e30f);
+  floor = to_f<T>(from_f<T>(f));
+  return r.sh == 0.f && fmaf(floor, q.kl, -r.k) <= -200.f;
+}
+// The same where the terms are cut off one by one.
+constexpr float kNoTerm = -200.f;
 
 __device__ __forceinline__ float redux_max(float v) {  // over the warp; NaN is passed over
   float r;

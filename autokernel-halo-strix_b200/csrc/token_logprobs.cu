@@ -541,11 +541,17 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
     const float y = CAP ? squash_far(x, q) : x;
     const float d = exponent(y, ref, q);
     float o = ex2(d);
-    o *= ENT ? fmaf(c1, fmaxf(d, -1e30f), c0) : c0;
+    o *= ENT ? fmaf(c1, fmaxf(d, kNoTerm), c0) : c0;
     if (i == ti) o += ct;
     return o * squash_slope<CAP>(y, q);
   };
-  const bool quick = CAP ? ref.sh == 0.f : ENT ? can_raise<T>(ref, q) : ref.sh == 0.f;
+  [[maybe_unused]] uint32_t floor = 0;
+  bool quick = ref.sh == 0.f;
+  if constexpr (ENT && !CAP) {
+    float f;
+    quick = raise_to<T>(f, ref, q);
+    floor = floor_word<T>(f);
+  }
   const float2 kl = both(q.kl), nk = both(-ref.k), c02 = both(c0), c12 = both(c1);
 
   const int gbeg = seg * kBwdGroups;
@@ -572,7 +578,7 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
           uint32_t w[W];
 #pragma unroll
           for (int i = 0; i < W; ++i)
-            w[i] = ENT && !CAP ? word_max_nan(raw[u].r[h].w[i], floor_word<T>(), (const T*)nullptr) : raw[u].r[h].w[i];
+            w[i] = ENT && !CAP ? word_max_nan(raw[u].r[h].w[i], floor, (const T*)nullptr) : raw[u].r[h].w[i];
           if (CAP && !all_near<T>(w, words_max<T>(w), q)) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -587,7 +593,7 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
             float2 y = word_pair<T>(w, i);
             if constexpr (CAP) y = squash_near(y, q);
             float2 d = __ffma2_rn(y, kl, nk);
-            if constexpr (CAP && ENT) d = make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f));
+            if constexpr (CAP && ENT) d = make_float2(fmaxf(d.x, kNoTerm), fmaxf(d.y, kNoTerm));
             float2 o = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), ENT ? __ffma2_rn(c12, d, c02) : c02);
             if constexpr (CAP) o = __fmul2_rn(o, squash_slope_near(y, q));
             x[h * 2 * P + 2 * i] = o.x;
@@ -630,8 +636,8 @@ int check_rows(const char* what, const void* logits, int64_t rows, int64_t inner
   AK_REQUIRE(valid_dtype(dt), AK_ERR_DTYPE, "%s: unsupported dtype %d", what, dt);
   AK_REQUIRE(rows >= 0 && inner > 0 && V > 0 && V < (1LL << 30) && rows < (1LL << 27), AK_ERR_SHAPE,
              "%s: bad shape: %lld rows of %lld", what, (long long)rows, (long long)V);
-  AK_REQUIRE(temperature > 0.f && temperature < INFINITY, AK_ERR_ARG, "%s: temperature must be positive and finite",
-             what);
+  AK_REQUIRE(temperature >= kLowestTemperature && temperature < INFINITY, AK_ERR_ARG,
+             "%s: temperature must be at least 2^-100 and finite", what);
   AK_REQUIRE(softcap >= 0.f && softcap < INFINITY, AK_ERR_ARG, "%s: softcap must be >= 0 and finite", what);
   AK_REQUIRE(rows == 0 || logits, AK_ERR_ARG, "%s: null pointer", what);
   AK_REQUIRE((reinterpret_cast<uintptr_t>(logits) % elem_size(dt)) == 0, AK_ERR_ARG,

@@ -1,0 +1,66 @@
+"""Token log-probabilities: calls at the edges of what their documentation allows."""
+import pytest
+import torch
+
+from oracle import logit_row_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def masked(n, v, dtype, seed, scale=1.0, share=0.3):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, v, generator=g) * scale
+    t = torch.randint(0, v, (n,), generator=g)
+    gone = torch.rand(n, v, generator=g) < share
+    gone[torch.arange(n), t] = False
+    x[gone] = -torch.inf
+    return x.to(dtype), t, gone
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,scale,T,up", [(3, 777, 0.05, 0.01, 65536.0 * 1e4), (70, 515, 0.05, 0.01, 1e10), (2, 40000, 20.0, 0.01, 1e12),
+                                            (4, 300, 1.0, 1.0, 1e25), (3, 5003, 900.0, 0.001, 1e9),
+                                            (2, 1000, 1e-4, 1e-6, 1e15)])
+def test_masked_tokens_under_a_large_upstream_of_the_entropy(n, v, scale, T, up, dtype):
+    """A token without probability has gradient 0, however large T^-2 times the upstream gradient."""
+    from kernels.token_logprobs import token_logprobs
+    x, t, gone = masked(n, v, dtype, 3, scale)
+    gl, ge = torch.full((n,), 0.5), torch.full((n,), up)
+    if dtype == torch.float16:             # its largest value is not the subject
+        ge = ge * 1e-25
+    for kw in (dict(temperature=T), dict(temperature=T, softcap=scale * 5)):
+        leaf = x.to(DEV).requires_grad_(True)
+        r = token_logprobs(leaf, t.to(DEV), entropy=True, **kw)
+        got, = torch.autograd.grad([r.logprobs, r.entropy], leaf, [gl.to(DEV), ge.to(DEV)])
+        assert (got[gone.to(DEV)] == 0).all()
+        ref, tol = O.token_logprobs_grad(x.double(), t, gl, ge, **kw)
+        # a gradient half a step beyond the type's largest value, (2 - eps / 2) 2^e, rounds to infinity
+        info = torch.finfo(dtype)
+        over = ref.abs() >= info.max * (1 + info.eps / 4 / (1 - info.eps / 2))
+        O.assert_within(got, torch.where(over, ref.sign() * torch.inf, ref), tol, f"grad {kw}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1e-9, 1e-20, 2.0 ** -100])
+def test_masked_tokens_at_the_lowest_temperatures(T, dtype):
+    """The entropy of rows whose exponents leave fp32's range where they are masked: two equal
+    largest tokens, all others masked or far below."""
+    from kernels.token_logprobs import token_logprobs
+    for n, v in ((3, 700), (700, 64), (4, 20011)):
+        x = torch.full((n, v), -torch.inf)
+        x[:, 5], x[:, v - 2] = 0.0, 0.0
+        x[1, 7:20] = -1.0
+        x[2, :] = torch.finfo(dtype).min
+        x[2, 1], x[2, 2] = 0.0, 0.0
+        x = x.to(dtype).to(DEV)
+        r = token_logprobs(x, torch.full((n,), 5, device=DEV), entropy=True, temperature=T)
+        half = torch.log(torch.tensor(2.0)).item()
+        # log 2 and 0.5 log 2 twice: a few roundings of numbers below 1
+        assert ((r.entropy - half).abs() <= 8 * O.U).all()
+        assert ((r.logprobs[:2] + half).abs() <= 8 * O.U).all()
+        leaf = x.clone().requires_grad_(True)
+        q = token_logprobs(leaf, torch.full((n,), 5, device=DEV), entropy=True, temperature=T)
+        g, = torch.autograd.grad(q.entropy, leaf, torch.full((n,), T, device=DEV))
+        assert (g.abs() <= 8 * O.U).all()  # p (log p + H) = 0 for both

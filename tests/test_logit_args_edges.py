@@ -1,0 +1,31 @@
+"""Arguments at the edge of what the operators over logits take, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from kernels import _ak
+from kernels import token_logprobs as TL
+
+
+def on_gpu(monkeypatch):
+    """Lets CPU tensors pass the device check, so that the checks behind it are reached."""
+    monkeypatch.setattr(_ak, "require_cuda", lambda *t: torch.device("cpu"))
+
+
+def test_temperatures_too_low_for_fp32_are_refused(monkeypatch):
+    """Below 2^-100 products of masked logits with 1 / temperature leave fp32's range."""
+    on_gpu(monkeypatch)
+    lib = _ak.lib()
+    fake = ctypes.c_void_p(256)  # never dereferenced: each call fails its checks first
+    for T in (1e-31, 1e-39, 1e-45):
+        with pytest.raises(ValueError, match="2\\^-100"):
+            TL.token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.long), temperature=T)
+        with pytest.raises(ValueError, match="2\\^-100"):
+            TL.linear_token_logprobs(torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(9, 8), temperature=T)
+        assert lib.ak_token_logprobs_fwd(fake, None, fake, None, None, None, fake, fake, 2, 2, 0, 64, 64, 0, T, 0.0, -100,
+                                         1, None) == 1
+        assert lib.ak_distill_topk_fwd(fake, fake, None, None, None, None, fake, fake, fake, None, 2, 2, 0, 64, 64, 3, T,
+                                       0.0, 0, 1, None, None) == 1
+        assert lib.ak_linear_logprobs_fwd(None, None, fake, None, fake, 1 << 20, fake, fake, None, 8, 64, 100, T, 0.0,
+                                          -100, 1, None, None) == 1
