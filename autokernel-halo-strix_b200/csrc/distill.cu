@@ -315,16 +315,27 @@ __device__ __forceinline__ void Teacher::work(RowStats<CAP, false>& top, Picked&
   const Squash sq = a.q;
   bad = __any_sync(0xffffffffu, p.bad);
   const bool any = __any_sync(0xffffffffu, p.any);
-  float qsum = 0.f;
+  // 1 - sum q would cancel in 32 bits: a teacher's 64 entries may leave 1e-5, of which their
+  // exponentials' roundings are a tenth.  So the masses and their sum are formed in 64.
   if (a.tail) {
+    double all = 0.0;
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       q[j] = 0.f;
       logq[j] = p.t[j];
-      if (32 * j < a.K) qsum += q[j] = p.idx[j] >= 0 ? expf(p.t[j]) : 0.f;
+      if (32 * j < a.K) {
+        const double e = p.idx[j] >= 0 ? exp((double)p.t[j]) : 0.0;
+        q[j] = (float)e;
+        all += e;
+      }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    none = !any;
+    rest = (float)fmax(1.0 - all, 0.0);
+    total = (float)all;
   } else {
-    float tm = p.t[0], z = 0.f;
+    float tm = p.t[0], z = 0.f, qsum = 0.f;
 #pragma unroll
     for (int j = 1; j < kSlots; ++j) tm = fmaxf(tm, p.t[j]);
     tm = redux_max(tm);
@@ -341,11 +352,10 @@ __device__ __forceinline__ void Teacher::work(RowStats<CAP, false>& top, Picked&
       logq[j] = p.t[j] - tm - logz;
       qsum += q[j];
     }
+    none = warp_sum(qsum) == 0.f;  // no teacher: loss 0, no gradient
+    rest = 0.f;
+    total = 1.f;
   }
-  qsum = warp_sum(qsum);
-  none = a.tail ? !any : qsum == 0.f;  // no teacher: loss 0, no gradient
-  rest = a.tail ? fmaxf(1.f - qsum, 0.f) : 0.f;
-  total = a.tail ? qsum : 1.f;
   // entries of one token: its logit counts once, at the first of them; their masses add up
   uint32_t later = 0;
 #pragma unroll

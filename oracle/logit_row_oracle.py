@@ -135,8 +135,9 @@ def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=Fals
     """dict of loss, losses, grad of double rows (N, V) and the fp32 bounds tol_loss, tol_losses, tol_grad.
 
     Student log-probabilities are off as in token_logprobs.  q: an exponential off by 4 u, its
-    argument t - max by u each, K additions and a division; 1 - sum q by (K + 6) u; losses are sums of
-    K terms, and the mean one of N / 1024 + 64."""
+    argument t - max by u each, K additions and a division, with a tail rounded once from 64 bits;
+    1 - sum q is formed in 64 bits and rounded (sums of K terms, off by K 2^-52); losses are sums of K
+    terms, and the mean one of N / 1024 + 64."""
     n, v = x.shape
     k = idx.shape[1]
     live = torch.ones(n, dtype=torch.bool, device=x.device) if mask is None else mask
@@ -149,7 +150,7 @@ def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=Fals
     if tail:
         none = ~used.any(1)
         q, logq = torch.where(used, t.exp(), 0.0), t
-        rel_q = torch.full_like(q, 4 * U)
+        rel_q = torch.full_like(q, U)
         rest = (1 - q.sum(1)).clamp(min=0)
     else:
         tm = t.amax(1, keepdim=True)
@@ -172,7 +173,7 @@ def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=Fals
     y = squash(x, 1.0, softcap)[0]
     low = torch.where(outside, y, torch.full_like(y, -torch.inf)).amax(1) - y.amax(1)
     has_rest = outside.any(1) & ~none & (torch.tensor(tail, device=x.device)) & (low >= -3e4)
-    dr = (k + 6) * U
+    dr = rest * U + (k + 4) * 2.0 ** -52
     tail_term = torch.where(has_rest & (rest > 0), rest * (torch.log(rest) - logpr), torch.zeros_like(rest))
     losses = terms.sum(1) + tail_term
     tol_lp = r["tol_logs"][:, None] + 8 * U * (lpk.abs().nan_to_num(0, 0, 0) + torch.log(torch.tensor(v + 1.0)).item()) + CAP * U * softcap / temperature
@@ -201,7 +202,7 @@ def distill_topk(x, idx, tlp, mask=None, temperature=1.0, softcap=0.0, tail=Fals
     rel = 10 * U + (4 * lgp.abs() + 6 * logv + 6 * lpr) * U + 2 * r["tol_logs"][:, None] + 2 * CAP * U * softcap / temperature
     relm = torch.zeros_like(p).scatter_add_(1, at, torch.where(used, q * (rel_q + k * U), torch.zeros_like(q)))
     rel_t = (q * (rel_q + k * U)).sum(1, keepdim=True)  # of total, absolute
-    tg = p * (total * rel + rel_t) + torch.where(inside, relm, cond * (rest[:, None] * rel + dr))
+    tg = p * (total * rel + rel_t) + torch.where(inside, relm, cond * (rest[:, None] * rel + dr[:, None]))
     tg = tg + 6 * U * g.abs() + 2 * FLUSH
     tg = tg * dy.abs() + (g.abs() * 20 * U / temperature if softcap > 0 else 0.0)
     off = (none | empty | ~live)[:, None]

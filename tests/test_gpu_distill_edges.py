@@ -91,3 +91,21 @@ def test_masked_rest_against_differences():
     ref = O.distill_topk(x.double().cpu(), *args, tail=True)
     bound = h * h / 6 * 8 + ((ref["tol_grad"] + O.U * ref["grad"].abs()) * d.abs()).sum() + 1e-11
     assert abs((f[0] - f[1]) / (2 * h) - (g.double().cpu() * d).sum()) <= bound
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,v,k", [(40, 2000, 64), (700, 1500, 128), (6, 50257, 64), (300, 20011, 100)])
+def test_teachers_that_leave_little(n, v, k, dtype):
+    """A teacher's entries cover all but 1e-2 to 1e-7 of its mass: the rest of it, 1 - sum q, and what
+    follows from it keep their leading bits.  The student's own rest is as small, so the rest's term
+    and its gradient p_i (1 - r / p_r) count."""
+    g = torch.Generator().manual_seed(7)
+    rest = 10.0 ** -(2 + 5 * torch.rand(n, 1, generator=g, dtype=torch.float64))
+    idx = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(n)])
+    lp = torch.log_softmax(torch.randn(n, k, generator=g, dtype=torch.float64), 1) + torch.log1p(-rest)
+    x = torch.randn(n, v, generator=g, dtype=torch.float64) + torch.log(rest / v)
+    x.scatter_(1, idx, lp + 0.1 * torch.randn(n, k, generator=g, dtype=torch.float64))
+    x, idx, tlp = x.to(dtype).to(DEV), idx.to(DEV), lp.float().to(DEV)
+    check(x, idx, tlp, tail=True)
+    check(x, idx, tlp, tail=True, upstream=2.0 ** 20, modes=("tiny",))
+    check(x, idx, tlp, tail=False)
