@@ -276,13 +276,16 @@ struct Picked {
 constexpr int kTags = 2048;
 __device__ __forceinline__ int mix_bits(int i) { return (int)(((uint32_t)i * 2654435761u) >> 21); }  // 11 bits
 
-// Whether a token may come twice: two tables of who came last to a place that its low and its mixed
-// bits name.  One that comes twice is not the last in either table at one of its entries; so,
-// rarely, is one that shares its places with others, which costs a comparison of all with all.
-__device__ __forceinline__ bool maybe_twice(const Picked& p, uint8_t (*tag)[kTags]) {
+// Whether a token may come twice: two tables of who holds a place that its low and its mixed bits
+// name.  Which of several entries holds it is not known (lanes of one store go in any order), but it
+// is one of them: where the holder has the same token, that comes twice; where both places are held
+// by other tokens it may, which costs a comparison of all with all.  A token that comes twice meets
+// one of the two at an entry that does not hold its place.
+__device__ __forceinline__ bool maybe_twice(const Picked& p, uint8_t (*tag)[kTags], int* s_idx) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int j = 0; j < kSlots; ++j) {
+    s_idx[32 * j + lane] = p.idx[j];
     if (p.idx[j] >= 0) {
       tag[0][p.idx[j] & (kTags - 1)] = (uint8_t)(32 * j + lane);
       tag[1][mix_bits(p.idx[j])] = (uint8_t)(32 * j + lane);
@@ -291,10 +294,11 @@ __device__ __forceinline__ bool maybe_twice(const Picked& p, uint8_t (*tag)[kTag
   __syncwarp();
   bool twice = false;
 #pragma unroll
-  for (int j = 0; j < kSlots; ++j)
-    if (p.idx[j] >= 0)
-      twice |= tag[0][p.idx[j] & (kTags - 1)] != (uint8_t)(32 * j + lane) &&
-               tag[1][mix_bits(p.idx[j])] != (uint8_t)(32 * j + lane);
+  for (int j = 0; j < kSlots; ++j) {
+    if (p.idx[j] < 0) continue;
+    const int a = tag[0][p.idx[j] & (kTags - 1)], b = tag[1][mix_bits(p.idx[j])], me = 32 * j + lane;
+    twice |= (a != me && (b != me || s_idx[a] == p.idx[j])) || (b != me && s_idx[b] == p.idx[j]);
+  }
   return __any_sync(0xffffffffu, twice);
 }
 
@@ -516,7 +520,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
         if (lane < sh.head_here) e0 = to_f<T>(sh.row[lane]);
         if (lane < sh.tail_here) e1 = to_f<T>(sh.row[sh.tail0 + lane]);
         p.pick(now, a, [&](int i) { return to_f<T>(sh.row[i]); });
-        const bool twice = maybe_twice(p, s_tag);
+        const bool twice = maybe_twice(p, s_tag, s_idx);
         te.template work<CAP>(top, p, twice, a, s_idx, s_q);
       }
       wait.operator()<false>(&done[b], ((uint32_t)(it >> 1) & 1u) ^ 1u);

@@ -109,3 +109,25 @@ def test_teachers_that_leave_little(n, v, k, dtype):
     check(x, idx, tlp, tail=True)
     check(x, idx, tlp, tail=True, upstream=2.0 ** 20, modes=("tiny",))
     check(x, idx, tlp, tail=False)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("n,v,k", [(400, 9000, 128), (60, 50257, 70), (8, 131073, 33), (700, 2000, 128)])
+def test_repeated_tokens_beside_others_of_their_places(n, v, k, tail):
+    """Tokens that come twice or often, within a group of 32 entries and across groups, among tokens
+    that agree with them in their low 11 bits."""
+    x, idx, tlp = rows(n, v, k, torch.float32, 9, rest=0.25)
+    g = torch.Generator().manual_seed(10)
+    idx = idx.cpu()
+    for r in range(n):
+        kind = r % 4
+        if kind == 0:                      # one pair
+            a, b = torch.randperm(k, generator=g)[:2].tolist()
+            idx[r, a] = idx[r, b]
+        elif kind == 1:                    # a few tokens, all often
+            idx[r] = idx[r, torch.randint(0, 5, (k,), generator=g)]
+        elif kind == 2:                    # pairs among tokens 2048 apart
+            base = int(torch.randint(0, min(v, 2048), (1,), generator=g))
+            pool = torch.arange(base, v, 2048)
+            idx[r] = pool[torch.randint(0, len(pool), (k,), generator=g)]
+    check(x, idx.to(DEV), tlp, tail=tail)
