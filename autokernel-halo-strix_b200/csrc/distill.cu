@@ -1012,7 +1012,10 @@ int launch_width(const T* logits, DistillArgs& a, int64_t share, cudaStream_t st
   const int cs = 1 << a.log_cs;
   a.piece = (uint32_t)((share + kPieces * 16 - 1) / (kPieces * 16) * 16);
   const size_t smem = (size_t)std::max<int64_t>(share, 16);
-  AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+  // the most that this instance is launched with, not this call's: the attribute is the kernel's, and
+  // another thread may launch it for a longer row between here and the launch
+  AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   W == kWide ? kShareMost : kShareNarrow),
               "ak_distill_topk_fwd: shared memory");
   int64_t grid = a.rows * cs;
   if (grid > sm_count()) {  // fewer have an SM each
@@ -1032,7 +1035,7 @@ int launch_fwd(const T* logits, DistillArgs& a, cudaStream_t st) {
     auto kern = a.grad ? (cap ? distill_warp_kernel<T, true, true> : distill_warp_kernel<T, false, true>)
                        : (cap ? distill_warp_kernel<T, true, false> : distill_warp_kernel<T, false, false>);
     const size_t smem = (size_t)kRowWarps * warp_row_bytes(a.V * (int)sizeof(T));
-    AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+    AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowWarps * kShortBytes),
                 "ak_distill_topk_fwd: shared memory");
     AK_CUDA_TRY(launch_rows(kern, (a.rows + kRowWarps - 1) / kRowWarps, 32 * kRowWarps, 1, smem, st, logits,
                             (const DistillArgs&)a),

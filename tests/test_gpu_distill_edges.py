@@ -131,3 +131,46 @@ def test_repeated_tokens_beside_others_of_their_places(n, v, k, tail):
             pool = torch.arange(base, v, 2048)
             idx[r] = pool[torch.randint(0, len(pool), (k,), generator=g)]
     check(x, idx.to(DEV), tlp, tail=tail)
+
+
+@pytest.mark.parametrize("sizes", [(60000, 24000), (21000, 9000), (4000, 900)])
+def test_two_threads_with_different_vocabularies(sizes):
+    """Calls from two host threads at once, each with its own vocabulary and stream, over kernels that
+    they share: none is refused and each gives what it gives alone.  The library is called as often
+    as it can be, on buffers made before."""
+    import threading
+
+    from kernels import _ak
+    n, k, times = 640, 16, 6000
+    device = torch.device(DEV, torch.cuda.current_device())
+    mask = torch.zeros(n, dtype=torch.bool, device=DEV)
+    mask[::80] = True                      # short calls: host threads meet in the library, not on the GPU
+    calls, errors, start = [], [], threading.Barrier(len(sizes))
+    for v in sizes:
+        x, idx, tlp = rows(n, v, k, torch.bfloat16, 11)
+        want = _ak.distill_topk_fwd(x, idx, tlp, mask, tail=True, want_grad=True)
+        out = [torch.empty_like(t) for t in (want[0], want[1], want[2], want[3])]
+        args = [_ak.ptr(t) for t in out] + [None, None, _ak.ptr(x), _ak.ptr(idx), _ak.ptr(tlp), _ak.ptr(mask), n, n, 0, v, v, k,
+                                            1.0, 0.0, 1, _ak.dtype_code(x),
+                                            _ak.status_ptr(device, "distill_topk")]
+        calls.append((args, out, want, (x, idx, tlp)))
+    torch.cuda.synchronize()
+
+    def work(args, out, want, _):
+        try:
+            stream = torch.cuda.Stream()
+            start.wait(timeout=60)
+            for _ in range(times):
+                _ak.call("ak_distill_topk_fwd", *args, stream.cuda_stream)
+            stream.synchronize()
+            assert torch.equal(out[1], want[1]) and torch.equal(out[3][mask], want[3][mask])
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=c) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    _ak.check_status(device)
