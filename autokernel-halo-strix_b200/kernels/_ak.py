@@ -450,7 +450,7 @@ def scale_by_device_scalar_(x: torch.Tensor, scale: torch.Tensor) -> torch.Tenso
     dev = require_cuda(x, scale)
     if not x.is_contiguous():
         raise ValueError("scale_by_device_scalar_: x must be contiguous")
-    s = f32_dense(scale)
+    s = f32_dense(scale.reshape(1))  # one element, or an error
     if x.numel():
         call_on(dev, "ak_scale_by_device_scalar", ptr(x), x.numel(), ptr(s), dtype_code(x), stream(dev))
     return x
