@@ -154,10 +154,15 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=1024)
-def _size_query(name: str, *dims: int) -> int:
+def _size_on(index: Optional[int], name: str, *dims: int) -> int:
     out = ctypes.c_size_t(0)
-    call(name, *dims, ctypes.byref(out))
+    call_on(torch.device("cuda", index) if index is not None else torch.device("cpu"), name, *dims, ctypes.byref(out))
     return int(out.value)
+
+
+def _size_query(device: torch.device, name: str, *dims: int) -> int:
+    """Bytes that `name` asks for on `device`, whose number of SMs may count; remembered."""
+    return _size_on(device.index, name, *dims)
 
 
 # ---------------------------------------------------------------------------
@@ -257,7 +262,7 @@ def rmsnorm_bwd(x: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, eps: float =
     M = x.numel() // N if N else 0
     dx = torch.empty_like(x)
     dw = torch.empty(N, dtype=dw_dtype, device=dev)
-    ws_bytes = _size_query("ak_rmsnorm_bwd_workspace_size", M, N)
+    ws_bytes = _size_query(dev, "ak_rmsnorm_bwd_workspace_size", M, N)
     ws = workspace(ws_bytes, dev)
     call("ak_rmsnorm_bwd", ptr(dx), ptr(dw), _DT[dw_dtype], ptr(ws), ws_bytes, ptr(dy), ptr(x), ptr(w), M, N,
          float(eps), dtype_code(x), dtype_code(w), stream(dev))
@@ -298,7 +303,7 @@ def fused_res_rmsnorm_bwd(hidden: torch.Tensor, w: torch.Tensor, grad_hidden: Op
     M = hidden.numel() // N if N else 0
     dx = torch.empty_like(hidden)
     dw = torch.empty(N, dtype=dw_dtype, device=dev)
-    ws_bytes = _size_query("ak_rmsnorm_bwd_workspace_size", M, N)
+    ws_bytes = _size_query(dev, "ak_rmsnorm_bwd_workspace_size", M, N)
     ws = workspace(ws_bytes, dev)
     call("ak_fused_res_rmsnorm_bwd", ptr(dx), ptr(dw), _DT[dw_dtype], ptr(ws), ws_bytes, ptr(gh), ptr(gn),
          ptr(hidden), ptr(w), M, N, float(eps), dtype_code(hidden), dtype_code(w), stream(dev))
@@ -344,7 +349,7 @@ def rmsnorm_bwd_mixed(x: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, eps: f
     dx = torch.empty_like(x)
     dx2 = torch.empty_like(dy) if want_lo else None
     dw = torch.empty(N, dtype=torch.float32, device=dev)
-    ws_bytes = _size_query("ak_rmsnorm_bwd_workspace_size", M, N)
+    ws_bytes = _size_query(dev, "ak_rmsnorm_bwd_workspace_size", M, N)
     ws = workspace(ws_bytes, dev)
     call("ak_rmsnorm_bwd_mixed", ptr(dx), ptr(dx2), ptr(dw), F32, ptr(ws), ws_bytes, ptr(gh), ptr(dy),
          dtype_code(dy), ptr(x), dtype_code(x), ptr(w), dtype_code(w), M, N, float(eps), stream(dev))
@@ -727,7 +732,7 @@ def linear_ce_logits_grad(hidden, weight, labels, ignore_index=-100):
     loss = torch.empty((), dtype=torch.float32, device=dev)
     lse = torch.empty(N, dtype=torch.float32, device=dev)
     G = torch.empty(N, V, dtype=h.dtype, device=dev)
-    ws_bytes = _size_query("ak_linear_ce_logits_grad_workspace_size", N, V)
+    ws_bytes = _size_query(dev, "ak_linear_ce_logits_grad_workspace_size", N, V)
     ws = workspace(ws_bytes, dev)
     call("ak_linear_ce_logits_grad", ptr(loss), ptr(lse), ptr(G), ptr(ws), ws_bytes, ptr(h), ptr(w), ptr(lab), N, D,
          V, int(ignore_index), dtype_code(h), status_ptr(dev, "linear_ce"), stream(dev))
@@ -750,7 +755,7 @@ def linear_ce_fwdbwd(hidden, weight, labels, ignore_index=-100, need_dh=True, ne
     lse = torch.empty(N, dtype=torch.float32, device=dev)
     dH = torch.empty_like(h) if need_dh else None
     dW = torch.empty_like(w) if need_dw else None
-    ws_bytes = _size_query("ak_linear_ce_workspace_size", N, D, V)
+    ws_bytes = _size_query(dev, "ak_linear_ce_workspace_size", N, D, V)
     ws = workspace(ws_bytes, dev)
     if inv_valid is not None:
         inv_valid = inv_valid.reshape(1).to(torch.float32).contiguous()
@@ -771,7 +776,7 @@ def linear_logprobs_fwd(hidden, weight, targets, temperature=1.0, softcap=0.0, i
     ent = torch.empty(N, **f32) if want_entropy else None
     lse = torch.empty(N, **f32)
     stats = torch.empty(N, 4, **f32) if want_stats else None
-    ws_bytes = _size_query("ak_linear_logprobs_workspace_size", N, D, V, 0)
+    ws_bytes = _size_query(dev, "ak_linear_logprobs_workspace_size", N, D, V, 0)
     ws = workspace(ws_bytes, dev)
     call_on(dev, "ak_linear_logprobs_fwd", ptr(lp), ptr(ent), ptr(lse), ptr(stats), ptr(ws), ws_bytes, ptr(hidden),
             ptr(weight), ptr(targets), N, D, V, temperature, softcap, ignore_index, dtype_code(hidden),
@@ -788,7 +793,7 @@ def linear_logprobs_bwd(hidden, weight, targets, row_stats, g_logprobs, g_entrop
     dH = torch.empty_like(hidden) if need_dh else None
     dW = (torch.empty_like(weight) if N else torch.zeros_like(weight)) if need_dw else None
     glp, gent = f32_dense(g_logprobs), f32_dense(g_entropy)
-    ws_bytes = _size_query("ak_linear_logprobs_workspace_size", N, D, V, 1)
+    ws_bytes = _size_query(dev, "ak_linear_logprobs_workspace_size", N, D, V, 1)
     ws = workspace(ws_bytes, dev)
     call_on(dev, "ak_linear_logprobs_bwd", ptr(dH), ptr(dW), ptr(ws), ws_bytes, ptr(hidden), ptr(weight),
             ptr(targets), ptr(row_stats), ptr(glp), ptr(gent), N, D, V, temperature, softcap,
@@ -844,7 +849,7 @@ def scan1_fwd(dA, dBx, C, D, x, save_carries: bool = False):
     y = torch.empty_like(dA)
     carries = None
     if save_carries:
-        nbytes = _size_query("ak_scan1_carries_size", B, L, d)
+        nbytes = _size_query(dev, "ak_scan1_carries_size", B, L, d)
         carries = torch.empty(max(nbytes // 4, 1), dtype=torch.float32, device=dev)
     call("ak_scan1_fwd_ex", ptr(y), ptr(carries), ptr(dA), ptr(dBx), ptr(C), ptr(D), ptr(x), B, L, d, stream(dev))
     return (y, carries) if save_carries else y
@@ -859,12 +864,12 @@ def scan1_bwd(dA, dBx, C, D, x, gy, carries=None):
     gdA, gdBx, gC, gx = (torch.empty_like(dA) for _ in range(4))
     gD = torch.empty(d, dtype=torch.float32, device=dev)
     if carries is not None:
-        need = _size_query("ak_scan1_carries_size", B, L, d)
+        need = _size_query(dev, "ak_scan1_carries_size", B, L, d)
         if carries.dtype != torch.float32 or not carries.is_contiguous() or carries.numel() * 4 < need:
             raise ValueError("scan1_bwd: carries do not match this shape (use scan1_fwd(save_carries=True))")
         ws_bytes = max(B * d * 4, 4)
     else:
-        ws_bytes = _size_query("ak_scan1_bwd_workspace_size", B, L, d)
+        ws_bytes = _size_query(dev, "ak_scan1_bwd_workspace_size", B, L, d)
     ws = workspace(ws_bytes, dev)
     call("ak_scan1_bwd_ex", ptr(gdA), ptr(gdBx), ptr(gC), ptr(gD), ptr(gx), ptr(ws), ws_bytes, ptr(carries),
          ptr(dA), ptr(dBx), ptr(C), ptr(D), ptr(x), ptr(gy), B, L, d, stream(dev))
@@ -942,7 +947,7 @@ def selective_scan_bwd(dout, u, delta, A, B, C, D, z, delta_bias, delta_softplus
     dD = torch.empty(dim, **f32) if D is not None else None
     dz = torch.empty_like(u) if z is not None else None
     dbias = torch.empty(dim, **f32) if delta_bias is not None else None
-    ws_bytes = _size_query("ak_selective_scan_bwd_workspace_size", batch, dim, L, N, G)
+    ws_bytes = _size_query(dev, "ak_selective_scan_bwd_workspace_size", batch, dim, L, N, G)
     ws = workspace(ws_bytes, dev)
     call("ak_selective_scan_bwd", ptr(du), ptr(ddelta), ptr(dA), ptr(dB), ptr(dC), ptr(dD), ptr(dz), ptr(dbias),
          ptr(ws), ws_bytes, ptr(dout), ptr(u), ptr(delta), ptr(A), ptr(B4), ptr(C4), ptr(D), ptr(z),
@@ -986,7 +991,7 @@ def causal_conv1d_bwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torc
     dx = torch.empty_like(x)
     dw = torch.empty(D, K, dtype=torch.float32, device=dev)
     db = torch.empty(D, dtype=torch.float32, device=dev) if bias is not None else None
-    ws_bytes = _size_query("ak_causal_conv1d_bwd_workspace_size", B, D, T, K)
+    ws_bytes = _size_query(dev, "ak_causal_conv1d_bwd_workspace_size", B, D, T, K)
     ws = workspace(ws_bytes, dev)
     call("ak_causal_conv1d_bwd", ptr(dx), ptr(dw), ptr(db), ptr(ws), ws_bytes, ptr(x), ptr(w32), ptr(b32), ptr(dy), B, D, T, K, int(bool(silu)), dtype_code(x),
          stream(dev))

@@ -26,3 +26,30 @@ def test_a_scale_of_one_element_is_taken(monkeypatch, scale):
     s, args = seen
     assert s.dtype == torch.float32 and s.numel() == 1 and s.item() == 2.0
     assert args[2] == s.data_ptr() and args[1] == 4
+
+
+def test_sizes_are_remembered_for_each_device(monkeypatch):
+    """A size may depend on the device's SMs: what one device was told is not the other's answer, and
+    the question is put with the device of the tensors current."""
+    asked = []
+
+    def answer(device, name, *args):
+        asked.append((device.index, name, args[:-1]))
+        args[-1]._obj.value = 100 * (device.index or 0) + args[0]
+
+    monkeypatch.setattr(_ak, "call_on", answer)
+    _ak._size_on.cache_clear()
+    try:
+        for _ in range(2):
+            for index in (0, 1):
+                assert _ak._size_query(torch.device("cuda", index), "ak_rmsnorm_bwd_workspace_size", 7, 64) == 100 * index + 7
+        assert asked == [(i, "ak_rmsnorm_bwd_workspace_size", (7, 64)) for i in (0, 1)]
+    finally:
+        _ak._size_on.cache_clear()
+
+
+def test_sizes_come_from_the_library():
+    n = _ak._size_query(torch.device("cpu"), "ak_linear_logprobs_workspace_size", 8, 64, 100, 0)
+    assert n > 8 * 2 * 12
+    with pytest.raises(_ak.AkError):
+        _ak._size_query(torch.device("cpu"), "ak_linear_logprobs_workspace_size", 8, 0, 100, 0)
