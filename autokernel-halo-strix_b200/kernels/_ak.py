@@ -15,6 +15,7 @@ from pathlib import Path
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "libak_b200.so"
 
@@ -147,6 +148,16 @@ def require_cuda(*tensors: Optional[torch.Tensor]) -> torch.device:
     if dev is None:
         raise RuntimeError("no tensor given")
     return dev
+
+
+def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode derivatives are not formed.  A dual input is refused where the library is called
+    directly, as an autograd function without a jvp refuses it; its tangent would be lost."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -128,6 +128,7 @@ class _CrossEntropyHIP(torch.autograd.Function):
 
 def kernel_fn(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """Mean CE over rows with target != -100 (reference.cross_entropy_ref semantics)."""
+    _ak.refuse_tangents("ce_fused", logits)
     assert logits.is_cuda and targets.is_cuda
     if not (logits.requires_grad and torch.is_grad_enabled()):
         losses, lse, _, _, _ = _ak.ce_rows_fwd(logits, targets, 0.0, -100, 0.0)

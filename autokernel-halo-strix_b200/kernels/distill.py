@@ -78,6 +78,7 @@ def distill_topk(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_lo
     """
     what = "distill_topk"
     _ak.dtype_code(logits)
+    _ak.refuse_tangents(what, logits, teacher_logprobs)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"{what}: logits must be (..., V) with V >= 1, got {tuple(logits.shape)}")
     lead = logits.shape[:-1]

@@ -111,6 +111,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     """
     what = "token_logprobs"
     _ak.dtype_code(logits)
+    _ak.refuse_tangents(what, logits)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"{what}: logits must be (..., V) with V >= 1, got {tuple(logits.shape)}")
     if targets is not None:
@@ -176,6 +177,7 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: O
     finite where a gradient of weight is wanted (they enter it times 0).
     """
     what = "linear_token_logprobs"
+    _ak.refuse_tangents(what, hidden, weight)
     if hidden.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"{what}: hidden must be bfloat16 or float16, got {hidden.dtype}")
     _ak.dtype_code(weight)

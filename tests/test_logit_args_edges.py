@@ -29,3 +29,27 @@ def test_temperatures_too_low_for_fp32_are_refused(monkeypatch):
                                        0.0, 0, 1, None, None) == 1
         assert lib.ak_linear_logprobs_fwd(None, None, fake, None, fake, 1 << 20, fake, fake, None, 8, 64, 100, T, 0.0,
                                           -100, 1, None, None) == 1
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """Without requires_grad nothing else would stop a dual input, whose tangent the library drops."""
+    from kernels import ce_fused
+    from kernels.distill import distill_topk
+    on_gpu(monkeypatch)
+    monkeypatch.setattr(_ak, "call", lambda *a: pytest.fail("launched"))
+    monkeypatch.setattr(_ak, "call_on", lambda *a: pytest.fail("launched"))
+    ad = torch.autograd.forward_ad
+    x, t = torch.randn(2, 8), torch.zeros(2, dtype=torch.long)
+    h, w = torch.randn(2, 8, dtype=torch.bfloat16), torch.randn(9, 8, dtype=torch.bfloat16)
+    idx, lp = torch.zeros(2, 3, dtype=torch.long), torch.full((2, 3), -1.5)
+    with ad.dual_level():
+        def dual(a):
+            return ad.make_dual(a, torch.ones_like(a))
+        for call in (lambda: TL.token_logprobs(dual(x), t), lambda: TL.token_logprobs(dual(x), top_k=2),
+                     lambda: TL.linear_token_logprobs(dual(h), w, t), lambda: TL.linear_token_logprobs(h, dual(w), t),
+                     lambda: distill_topk(dual(x), idx, lp), lambda: distill_topk(x, idx, dual(lp)),
+                     lambda: ce_fused.kernel_fn(dual(x), t)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        _ak.refuse_tangents("an input without a tangent", x, None)
