@@ -1490,7 +1490,7 @@ int logp_fwd(float* logprobs, float* entropy, float* lse, float4* stats, const L
 }
 
 template <typename T>
-int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, const int64_t* labels,
+int logp_bwd(void* dH, void* dW, bool dw_f32, const LogpWs& w, const void* H, const void* W, const int64_t* labels,
              const float4* stats, const float* g_lp, const float* g_ent, int64_t N, int64_t D, int64_t V,
              const Squash& q, int64_t ignore_index, int* status, cudaStream_t st) {
   const int64_t Nc = chunk_rows(N), ldg = (V + 7) / 8 * 8;
@@ -1535,7 +1535,9 @@ int logp_bwd(void* dH, void* dW, const LogpWs& w, const void* H, const void* W, 
       P.epi = EPI_STORE;
       P.ldc = D;
       P.scale = scale;
-      if (first && last) {
+      if (dw_f32) {  // the chunks add up in the result itself
+        P.C = dW; P.c_f32 = 1; P.accumulate = first ? 0 : 1;
+      } else if (first && last) {
         P.C = dW;
       } else if (!last) {
         P.C = w.dWacc; P.c_f32 = 1; P.accumulate = first ? 0 : 1;
@@ -1750,9 +1752,20 @@ extern "C" int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_
                                       const float* g_logprobs, const float* g_entropy, int64_t N, int64_t D, int64_t V,
                                       float temperature, float softcap, int64_t ignore_index, int dt, int* status,
                                       void* stream) {
+  return ak_linear_logprobs_bwd_ex(dH, dW, dt, workspace, ws_bytes, H, W, targets, row_stats, g_logprobs, g_entropy, N,
+                                   D, V, temperature, softcap, ignore_index, dt, status, stream);
+}
+
+extern "C" int ak_linear_logprobs_bwd_ex(void* dH, void* dW, int dt_dw, void* workspace, size_t ws_bytes,
+                                         const void* H, const void* W, const int64_t* targets, const float* row_stats,
+                                         const float* g_logprobs, const float* g_entropy, int64_t N, int64_t D,
+                                         int64_t V, float temperature, float softcap, int64_t ignore_index, int dt,
+                                         int* status, void* stream) {
   clear_error();
   const int rc = check_logp("ak_linear_logprobs_bwd", H, W, N, D, V, temperature, softcap, dt);
   if (rc) return rc;
+  AK_REQUIRE(dt_dw == dt || dt_dw == AK_F32, AK_ERR_DTYPE,
+             "ak_linear_logprobs_bwd: dW must be fp32 or of the hidden states' type");
   if (N == 0 || (!dH && !dW)) return AK_OK;
   AK_REQUIRE(row_stats && aligned16(row_stats), AK_ERR_ARG,
              "ak_linear_logprobs_bwd: null pointer, or row_stats not 16-byte aligned");
@@ -1765,6 +1778,6 @@ extern "C" int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_
   const LogpWs w = carve_logp(base, N, D, V, true);
   const Squash q = make_squash(temperature, softcap);
   auto fn = dt == AK_BF16 ? logp_bwd<__nv_bfloat16> : logp_bwd<__half>;
-  return fn(dH, dW, w, H, W, targets, reinterpret_cast<const float4*>(row_stats), g_logprobs, g_entropy, N, D, V, q,
+  return fn(dH, dW, dt_dw == AK_F32, w, H, W, targets, reinterpret_cast<const float4*>(row_stats), g_logprobs, g_entropy, N, D, V, q,
             ignore_index, status, (cudaStream_t)stream);
 }

@@ -56,6 +56,7 @@ SIGNATURES = {
     "ak_linear_logprobs_workspace_size": [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)],
     "ak_linear_logprobs_fwd": [_vp] * 5 + [_sz] + [_vp] * 3 + [_i64] * 3 + [_f, _f, _i64, _i, _vp, _vp],
     "ak_linear_logprobs_bwd": [_vp] * 3 + [_sz] + [_vp] * 6 + [_i64] * 3 + [_f, _f, _i64, _i, _vp, _vp],
+    "ak_linear_logprobs_bwd_ex": [_vp, _vp, _i, _vp, _sz] + [_vp] * 6 + [_i64] * 3 + [_f, _f, _i64, _i, _vp, _vp],
     "ak_linear_ce_logits_grad_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
     "ak_linear_ce_logits_grad": [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp],
     "ak_linear_ce_workspace_size": [_i64, _i64, _i64, ctypes.POINTER(_sz)],
@@ -796,17 +797,19 @@ def linear_logprobs_fwd(hidden, weight, targets, temperature=1.0, softcap=0.0, i
 
 
 def linear_logprobs_bwd(hidden, weight, targets, row_stats, g_logprobs, g_entropy, temperature=1.0,
-                        softcap=0.0, ignore_index=-100, need_dh=True, need_dw=True):
-    """Returns (dH or None, dW or None) from the gradients of logprobs and entropy (either may be None)."""
+                        softcap=0.0, ignore_index=-100, need_dh=True, need_dw=True, dw_dtype=None):
+    """Returns (dH or None, dW or None) from the gradients of logprobs and entropy (either may be None);
+    dW in dw_dtype, fp32 or (default) weight's."""
     dev = require_cuda(hidden, weight, targets, row_stats, g_logprobs, g_entropy)
     N, D = hidden.shape
     V = weight.shape[0]
     dH = torch.empty_like(hidden) if need_dh else None
-    dW = (torch.empty_like(weight) if N else torch.zeros_like(weight)) if need_dw else None
+    dw_dtype = dw_dtype or weight.dtype
+    dW = (torch.empty_like(weight, dtype=dw_dtype) if N else torch.zeros_like(weight, dtype=dw_dtype)) if need_dw else None
     glp, gent = f32_dense(g_logprobs), f32_dense(g_entropy)
     ws_bytes = _size_query(dev, "ak_linear_logprobs_workspace_size", N, D, V, 1)
     ws = workspace(ws_bytes, dev)
-    call_on(dev, "ak_linear_logprobs_bwd", ptr(dH), ptr(dW), ptr(ws), ws_bytes, ptr(hidden), ptr(weight),
+    call_on(dev, "ak_linear_logprobs_bwd_ex", ptr(dH), ptr(dW), _DT[dw_dtype], ptr(ws), ws_bytes, ptr(hidden), ptr(weight),
             ptr(targets), ptr(row_stats), ptr(glp), ptr(gent), N, D, V, temperature, softcap,
             ignore_index, dtype_code(hidden), status_ptr(dev, "linear_logprobs"), stream(dev))
     return dH, dW

@@ -135,8 +135,10 @@ def _linear_token_logprobs_backward(ctx, g_lp, g_ent):
     if g_lp is None and g_ent is None:
         return (None,) * 7
     hidden, w, targets, stats = ctx.saved_tensors
+    # a weight of another type than hidden's has its gradient rounded from fp32 to that type, if at all
     dh, dw = _ak.linear_logprobs_bwd(hidden, w, targets, stats, g_lp, g_ent, *ctx.args,
-                                     need_dh=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
+                                     need_dh=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1],
+                                     dw_dtype=w.dtype if ctx.weight_dtype == w.dtype else torch.float32)
     return (dh, dw.to(ctx.weight_dtype) if dw is not None else None) + (None,) * 5
 
 
@@ -171,7 +173,7 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: O
     """`token_logprobs(hidden @ weight.T, targets, ...)` without the logits and without alternatives.
 
     hidden (..., D): bf16 or fp16 on the GPU, D a multiple of 8; weight (V, D): cast to hidden's type
-    if it has another.  The log-probabilities are of the fp32 accumulators: nothing between the
+    if it has another (its gradient is rounded to its own type only; an fp32 weight's is not).  The log-probabilities are of the fp32 accumulators: nothing between the
     products and the result is rounded to 16 bits.  In the backward the gradient of the logits is, as
     the operand of the two products that follow.  The hidden states of ignored rows have to be
     finite where a gradient of weight is wanted (they enter it times 0).

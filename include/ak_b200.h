@@ -338,6 +338,15 @@ AK_API int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_t ws
                                   float temperature, float softcap, int64_t ignore_index, int dt,
                                   int* status, void* stream);
 
+/* The same with dW in dt_dw: dt, or fp32 for a weight that is kept in fp32 (its gradient is then the
+ * accumulators', not rounded to 16 bits). */
+AK_API int ak_linear_logprobs_bwd_ex(void* dH, void* dW, int dt_dw, void* workspace,
+                                     size_t ws_bytes, const void* H, const void* W,
+                                     const int64_t* targets, const float* row_stats,
+                                     const float* g_logprobs, const float* g_entropy, int64_t N,
+                                     int64_t D, int64_t V, float temperature, float softcap,
+                                     int64_t ignore_index, int dt, int* status, void* stream);
+
 /* ------------------------------------------------------------------------ *
  * Collapsed (single-state) selective scan, fp32, layout (B, L, d)
  * ------------------------------------------------------------------------ */

@@ -53,3 +53,18 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
                 with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
                     call()
         _ak.refuse_tangents("an input without a tangent", x, None)
+
+
+def test_the_type_of_a_weight_gradient():
+    lib, n = _ak.lib(), ctypes.c_size_t(0)
+    fake = ctypes.c_void_p(256)  # never dereferenced: each call fails its checks first
+    assert lib.ak_linear_logprobs_workspace_size(8, 64, 100, 1, ctypes.byref(n)) == 0
+
+    def bwd(dt_dw, dt=1, rows=8, dW=fake):
+        return lib.ak_linear_logprobs_bwd_ex(fake, dW, dt_dw, fake, n, fake, fake, fake, fake, fake, None, rows, 64, 100,
+                                             1.0, 0.0, -100, dt, None, None)
+
+    assert bwd(2) == 2 and bwd(1, dt=2) == 2 and bwd(7) == 2 and bwd(0, dt=0) == 2
+    assert bwd(0, dW=ctypes.c_void_p(264)) == 1
+    for dt_dw in (0, 1):
+        assert bwd(dt_dw, rows=0) == 0
