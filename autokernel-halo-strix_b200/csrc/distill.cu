@@ -997,7 +997,8 @@ int check_args(const char* what, const void* logits, int64_t rows, int64_t inner
              "%s: a row of %lld elements does not fit the shared memory of %d CTAs", what, (long long)V, kMaxCluster);
   AK_REQUIRE(temperature >= kLowestTemperature && temperature < INFINITY, AK_ERR_ARG,
              "%s: temperature must be at least 2^-100 and finite", what);
-  AK_REQUIRE(softcap >= 0.f && softcap < INFINITY, AK_ERR_ARG, "%s: softcap must be >= 0 and finite", what);
+  AK_REQUIRE(softcap == 0.f || (softcap >= kLowestSoftcap && softcap < INFINITY), AK_ERR_ARG,
+             "%s: softcap must be 0, or at least 2^-100 and finite", what);
   AK_REQUIRE(rows == 0 || logits, AK_ERR_ARG, "%s: null pointer", what);
   AK_REQUIRE((reinterpret_cast<uintptr_t>(logits) % elem_size(dt)) == 0, AK_ERR_ARG,
              "%s: logits not aligned to their type", what);

@@ -1601,7 +1601,8 @@ int check_logp(const char* what, const void* H, const void* W, int64_t N, int64_
              (long long)N, (long long)D, (long long)V);
   AK_REQUIRE(temperature >= kLowestTemperature && temperature < INFINITY, AK_ERR_ARG,
              "%s: temperature must be at least 2^-100 and finite", what);
-  AK_REQUIRE(softcap >= 0.f && softcap < INFINITY, AK_ERR_ARG, "%s: softcap must be >= 0 and finite", what);
+  AK_REQUIRE(softcap == 0.f || (softcap >= kLowestSoftcap && softcap < INFINITY), AK_ERR_ARG,
+             "%s: softcap must be 0, or at least 2^-100 and finite", what);
   AK_REQUIRE(N == 0 || (H && W && aligned16(H) && aligned16(W)), AK_ERR_ARG,
              "%s: hidden states and weight must be 16-byte aligned", what);
   return AK_OK;

@@ -25,7 +25,8 @@ struct RowAddr {
 // What a logit x means: y = softcap(x), log-probabilities of y / temperature.
 // kl = log2(e) / temperature turns a difference of y into an exponent of 2.
 // -inf stays -inf under softcap: a masked token has no probability there either.
-// temperature >= kLowestTemperature: its reciprocal and products with raise_floor stay finite.
+// temperature >= kLowestTemperature: its reciprocal and products with raise_floor stay finite; so does
+// the reciprocal of a softcap >= kLowestSoftcap.
 struct Squash {
   float cap, inv_cap, inv_t, kl;
   float rkl;   // 1 / kl
@@ -33,7 +34,7 @@ struct Squash {
   float near;  // softcap by the polynomial up to this |x|
 };
 
-constexpr float kLowestTemperature = 7.888609052210118e-31f;  // 2^-100
+constexpr float kLowestTemperature = 7.888609052210118e-31f, kLowestSoftcap = kLowestTemperature;  // 2^-100
 
 inline Squash make_squash(float temperature, float softcap) {
   Squash q;

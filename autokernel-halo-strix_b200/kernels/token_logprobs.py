@@ -24,7 +24,7 @@ KERNEL_TYPE = "token_logprobs"
 BACKEND = "cuda_sm100a"
 
 MAX_TOP_K = 128
-LOWEST_TEMPERATURE = 2.0 ** -100
+LOWEST_TEMPERATURE = LOWEST_SOFTCAP = 2.0 ** -100
 
 
 class TokenLogprobs(NamedTuple):
@@ -75,8 +75,8 @@ def check_scales(what: str, temperature: float, softcap: float):
     temperature, softcap = float(temperature), float(softcap)
     if not (temperature >= LOWEST_TEMPERATURE and math.isfinite(temperature)):
         raise ValueError(f"{what}: temperature must be at least 2^-100 and finite, got {temperature}")
-    if not (softcap >= 0.0 and math.isfinite(softcap)):
-        raise ValueError(f"{what}: softcap must be >= 0 (0: none) and finite, got {softcap}")
+    if not (softcap == 0.0 or (softcap >= LOWEST_SOFTCAP and math.isfinite(softcap))):
+        raise ValueError(f"{what}: softcap must be 0 (none), or at least 2^-100 and finite, got {softcap}")
     return temperature, softcap
 
 
@@ -104,7 +104,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     top_k: alternatives per row, at most 128 (of at most 1,048,320 tokens): `top_logprobs` and `top_indices` (..., top_k), most
     likely first, equal logits by lowest index.  They and `lse` carry no gradient.
     entropy: whether to compute the entropy (nats).
-    temperature: at least 2^-100.
+    temperature: at least 2^-100; softcap: 0 for none, or at least 2^-100.
 
     -inf logits are tokens without probability.  A row of nothing else has log-probabilities -inf,
     entropy 0 and no gradient; a row with NaN is NaN.

@@ -180,7 +180,7 @@ AK_API int ak_scale_by_device_scalar(void* x, int64_t n, const float* scale, int
  * ------------------------------------------------------------------------ */
 
 /* For each row x of logits: y = softcap(x) / temperature (softcap(x) = c tanh(x / c),
- * c = softcap; 0 leaves x; -inf stays -inf; temperature >= 2^-100), lse = log sum exp y, p = exp(y - lse):
+ * c = softcap; 0 leaves x; -inf stays -inf; temperature and a softcap >= 2^-100), lse = log sum exp y, p = exp(y - lse):
  *   logprobs[rows]  y_target - lse; 0 where target == ignore_index, NaN where it is no token
  *   entropy[rows]   -sum p log p; 0 where target == ignore_index
  *   lse[rows]

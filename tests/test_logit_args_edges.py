@@ -68,3 +68,18 @@ def test_the_type_of_a_weight_gradient():
     assert bwd(0, dW=ctypes.c_void_p(264)) == 1
     for dt_dw in (0, 1):
         assert bwd(dt_dw, rows=0) == 0
+
+
+def test_softcaps_too_low_for_fp32_are_refused(monkeypatch):
+    on_gpu(monkeypatch)
+    lib = _ak.lib()
+    fake = ctypes.c_void_p(256)  # never dereferenced: each call fails its checks first
+    for cap in (1e-31, 1e-39, 1e-45):
+        with pytest.raises(ValueError, match="2\\^-100"):
+            TL.token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.long), softcap=cap)
+        assert lib.ak_token_logprobs_fwd(fake, None, fake, None, None, None, fake, fake, 2, 2, 0, 64, 64, 0, 1.0, cap, -100,
+                                         1, None) == 1
+        assert lib.ak_distill_topk_fwd(fake, fake, None, None, None, None, fake, fake, fake, None, 2, 2, 0, 64, 64, 3,
+                                       1.0, cap, 0, 1, None, None) == 1
+        assert lib.ak_linear_logprobs_fwd(None, None, fake, None, fake, 1 << 20, fake, fake, None, 8, 64, 100, 1.0, cap,
+                                          -100, 1, None, None) == 1
