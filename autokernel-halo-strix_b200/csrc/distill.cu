@@ -91,15 +91,18 @@ __device__ __forceinline__ float grad_scale(const DistillArgs& a) {
 }
 
 // The gradient at a logit outside the teacher's tokens.  c = 0 gives 0 whatever x is.
-template <bool CAP>
-__device__ __forceinline__ float rest_grad(float x, const Ref& ref, float c, const Squash& q) {
+template <int CAP>
+__device__ __forceinline__ float rest_grad_at(float y, const Ref& ref, float c, const Squash& q) {  // y: squashed
   if (c == 0.f) return 0.f;
-  const float y = CAP ? squash_far(x, q) : x;
   return ex2(exponent(y, ref, q)) * c * squash_slope<CAP>(y, q);
+}
+template <int CAP>
+__device__ __forceinline__ float rest_grad(float x, const Ref& ref, float c, const Squash& q) {
+  return rest_grad_at<CAP>(squash<CAP>(x, q), ref, c, q);
 }
 
 // The same for the values of NW words, two at a time where it can.
-template <typename T, bool CAP, int NW>
+template <typename T, int CAP, int NW>
 __device__ __forceinline__ void rest_grads(float* x, const uint32_t (&w)[NW], const Ref& ref, float c, const Squash& q) {
   constexpr int P = NW * elems_per_word<T>() / 2;
   const float2 kl = both(q.kl), nk = both(-ref.k), c2 = both(c);
@@ -124,14 +127,14 @@ __device__ __forceinline__ void rest_grads(float* x, const uint32_t (&w)[NW], co
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const float2 v = word_pair<T>(w, i);
-      x[2 * i] = rest_grad<CAP>(v.x, ref, c, q);
-      x[2 * i + 1] = rest_grad<CAP>(v.y, ref, c, q);
+      x[2 * i] = rest_grad_at<CAP>(CAP ? squash_far<CAP>(v.x, q) : v.x, ref, c, q);
+      x[2 * i + 1] = rest_grad_at<CAP>(CAP ? squash_far<CAP>(v.y, q) : v.y, ref, c, q);
     }
   }
 }
 
 // The gradients of one 16-byte vector, rounded to T and stored.
-template <typename T, bool CAP>
+template <typename T, int CAP>
 __device__ __forceinline__ void store_grads(T* out, const uint4& f, const Ref& ref, float c, const Squash& q, bool vec) {
   constexpr int VEC = 16 / sizeof(T);
   const uint32_t w[4] = {f.x, f.y, f.z, f.w};
@@ -307,12 +310,12 @@ struct Teacher {
   float q[kSlots], logq[kSlots], y[kSlots], mass[kSlots];
   float rest, total;
   bool none, bad;
-  template <bool CAP>
+  template <int CAP>
   __device__ __forceinline__ void work(RowStats<CAP, false>& top, Picked& p, bool twice, const DistillArgs& a, int* s_idx,
                                        float* s_q);
 };
 
-template <bool CAP>
+template <int CAP>
 __device__ __forceinline__ void Teacher::work(RowStats<CAP, false>& top, Picked& p, bool twice, const DistillArgs& a,
                                               int* s_idx, float* s_q) {
   const int lane = threadIdx.x & 31;
@@ -396,7 +399,7 @@ __device__ __forceinline__ void Teacher::work(RowStats<CAP, false>& top, Picked&
 }
 
 // A row's coefficients from the statistics of the rest and of the teacher's tokens.
-template <bool CAP>
+template <int CAP>
 __device__ __forceinline__ FinishRow coefficients(const RowStats<CAP, false>& st, const RowStats<CAP, false>& top,
                                                   float rest, float total, bool none, bool bad, const Squash& q) {
   RowStats<CAP, false> all = st;
@@ -425,7 +428,7 @@ __device__ __forceinline__ FinishRow coefficients(const RowStats<CAP, false>& st
 }
 
 // One entry's term of the loss, added to it, and its token's gradient before the scale.
-template <bool CAP>
+template <int CAP>
 __device__ __forceinline__ float entry_grad(float& loss, int idx, float qk, float logq, float y, float mass,
                                             const FinishRow& f, bool none, bool bad, const Squash& q) {
   const float lpk = (f.empty || y == -INFINITY) ? -INFINITY : log_prob(y, f.all, f.logs, q);
@@ -434,7 +437,7 @@ __device__ __forceinline__ float entry_grad(float& loss, int idx, float qk, floa
   return (idx >= 0 && !none && !f.empty) ? fmaf(f.mass, expf(lpk), -mass) * squash_slope<CAP>(y, q) : 0.f;
 }
 
-template <typename T, bool CAP, bool GRAD, int W>
+template <typename T, int CAP, bool GRAD, int W>
 __global__ void __launch_bounds__(32 * (W + kRoles), W == kWide ? 2 : 4)
 distill_fwd_kernel(const T* __restrict__ logits, const DistillArgs a) {
   using Stats = RowStats<CAP, false>;
@@ -729,7 +732,7 @@ constexpr int kRowWarps = 8;
 
 __host__ __device__ constexpr int warp_row_bytes(int bytes) { return (bytes + 15) / 16 * 16; }
 
-template <typename T, bool CAP, bool GRAD>
+template <typename T, int CAP, bool GRAD>
 __global__ void __launch_bounds__(32 * kRowWarps, 3)
 distill_warp_kernel(const T* __restrict__ logits, const DistillArgs a) {
   using Stats = RowStats<CAP, false>;
@@ -877,7 +880,7 @@ constexpr int kBwdGroups = 32 * kBwdBatch;  // groups of one warp
 
 // The gradient from the forward's reference, c and K numbers a row: each warp takes one segment of a
 // row, then writes those of the teacher's tokens that lie in it.
-template <typename T, bool CAP>
+template <typename T, int CAP>
 __global__ void __launch_bounds__(kThreads)
 distill_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const DistillBwdArgs a) {
   const int tid = threadIdx.x & 31;
@@ -1007,9 +1010,8 @@ int check_args(const char* what, const void* logits, int64_t rows, int64_t inner
 
 template <typename T, int W>
 int launch_width(const T* logits, DistillArgs& a, int64_t share, cudaStream_t st) {
-  const bool cap = a.q.cap > 0.f;
-  auto kern = a.grad ? (cap ? distill_fwd_kernel<T, true, true, W> : distill_fwd_kernel<T, false, true, W>)
-                     : (cap ? distill_fwd_kernel<T, true, false, W> : distill_fwd_kernel<T, false, false, W>);
+  auto kern = distill_fwd_kernel<T, kNoCap, true, W>;
+  AK_DISPATCH_CAP(a.q, CAP, kern = a.grad ? distill_fwd_kernel<T, CAP, true, W> : distill_fwd_kernel<T, CAP, false, W>);
   const int cs = 1 << a.log_cs;
   a.piece = (uint32_t)((share + kPieces * 16 - 1) / (kPieces * 16) * 16);
   const size_t smem = (size_t)std::max<int64_t>(share, 16);
@@ -1031,10 +1033,9 @@ int launch_width(const T* logits, DistillArgs& a, int64_t share, cudaStream_t st
 
 template <typename T>
 int launch_fwd(const T* logits, DistillArgs& a, cudaStream_t st) {
-  const bool cap = a.q.cap > 0.f;
   if ((int64_t)a.V * (int64_t)sizeof(T) <= kShortBytes && a.rows >= 4 * sm_count()) {
-    auto kern = a.grad ? (cap ? distill_warp_kernel<T, true, true> : distill_warp_kernel<T, false, true>)
-                       : (cap ? distill_warp_kernel<T, true, false> : distill_warp_kernel<T, false, false>);
+    auto kern = distill_warp_kernel<T, kNoCap, true>;
+    AK_DISPATCH_CAP(a.q, CAP, kern = a.grad ? distill_warp_kernel<T, CAP, true> : distill_warp_kernel<T, CAP, false>);
     const size_t smem = (size_t)kRowWarps * warp_row_bytes(a.V * (int)sizeof(T));
     AK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowWarps * kShortBytes),
                 "ak_distill_topk_fwd: shared memory");
@@ -1118,9 +1119,9 @@ extern "C" int ak_distill_topk_bwd(void* grad, const void* logits, const int64_t
   a.segs = (int)std::max<int64_t>(1, (V / kGroup + kBwdGroups - 1) / kBwdGroups);
   a.q = make_squash(temperature, softcap);
   AK_REQUIRE(rows * a.segs < (1LL << 32) - 8, AK_ERR_SHAPE, "ak_distill_topk_bwd: too many rows");
-  const bool cap = a.q.cap > 0.f;
   AK_DISPATCH_DTYPE(dt, T, {
-    auto kern = cap ? distill_bwd_kernel<T, true> : distill_bwd_kernel<T, false>;
+    auto kern = distill_bwd_kernel<T, kNoCap>;
+    AK_DISPATCH_CAP(a.q, CAP, kern = distill_bwd_kernel<T, CAP>);
     kern<<<(unsigned)((rows * a.segs + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, (cudaStream_t)stream>>>(
         (T*)grad, (const T*)logits, a);
   });

@@ -589,8 +589,8 @@ __device__ __forceinline__ void epi_store(const Prob& P, uint32_t tbase, int row
 }
 
 // One 32-column chunk into a row's statistics; columns from P.N on hold nothing.
-template <bool CAP, bool ENT>
-__device__ __forceinline__ void logp_chunk(const uint32_t (&v)[32], RowStats<true, true>& st, const Squash& q) {
+template <int CAP, bool ENT>
+__device__ __forceinline__ void logp_chunk(const uint32_t (&v)[32], RowStats<kCap, true>& st, const Squash& q) {
   RowStats<CAP, ENT> a;
   a.m = st.m; a.lim = st.lim; a.s = st.s; a.r = st.r;
   if constexpr (ENT) a.w = st.w;
@@ -608,7 +608,7 @@ __device__ __forceinline__ void epi_logp(const Prob& P, uint32_t tbase, int row0
   const int c0 = eg * kGroupCols;
   const Squash q = P.q;
   const bool cap = q.cap > 0.f, ent = P.want_ent != 0;
-  RowStats<true, true> st;
+  RowStats<kCap, true> st;
   st.init();
   Tm32 buf[2];
   __syncwarp();
@@ -632,10 +632,10 @@ __device__ __forceinline__ void epi_logp(const Prob& P, uint32_t tbase, int row0
       for (int j = 0; j < 32; ++j)
         if (cbase + j >= P.N) v[j] = __float_as_uint(-INFINITY);
     }
-    if (!cap && ent) logp_chunk<false, true>(v, st, q);
-    else if (!cap) logp_chunk<false, false>(v, st, q);
-    else if (ent) logp_chunk<true, true>(v, st, q);
-    else logp_chunk<true, false>(v, st, q);
+    if (!cap && ent) logp_chunk<kNoCap, true>(v, st, q);
+    else if (!cap) logp_chunk<kNoCap, false>(v, st, q);
+    else if (ent) logp_chunk<kWideCap, true>(v, st, q);
+    else logp_chunk<kWideCap, false>(v, st, q);
     if (k + 1 < kGroupCols / 32) tmem_ld_wait(buf[(k + 1) & 1]);
   }
   if (row < P.M)
@@ -714,16 +714,16 @@ __device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int
         const float d = exponent(y, lr.ref, q);
         float o = ex2(d) * fmaf(lr.c1, fmaxf(d, -1e4f), lr.c0);
         if (j == rel) o += lr.ct;
-        v[j] = o * squash_slope<true>(y, q);
+        v[j] = o * squash_slope<kCap>(y, q);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        const float y = squash_far(v[j], q);
+        const float y = squash_far<kWideCap>(v[j], q);
         const float d = exponent(y, lr.ref, q);
         float o = ex2(d) * fmaf(lr.c1, fmaxf(d, -1e4f), lr.c0);
         if (j == rel) o += lr.ct;
-        v[j] = o * squash_slope<true>(y, q);
+        v[j] = o * squash_slope<kCap>(y, q);
       }
     }
     if (P.C2 != nullptr && row < P.M) {
@@ -1047,7 +1047,7 @@ lce_grad_inplace(T* __restrict__ L, const float* __restrict__ lse, const int64_t
 // Merge the per-tile partials of a row (one CTA each) into its log-probability, entropy and lse.
 constexpr int kRowThreads = 128;
 
-template <bool CAP>
+template <int CAP>
 __global__ void __launch_bounds__(kRowThreads)
 logp_rows_reduce(float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ lse,
                  float4* __restrict__ stats, const float4* __restrict__ part, const float* __restrict__ tlogit,
@@ -1480,7 +1480,7 @@ int logp_fwd(float* logprobs, float* entropy, float* lse, float4* stats, const L
     P.q = q;
     const int rc = launch_group<T>(A, B, g, st);
     if (rc) return rc;
-    auto kern = q.cap > 0.f ? logp_rows_reduce<true> : logp_rows_reduce<false>;
+    auto kern = q.cap > 0.f ? logp_rows_reduce<kCap> : logp_rows_reduce<kNoCap>;
     kern<<<(unsigned)nr, kRowThreads, 0, st>>>(
         logprobs ? logprobs + r0 : nullptr, entropy ? entropy + r0 : nullptr, lse + r0, stats ? stats + r0 : nullptr,
         w.part, w.tlogit, P.labels, (int)V, nparts, ignore_index, q);

@@ -31,8 +31,12 @@ struct Squash {
   float cap, inv_cap, inv_t, kl;
   float rkl;   // 1 / kl
   float kc;    // -2 log2(e) / cap
-  float near;  // softcap by the polynomial up to this |x|
 };
+
+// What the kernels are instantiated for (CAP): no softcap, one, or one so wide that its far form has
+// to keep small logits as well.
+enum SoftcapForm : int { kNoCap = 0, kCap = 1, kWideCap = 2 };
+inline int cap_form(const Squash& q) { return q.cap == 0.f ? kNoCap : q.cap <= 64.f ? kCap : kWideCap; }
 
 constexpr float kLowestTemperature = 7.888609052210118e-31f, kLowestSoftcap = kLowestTemperature;  // 2^-100
 
@@ -44,10 +48,18 @@ inline Squash make_squash(float temperature, float softcap) {
   q.inv_t = 1.f / temperature;
   q.kl = (float)(1.4426950408889634 / (double)temperature);
   q.rkl = 1.f / q.kl;
-  // there products with kl stay finite
-  q.near = q.cap * q.kl < 1e30f ? q.cap : 0.f;
   return q;
 }
+
+// A statement with CAP as the constant that q's softcap stands for.
+#define AK_DISPATCH_CAP(q, CAP, ...)                                                  \
+  do {                                                                                \
+    switch (cap_form(q)) {                                                            \
+      case kNoCap: { constexpr int CAP = kNoCap; __VA_ARGS__; } break;                \
+      case kCap: { constexpr int CAP = kCap; __VA_ARGS__; } break;                    \
+      default: { constexpr int CAP = kWideCap; __VA_ARGS__; } break;                  \
+    }                                                                                 \
+  } while (0)
 
 // cap tanh(x / cap), by one of two forms.  u = 2^-24.
 //
@@ -59,7 +71,11 @@ inline Squash make_squash(float temperature, float softcap) {
 // Beyond: (1 - E) / (1 + E) with E = e^(-2 |x| / cap) and x's sign, two special-unit operations.  E's
 // argument is off by 2 u relative and the hardware's exponential by 4 u, which reaches tanh as
 // 2 E / (1 + E)^2 (4 |x / cap| + 4) u <= 2.4 u; the difference, the sum and the quick division add
-// 6 u of tanh itself: at most 8 u of cap.
+// 6 u of tanh itself: at most 8 u of cap.  1 - E cancels for small logits, which come here beside one
+// beyond the cap (a mask of the type's lowest value).  Up to a cap of 64 that is 3e-5 at most.  Above
+// it (kWideCap) logits below cap / 16 take x (1 - w / 3 + 2 w^2 / 15), whose next term is 0.05 u, so that
+// each is within 40 u of its value as well.  Taken under every cap, that cost the softcap's cases 2 to
+// 20 % (4096 x 50304 bf16, most logits beyond the cap: 175 + 227 us to 200 + 277).
 //
 // The second form holds everywhere, but its special-unit operations bound the kernels.  With the first
 // where a warp's logits allow it, 4096 x 50304 bf16 under a softcap of 30 takes 121 us forward and 160
@@ -85,20 +101,25 @@ __device__ __forceinline__ float2 squash_near(float2 x, const Squash& q) {
   return __fmul2_rn(x, __ffma2_rn(p, w, make_float2(1.f, 1.f)));
 }
 
+template <int CAP>
 __device__ __forceinline__ float squash_far(float x, const Squash& q) {  // holds for every x
   const float e = ex2(fabsf(x) * q.kc);
-  const float y = copysignf(q.cap * __fdividef(1.f - e, 1.f + e), x);
+  float y = copysignf(q.cap * __fdividef(1.f - e, 1.f + e), x);
+  if constexpr (CAP == kWideCap) {
+    const float z = x * q.inv_cap, w = z * z;
+    if (w < 0.00390625f) y = x * fmaf(fmaf(w, 2.f / 15.f, -1.f / 3.f), w, 1.f);
+  }
   return x == -INFINITY ? x : y;
 }
 
-template <bool CAP>
-__device__ __forceinline__ float squash(float x, const Squash& q) {
+template <int CAP>
+__device__ __forceinline__ float squash(float x, const Squash& q) {  // one logit
   if constexpr (!CAP) return x;
-  return fabsf(x) <= q.near ? squash_near(x, q) : squash_far(x, q);
+  return fabsf(x) <= q.cap ? squash_near(x, q) : squash_far<kCap>(x, q);
 }
 
 // Derivative of squash at its output y.
-template <bool CAP>
+template <int CAP>
 __device__ __forceinline__ float squash_slope(float y, const Squash& q) {
   if constexpr (!CAP) return 1.f;
   const float t = y * q.inv_cap;
@@ -265,7 +286,7 @@ __device__ __forceinline__ float2 word_pair(const uint32_t (&w)[NW], int i) {
   else return unpack2(w[i], (const T*)nullptr);
 }
 
-// Whether squash_near holds for all NW words, lm their largest value: none beyond q.near but -inf and
+// Whether squash_near holds for all NW words, lm their largest value: none beyond the cap but -inf and
 // NaN, which it passes on (its last coefficient is positive).  One answer for the lanes that are here
 // together: the form that holds everywhere is cheaper than both in turn.
 __device__ __forceinline__ uint32_t abs_but_inf(uint32_t w, const __nv_bfloat16*) {
@@ -283,13 +304,13 @@ __device__ __forceinline__ bool all_near(const uint32_t (&w)[NW], float lm, cons
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < NW; ++i) m = max(m, 2u * w[i] + 0x01000000u);
-    return __all_sync(__activemask(), m <= 2u * __float_as_uint(q.near) + 0x01000000u && lm <= q.near);
+    return __all_sync(__activemask(), m <= 2u * __float_as_uint(q.cap) + 0x01000000u && lm <= q.cap);
   } else {
     uint32_t m = abs_but_inf(w[0], (const T*)nullptr);
 #pragma unroll
     for (int i = 1; i < NW; ++i) m = word_max(m, abs_but_inf(w[i], (const T*)nullptr), (const T*)nullptr);
     const float2 v = unpack2(m, (const T*)nullptr);
-    return __all_sync(__activemask(), fmaxf(v.x, v.y) <= q.near && lm <= q.near);
+    return __all_sync(__activemask(), fmaxf(v.x, v.y) <= q.cap && lm <= q.cap);
   }
 }
 
@@ -380,7 +401,7 @@ constexpr float kSlack = 16.f;              // a maximum this far above the refe
 //   r    the reference;  lim  the y above which it moves (-inf: nothing seen yet)
 //   s    sum of e;  w  sum of e * d (entropy only)
 // A -inf logit adds nothing (its term of w is cut off at a finite d); a NaN reaches s.
-template <bool CAP, bool ENT>
+template <int CAP, bool ENT>
 struct RowStats {
   float m, lim, s, w;
   Ref r;
@@ -453,7 +474,7 @@ struct RowStats {
       for (int i = 0; i < P; ++i) {
         const float2 x = word_pair<T>(w_, i);
         // without the polynomial: both forms in one unrolled loop cost more than they save
-        const float2 y = CAP ? make_float2(squash_far(x.x, q), squash_far(x.y, q)) : x;
+        const float2 y = CAP ? make_float2(squash_far<CAP>(x.x, q), squash_far<CAP>(x.y, q)) : x;
         const float2 d = make_float2(exponent(y.x, r, q), exponent(y.y, r, q));
         const float2 e = make_float2(ex2(d.x), ex2(d.y));
         s2 = __fadd2_rn(s2, e);

@@ -286,11 +286,11 @@ struct FwdArgs {
 constexpr int kBatch = 2;  // groups of a thread in flight
 // CTAs on an SM: 16-bit groups take 32 registers a thread with two in flight, which hides the
 // row's start and end behind seven other rows; fp32 groups are twice as large
-template <typename T, bool CAP, int NT>
+template <typename T, int CAP, int NT>
 constexpr int resident() { return (sizeof(T) == 4 ? 4 : (CAP ? 5 : 8)) * (kThreads / NT); }
 
 // A row's results from its joined and centred statistics.
-template <typename T, bool CAP, bool ENT>
+template <typename T, int CAP, bool ENT>
 __device__ __forceinline__ void write_row(const FwdArgs& a, int64_t r, const T* row, const RowStats<CAP, ENT>& st,
                                           float logs) {
   const int64_t t = a.targets ? a.targets[r] : 0;
@@ -313,7 +313,7 @@ __device__ __forceinline__ void write_row(const FwdArgs& a, int64_t r, const T* 
   if (a.stats) a.stats[r] = make_float4(st.r.sh, st.r.k, logs, H);
 }
 
-template <typename T, bool CAP, bool ENT, bool TOP, int NT>
+template <typename T, int CAP, bool ENT, bool TOP, int NT>
 __global__ void __launch_bounds__(NT, (resident<T, CAP, NT>()))
 token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
   constexpr int kWarps = NT / 32;
@@ -459,7 +459,7 @@ token_logprobs_fwd_kernel(const T* __restrict__ logits, const FwdArgs a) {
 }
 
 // Many short rows: one warp a row, nothing shared.
-template <typename T, bool CAP, bool ENT>
+template <typename T, int CAP, bool ENT>
 __global__ void __launch_bounds__(kThreads)
 token_logprobs_warp_kernel(const T* __restrict__ logits, const FwdArgs a, int64_t rows) {
   const int lane = threadIdx.x & 31;
@@ -509,7 +509,7 @@ constexpr int kBwdBatch = 4;
 constexpr int kBwdGroups = 32 * kBwdBatch;  // groups of one warp
 
 // Elementwise from the forward's numbers: each warp takes one segment of a row.
-template <typename T, bool CAP, bool ENT>
+template <typename T, int CAP, bool ENT>
 __global__ void __launch_bounds__(kThreads)
 token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, const BwdArgs a) {
   const int tid = threadIdx.x & 31;
@@ -537,14 +537,14 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
   const float c0 = (ge * (logs - H) - gl) * f, c1 = -ge * kLn2 * f, ct = gl * q.inv_t;
   const int ti = (a.targets && t >= 0 && t < a.V) ? (int)t : -1;
 
-  auto one = [&](float x, int i) {
-    const float y = CAP ? squash_far(x, q) : x;
+  auto one_at = [&](float y, int i) {  // y: squashed
     const float d = exponent(y, ref, q);
     float o = ex2(d);
     o *= ENT ? fmaf(c1, fmaxf(d, kNoTerm), c0) : c0;
     if (i == ti) o += ct;
     return o * squash_slope<CAP>(y, q);
   };
+  auto one = [&](float x, int i) { return one_at(squash<CAP>(x, q), i); };
   [[maybe_unused]] uint32_t floor = 0;
   bool quick = ref.sh == 0.f;
   if constexpr (ENT && !CAP) {
@@ -583,8 +583,8 @@ token_logprobs_bwd_kernel(T* __restrict__ grad, const T* __restrict__ logits, co
 #pragma unroll
             for (int i = 0; i < P; ++i) {
               const float2 v = word_pair<T>(w, i);
-              x[h * 2 * P + 2 * i] = one(v.x, -2);  // the target's part follows
-              x[h * 2 * P + 2 * i + 1] = one(v.y, -2);
+              x[h * 2 * P + 2 * i] = one_at(squash_far<CAP>(v.x, q), -2);  // the target's part follows
+              x[h * 2 * P + 2 * i + 1] = one_at(squash_far<CAP>(v.y, q), -2);
             }
             continue;
           }
@@ -652,28 +652,27 @@ int check_rows(const char* what, const void* logits, int64_t rows, int64_t inner
 constexpr int64_t kShortRow = 4096, kSmallRow = 8192;
 
 template <typename T, int NT>
-void (*pick_fwd(bool cap, bool ent, bool top))(const T*, FwdArgs) {
-#define AK_PICK(C, E, P) \
-  if (cap == C && ent == E && top == P) return token_logprobs_fwd_kernel<T, C, E, P, NT>;
-  AK_PICK(false, false, false) AK_PICK(false, false, true) AK_PICK(false, true, false) AK_PICK(false, true, true)
-  AK_PICK(true, false, false) AK_PICK(true, false, true) AK_PICK(true, true, false)
-#undef AK_PICK
-  return token_logprobs_fwd_kernel<T, true, true, true, NT>;
+void (*pick_fwd(const Squash& q, bool ent, bool top))(const T*, FwdArgs) {
+  AK_DISPATCH_CAP(q, CAP, return ent ? (top ? token_logprobs_fwd_kernel<T, CAP, true, true, NT>
+                                            : token_logprobs_fwd_kernel<T, CAP, true, false, NT>)
+                                     : (top ? token_logprobs_fwd_kernel<T, CAP, false, true, NT>
+                                            : token_logprobs_fwd_kernel<T, CAP, false, false, NT>));
 }
 
 template <typename T>
 int launch_fwd(const T* logits, const FwdArgs& a, int64_t rows, cudaStream_t st) {
-  const bool cap = a.q.cap > 0.f, ent = a.entropy != nullptr, top = a.k > 0;
+  const bool ent = a.entropy != nullptr, top = a.k > 0;
   if (!top && a.V <= kShortRow && rows >= 4 * sm_count()) {
-    auto kern = cap ? (ent ? token_logprobs_warp_kernel<T, true, true> : token_logprobs_warp_kernel<T, true, false>)
-                    : (ent ? token_logprobs_warp_kernel<T, false, true> : token_logprobs_warp_kernel<T, false, false>);
+    auto kern = token_logprobs_warp_kernel<T, kNoCap, true>;
+    AK_DISPATCH_CAP(a.q, CAP, kern = ent ? token_logprobs_warp_kernel<T, CAP, true>
+                                         : token_logprobs_warp_kernel<T, CAP, false>);
     const int64_t grid = (rows + kThreads / 32 - 1) / (kThreads / 32);
     AK_CUDA_TRY(launch_rows(kern, grid, kThreads, 1, 0, st, logits, a, rows), "ak_token_logprobs_fwd");
     return AK_OK;
   }
   const bool few = a.V <= kSmallRow && a.cs == 1;
   const int nt = few ? kFew : kThreads;
-  auto kern = few ? pick_fwd<T, kFew>(cap, ent, top) : pick_fwd<T, kThreads>(cap, ent, top);
+  auto kern = few ? pick_fwd<T, kFew>(a.q, ent, top) : pick_fwd<T, kThreads>(a.q, ent, top);
   const size_t smem = top ? ((size_t)(a.V / kGroup) / a.cs + 3 + 4) * 4 : 0;  // read four at a time
   AK_CUDA_TRY(launch_rows(kern, rows * a.cs, nt, a.cs, smem, st, logits, a), "ak_token_logprobs_fwd");
   return AK_OK;
@@ -734,10 +733,10 @@ extern "C" int ak_token_logprobs_bwd(void* grad, const void* logits, const int64
   a.segs = (int)std::max<int64_t>(1, (V / kGroup + kBwdGroups - 1) / kBwdGroups);
   a.q = make_squash(temperature, softcap);
   AK_REQUIRE(rows * a.segs < (1LL << 32) - 8, AK_ERR_SHAPE, "ak_token_logprobs_bwd: too many rows");
-  const bool cap = a.q.cap > 0.f, ent = g_entropy != nullptr;
+  const bool ent = g_entropy != nullptr;
   AK_DISPATCH_DTYPE(dt, T, {
-    auto kern = cap ? (ent ? token_logprobs_bwd_kernel<T, true, true> : token_logprobs_bwd_kernel<T, true, false>)
-                    : (ent ? token_logprobs_bwd_kernel<T, false, true> : token_logprobs_bwd_kernel<T, false, false>);
+    auto kern = token_logprobs_bwd_kernel<T, kNoCap, true>;
+    AK_DISPATCH_CAP(a.q, CAP, kern = ent ? token_logprobs_bwd_kernel<T, CAP, true> : token_logprobs_bwd_kernel<T, CAP, false>);
     kern<<<(unsigned)((rows * a.segs + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, (cudaStream_t)stream>>>(
         (T*)grad, (const T*)logits, a);
   });

@@ -64,3 +64,36 @@ def test_masked_tokens_at_the_lowest_temperatures(T, dtype):
         q = token_logprobs(leaf, torch.full((n,), 5, device=DEV), entropy=True, temperature=T)
         g, = torch.autograd.grad(q.entropy, leaf, torch.full((n,), T, device=DEV))
         assert (g.abs() <= 8 * O.U).all()  # p (log p + H) = 0 for both
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cap", [100.0, 2.0e4, 1e12, 1e30, 3e38])
+def test_small_logits_beside_masks_of_the_lowest_value(monkeypatch, cap, dtype):
+    """A warp with a logit beyond the cap takes another form of the softcap, which has to keep the
+    small logits of that warp as well: within 40 u of their own value, not of the cap."""
+    from kernels.token_logprobs import token_logprobs
+    low = torch.finfo(dtype).min
+    monkeypatch.setattr(O, "CAP", 0)       # the softcap's error is counted here
+    for n, v in ((3, 4001), (700, 515), (40, 9000)):
+        g = torch.Generator().manual_seed(n)
+        x = (torch.randn(n, v, generator=g) * 6).to(dtype)
+        x[torch.rand(n, v, generator=g) < 0.05] = low
+        t = torch.randint(0, v, (n,), generator=g)
+        x[torch.arange(n), t] = 1.25
+        x[0, 7] = min(cap * 3, 6e4) if cap < 1e4 else 1.0
+        ref = O.token_logprobs(x.double(), t, softcap=cap)
+        size = torch.where(x == low, 0.0, x.double()).abs().amax(1).clamp(max=cap)
+        # a masked token at -cap counts where exp(-cap) does: under 100 with an error of 8 u cap
+        e = 40 * O.U * size + (8 * O.U * cap if cap <= 100 else 0.0)
+        r = token_logprobs(x.to(DEV), t.to(DEV), entropy=True, softcap=cap)
+        O.assert_within(r.lse, ref["lse"], ref["tol_lse"] + e, "lse")
+        O.assert_within(r.logprobs, ref["logprobs"], ref["tol_logprobs"] + 2 * e, "logprobs")
+        O.assert_within(r.entropy, ref["entropy"], ref["tol_entropy"] + 2 * e * (1 + 2 * ref["entropy"].abs()), "entropy")
+        leaf = x.to(DEV).requires_grad_(True)
+        gl = torch.randn(n, generator=g)
+        got, = torch.autograd.grad(token_logprobs(leaf, t.to(DEV), softcap=cap).logprobs, leaf, gl.to(DEV))
+        want, tol = O.token_logprobs_grad(x.double(), t, gl, None, softcap=cap)
+        p = ref["p"]
+        # p is off by 2 e relative, the slope 1 - (y / cap)^2 by 20 u
+        tol = tol + p * 2 * e[:, None] * gl.abs()[:, None].double() + want.abs() * 24 * O.U
+        O.assert_within(got, want, tol + 24 * O.U * gl.abs()[:, None].double() * (p + (torch.arange(v) == t[:, None])), "grad")
