@@ -64,14 +64,15 @@ inline Squash make_squash(float temperature, float softcap) {
 // cap tanh(x / cap), by one of two forms.  u = 2^-24.
 //
 // |x| <= cap: x P(w), w = (x / cap)^2, where P is the polynomial of degree 6 with P(0) = 1 whose largest
-// relative distance from tanh(z) / z on 0 < z <= 1 is smallest (found by exchange of its extrema):
-// 0.93 u.  With the roundings of w (5 u, of which 0.22 reach tanh(z) / z), of Horner's steps and of the
-// product it is within 5 u of its value, small logits under a large cap too.
+// relative distance from tanh(z) / z on 0 < z <= 1 is smallest.  Its coefficients were rounded to fp32
+// one after the other, the later ones fitted anew to those that were (linear programs over a grid of
+// w): 0.93 u, as without the rounding.  w is off by 5 u, of which 0.22 reach tanh(z) / z; Horner's
+// steps add 1.2 u and the product 1 u: within 5 u of its value, small logits under a large cap too.
 //
 // Beyond: (1 - E) / (1 + E) with E = e^(-2 |x| / cap) and x's sign, two special-unit operations.  E's
 // argument is off by 2 u relative and the hardware's exponential by 4 u, which reaches tanh as
 // 2 E / (1 + E)^2 (4 |x / cap| + 4) u <= 2.4 u; the difference, the sum and the quick division add
-// 6 u of tanh itself: at most 8 u of cap.  1 - E cancels for small logits, which come here beside one
+// 6 u of tanh itself: at most 9 u of cap.  1 - E cancels for small logits, which come here beside one
 // beyond the cap (a mask of the type's lowest value).  Up to a cap of 64 that is 3e-5 at most.  Above
 // it (kWideCap) logits below cap / 16 take x (1 - w / 3 + 2 w^2 / 15), whose next term is 0.05 u, so that
 // each is within 40 u of its value as well.  Taken under every cap, that cost the softcap's cases 2 to
@@ -82,7 +83,7 @@ inline Squash make_squash(float temperature, float softcap) {
 // backward (167 and 198 without it), distillation of 8192 rows 696 us (917); logits that mostly lie
 // beyond the cap pay 5 to 19 % for the test.
 __device__ constexpr float tanh_coef(int i) {  // of w^(i + 1)
-  const float c[6] = {-0.333329856f, 0.133264095f, -0.0534987077f, 0.0203597602f, -0.00625933986f, 0.00105826487f};
+  const float c[6] = {-0.333329886f, 0.133264288f, -0.0534994751f, 0.0203611124f, -0.00626045559f, 0.00105861423f};
   return c[i];
 }
 
