@@ -174,3 +174,33 @@ def test_two_threads_with_different_vocabularies(sizes):
         t.join()
     assert not errors, errors
     _ak.check_status(device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 2, 22])
+def test_the_longest_rows(n, dtype):
+    """As many elements as eight CTAs' shared memory holds: 851,968 of 16 bits or 425,984 of fp32 (and
+    the rest of a group); more rows than the GPU takes clusters at once; rows that start anywhere."""
+    from kernels import _ak
+    from kernels.distill import distill_topk
+    v = (425_984 if dtype == torch.float32 else 851_968) + 15
+    full, _, _ = rows(n, v + 1, 1, dtype, 12)
+    g = torch.Generator().manual_seed(13)
+    for x in (full[:, :v], full[:, 1:]):
+        idx = torch.randint(0, v, (n, 64), generator=g).to(DEV)
+        idx[:, 0], idx[:, 1] = 0, v - 1
+        tlp = torch.log_softmax(torch.randn(n, 64, generator=g), 1).to(DEV) - 0.2
+        if n <= 2:
+            check(x, idx, tlp, tail=True)
+            continue
+        mask = torch.rand(n, generator=g).to(DEV) < 0.8
+        mask[n - 1] = True
+        loss, losses, _, grad, _, _ = _ak.distill_topk_fwd(x, idx, tlp, mask, tail=True, want_grad=True)
+        at = [0, n // 2, n - 1]
+        ref = O.distill_topk(x[at].double().cpu(), idx[at].cpu(), tlp[at].cpu(), mask[at].cpu(), tail=True)
+        O.assert_within(losses[at], ref["losses"], ref["tol_losses"], "losses")
+        f = max(1, int(mask[at].sum())) / int(mask.sum())
+        O.assert_within(grad[at], ref["grad"] * f, ref["tol_grad"] * f, "grad")
+    _ak.check_status(torch.device(DEV))
+    with pytest.raises(RuntimeError, match="does not fit"):
+        distill_topk(torch.zeros(1, v + 1 + 8 * 16, dtype=dtype, device=DEV), idx[:1], tlp[:1])

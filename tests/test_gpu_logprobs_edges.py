@@ -97,3 +97,35 @@ def test_small_logits_beside_masks_of_the_lowest_value(monkeypatch, cap, dtype):
         # p is off by 2 e relative, the slope 1 - (y / cap)^2 by 20 u
         tol = tol + p * 2 * e[:, None] * gl.abs()[:, None].double() + want.abs() * 24 * O.U
         O.assert_within(got, want, tol + 24 * O.U * gl.abs()[:, None].double() * (p + (torch.arange(v) == t[:, None])), "grad")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", [(1, 128), (3, 7), (40, 20)])
+def test_the_largest_vocabulary_with_alternatives(n, k, dtype):
+    """1,048,320 tokens: eight CTAs a row, each with as many group maxima as its buffer holds; rows
+    that start anywhere, ties that go through the exact selection, and the last token among the best."""
+    from kernels.token_logprobs import token_logprobs
+    v = 1_048_320
+    g = torch.Generator(device=DEV).manual_seed(n)
+    full = torch.randn(n, v + 3, generator=g, device=DEV).mul_(2).to(dtype)
+    for x in (full[:, :v], full[:, 3:]):
+        x[0, v - 1] = 20.0
+        x[0, 0] = 20.0
+        if n > 2:
+            x[1] = 1.0                     # constant: the lowest indices
+            x[2] = -torch.inf
+            x[2, v - 5:] = 0.5
+        t = torch.full((n,), v - 1, device=DEV)
+        r = token_logprobs(x, t, top_k=k, entropy=True)
+        for i in range(0, n, max(1, n // 5)):
+            s = slice(i, i + 1)
+            ref = O.token_logprobs(x[s].double().cpu(), t[s].cpu(), top_k=k)
+            assert torch.equal(r.top_indices[s].cpu(), ref["top_indices"])
+            for f, tol in (("logprobs", "tol_logprobs"), ("entropy", "tol_entropy"), ("lse", "tol_lse"), ("top_logprobs", "tol_top")):
+                O.assert_within(getattr(r, f)[s], ref[f], ref[tol], f)
+        if n > 2:
+            assert torch.equal(r.top_indices[1].cpu(), torch.arange(k))
+            assert torch.equal(r.top_indices[2, :min(k, 5)].cpu(), torch.arange(v - 5, v)[:k])
+    with pytest.raises(RuntimeError, match="too large for top_k"):
+        token_logprobs(torch.zeros(1, v + 1, dtype=dtype, device=DEV), top_k=1)
+    assert token_logprobs(torch.zeros(1, v + 17, dtype=dtype, device=DEV)).lse.shape == (1,)
