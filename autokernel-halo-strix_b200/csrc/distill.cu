@@ -28,14 +28,17 @@
 // Rows of up to 8 KB take one warp each instead: their fixed steps overlap across many rows.
 //
 // What it measured (loss and gradient, GPU time, floors at the measured 6551 GB/s):
-//   8192 x 50304 bf16, K 64       372 us, floor 253: two CTAs an SM hold two rows; leaving out the
-//                                 stores changes nothing, leaving out either pass's exponentials 10 %,
-//                                 so it is bound by the issue slots of the two passes (16.6
-//                                 instructions an element, the waits among them)
-//   3000 x 50257 fp32, K 20       247 us, floor 184
-//   60000 x 4000 bf16, K 32       217 us, floor 146 (a warp each)
-//   100000 x 1500 bf16, K 8       233 us, floor 92 (a warp each)
-//   1023 x 50257 fp16, K 33       38 us forward + 36 us backward, floors 16 + 31
+//   8192 x 50304 bf16, K 64       381 us, floor 253: no unit is saturated (issue slots 48 % active,
+//                                 special units 48 %, 40 % of the warps): it waits.  Two CTAs an SM
+//                                 hold one row each, so nothing is left to load during a row's
+//                                 statistics.  Leaving out the stores changes nothing, leaving out
+//                                 either pass's exponentials 10 %
+//   the same, softcap 30          711 us: issue slots 56 %, twice the instructions
+//   3000 x 50257 fp32, K 20       252 us, floor 184
+//   16000 x 20000 bf16, K 100     450 us, floor 195: the teacher's warp
+//   60000 x 4000 bf16, K 32       220 us, floor 146 (a warp each)
+//   100000 x 1500 bf16, K 8       240 us, floor 92 (a warp each)
+//   1023 x 50257 fp16, K 33       38 us forward + 37 us backward, floors 16 + 31
 // Tried and dropped: one CTA with two row buffers (405 us), no roles (398 us), two teacher warps
 // (423 us), four CTAs of half rows (480 us).
 #include "logit_rows.cuh"

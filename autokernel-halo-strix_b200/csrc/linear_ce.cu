@@ -42,8 +42,8 @@
 // their gradients (EPI_LOGP_GRAD: the logits are formed again and leave the accumulators as
 // dL/dlogits in 16 bits, from the forward's statistics; then the grouped dW / dH launch).  Measured:
 // 4096 x 768 x 50304 bf16 270-320 us forward (1.0-1.2 PFLOP/s, tensor cores; clocks under the power
-// cap) and 840-900 us backward (three products and the logits again); 2001 x 1536 x 32000 fp16 172 us
-// forward; 8 x 768 x 50304 bf16 27 us, floor 12 (the weight once): 2.7 rounds of tiles and the row join.
+// cap) and 840-900 us backward (three products and the logits again); 2001 x 1536 x 32000 fp16 170 us
+// forward; 8 x 768 x 50304 bf16 28 us, floor 12 (the weight once): 2.7 rounds of tiles and the row join.
 #include "logit_rows.cuh"
 
 #include <cfloat>
@@ -673,7 +673,12 @@ __device__ __forceinline__ LogpRow load_logp_row(const Prob& P, int row) {
   return r;
 }
 
-// The logits' gradient, rounded to T once: the operand type of the dW / dH products.
+// The logits' gradient, rounded to T once: the operand type of the dW / dH products.  That rounding is
+// seen in the result, as it is in any product of 16-bit gradients: 4096 x 768 x 50304 bf16, dW and dH
+// are off by 2.3e-3 of their norm, where an fp32 gradient leaves 1.7e-3 (the results' own rounding).
+// Keeping what it left over as a second matrix (C2) reaches that 1.7e-3, but each product is paid
+// twice: 3.5 ms for 0.84 at 4096 rows, 457 us for 157 at 257.  So only up to kFewRows rows, whose
+// roundings have little to average over, have it.
 template <typename T>
 __device__ __forceinline__ void epi_logp_grad(const Prob& P, uint32_t tbase, int row0, int lane, const LogpRow& lr,
                                               int col0, int eg, uint32_t stg) {

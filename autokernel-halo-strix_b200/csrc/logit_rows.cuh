@@ -79,9 +79,9 @@ inline Squash make_squash(float temperature, float softcap) {
 // 20 % (4096 x 50304 bf16, most logits beyond the cap: 175 + 227 us to 200 + 277).
 //
 // The second form holds everywhere, but its special-unit operations bound the kernels.  With the first
-// where a warp's logits allow it, 4096 x 50304 bf16 under a softcap of 30 takes 121 us forward and 160
-// backward (167 and 198 without it), distillation of 8192 rows 696 us (917); logits that mostly lie
-// beyond the cap pay 5 to 19 % for the test.
+// where a warp's logits allow it, 4096 x 50304 bf16 under a softcap of 30 takes 121 us forward and 165
+// backward (167 and 198 without it), distillation of 8192 rows 711 us (917); logits that mostly lie
+// beyond the cap pay 5 to 24 % for the test.
 __device__ constexpr float tanh_coef(int i) {  // of w^(i + 1)
   const float c[6] = {-0.333329886f, 0.133264288f, -0.0534994751f, 0.0203611124f, -0.00626045559f, 0.00105861423f};
   return c[i];

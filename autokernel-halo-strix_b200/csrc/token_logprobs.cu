@@ -16,14 +16,14 @@
 // they are read again, from L2.
 //
 // What bounds it and what it measured (GPU time; 6551 GB/s is the measured copy rate):
-//   8192 x 50304 bf16, entropy   131 us = 6.3 TB/s: HBM; one exponential an element keeps the special
+//   8192 x 50304 bf16, entropy   129-133 us = 6.2-6.4 TB/s: HBM; one exponential an element keeps the special
 //                                units at 2/3
-//   4096 x 32768 fp16, entropy   48.5 us = 5.5 TB/s
+//   4096 x 32768 fp16, entropy   48.2 us = 5.6 TB/s
 //   8192 x 50304 bf16, top 64    163 us: the selection costs 35 us (its barriers and a few hundred
 //                                instructions a warp; ranking by counting among the ~75 candidates)
 //   64 x 131072 fp32, softcap    17 us, floor 5.1 us (18.4 with the softcap by special units alone)
-//   1 x 50304 bf16, top 20       9.5 us: latency of one cluster (load, two reductions, selection, join)
-//   backward 8192 x 50304 bf16   237 us = 6.95 TB/s: HBM
+//   1 x 50304 bf16, top 20       9.8 us: latency of one cluster (load, two reductions, selection, join)
+//   backward 8192 x 50304 bf16   238 us = 6.9 TB/s: HBM
 #include "logit_rows.cuh"
 
 #include <algorithm>

@@ -57,14 +57,16 @@ class _DistillTopK(torch.autograd.Function):
 def distill_topk(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_logprobs: torch.Tensor, *,
                  mask: Optional[torch.Tensor] = None, temperature: float = 1.0, softcap: float = 0.0,
                  tail: bool = False, mode: Optional[str] = None) -> torch.Tensor:
-    """temperature^2 * mean over the rows of KL(teacher || student), a scalar.
+    """temperature^2 * mean over the rows of sum_k q_k (log q_k - log p_k), a scalar: KL(teacher ||
+    student) where a row's tokens are all different.
 
     logits (..., V): the student's, fp32, bf16 or fp16 on the GPU; p = softmax(softcap(logits) /
     temperature).  Row views are read in place, as in `token_logprobs`.
     teacher_indices, teacher_logprobs (..., K), K <= 128: the teacher's tokens and their
     log-probabilities at the same temperature.  A negative index is padding; a row of padding alone
     has loss 0 and no gradient.  An index outside the vocabulary makes its row NaN.  Several entries
-    of one token add up.
+    of one token have a term each; their masses add up in the gradient (a constant away from the KL
+    of the merged teacher).
     tail: False renormalises the teacher over its K entries; True takes exp(teacher_logprobs) as they
     are and compares the rest of both distributions as one bucket, left out where the student has
     masked it (no logit outside the teacher's tokens within 30000 of its largest) and where the

@@ -228,7 +228,8 @@ AK_API int ak_token_logprobs_bwd(void* grad, const void* logits, const int64_t* 
  *             the terms that are there: T dL/dx_i = Q p_i - q_i (- r p_i / p_r outside the K
  *             tokens), Q = sum q + r, or sum q without the rest's term
  * A negative index is padding; a row of nothing else has loss 0 and no gradient (it counts in the
- * mean).  An index >= V makes its row's loss and gradient NaN.  Entries of one token add up.
+ * mean).  An index >= V makes its row's loss and gradient NaN.  Entries of one token: each has its
+ * term in the loss, and the gradient is that of their summed mass.
  * losses[rows] fp32: the rows' divergences (0 without mask).  inv_n (needed with a mask): receives
  * 1 / max(1, rows with mask).
  * grad (nullable): d loss / d logits, dense [rows][V] dt.  Without it, rest_stats [rows][4] and
@@ -327,10 +328,14 @@ AK_API int ak_linear_logprobs_fwd(float* logprobs, float* entropy, float* lse, f
 
 /* dH[N, D] and dW[V, D] (dt, each nullable) from the gradients of logprobs and entropy (fp32 [N],
  * each nullable) and the forward's row_stats.  Per chunk of at most 16384 rows the
- * logits are formed again and leave the accumulators as their gradient, rounded to dt once (in
- * fp16 divided by the largest upstream gradient, which the next products' fp32 accumulators
- * restore); then dW += G^T H and dH = G W in one launch.  Ignored rows have G = 0: their hidden
- * states enter dW as 0 * h. */
+ * logits are formed again and leave the accumulators as their gradient G in dt, the operand of
+ * dW += G^T H and dH = G W:
+ *   - rounded once; for up to 256 rows what the rounding left over is kept as a second matrix;
+ *   - in fp16 divided by the largest upstream gradient of the rows that count (at temperatures
+ *     below 1/256 by more), which the products' fp32 accumulators restore;
+ *   - both products run in one launch, but for few rows, where dH's long sum over the vocabulary is
+ *     cut into runs that are added up afterwards.
+ * Ignored rows have G = 0: their hidden states enter dW as 0 * h. */
 AK_API int ak_linear_logprobs_bwd(void* dH, void* dW, void* workspace, size_t ws_bytes,
                                   const void* H, const void* W, const int64_t* targets,
                                   const float* row_stats, const float* g_logprobs,
